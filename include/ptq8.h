@@ -1,5 +1,6 @@
 /*
- * ptq8.h - C ABI of the B200-native (sm_100a) W8A8 / W4A8 quantized-conv engine.
+ * ptq8.h - C ABI of the B200-native (sm_100a) W8A8 / W4A8 quantized-conv engine and of its
+ * token operators (per-token quantization, linear layers, experts).
  *
  * Drop-in boundary for the reference's int8 engine (PaperTigerL/ptq-int8-lab,
  * 06-gpu-int8/cpp).  Each entry point names the reference interface it
@@ -279,6 +280,90 @@ int ptq8_capture_graph(ptq8_engine* e, int n);
 /* Destroy an engine and, when it came from ptq8_load, its model. */
 void ptq8_destroy(ptq8_engine* e);
 const char* ptq8_last_error(const ptq8_engine* e);
+
+/* ---- token operators ---------------------------------------------------------
+ *
+ * The engine's arithmetic for a language model's layers: int8 activations with one
+ * scale per token, int8 (or packed int4) weights with one scale per output channel,
+ * exact int32 sums.  No reference counterpart (its engine runs convolutions with
+ * static activation ranges).  All tensors are device memory of the handle's device;
+ * every call only enqueues work on `stream` (a cudaStream_t, NULL: the legacy default
+ * stream), allocates nothing and may be captured in a CUDA graph.  Row pitches are in
+ * elements of the tensor, and may exceed the row's width.  One handle per device per
+ * host thread; handles are independent of engines. */
+
+typedef struct ptq8_ops ptq8_ops;
+
+/* element types */
+#define PTQ8_F32 0
+#define PTQ8_F16 1
+#define PTQ8_BF16 2
+
+/* what a product does with its channels */
+#define PTQ8_EPI_NONE 0
+#define PTQ8_EPI_SWIGLU 1 /* weights hold 2*out_features channels, gate then up: y = silu(gate) * up */
+
+/* int32 sums of in_features products of codes of magnitude <= 128 never overflow up to here */
+#define PTQ8_MAX_IN_FEATURES 131071
+#define PTQ8_MAX_GROUPS 1024
+
+ptq8_ops* ptq8_ops_create(int device, char* err, size_t errlen);
+void ptq8_ops_destroy(ptq8_ops* ops); /* the caller has synchronised the streams it used */
+const char* ptq8_ops_last_error(const ptq8_ops* ops);
+/* Waits for `stream`, then reports (and clears) a bounded device wait that ran out: PTQ8_ERR_TIMEOUT.
+ * Until it is cleared here, every further call on the handle returns PTQ8_ERR_TIMEOUT too. */
+int ptq8_ops_check_device_error(ptq8_ops* ops, void* stream);
+/* Failure-detection test hook: wait limit in clock cycles (0: the default, about 2 s), and a switch that makes
+ * the tensor-core product announce the first operand load of its first block without issuing it. */
+int ptq8_ops_set_wait_test(ptq8_ops* ops, long long wait_limit_cycles, int stall_first_load);
+
+/* int8 codes with one scale per row (token):
+ *   scale[r] = max(fl32(max_k |x[row(r)][k]| / 127), 1e-8)
+ *   codes[r][k] = round_half_away(x[row(r)][k] / scale[r])   (the exact quotient; within +-127)
+ * row(r) = rows[r], or r where rows is NULL.  A row whose index is outside [0, x_rows) gets codes 0 and scale 0.
+ * A row that holds NaN or an infinity gets codes 0 and scale NaN or infinity, so that its products are NaN. */
+typedef struct {
+    const void* x;       /* [x_rows][width], pitch ldx */
+    long long ldx;
+    long long x_rows;
+    const int* rows;     /* [n_rows] or NULL (then n_rows == x_rows) */
+    long long n_rows;
+    int8_t* codes;       /* [n_rows][width], pitch ldc; must not overlap x */
+    long long ldc;
+    float* scale;        /* [n_rows] */
+    int width;
+    int x_type;          /* PTQ8_F32 / F16 / BF16 */
+} ptq8_rows_args;
+int ptq8_quantize_rows(ptq8_ops* ops, const ptq8_rows_args* args, void* stream);
+
+/* y[t][c] = fl(fl(float(sum_k x[t][k] * w[c][k]) * fl(x_scale[t] * w_scale[c])) + bias[c]), then the epilogue,
+ * then one rounding to y's type.  w_bits 4: codes two per byte, code k in the low (k even) or high half of byte k/2.
+ * The tensor-core kernels need x, w (and a group's weights) to start at multiples of 16 bytes and row pitches that
+ * are multiples of 16 bytes; any other layout runs on a slower kernel.
+ * ptq8_linear_grouped: rows offsets[g] .. offsets[g+1]-1 meet group g's weights (offsets: device memory, groups+1
+ * values, not decreasing, within [0, rows]; values outside are clamped); rows of no group are not written. */
+typedef struct {
+    const int8_t* x;       /* [rows][in_features], pitch ldx */
+    long long ldx;
+    const float* x_scale;  /* [rows] */
+    const void* w;         /* [groups][channels][in_features], pitch ldw bytes, groups w_group_stride bytes apart */
+    long long ldw;
+    long long w_group_stride;
+    const float* w_scale;  /* [groups][channels] */
+    const float* bias;     /* [groups][channels] or NULL */
+    void* y;               /* [rows][out_features], pitch ldy; must not overlap the inputs */
+    long long ldy;
+    const int* offsets;    /* ptq8_linear_grouped only */
+    long long rows;
+    int in_features;
+    int out_features;      /* channels = out_features, or twice that with PTQ8_EPI_SWIGLU */
+    int groups;            /* ptq8_linear_grouped only */
+    int w_bits;            /* 8 or 4 */
+    int epilogue;          /* PTQ8_EPI_* */
+    int y_type;            /* PTQ8_F32 / F16 / BF16 */
+} ptq8_linear_args;
+int ptq8_linear(ptq8_ops* ops, const ptq8_linear_args* args, void* stream);
+int ptq8_linear_grouped(ptq8_ops* ops, const ptq8_linear_args* args, void* stream);
 
 #ifdef __cplusplus
 }

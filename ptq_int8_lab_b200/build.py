@@ -18,25 +18,32 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 
 
-def _run(cmd):
-    print(" ".join(cmd), flush=True)
-    subprocess.check_call(cmd)
+# (source, object, further nvcc flags)
+SOURCES = (
+    ("ptq8_model.cpp", "ptq8_model.o", ["-x", "c++"]),
+    ("ptq8_engine.cu", "ptq8_engine.o", ["-lineinfo"]),
+    ("ptq8_ops.cu", "ptq8_ops.o", ["-lineinfo"]),
+)
 
 
 def build(verbose_ptxas: bool = False) -> Path:
     OUT.mkdir(exist_ok=True)
     lib = OUT / "libptq8.so"
-    objs = []
-    common = ["-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-I", str(HERE.parent / "include")]
-    o1 = OUT / "ptq8_model.o"
-    _run([NVCC, *common, *ARCH, "-x", "c++", "-c", str(SRC / "ptq8_model.cpp"), "-o", str(o1)])
-    objs.append(o1)
-    o2 = OUT / "ptq8_engine.o"
-    extra = ["-Xptxas", "-v"] if verbose_ptxas else []
-    _run([NVCC, *common, *ARCH, "-lineinfo", *extra, "-c", str(SRC / "ptq8_engine.cu"), "-o", str(o2)])
-    objs.append(o2)
+    common = ["-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-I", str(HERE.parent / "include"), *ARCH]
+    objs, running = [], []
+    for src, obj, flags in SOURCES:      # one compiler process per source, side by side
+        extra = ["-Xptxas", "-v"] if verbose_ptxas and src.endswith(".cu") else []
+        cmd = [NVCC, *common, *flags, *extra, "-c", str(SRC / src), "-o", str(OUT / obj)]
+        print(" ".join(cmd), flush=True)
+        objs.append(OUT / obj)
+        running.append((cmd, subprocess.Popen(cmd)))
+    failed = [cmd for cmd, p in running if p.wait() != 0]
+    if failed:
+        raise subprocess.CalledProcessError(1, failed[0])
     tmp = OUT / "libptq8.so.tmp"
-    _run([NVCC, "-shared", *ARCH, *[str(o) for o in objs], "-o", str(tmp), "-lcudart"])
+    cmd = [NVCC, "-shared", *ARCH, *[str(o) for o in objs], "-o", str(tmp), "-lcudart"]
+    print(" ".join(cmd), flush=True)
+    subprocess.check_call(cmd)
     os.replace(tmp, lib)
     for o in objs:
         o.unlink()

@@ -1,0 +1,285 @@
+// Token operators: host side of ptq8_quantize_rows, ptq8_linear and ptq8_linear_grouped
+// (argument checks, kernel choice, launches) and their extern "C" boundary.
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <cstdarg>
+#include <cstdio>
+#include <cstring>
+#include <exception>
+#include <new>
+#include <string>
+
+#include "ptq8.h"
+#include "ptq8_linear.cuh"
+#include "ptq8_rows.cuh"
+
+using namespace ptq8;
+
+struct ptq8_ops {
+    int device = 0;
+    int sms = 0;
+    int* error = nullptr;       // pinned host word that a kernel whose bounded wait ran out sets
+    int* error_dev = nullptr;   // its device address
+    long long wait_limit = kWaitLimitCycles;
+    int stall = 0;
+    std::string err;
+};
+
+namespace {
+
+int fail(ptq8_ops* o, int status, const char* f, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, f);
+    std::vsnprintf(buf, sizeof buf, f, ap);
+    va_end(ap);
+    o->err = buf;
+    return status;
+}
+
+void say(char* err, size_t n, const std::string& m) {
+    if (err && n) std::snprintf(err, n, "%s", m.c_str());
+}
+
+// The device becomes current for the call and is given back: a process may drive several.
+struct OnDevice {
+    int before = -1;
+    cudaError_t rc;
+    explicit OnDevice(int device) {
+        rc = cudaGetDevice(&before);
+        if (rc == cudaSuccess && before != device) rc = cudaSetDevice(device);
+        if (before == device) before = -1;
+    }
+    ~OnDevice() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
+// One launch with programmatic stream serialization: the kernel may be scheduled while the kernel
+// before it on the stream drains, and waits (griddepcontrol.wait) before it touches global memory.
+template <typename... P, typename... A>
+cudaError_t launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+size_t type_size(int t) { return t == PTQ8_F32 ? 4 : 2; }
+
+// What every call checks first: a wait of an earlier call that ran out, until it is cleared.
+int ready(ptq8_ops* o) {
+    if (*static_cast<volatile int*>(o->error))
+        return fail(o, PTQ8_ERR_TIMEOUT, "a device wait of an earlier call ran out (code %d); its outputs are invalid",
+                    *o->error);
+    return PTQ8_OK;
+}
+
+int cuda_fail(ptq8_ops* o, const char* what, cudaError_t e) {
+    cudaGetLastError();   // reported here: the process's next check must not find it again
+    return fail(o, PTQ8_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+}
+
+int check_rows(ptq8_ops* o, const ptq8_rows_args& a) {
+    const char* w = "quantize_rows";
+    if (a.x_type < PTQ8_F32 || a.x_type > PTQ8_BF16) return fail(o, PTQ8_ERR_INVALID, "%s: x_type %d", w, a.x_type);
+    if (a.width <= 0) return fail(o, PTQ8_ERR_INVALID, "%s: width %d", w, a.width);
+    if (a.x_rows < 0 || a.n_rows < 0 || a.n_rows > 0x7FFFFFFFLL)
+        return fail(o, PTQ8_ERR_INVALID, "%s: x_rows %lld, n_rows %lld", w, a.x_rows, a.n_rows);
+    if (!a.rows && a.n_rows != a.x_rows)
+        return fail(o, PTQ8_ERR_INVALID, "%s: n_rows %lld without a row index, but x has %lld rows", w, a.n_rows, a.x_rows);
+    if (a.ldx < a.width && a.x_rows > 1) return fail(o, PTQ8_ERR_INVALID, "%s: ldx %lld < width %d", w, a.ldx, a.width);
+    if (a.ldc < a.width && a.n_rows > 1) return fail(o, PTQ8_ERR_INVALID, "%s: ldc %lld < width %d", w, a.ldc, a.width);
+    if (a.n_rows == 0) return PTQ8_OK;
+    if ((!a.x && a.x_rows) || !a.codes || !a.scale) return fail(o, PTQ8_ERR_INVALID, "%s: null pointer", w);
+    if (reinterpret_cast<uintptr_t>(a.x) % type_size(a.x_type))
+        return fail(o, PTQ8_ERR_INVALID, "%s: x is not aligned to its element type", w);
+    return PTQ8_OK;
+}
+
+int check_linear(ptq8_ops* o, const ptq8_linear_args& a, bool grouped) {
+    const char* w = grouped ? "linear_grouped" : "linear";
+    if (a.w_bits != 8 && a.w_bits != 4) return fail(o, PTQ8_ERR_INVALID, "%s: w_bits %d (8 or 4)", w, a.w_bits);
+    if (a.epilogue != PTQ8_EPI_NONE && a.epilogue != PTQ8_EPI_SWIGLU)
+        return fail(o, PTQ8_ERR_INVALID, "%s: epilogue %d", w, a.epilogue);
+    if (a.y_type < PTQ8_F32 || a.y_type > PTQ8_BF16) return fail(o, PTQ8_ERR_INVALID, "%s: y_type %d", w, a.y_type);
+    if (a.in_features <= 0 || a.in_features > PTQ8_MAX_IN_FEATURES)
+        return fail(o, PTQ8_ERR_INVALID, "%s: in_features %d (1 to %d: int32 sums)", w, a.in_features, PTQ8_MAX_IN_FEATURES);
+    if (a.out_features <= 0 || a.out_features > (1 << 24))
+        return fail(o, PTQ8_ERR_INVALID, "%s: out_features %d", w, a.out_features);
+    if (a.rows < 0 || a.rows > 0x7FFFFF00LL) return fail(o, PTQ8_ERR_INVALID, "%s: rows %lld", w, a.rows);
+    const long long wide = a.w_bits == 4 ? (a.in_features + 1) / 2 : a.in_features;
+    const long long channels = static_cast<long long>(a.out_features) * (a.epilogue == PTQ8_EPI_SWIGLU ? 2 : 1);
+    if (a.ldx < a.in_features && a.rows > 1) return fail(o, PTQ8_ERR_INVALID, "%s: ldx %lld < in_features %d", w, a.ldx, a.in_features);
+    if (a.ldw < wide && channels > 1) return fail(o, PTQ8_ERR_INVALID, "%s: ldw %lld < %lld bytes of a weight row", w, a.ldw, wide);
+    if (a.ldy < a.out_features && a.rows > 1) return fail(o, PTQ8_ERR_INVALID, "%s: ldy %lld < out_features %d", w, a.ldy, a.out_features);
+    if (grouped) {
+        if (a.groups <= 0 || a.groups > PTQ8_MAX_GROUPS)
+            return fail(o, PTQ8_ERR_INVALID, "%s: groups %d (1 to %d)", w, a.groups, PTQ8_MAX_GROUPS);
+        if (a.groups > 1 && a.w_group_stride < a.ldw * (channels - 1) + wide)
+            return fail(o, PTQ8_ERR_INVALID, "%s: w_group_stride %lld: groups overlap", w, a.w_group_stride);
+        if (!a.offsets) return fail(o, PTQ8_ERR_INVALID, "%s: null offsets", w);
+    }
+    if (a.rows == 0) return PTQ8_OK;
+    if (!a.x || !a.x_scale || !a.w || !a.w_scale || !a.y) return fail(o, PTQ8_ERR_INVALID, "%s: null pointer", w);
+    if (reinterpret_cast<uintptr_t>(a.y) % type_size(a.y_type))
+        return fail(o, PTQ8_ERR_INVALID, "%s: y is not aligned to its element type", w);
+    return PTQ8_OK;
+}
+
+int run_rows(ptq8_ops* o, const ptq8_rows_args& a, cudaStream_t st) {
+    RowsParams p{a.x, a.codes, a.scale, a.rows, static_cast<size_t>(a.ldx), static_cast<size_t>(a.ldc), a.x_rows, a.width};
+    auto kernel = a.x_type == PTQ8_F32 ? rows_kernel<float> : a.x_type == PTQ8_F16 ? rows_kernel<__half> : rows_kernel<__nv_bfloat16>;
+    const cudaError_t e = launch(kernel, dim3(static_cast<unsigned>(a.n_rows)), dim3(256), 0, st, p);
+    return e == cudaSuccess ? PTQ8_OK : cuda_fail(o, "quantize_rows", e);
+}
+
+int run_linear(ptq8_ops* o, const ptq8_linear_args& a, bool grouped, cudaStream_t st) {
+    LinearParams p{};
+    p.x = a.x;
+    p.w = static_cast<const uint8_t*>(a.w);
+    p.xs = a.x_scale;
+    p.ws = a.w_scale;
+    p.bias = a.bias;
+    p.y = a.y;
+    p.offsets = grouped ? a.offsets : nullptr;
+    p.ldx = a.ldx;
+    p.ldw = a.ldw;
+    p.gstride = grouped ? a.w_group_stride : 0;
+    p.ldy = a.ldy;
+    p.rows = a.rows;
+    p.k = a.in_features;
+    p.n = a.out_features;
+    p.groups = grouped ? a.groups : 1;
+    p.y_type = a.y_type;
+    const bool gated = a.epilogue == PTQ8_EPI_SWIGLU, w4 = a.w_bits == 4;
+    const long long row_tiles = (a.rows + kAnyTile - 1) / kAnyTile;
+    // blocks stride over the channel tiles (x) and over a group's row tiles (y)
+    const dim3 grid(static_cast<unsigned>((a.out_features + kAnyTile - 1) / kAnyTile),
+                    static_cast<unsigned>(std::min<long long>(row_tiles, grouped ? 64 : 65535)), static_cast<unsigned>(p.groups));
+    auto kernel = w4 ? (gated ? linear_any_kernel<true, true> : linear_any_kernel<true, false>)
+                     : (gated ? linear_any_kernel<false, true> : linear_any_kernel<false, false>);
+    const cudaError_t e = launch(kernel, grid, dim3(256), 0, st, p);
+    return e == cudaSuccess ? PTQ8_OK : cuda_fail(o, "linear", e);
+}
+
+int product(ptq8_ops* o, const ptq8_linear_args* a, bool grouped, void* stream) {
+    if (!o) return PTQ8_ERR_INVALID;
+    try {
+        if (!a) return fail(o, PTQ8_ERR_INVALID, "null arguments");
+        if (const int rc = check_linear(o, *a, grouped)) return rc;
+        if (const int rc = ready(o)) return rc;
+        if (a->rows == 0) return PTQ8_OK;
+        OnDevice on(o->device);
+        if (on.rc != cudaSuccess) return cuda_fail(o, "cudaSetDevice", on.rc);
+        return run_linear(o, *a, grouped, static_cast<cudaStream_t>(stream));
+    } catch (const std::exception& ex) {
+        return PTQ8_ERR_INVALID;
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+ptq8_ops* ptq8_ops_create(int device, char* err, size_t errlen) {
+    try {
+        cudaDeviceProp prop;
+        cudaError_t e = cudaGetDeviceProperties(&prop, device);
+        if (e == cudaSuccess && prop.major != 10) {
+            say(err, errlen, std::string("device is not sm_100: ") + prop.name);
+            return nullptr;
+        }
+        OnDevice on(device);
+        if (e == cudaSuccess) e = on.rc;
+        int* host = nullptr;
+        int* dev = nullptr;
+        if (e == cudaSuccess) e = cudaHostAlloc(&host, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable);
+        if (e == cudaSuccess) {
+            *host = 0;
+            e = cudaHostGetDevicePointer(&dev, host, 0);
+        }
+        if (e != cudaSuccess) {
+            if (host) cudaFreeHost(host);
+            cudaGetLastError();   // reported here: the process's next check must not find it again
+            say(err, errlen, std::string("ptq8_ops_create: ") + cudaGetErrorString(e));
+            return nullptr;
+        }
+        auto* o = new (std::nothrow) ptq8_ops();
+        if (!o) {
+            cudaFreeHost(host);
+            say(err, errlen, "ptq8_ops_create: out of host memory");
+            return nullptr;
+        }
+        o->device = device;
+        o->sms = prop.multiProcessorCount;
+        o->error = host;
+        o->error_dev = dev;
+        say(err, errlen, "");
+        return o;
+    } catch (const std::exception& ex) {
+        say(err, errlen, ex.what());
+        return nullptr;
+    }
+}
+
+void ptq8_ops_destroy(ptq8_ops* o) {
+    if (!o) return;
+    cudaFreeHost(o->error);
+    delete o;
+}
+
+const char* ptq8_ops_last_error(const ptq8_ops* o) { return o ? o->err.c_str() : "null handle"; }
+
+int ptq8_ops_check_device_error(ptq8_ops* o, void* stream) {
+    if (!o) return PTQ8_ERR_INVALID;
+    try {
+        OnDevice on(o->device);
+        cudaError_t e = on.rc;
+        if (e == cudaSuccess) e = cudaStreamSynchronize(static_cast<cudaStream_t>(stream));
+        if (e != cudaSuccess) return cuda_fail(o, "cudaStreamSynchronize", e);
+        const int rc = ready(o);
+        *static_cast<volatile int*>(o->error) = 0;
+        return rc;
+    } catch (const std::exception& ex) {
+        return PTQ8_ERR_INVALID;
+    }
+}
+
+int ptq8_ops_set_wait_test(ptq8_ops* o, long long wait_limit_cycles, int stall_first_load) {
+    if (!o) return PTQ8_ERR_INVALID;
+    o->wait_limit = wait_limit_cycles > 0 ? wait_limit_cycles : kWaitLimitCycles;
+    o->stall = stall_first_load != 0;
+    return PTQ8_OK;
+}
+
+int ptq8_quantize_rows(ptq8_ops* o, const ptq8_rows_args* a, void* stream) {
+    if (!o) return PTQ8_ERR_INVALID;
+    try {
+        if (!a) return fail(o, PTQ8_ERR_INVALID, "null arguments");
+        if (const int rc = check_rows(o, *a)) return rc;
+        if (const int rc = ready(o)) return rc;
+        if (a->n_rows == 0) return PTQ8_OK;
+        OnDevice on(o->device);
+        if (on.rc != cudaSuccess) return cuda_fail(o, "cudaSetDevice", on.rc);
+        return run_rows(o, *a, static_cast<cudaStream_t>(stream));
+    } catch (const std::exception& ex) {
+        return PTQ8_ERR_INVALID;
+    }
+}
+
+int ptq8_linear(ptq8_ops* o, const ptq8_linear_args* a, void* stream) { return product(o, a, false, stream); }
+
+int ptq8_linear_grouped(ptq8_ops* o, const ptq8_linear_args* a, void* stream) { return product(o, a, true, stream); }
+
+}  // extern "C"

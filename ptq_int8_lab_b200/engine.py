@@ -52,6 +52,8 @@ EXPORTS = (
     "ptq8_engine_dump", "ptq8_engine_dump_range",
     "ptq8_engine_n_launches", "ptq8_engine_weight_bytes", "ptq8_engine_passes_log", "ptq8_engine_profile",
     "ptq8_load", "ptq8_forward", "ptq8_forward_debug", "ptq8_capture_graph", "ptq8_destroy", "ptq8_last_error",
+    "ptq8_ops_create", "ptq8_ops_destroy", "ptq8_ops_last_error", "ptq8_ops_check_device_error",
+    "ptq8_ops_set_wait_test", "ptq8_quantize_rows", "ptq8_linear", "ptq8_linear_grouped",
 )
 
 
@@ -137,6 +139,14 @@ def lib() -> ctypes.CDLL:
         "ptq8_capture_graph": (c_int, [c_void_p, c_int]),
         "ptq8_destroy": (None, [c_void_p]),
         "ptq8_last_error": (c_char_p, [c_void_p]),
+        "ptq8_ops_create": (c_void_p, [c_int, c_char_p, c_size]),
+        "ptq8_ops_destroy": (None, [c_void_p]),
+        "ptq8_ops_last_error": (c_char_p, [c_void_p]),
+        "ptq8_ops_check_device_error": (c_int, [c_void_p, c_void_p]),
+        "ptq8_ops_set_wait_test": (c_int, [c_void_p, ctypes.c_longlong, c_int]),
+        "ptq8_quantize_rows": (c_int, [c_void_p, c_void_p, c_void_p]),
+        "ptq8_linear": (c_int, [c_void_p, c_void_p, c_void_p]),
+        "ptq8_linear_grouped": (c_int, [c_void_p, c_void_p, c_void_p]),
     }
     for name, (res, args) in sig.items():
         f = getattr(L, name)
