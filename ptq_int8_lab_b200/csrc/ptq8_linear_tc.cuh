@@ -1,0 +1,662 @@
+// The tensor-core product: tcgen05 kind::i8 with the weights as the M operand.
+//
+// Output channels are the 128 rows (lanes) of an accumulator and tokens its columns, for every
+// number of tokens: a single token pads the 16-column minimum instead of 128 rows, one weight
+// tile layout serves all variants, and the epilogue's lanes hold consecutive channels, so that
+// plain stores of a warp are consecutive bytes of y whatever y's pitch and alignment.
+//
+//   CG 2: two CTAs share a tile of 256 channels (cta_group::2); each loads its 128 weight rows
+//         and half of the tokens' rows.
+//   S > 1 (CG 1): a cluster of S CTAs splits the sum over k; each sends the int32 partial sums
+//         of 1/S of the tokens to the CTA that finishes them.  Integer sums: the order of
+//         arrival changes nothing.
+//   GATED: two accumulators per tile, gate and up channels, joined in the epilogue.
+//   W4: weights arrive packed; four warps widen them into the swizzled operand tile as 16 times
+//       the code (the nibble moved to its byte's high half: no sign extension), and the
+//       channel's scale carries the exact factor 1/16.
+//
+// Warps: 0 TMA producer, 1 MMA issuer, 2 TMEM and the groups' tile list, 4.. epilogue, then
+// (W4) four unpackers.  All waits are bounded.
+#pragma once
+
+#include "ptq8_linear.cuh"
+
+namespace ptq8 {
+
+enum : int { ERR_WAIT_UNPACK = 5, ERR_WAIT_PARTIAL = 6 };
+
+constexpr int kMaxLinStages = 12;
+constexpr int kBand = 8;   // token tiles per band of the tile order: a band's operands stay in L2
+
+struct TcParams {
+    LinearParams l;
+    int kblocks;       // blocks of 128 input features
+    int stages;
+    int a_bufs;        // W4: unpacked operand tiles
+    int split;         // S
+    int list_bytes;    // shared memory of the groups' tile list
+    int ctiles;        // channel tiles
+    uint32_t tmem_cols;
+    int acc_bufs;
+    long long wait_limit;
+    int* err;
+    int stall;         // failure test: the first load is announced but not issued
+};
+
+template <int CG, int TN, bool W4, bool GATED>
+struct TcShape {
+    static constexpr int H = GATED ? 2 : 1;
+    static constexpr int XR = TN / CG;                     // token rows loaded by one CTA
+    static constexpr int kTile = H * 128 * 128;            // operand bytes of the weights, unpacked
+    static constexpr int kPacked = H * 128 * 64;
+    static constexpr int kW = W4 ? kPacked : kTile;        // what a stage holds of them
+    static constexpr int kX = XR * 128;
+    static constexpr int kStage = kW + kX;
+    static constexpr int kEpi = TN >= 128 ? 8 : 4;         // epilogue warps
+    static constexpr int kCW = TN / (kEpi / 4);            // accumulator columns of one warp
+    static constexpr int kThreads = 128 + 32 * kEpi + (W4 ? 128 : 0);
+    static constexpr int kCols = H * TN;                   // accumulator columns of a tile
+    static constexpr int kPerSm = TN <= 64 && !(W4 && GATED) ? 2 : 1;   // CTAs that share an SM
+};
+
+// ---- cluster-wide pieces
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Arrive on a barrier of any CTA of the cluster (address from mapa, or of the own CTA).
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// The same without release: frees an accumulator (see mbar_arrive_relaxed).
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t bar) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool mbar_try_cluster(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// A converged warp's bounded wait that also acquires what other CTAs released.
+__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, long long limit) {
+    bool ok = mbar_try_cluster(bar, parity);
+    if (!ok) {
+        const long long t0 = clock64();
+        while (!ok && clock64() - t0 <= limit) {
+#pragma unroll
+            for (int k = 0; k < 8 && !ok; ++k) ok = mbar_try_cluster(bar, parity);
+        }
+    }
+    return __all_sync(0xffffffffu, ok);
+}
+__device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+
+template <int CG>
+__device__ __forceinline__ void load_rows_2d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int c0, int c1) {
+    if constexpr (CG == 2)
+        asm volatile(
+            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0), "r"(c1)
+            : "memory");
+    else
+        tma_load_2d(dst, m, bar, c0, c1);
+}
+template <int CG>
+__device__ __forceinline__ void load_rows_3d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int c0, int c1, int c2) {
+    if constexpr (CG == 2)
+        asm volatile(
+            "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0),
+            "r"(c1), "r"(c2)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0),
+            "r"(c1), "r"(c2)
+            : "memory");
+}
+
+// The four K slices of one 128-byte block; the pair's form of mma_chunk_elect<4>.
+__device__ __forceinline__ void mma_pair_chunk_elect(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred e, p;\n\t.reg .b64 a1, b1, a2, b2, a3, b3;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t"
+        "add.s64 a1, %1, 2;\n\t"
+        "add.s64 b1, %2, 2;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::i8 [%0], a1, b1, %3, 1;\n\t"
+        "add.s64 a2, %1, 4;\n\t"
+        "add.s64 b2, %2, 4;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::i8 [%0], a2, b2, %3, 1;\n\t"
+        "add.s64 a3, %1, 6;\n\t"
+        "add.s64 b3, %2, 6;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::i8 [%0], a3, b3, %3, 1;\n\t}\n" ::"r"(d),
+        "l"(da), "l"(db), "r"(idesc), "r"(acc)
+        : "memory");
+}
+// Arrive on `bar` (the pair's: in both CTAs) when the MMAs issued so far have completed.
+template <int CG>
+__device__ __forceinline__ void commit_elect(uint32_t bar) {
+    if constexpr (CG == 2)
+        asm volatile(
+            "{\n\t.reg .pred e;\n\t.reg .b16 m;\n\tmov.u16 m, 3;\n\t"
+            "elect.sync _|e, 0xffffffff;\n\t"
+            "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], m;\n\t}\n" ::"r"(bar)
+            : "memory");
+    else
+        mma_commit_elect(bar);
+}
+
+// ---- tiles
+
+// Tile t of the launch: its group, first row, valid rows (0: none left) and channel tile.
+// Order inside a group: bands of kBand token tiles; a band goes through the channel tiles with its
+// token tiles innermost, so that CTAs running at the same time share both operands in L2.
+struct Tile {
+    int group, row0, valid, ct;
+};
+// Accumulator columns in use: as many as the tile has tokens, a multiple of 16 (of 32 for a pair).
+template <int CG, int TN>
+__device__ __forceinline__ int columns_of(const Tile& t) {
+    return min(TN, (t.valid + 16 * CG - 1) / (16 * CG) * (16 * CG));
+}
+
+template <int TN>
+struct Tiles {
+    const LinearParams& l;
+    const int* start;   // shared memory: first tile of each group, and the end; null: one group of all rows
+    int ctiles;
+    int g = 0;          // cursor: tiles are asked for in increasing order
+    __device__ Tiles(const LinearParams& lp, const int* s, int c) : l(lp), start(s), ctiles(c) {}
+    __device__ bool get(int t, Tile& o) {
+        long long beg = 0, end = l.rows;
+        int i = t;
+        if (start) {
+            while (g < l.groups && t >= start[g + 1]) ++g;
+            if (g >= l.groups) return false;
+            group_rows(l, g, beg, end);
+            i = t - start[g];
+        }
+        const int tt = static_cast<int>((end - beg + TN - 1) / TN);
+        const int full = kBand * ctiles, band = i / full, rest = i - band * full;
+        if (band * kBand >= tt) return false;
+        const int wide = min(kBand, tt - band * kBand);
+        o.ct = rest / wide;
+        const int k = band * kBand + (rest - o.ct * wide);
+        o.group = g;
+        o.row0 = static_cast<int>(beg) + k * TN;
+        o.valid = min(TN, static_cast<int>(end) - o.row0);
+        return true;
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// A lane's channel: scales and bias of the tile (two of each when gated).
+template <int H>
+struct Channel {
+    float ws[H], b[H];
+    bool ok;
+};
+
+template <int H, bool W4>
+__device__ __forceinline__ Channel<H> channel_of(const LinearParams& l, int group, int c) {
+    Channel<H> ch;
+    ch.ok = c < l.n;
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+        const size_t at = static_cast<size_t>(group) * (l.n * H) + h * l.n + c;
+        ch.ws[h] = ch.ok ? __ldg(l.ws + at) * (W4 ? 0.0625f : 1.0f) : 0.0f;
+        ch.b[h] = ch.ok && l.bias ? __ldg(l.bias + at) : 0.0f;
+    }
+    return ch;
+}
+
+template <int H>
+__device__ __forceinline__ float finish(const Channel<H>& ch, float xs, int a0, int a1) {
+    const float v = dequant(a0, xs, ch.ws[0], ch.b[0]);
+    return H == 2 ? swiglu(v, dequant(a1, xs, ch.ws[H - 1], ch.b[H - 1])) : v;
+}
+
+// Columns [c0, c1) of a warp's 32 accumulator lanes -> y.  xs: their token scales, from column c0 on.
+template <typename T, int H, int TN>
+__device__ __forceinline__ void store_columns(T* y, size_t ldy, uint32_t acc, const float* xs, const Channel<H>& ch, int c0,
+                                              int c1) {
+    for (int c = c0; c < c1; c += 16) {
+        uint32_t v[16], u[16];
+        tmem_ld16(acc + c, v);
+        if (H == 2) tmem_ld16(acc + TN + c, u);
+        tmem_wait_ld();
+        pin_after(v);
+        if (H == 2) pin_after(u);
+        T* out = y + static_cast<size_t>(c) * ldy;
+        const int left = c1 - c;
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+            const float4 x4 = *reinterpret_cast<const float4*>(xs + (c - c0) + j);
+            const float xf[4] = {x4.x, x4.y, x4.z, x4.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float r = finish<H>(ch, xf[i], static_cast<int>(v[j + i]), H == 2 ? static_cast<int>(u[j + i]) : 0);
+                if (ch.ok && j + i < left) *out = from_f32<T>(r);
+                out += ldy;
+            }
+        }
+    }
+}
+
+// The finishing half of a split tile: the S partial sums of this CTA's tokens.
+template <typename T, int H>
+__device__ __forceinline__ void store_partials(T* y, size_t ldy, const int* recv, int S, int tokens, const float* xs,
+                                               const Channel<H>& ch, int lane_c, int t0, int valid) {
+    for (int t = 0; t < tokens && t0 + t < valid; ++t) {
+        int a[2] = {0, 0};
+        for (int s = 0; s < S; ++s)
+#pragma unroll
+            for (int h = 0; h < H; ++h) a[h] += recv[((s * tokens + t) * H + h) * 128 + lane_c];
+        const float r = finish<H>(ch, xs[t0 + t], a[0], a[1]);
+        if (ch.ok) y[static_cast<size_t>(t0 + t) * ldy] = from_f32<T>(r);
+    }
+}
+
+// 16 packed bytes (32 codes) -> two 16-byte granules of 16 times the codes.
+__device__ __forceinline__ void widen(const uint4& p, uint4& lo, uint4& hi) {
+    const uint32_t m = 0xF0F0F0F0u;
+    uint32_t o[8];
+    const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t even = (w[i] << 4) & m, odd = w[i] & m;
+        o[2 * i] = __byte_perm(even, odd, 0x5140);
+        o[2 * i + 1] = __byte_perm(even, odd, 0x7362);
+    }
+    lo = make_uint4(o[0], o[1], o[2], o[3]);
+    hi = make_uint4(o[4], o[5], o[6], o[7]);
+}
+
+template <int CG, int TN, bool W4, bool GATED>
+__global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<CG, TN, W4, GATED>::kPerSm)
+    linear_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+                     const __grid_constant__ TcParams p) {
+    using Sh = TcShape<CG, TN, W4, GATED>;
+    constexpr int H = Sh::H;
+    extern __shared__ uint8_t dyn[];
+    __shared__ __align__(8) uint64_t bars[3 * kMaxLinStages + 16];
+    __shared__ uint32_t tmem_slot;
+    __shared__ __align__(16) float sxs_all[Sh::kEpi][Sh::kCW];   // token scales, each epilogue warp its own columns
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int S = CG == 1 ? p.split : 1;
+    const bool clustered = CG == 2 || S > 1;
+    const uint32_t rank = clustered ? cluster_rank() : 0;
+    const bool leader = CG == 1 || rank == 0;
+
+    const uint32_t base = (smem_u32(dyn) + 1023u) & ~1023u;
+    uint8_t* const base_p = dyn + (base - smem_u32(dyn));
+    const uint32_t a_ring = base + p.stages * Sh::kStage;                       // W4: unpacked tiles
+    const uint32_t after = a_ring + (W4 ? p.a_bufs * Sh::kTile : 0);            // tile list, or partial sums
+    int* const list = reinterpret_cast<int*>(base_p + (after - base));
+    const uint32_t recv = after + p.list_bytes;
+    const uint32_t b0 = smem_u32(bars);
+    const uint32_t full = b0, empty = full + 8 * p.stages, pfull = empty + 8 * p.stages;
+    const uint32_t afull = b0 + 8 * 3 * kMaxLinStages, aempty = afull + 32, accfull = aempty + 32, accempty = accfull + 16,
+                   partial = accempty + 16, drain = partial + 8;
+
+    if (warp == 0 && elect_one()) {
+        tma_prefetch(&map_x);
+        tma_prefetch(&map_w);
+    }
+    if (warp == 1 && lane == 0) {
+        for (int s = 0; s < p.stages; ++s) {
+            mbar_init(full + 8 * s, 1);
+            mbar_init(empty + 8 * s, 1);
+            mbar_init(pfull + 8 * s, 1);
+        }
+        for (int a = 0; a < 4; ++a) {
+            mbar_init(afull + 8 * a, 4 * CG);
+            mbar_init(aempty + 8 * a, 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(accfull + 8 * a, 1);
+            mbar_init(accempty + 8 * a, Sh::kEpi * CG);
+        }
+        mbar_init(partial, S * Sh::kEpi);
+        mbar_init(drain, 1);
+        fence_mbar_init();
+    }
+    if (warp == 2) {
+        if constexpr (CG == 2) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
+                         "r"(p.tmem_cols)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            tmem_alloc(smem_u32(&tmem_slot), p.tmem_cols);
+            tmem_relinquish();
+        }
+    }
+    griddep_launch();
+    griddep_wait();   // nothing above reads or writes global memory
+    const bool listed = p.l.offsets != nullptr;
+    if (listed && warp == 2) {   // first tile of each group
+        int sum = 0;
+        for (int g0 = 0; g0 < p.l.groups; g0 += 32) {
+            int n = 0;
+            if (g0 + lane < p.l.groups) {
+                long long beg, end;
+                group_rows(p.l, g0 + lane, beg, end);
+                n = static_cast<int>((end - beg + TN - 1) / TN) * p.ctiles;
+            }
+            int incl = n;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int o = __shfl_up_sync(0xffffffffu, incl, d);
+                if (lane >= d) incl += o;
+            }
+            if (g0 + lane < p.l.groups) list[g0 + lane] = sum + incl - n;
+            sum += __shfl_sync(0xffffffffu, incl, 31);
+        }
+        if (lane == 0) list[p.l.groups] = sum;
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (clustered) cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+
+    Tiles<TN> tiles(p.l, listed ? list : nullptr, p.ctiles);
+    const int per = CG == 2 ? 2 : S;
+    const int t0 = blockIdx.x / per, dt = gridDim.x / per;
+    const int kb0 = static_cast<int>(static_cast<long long>(p.kblocks) * (S > 1 ? rank : 0) / S);
+    const int kb1 = static_cast<int>(static_cast<long long>(p.kblocks) * (S > 1 ? rank + 1 : 1) / S);
+    const long long limit = p.wait_limit;
+    auto give_up = [&](int code) {
+        if (lane == 0) {
+            *static_cast<volatile int*>(p.err) = code;
+            __threadfence_system();
+        }
+    };
+    Tile tile;
+
+    if (warp == 0) {
+        // ---------------------------------------------------------------- producer
+        const uint32_t full_at = CG == 2 ? mapa(full, 0) : full;   // the pair's loads all count at the leader
+        int s = 0, issued = 0;
+        uint32_t ph = 1;
+        bool ok = true;
+        for (int t = t0; ok && tiles.get(t, tile); t += dt) {
+            const int c = (tile.ct * CG + static_cast<int>(CG == 2 ? rank : 0)) * 128;
+            // the pair's MMA takes the first half of its columns from CTA 0, the other from CTA 1
+            const int r = tile.row0 + (CG == 2 ? static_cast<int>(rank) * columns_of<CG, TN>(tile) / 2 : 0);
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!mbar_wait_warp(empty + 8 * s, ph, limit)) {
+                    give_up(ERR_WAIT_EMPTY);
+                    ok = false;
+                    break;
+                }
+                if (elect_one()) {
+                    const uint32_t wdst = base + s * Sh::kStage, xdst = wdst + Sh::kW;
+                    if (leader) mbar_expect_tx(full + 8 * s, CG * (W4 ? Sh::kX : Sh::kStage));
+                    if (W4) mbar_expect_tx(pfull + 8 * s, Sh::kPacked);
+                    if (!(p.stall && blockIdx.x == 0 && issued == 0)) {
+#pragma unroll
+                        for (int h = 0; h < H; ++h) {
+                            if constexpr (W4)
+                                load_rows_3d<1>(wdst + h * 8192, &map_w, pfull + 8 * s, kb * 64, h * p.l.n + c, tile.group);
+                            else
+                                load_rows_3d<CG>(wdst + h * 16384, &map_w, full_at + 8 * s, kb * 128, h * p.l.n + c, tile.group);
+                        }
+                        load_rows_2d<CG>(xdst, &map_x, full_at + 8 * s, kb * 128, r);
+                    }
+                }
+                __syncwarp();
+                ++issued;
+                if (++s == p.stages) {
+                    s = 0;
+                    ph ^= 1;
+                }
+            }
+            if (S > 1) break;
+        }
+        if (ok) {
+            // every stage consumed: no commit is on its way to this CTA's barriers when it ends
+            for (int i = 0; ok && i < p.stages; ++i) {
+                ok = mbar_wait_warp(empty + 8 * s, ph, limit);
+                if (++s == p.stages) {
+                    s = 0;
+                    ph ^= 1;
+                }
+            }
+            if (!ok) give_up(ERR_WAIT_EMPTY);
+        }
+        if (!ok) {
+            // own copies in flight must land before the CTA ends
+            const int n = min(issued, p.stages);
+            for (int i = 1; i <= n; ++i) {
+                const int back = issued - i;
+                if (leader) mbar_wait_warp(full + 8 * (back % p.stages), (back / p.stages) & 1, limit);
+                if (W4) mbar_wait_warp(pfull + 8 * (back % p.stages), (back / p.stages) & 1, limit);
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------------------------------------------------------- MMA issuer (the pair's leader)
+        int s = 0, ab = 0, buf = 0;
+        uint32_t ph = 0, aph = 0, accph = 1;
+        bool ok = leader;
+        for (int t = t0; ok && tiles.get(t, tile); t += dt) {
+            const int nn = columns_of<CG, TN>(tile);
+            const uint32_t idesc = (make_idesc_i8(nn) & ~(0x1Fu << 24)) | (static_cast<uint32_t>(128 * CG >> 4) << 24);
+            const uint32_t d = tmem + buf * Sh::kCols;
+            if (!mbar_wait_cluster(accempty + 8 * buf, accph, limit)) {
+                give_up(ERR_WAIT_ACC);
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            for (int kb = kb0; kb < kb1; ++kb) {
+                bool there = mbar_wait_cluster(full + 8 * s, ph, limit);
+                if (W4 && there) there = mbar_wait_cluster(afull + 8 * ab, aph, limit);
+                if (!there) {
+                    give_up(ERR_WAIT_FULL);
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t wsrc = W4 ? a_ring + ab * Sh::kTile : base + s * Sh::kStage;
+                const uint64_t db = make_sdesc(base + s * Sh::kStage + Sh::kW, 128);
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    const uint64_t da = make_sdesc(wsrc + h * 16384, 128);
+                    if constexpr (CG == 2)
+                        mma_pair_chunk_elect(d + h * TN, da, db, idesc, kb > kb0);
+                    else
+                        mma_chunk_elect<4>(d + h * TN, da, db, idesc, kb > kb0);
+                }
+                if (W4) {
+                    commit_elect<CG>(aempty + 8 * ab);
+                    if (++ab == p.a_bufs) {
+                        ab = 0;
+                        aph ^= 1;
+                    }
+                }
+                commit_elect<CG>(empty + 8 * s);
+                if (++s == p.stages) {
+                    s = 0;
+                    ph ^= 1;
+                }
+            }
+            if (!ok) break;
+            commit_elect<CG>(accfull + 8 * buf);
+            if (++buf == p.acc_bufs) {
+                buf = 0;
+                accph ^= 1;
+            }
+            if (S > 1) break;
+        }
+        if (leader && !ok) {   // MMAs in flight end before TMEM is freed
+            if constexpr (CG == 1) {
+                mma_commit_elect(drain);
+                mbar_wait_warp(drain, 0, limit);
+            } else {
+                commit_elect<2>(drain);
+                mbar_wait_warp(drain, 0, limit);
+            }
+        }
+    } else if (warp >= 4 && warp < 4 + Sh::kEpi) {
+        // ---------------------------------------------------------------- epilogue
+        const int quad = warp & 3, part = (warp - 4) >> 2;
+        float* const sxs = sxs_all[warp - 4];
+        const int lane_c = quad * 32 + lane;
+        const uint32_t accempty_at = CG == 2 ? mapa(accempty, 0) : accempty;
+        int buf = 0;
+        uint32_t accph = 0;
+        for (int t = t0; tiles.get(t, tile); t += dt) {
+            const int c = (tile.ct * CG + static_cast<int>(CG == 2 ? rank : 0)) * 128 + lane_c;
+            const Channel<H> ch = channel_of<H, W4>(p.l, tile.group, c);
+            const int c0 = part * Sh::kCW, c1 = min(c0 + Sh::kCW, tile.valid);
+            __syncwarp();
+            for (int i = lane; c0 + i < c1; i += 32) sxs[i] = __ldg(p.l.xs + tile.row0 + c0 + i);
+            __syncwarp();
+            if (!mbar_wait_cluster(accfull + 8 * buf, accph, limit)) {
+                give_up(ERR_WAIT_ACC);
+                break;
+            }
+            tc_fence_after();
+            const uint32_t acc = tmem + buf * Sh::kCols + (static_cast<uint32_t>(quad * 32) << 16);
+            const size_t at = static_cast<size_t>(tile.row0) * p.l.ldy + c;
+            if (CG == 2 || S == 1) {
+                if (p.l.y_type == Y_F32)
+                    store_columns<float, H, TN>(static_cast<float*>(p.l.y) + at, p.l.ldy, acc, sxs, ch, c0, c1);
+                else if (p.l.y_type == Y_F16)
+                    store_columns<__half, H, TN>(static_cast<__half*>(p.l.y) + at, p.l.ldy, acc, sxs, ch, c0, c1);
+                else
+                    store_columns<__nv_bfloat16, H, TN>(static_cast<__nv_bfloat16*>(p.l.y) + at, p.l.ldy, acc, sxs, ch, c0, c1);
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster_relaxed(accempty_at + 8 * buf);
+                if (++buf == p.acc_bufs) {
+                    buf = 0;
+                    accph ^= 1;
+                }
+            } else {
+                const int tokens = TN / S, shift = 31 - __clz(tokens);   // S is a power of two
+                for (int cc = c0; cc < c1; cc += 16) {
+                    uint32_t v[H][16];
+#pragma unroll
+                    for (int h = 0; h < H; ++h) tmem_ld16(acc + h * TN + cc, v[h]);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int h = 0; h < H; ++h) pin_after(v[h]);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        if (cc + j < c1) {
+                            const int to = (cc + j) >> shift, tk = (cc + j) & (tokens - 1);
+                            const uint32_t dst = mapa(recv + (((rank * tokens + tk) * H) * 128 + lane_c) * 4, to);
+#pragma unroll
+                            for (int h = 0; h < H; ++h) st_cluster(dst + h * 512, v[h][j]);
+                        }
+                    }
+                }
+                __syncwarp();
+                if (lane < S) mbar_arrive_cluster(mapa(partial, lane));
+                if (!mbar_wait_cluster(partial, 0, limit)) {
+                    give_up(ERR_WAIT_PARTIAL);
+                    break;
+                }
+                const int* got = reinterpret_cast<const int*>(base_p + (recv - base));
+                const int first = rank * tokens;
+                if (part == 0) {
+                    if (p.l.y_type == Y_F32)
+                        store_partials<float, H>(static_cast<float*>(p.l.y) + at, p.l.ldy, got, S, tokens, sxs, ch, lane_c, first, tile.valid);
+                    else if (p.l.y_type == Y_F16)
+                        store_partials<__half, H>(static_cast<__half*>(p.l.y) + at, p.l.ldy, got, S, tokens, sxs, ch, lane_c, first, tile.valid);
+                    else
+                        store_partials<__nv_bfloat16, H>(static_cast<__nv_bfloat16*>(p.l.y) + at, p.l.ldy, got, S, tokens, sxs, ch, lane_c, first, tile.valid);
+                }
+                break;
+            }
+        }
+    } else if (W4 && warp >= 4 + Sh::kEpi) {
+        // ---------------------------------------------------------------- unpackers
+        const int u = tid - 32 * (4 + Sh::kEpi);   // 0..127
+        const uint32_t afull_at = CG == 2 ? mapa(afull, 0) : afull;
+        int s = 0, ab = 0;
+        uint32_t ph = 0, aph = 1;
+        bool ok = true;
+        for (int t = t0; ok && tiles.get(t, tile); t += dt) {
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!mbar_wait_warp(pfull + 8 * s, ph, limit) || !mbar_wait_cluster(aempty + 8 * ab, aph, limit)) {
+                    give_up(ERR_WAIT_UNPACK);
+                    ok = false;
+                    break;
+                }
+                const uint8_t* src = base_p + s * Sh::kStage;
+                uint8_t* dst = base_p + (a_ring - base) + ab * Sh::kTile;
+#pragma unroll
+                for (int i = 0; i < 4 * H; ++i) {
+                    const int item = i * 128 + u, r = item >> 2, q = item & 3;   // row, 16-byte granule of the packed row
+                    uint4 lo, hi;
+                    widen(*reinterpret_cast<const uint4*>(src + item * 16), lo, hi);
+                    uint8_t* row = dst + r * 128;
+                    *reinterpret_cast<uint4*>(row + (((2 * q) ^ (r & 7)) << 4)) = lo;
+                    *reinterpret_cast<uint4*>(row + (((2 * q + 1) ^ (r & 7)) << 4)) = hi;
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(afull_at + 8 * ab);
+                if (++ab == p.a_bufs) {
+                    ab = 0;
+                    aph ^= 1;
+                }
+                if (++s == p.stages) {
+                    s = 0;
+                    ph ^= 1;
+                }
+            }
+            if (S > 1) break;
+        }
+    }
+
+    // No CTA of a cluster ends, and no TMEM is freed, while a peer may still reach it.
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (clustered) cluster_sync();
+    if (warp == 2) {
+        tc_fence_after();
+        if constexpr (CG == 2)
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols) : "memory");
+        else
+            tmem_dealloc(tmem, p.tmem_cols);
+    }
+}
+
+}  // namespace ptq8

@@ -14,6 +14,7 @@
 
 #include "ptq8.h"
 #include "ptq8_linear.cuh"
+#include "ptq8_linear_tc.cuh"
 #include "ptq8_rows.cuh"
 
 using namespace ptq8;
@@ -25,6 +26,7 @@ struct ptq8_ops {
     int* error_dev = nullptr;   // its device address
     long long wait_limit = kWaitLimitCycles;
     int stall = 0;
+    PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
     std::string err;
 };
 
@@ -61,17 +63,20 @@ struct OnDevice {
 // One launch with programmatic stream serialization: the kernel may be scheduled while the kernel
 // before it on the stream drains, and waits (griddepcontrol.wait) before it touches global memory.
 template <typename... P, typename... A>
-cudaError_t launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A... args) {
+cudaError_t launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, int cluster, cudaStream_t stream, const A&... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
@@ -140,8 +145,121 @@ int check_linear(ptq8_ops* o, const ptq8_linear_args& a, bool grouped) {
 int run_rows(ptq8_ops* o, const ptq8_rows_args& a, cudaStream_t st) {
     RowsParams p{a.x, a.codes, a.scale, a.rows, static_cast<size_t>(a.ldx), static_cast<size_t>(a.ldc), a.x_rows, a.width};
     auto kernel = a.x_type == PTQ8_F32 ? rows_kernel<float> : a.x_type == PTQ8_F16 ? rows_kernel<__half> : rows_kernel<__nv_bfloat16>;
-    const cudaError_t e = launch(kernel, dim3(static_cast<unsigned>(a.n_rows)), dim3(256), 0, st, p);
+    const cudaError_t e = launch(kernel, dim3(static_cast<unsigned>(a.n_rows)), dim3(256), 0, 1, st, p);
     return e == cudaSuccess ? PTQ8_OK : cuda_fail(o, "quantize_rows", e);
+}
+
+// ---- the tensor-core kernel's variants
+
+using TcKernel = void (*)(const CUtensorMap, const CUtensorMap, const TcParams);
+
+struct Variant {
+    int cg, tn;            // CTAs per tile, tokens per tile
+    bool w4, gated;
+    TcKernel kernel;
+    int threads, stage, tile, cols, x_rows, per_sm;
+};
+
+template <int CG, int TN, bool W4, bool GATED>
+Variant variant() {
+    using Sh = TcShape<CG, TN, W4, GATED>;
+    return {CG, TN, W4, GATED, linear_tc_kernel<CG, TN, W4, GATED>, Sh::kThreads, Sh::kStage, Sh::kTile, Sh::kCols, Sh::XR, Sh::kPerSm};
+}
+
+const Variant kVariants[] = {
+    variant<1, 16, false, false>(),  variant<1, 16, false, true>(),  variant<1, 16, true, false>(),  variant<1, 16, true, true>(),
+    variant<1, 32, false, false>(),  variant<1, 32, false, true>(),  variant<1, 32, true, false>(),  variant<1, 32, true, true>(),
+    variant<1, 64, false, false>(),  variant<1, 64, false, true>(),  variant<1, 64, true, false>(),  variant<1, 64, true, true>(),
+    variant<1, 128, false, false>(), variant<1, 128, false, true>(), variant<1, 128, true, false>(), variant<1, 128, true, true>(),
+    variant<2, 128, false, false>(), variant<2, 128, false, true>(), variant<2, 128, true, false>(), variant<2, 128, true, true>(),
+    variant<2, 256, false, false>(), variant<2, 256, true, false>(),
+};
+
+// Dynamic shared memory of a CTA that shares its SM with another, or not.
+constexpr int kSmemTwo = 110 * 1024, kSmemOne = 222 * 1024;
+
+struct Choice {
+    int cg, tn, split;
+};
+
+Choice choose(const ptq8_ops* o, const ptq8_linear_args& a, int groups, bool gated) {
+    const long long m = (a.rows + groups - 1) / groups;   // rows that a group has on average
+    const int kblocks = (a.in_features + 127) / 128;
+    Choice c{1, m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128, 1};
+    const long long tiles = (a.out_features + 127) / 128 * std::max<long long>(groups > 1 ? std::min<long long>(groups, a.rows) : 1, (a.rows + c.tn - 1) / c.tn);
+    if (c.tn == 128 && tiles > 2 * o->sms) c = {2, gated ? 128 : 256, 1};
+    if (c.tn <= 32)
+        while (c.split < 8 && tiles * c.split * 2 <= 2 * o->sms && kblocks >= 4 * c.split) c.split *= 2;
+    return c;
+}
+
+bool aligned16(long long v) { return v % 16 == 0; }
+
+// What TMA needs of the operands' layout (a pitch that no second row uses does not count).
+bool tc_layout(const ptq8_linear_args& a, bool grouped) {
+    return aligned16(reinterpret_cast<uintptr_t>(a.x)) && aligned16(reinterpret_cast<uintptr_t>(a.w)) &&
+           (aligned16(a.ldx) || a.rows == 1) && (aligned16(a.ldw) || a.out_features == 1 && a.epilogue == PTQ8_EPI_NONE) &&
+           (!grouped || a.groups == 1 || aligned16(a.w_group_stride)) && a.ldx < (1LL << 39) && a.ldw < (1LL << 39);
+}
+
+int encode(ptq8_ops* o, CUtensorMap* m, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
+           const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
+    const cuuint32_t one[3] = {1, 1, 1};
+    const CUresult r = o->encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(base), dims, strides, box, one,
+                                 CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? PTQ8_OK : fail(o, PTQ8_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+}
+
+int run_tc(ptq8_ops* o, const ptq8_linear_args& a, const LinearParams& l, cudaStream_t st) {
+    const bool gated = a.epilogue == PTQ8_EPI_SWIGLU, w4 = a.w_bits == 4;
+    const Choice c = choose(o, a, l.groups, gated);
+    const Variant* v = nullptr;
+    for (const Variant& k : kVariants)
+        if (k.cg == c.cg && k.tn == c.tn && k.w4 == w4 && k.gated == gated) v = &k;
+    if (!v) return fail(o, PTQ8_ERR_INVALID, "linear: no kernel for %d CTAs, %d tokens", c.cg, c.tn);
+    const long long channels = static_cast<long long>(a.out_features) * (gated ? 2 : 1);
+    const int wide = w4 ? (a.in_features + 1) / 2 : a.in_features;
+    CUtensorMap mx, mw;
+    {
+        const cuuint64_t dims[2] = {static_cast<cuuint64_t>(a.in_features), static_cast<cuuint64_t>(a.rows)};
+        const cuuint64_t pitch[1] = {static_cast<cuuint64_t>(a.rows > 1 ? a.ldx : (a.in_features + 15) / 16 * 16)};
+        const cuuint32_t box[2] = {128, static_cast<cuuint32_t>(v->x_rows)};
+        if (const int rc = encode(o, &mx, 2, a.x, dims, pitch, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+    }
+    {
+        const cuuint64_t ldw = channels > 1 ? a.ldw : (wide + 15) / 16 * 16;
+        const cuuint64_t dims[3] = {static_cast<cuuint64_t>(wide), static_cast<cuuint64_t>(channels), static_cast<cuuint64_t>(l.groups)};
+        const cuuint64_t pitch[2] = {ldw, l.groups > 1 ? static_cast<cuuint64_t>(l.gstride) : ldw};
+        const cuuint32_t box[3] = {w4 ? 64u : 128u, 128, 1};
+        if (const int rc = encode(o, &mw, 3, a.w, dims, pitch, box, w4 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B))
+            return rc;
+    }
+    TcParams p{};
+    p.l = l;
+    p.kblocks = (a.in_features + 127) / 128;
+    p.split = c.split;
+    p.ctiles = (a.out_features + 128 * c.cg - 1) / (128 * c.cg);
+    p.list_bytes = l.offsets ? ((l.groups + 1) * 4 + 127) / 128 * 128 : 0;
+    p.a_bufs = w4 ? 2 : 0;
+    p.acc_bufs = c.split > 1 ? 1 : 2;
+    p.tmem_cols = 32;
+    while (static_cast<int>(p.tmem_cols) < v->cols * p.acc_bufs) p.tmem_cols *= 2;
+    p.wait_limit = o->wait_limit;
+    p.err = o->error_dev;
+    p.stall = o->stall;
+    const int extra = 1024 + p.a_bufs * v->tile + p.list_bytes + (c.split > 1 ? v->cols * 128 * 4 : 0);
+    p.stages = std::min(kMaxLinStages, ((v->per_sm == 2 ? kSmemTwo : kSmemOne) - extra) / v->stage);
+    if (p.stages < 2) return fail(o, PTQ8_ERR_INVALID, "linear: %d stages", p.stages);
+    const int smem = extra + p.stages * v->stage;
+    // tiles at most: each group's last tile may be partly filled
+    const long long row_tiles = l.offsets ? a.rows / c.tn + std::min<long long>(l.groups, a.rows) : (a.rows + c.tn - 1) / c.tn;
+    const long long tiles = row_tiles * p.ctiles;
+    if (tiles > 0x3FFFFFFF / 8) return fail(o, PTQ8_ERR_INVALID, "linear: %lld tiles", tiles);
+    const int per = c.cg * c.split, slots = o->sms * v->per_sm / per;
+    const long long clusters = c.split > 1 ? tiles : std::min<long long>(tiles, slots);
+    const cudaError_t e = launch(v->kernel, dim3(static_cast<unsigned>(clusters * per)), dim3(v->threads), smem, per, st, mx, mw, p);
+    return e == cudaSuccess ? PTQ8_OK : cuda_fail(o, "linear", e);
 }
 
 int run_linear(ptq8_ops* o, const ptq8_linear_args& a, bool grouped, cudaStream_t st) {
@@ -163,13 +281,14 @@ int run_linear(ptq8_ops* o, const ptq8_linear_args& a, bool grouped, cudaStream_
     p.groups = grouped ? a.groups : 1;
     p.y_type = a.y_type;
     const bool gated = a.epilogue == PTQ8_EPI_SWIGLU, w4 = a.w_bits == 4;
+    if (tc_layout(a, grouped)) return run_tc(o, a, p, st);
     const long long row_tiles = (a.rows + kAnyTile - 1) / kAnyTile;
     // blocks stride over the channel tiles (x) and over a group's row tiles (y)
     const dim3 grid(static_cast<unsigned>((a.out_features + kAnyTile - 1) / kAnyTile),
                     static_cast<unsigned>(std::min<long long>(row_tiles, grouped ? 64 : 65535)), static_cast<unsigned>(p.groups));
     auto kernel = w4 ? (gated ? linear_any_kernel<true, true> : linear_any_kernel<true, false>)
                      : (gated ? linear_any_kernel<false, true> : linear_any_kernel<false, false>);
-    const cudaError_t e = launch(kernel, grid, dim3(256), 0, st, p);
+    const cudaError_t e = launch(kernel, grid, dim3(256), 0, 1, st, p);
     return e == cudaSuccess ? PTQ8_OK : cuda_fail(o, "linear", e);
 }
 
@@ -215,6 +334,20 @@ ptq8_ops* ptq8_ops_create(int device, char* err, size_t errlen) {
             say(err, errlen, std::string("ptq8_ops_create: ") + cudaGetErrorString(e));
             return nullptr;
         }
+        void* encode = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &encode, cudaEnableDefault, &q);
+        if (e == cudaSuccess && q != cudaDriverEntryPointSuccess) e = cudaErrorNotSupported;
+        for (const Variant& v : kVariants)
+            if (e == cudaSuccess)
+                e = cudaFuncSetAttribute(reinterpret_cast<const void*>(v.kernel), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         v.per_sm == 2 ? kSmemTwo : kSmemOne);
+        if (e != cudaSuccess) {
+            cudaFreeHost(host);
+            cudaGetLastError();
+            say(err, errlen, std::string("ptq8_ops_create: ") + cudaGetErrorString(e));
+            return nullptr;
+        }
         auto* o = new (std::nothrow) ptq8_ops();
         if (!o) {
             cudaFreeHost(host);
@@ -225,6 +358,7 @@ ptq8_ops* ptq8_ops_create(int device, char* err, size_t errlen) {
         o->sms = prop.multiProcessorCount;
         o->error = host;
         o->error_dev = dev;
+        o->encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(encode);
         say(err, errlen, "");
         return o;
     } catch (const std::exception& ex) {

@@ -237,6 +237,30 @@ def test_linear_shapes(ops, rows, k, n, bits, gated):
     check(lambda t: ops.linear(*a, bits=bits, act=1 if gated else 0, dtype=t), plain_product(x, xs, w, ws, b), n, gated, dtype)
 
 
+@pytest.mark.parametrize("rows,k,n", [(2500, 272, 2100), (5000, 130, 1111), (4097, 640, 1290), (9000, 48, 530)])
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("gated", [False, True])
+def test_linear_many_tiles(ops, rows, k, n, bits, gated):
+    """More tiles than the device runs at once: every CTA takes several."""
+    rng = np.random.default_rng(rows)
+    x, xs, w, ws, b = case(rng, rows, k, n, bits, gated, True)
+    a = (laid(x), dev(xs), laid(w if bits == 8 else pack4(w)), dev(ws), dev(b))
+    check(lambda t: ops.linear(*a, bits=bits, act=1 if gated else 0, dtype=t), plain_product(x, xs, w, ws, b), n, gated, "bf16")
+
+
+@pytest.mark.parametrize("counts", [[900, 0, 3, 2000, 1, 515, 30, 1300], [257] * 20], ids=["uneven", "even"])
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("gated", [False, True])
+def test_grouped_many_tiles(ops, counts, bits, gated):
+    rng = np.random.default_rng(len(counts))
+    offs = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    k, n = 400, 1000
+    x, xs, w, ws, b = case(rng, int(offs[-1]), k, n, bits, gated, True, len(counts))
+    a = (laid(x), dev(xs), dev(offs), laid(w if bits == 8 else pack4(w)), dev(ws), dev(b))
+    check(lambda t: ops.linear_grouped(*a, bits=bits, act=1 if gated else 0, dtype=t), plain_grouped(x, xs, offs, w, ws, b), n,
+          gated, "f16")
+
+
 @pytest.mark.parametrize("bits", [8, 4])
 @pytest.mark.parametrize("gated", [False, True])
 @pytest.mark.parametrize("rows", [1, 6, 40, 300])
