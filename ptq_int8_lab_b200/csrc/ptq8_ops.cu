@@ -142,10 +142,38 @@ int check_linear(ptq8_ops* o, const ptq8_linear_args& a, bool grouped) {
     return PTQ8_OK;
 }
 
+using RowsKernel = void (*)(RowsParams);
+
+struct RowsVariant {
+    int tpr;      // threads per row
+    int vecs;     // vectors of 16 bytes that they hold (0: any number, read twice)
+    RowsKernel aligned, shifted;
+};
+
+template <typename T, int TPR, int NV>
+RowsVariant rows_variant() {
+    return {TPR, TPR * NV, rows_kernel<T, TPR, NV, false>, rows_kernel<T, TPR, NV, true>};
+}
+
+// By row length, four vectors a thread at most: 64 KB of loads in flight on an SM full of threads.
+template <typename T>
+const RowsVariant& rows_for(int vecs) {
+    static const RowsVariant k[] = {rows_variant<T, 32, 1>(),  rows_variant<T, 32, 2>(),  rows_variant<T, 32, 4>(),
+                                    rows_variant<T, 128, 2>(), rows_variant<T, 128, 4>(), rows_variant<T, 256, 4>(),
+                                    rows_variant<T, 512, 4>(), rows_variant<T, 1024, 4>()};
+    static const RowsVariant any = rows_variant<T, 512, 0>();
+    for (const RowsVariant& v : k)
+        if (vecs <= v.vecs) return v;
+    return any;
+}
+
 int run_rows(ptq8_ops* o, const ptq8_rows_args& a, cudaStream_t st) {
-    RowsParams p{a.x, a.codes, a.scale, a.rows, static_cast<size_t>(a.ldx), static_cast<size_t>(a.ldc), a.x_rows, a.width};
-    auto kernel = a.x_type == PTQ8_F32 ? rows_kernel<float> : a.x_type == PTQ8_F16 ? rows_kernel<__half> : rows_kernel<__nv_bfloat16>;
-    const cudaError_t e = launch(kernel, dim3(static_cast<unsigned>(a.n_rows)), dim3(256), 0, 1, st, p);
+    const RowsParams p{a.x, a.codes, a.scale, a.rows, static_cast<size_t>(a.ldx), static_cast<size_t>(a.ldc), a.x_rows, a.n_rows, a.width};
+    const int size = static_cast<int>(type_size(a.x_type)), vecs = (a.width + 16 / size - 1) / (16 / size);
+    const RowsVariant& v = a.x_type == PTQ8_F32 ? rows_for<float>(vecs) : a.x_type == PTQ8_F16 ? rows_for<__half>(vecs) : rows_for<__nv_bfloat16>(vecs);
+    const bool aligned = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && (a.x_rows <= 1 || a.ldx * size % 16 == 0);
+    const int block = std::max(256, v.tpr), per = block / v.tpr;
+    const cudaError_t e = launch(aligned ? v.aligned : v.shifted, dim3(static_cast<unsigned>((a.n_rows + per - 1) / per)), dim3(block), 0, 1, st, p);
     return e == cudaSuccess ? PTQ8_OK : cuda_fail(o, "quantize_rows", e);
 }
 

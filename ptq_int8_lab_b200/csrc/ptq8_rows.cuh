@@ -14,13 +14,9 @@ struct RowsParams {
     float* scale;
     const int* rows;   // gathered row per output row, or null
     size_t ldx, ldc;   // elements
-    long long x_rows;
+    long long x_rows, n_rows;
     int width;
 };
-
-__device__ __forceinline__ float to_f32(float v) { return v; }
-__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 
 // Exact code of y for the 32-bit scale s: round_half_away(y / s).  double(y) / double(s) never
 // rounds onto a half-integer that it is not: the quotient of two 24-bit numbers differs from
@@ -30,31 +26,212 @@ __device__ __forceinline__ int row_code_exact(float y, float s) {
     return static_cast<int>(v >= 0.0 ? floor(v + 0.5) : ceil(v - 0.5));
 }
 
-// The simple kernel: one block per row, two passes over the row.
+// How one 16-byte vector of T is read: its largest magnitude as a bit pattern (NaN above infinity
+// above every number, so a maximum of patterns loses neither), and its values.
 template <typename T>
-__global__ void __launch_bounds__(256) rows_kernel(RowsParams p) {
+struct Vec;
+template <>
+struct Vec<float> {
+    static constexpr int V = 4;
+    static __device__ __forceinline__ uint32_t join(uint32_t m, uint32_t w) { return max(m, w & 0x7FFFFFFFu); }
+    static __device__ __forceinline__ uint32_t top(uint32_t m) { return m; }
+    static __device__ __forceinline__ void values(const uint4& v, float (&f)[4]) {
+        f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y), f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
+    }
+};
+template <>
+struct Vec<__nv_bfloat16> {
+    static constexpr int V = 8;
+    static __device__ __forceinline__ uint32_t join(uint32_t m, uint32_t w) { return __vmaxu2(m, w & 0x7FFF7FFFu); }
+    static __device__ __forceinline__ uint32_t top(uint32_t m) { return max(m & 0xFFFFu, m >> 16) << 16; }
+    static __device__ __forceinline__ void values(const uint4& v, float (&f)[8]) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f[2 * i] = __uint_as_float(w[i] << 16);
+            f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+    }
+};
+template <>
+struct Vec<__half> {
+    static constexpr int V = 8;
+    static __device__ __forceinline__ uint32_t join(uint32_t m, uint32_t w) { return __vmaxu2(m, w & 0x7FFF7FFFu); }
+    static __device__ __forceinline__ uint32_t top(uint32_t m) {
+        return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(max(m & 0xFFFFu, m >> 16)))));
+    }
+    static __device__ __forceinline__ void values(const uint4& v, float (&f)[8]) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            f[2 * i] = p.x;
+            f[2 * i + 1] = p.y;
+        }
+    }
+};
+
+__device__ __forceinline__ uint4 load16(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+// The first n (>= 1) elements of a vector one by one; the others are zero (code 0, no part in the maximum).
+template <typename T>
+__device__ __forceinline__ uint4 load_part(const T* p, int n) {
+    uint4 v = make_uint4(0, 0, 0, 0);
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < Vec<T>::V; ++i) {
+        if (i >= n) break;
+        if (sizeof(T) == 4)
+            w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+        else
+            w[i / 2] |= static_cast<uint32_t>(reinterpret_cast<const unsigned short*>(p)[i]) << (16 * (i & 1));
+    }
+    v = make_uint4(w[0], w[1], w[2], w[3]);
+    return v;
+}
+
+// A whole vector that starts at any element: two aligned loads joined, where both lie inside the
+// tensor [lo, hi); one by one at its very ends.
+template <typename T>
+__device__ __forceinline__ uint4 load_shifted(const T* p, const char* lo, const char* hi) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    const uint32_t off = at & 15;
+    const char* a = reinterpret_cast<const char*>(at - off);
+    if (a < lo || a + 32 > hi) return load_part(p, Vec<T>::V);
+    const uint4 x = load16(a), y = load16(a + 16);
+    uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+    if (off & 8)
+#pragma unroll
+        for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+    if (off & 4)
+#pragma unroll
+        for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+    if (sizeof(T) == 2) {
+        const uint32_t bits = (off & 2) * 8;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], bits);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Codes of one vector.  Multipliers that bracket 1/s, each in one FMA with 1.5 * 2^23 added: the sum
+// lies in [2^23, 2^24) where floats are 1 apart, so it is rounded to the nearest integer and its low
+// byte is the code (|y / s| <= 127 (1 + 2^-23): s is the row's own).  Where both agree, every number
+// between y * inv_lo and y * inv_hi rounds to that integer, and so does the exact quotient, which lies
+// strictly inside; where they do not, a half-integer lies between them and the exact form decides.
+template <int V>
+__device__ __forceinline__ void codes_of(const float (&f)[V], float inv_lo, float inv_hi, float s, uint32_t (&out)[V / 4]) {
+    constexpr float kMagic = 12582912.0f;
+    const float2 lo = make_float2(inv_lo, inv_lo), hi = make_float2(inv_hi, inv_hi), mg = make_float2(kMagic, kMagic);
+    uint32_t m[V], flag = 0;
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+        const float2 y = make_float2(f[i], f[i + 1]);
+        const float2 a = __ffma2_rn(y, lo, mg), b = __ffma2_rn(y, hi, mg);
+        flag |= (__float_as_uint(a.x) ^ __float_as_uint(b.x)) | (__float_as_uint(a.y) ^ __float_as_uint(b.y));
+        m[i] = __float_as_uint(a.x);
+        m[i + 1] = __float_as_uint(a.y);
+    }
+    if (flag) {
+#pragma unroll 1
+        for (int i = 0; i < V; ++i) {
+            float y = f[0];
+#pragma unroll
+            for (int j = 1; j < V; ++j) y = i == j ? f[j] : y;
+            const uint32_t c = static_cast<uint32_t>(row_code_exact(y, s));
+#pragma unroll
+            for (int j = 0; j < V; ++j) m[j] = i == j ? c : m[j];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < V / 4; ++k)
+        out[k] = __byte_perm(__byte_perm(m[4 * k], m[4 * k + 1], 0x0040), __byte_perm(m[4 * k + 2], m[4 * k + 3], 0x0040), 0x5410);
+}
+
+// One pass over the data: TPR threads per row hold it in registers, NV vectors of 16 bytes each,
+// between its maximum and its codes.  (NV 0, for rows longer than that: a loop that reads them twice.)
+// SHIFT: rows that do not start at multiples of 16 bytes.
+template <typename T, int TPR, int NV, bool SHIFT>
+__global__ void __launch_bounds__(TPR > 256 ? TPR : 256) rows_kernel(RowsParams p) {
+    constexpr int V = Vec<T>::V, kBlock = TPR > 256 ? TPR : 256, kWarps = TPR / 32;
+    __shared__ uint32_t part[kBlock / 32];
     griddep_launch();
     griddep_wait();
-    __shared__ uint32_t part[8];
-    const size_t r = blockIdx.x;
-    const long long src = p.rows ? p.rows[r] : static_cast<long long>(r);
-    int8_t* out = p.codes + r * p.ldc;
-    if (src < 0 || src >= p.x_rows) {
-        for (int k = threadIdx.x; k < p.width; k += blockDim.x) out[k] = 0;
-        if (threadIdx.x == 0) p.scale[r] = 0.0f;
-        return;
+    const int lane = threadIdx.x % TPR;
+    const size_t r = static_cast<size_t>(blockIdx.x) * (kBlock / TPR) + threadIdx.x / TPR;
+    const bool there = r < static_cast<size_t>(p.n_rows);
+    const long long src = !there ? -1 : p.rows ? p.rows[r] : static_cast<long long>(r);
+    const bool read = src >= 0 && src < p.x_rows;
+    const T* x = static_cast<const T*>(p.x) + static_cast<size_t>(read ? src : 0) * p.ldx;
+    const char* lo = static_cast<const char*>(p.x);
+    const char* hi = SHIFT ? lo + (static_cast<size_t>(p.x_rows - 1) * p.ldx + p.width) * sizeof(T) : nullptr;
+    auto fetch = [&](int v) {
+        const int k = v * V;
+        if (!read || k >= p.width) return make_uint4(0, 0, 0, 0);
+        if (k + V > p.width) return load_part(x + k, p.width - k);
+        return SHIFT ? load_shifted(x + k, lo, hi) : load16(x + k);
+    };
+    uint4 d[NV ? NV : 1];
+    uint32_t top = 0;
+    auto join = [&](const uint4& q) { top = Vec<T>::join(Vec<T>::join(Vec<T>::join(Vec<T>::join(top, q.x), q.y), q.z), q.w); };
+    const int vecs = (p.width + V - 1) / V;
+    if (NV) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) d[i] = fetch(lane + i * TPR);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) join(d[i]);
+    } else {
+        for (int v = lane; v < vecs; v += TPR) join(fetch(v));
     }
-    const T* x = static_cast<const T*>(p.x) + static_cast<size_t>(src) * p.ldx;
-    uint32_t top = 0;   // magnitudes compared as bit patterns: NaN is above infinity is above every number
-    for (int k = threadIdx.x; k < p.width; k += blockDim.x) top = max(top, __float_as_uint(to_f32(x[k])) & 0x7FFFFFFFu);
-    top = __reduce_max_sync(0xffffffffu, top);
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
-    __syncthreads();
-    for (int w = 0; w < 8; ++w) top = max(top, part[w]);
-    const float s = top < 0x7F800000u ? fmaxf(__fdiv_rn(__uint_as_float(top), 127.0f), 1e-8f) : __uint_as_float(top);
-    for (int k = threadIdx.x; k < p.width; k += blockDim.x)
-        out[k] = top < 0x7F800000u ? static_cast<int8_t>(row_code_exact(to_f32(x[k]), s)) : 0;
-    if (threadIdx.x == 0) p.scale[r] = s;
+    top = __reduce_max_sync(0xffffffffu, Vec<T>::top(top));
+    if (kWarps > 1) {
+        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
+        __syncthreads();
+        const int w0 = threadIdx.x / TPR * kWarps;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = max(top, part[w0 + w]);
+    }
+    if (!there) return;
+    const bool finite = top < 0x7F800000u;
+    float s = __uint_as_float(top), inv_lo = 0.0f, inv_hi = 0.0f;   // not finite: codes 0
+    if (finite) {
+        s = fmaxf(__fdiv_rn(s, 127.0f), 1e-8f);
+        // 1/s within half a unit, then at least 2^-23 relative to both sides
+        const float inv = __frcp_rn(s);
+        inv_lo = __fmul_rd(inv, 1.0f - 0x1p-22f);
+        inv_hi = __fmul_ru(inv, 1.0f + 0x1p-22f);
+    }
+    if (lane == 0) p.scale[r] = read ? s : 0.0f;
+    int8_t* out = p.codes + r * p.ldc;
+    const bool whole = (reinterpret_cast<uintptr_t>(out) & (V - 1)) == 0;
+    auto emit = [&](int v, const uint4& q) {
+        const int k = v * V;
+        if (k >= p.width) return;
+        float f[V];
+        uint32_t c[V / 4] = {};
+        Vec<T>::values(q, f);
+        if (finite) codes_of<V>(f, inv_lo, inv_hi, s, c);
+        if (whole && k + V <= p.width) {
+            if (V == 8)
+                *reinterpret_cast<uint2*>(out + k) = make_uint2(c[0], c[V / 4 - 1]);
+            else
+                *reinterpret_cast<uint32_t*>(out + k) = c[0];
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (k + i < p.width) out[k + i] = static_cast<int8_t>(c[i / 4] >> (8 * (i & 3)));
+        }
+    };
+    if (NV) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) emit(lane + i * TPR, d[i]);
+    } else {
+        for (int v = lane; v < vecs; v += TPR) emit(v, fetch(v));
+    }
 }
 
 }  // namespace ptq8
