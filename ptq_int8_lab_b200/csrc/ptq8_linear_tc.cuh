@@ -11,12 +11,14 @@
 //         of 1/S of the tokens to the CTA that finishes them.  Integer sums: the order of
 //         arrival changes nothing.
 //   GATED: two accumulators per tile, gate and up channels, joined in the epilogue.
-//   W4: weights arrive packed; four warps widen them into the swizzled operand tile as 16 times
-//       the code (the nibble moved to its byte's high half: no sign extension), and the
-//       channel's scale carries the exact factor 1/16.
+//   W4: weights arrive packed; eight warps widen them as 16 times the code (the nibble moved to
+//       its byte's high half: no sign extension; the channel's scale carries the exact factor
+//       1/16) and write them to TMEM, from where the MMA takes its M operand.  A thread owns
+//       a channel, which is a TMEM lane.  Through shared memory the same took twice the time:
+//       writing the widened tile and the MMA's reads of it filled shared memory's bandwidth.
 //
 // Warps: 0 TMA producer, 1 MMA issuer, 2 TMEM and the groups' tile list, 4.. epilogue, then
-// (W4) four unpackers.  All waits are bounded.
+// (W4) the unpackers.  All waits are bounded.
 #pragma once
 
 #include "ptq8_linear.cuh"
@@ -32,7 +34,7 @@ struct TcParams {
     LinearParams l;
     int kblocks;       // blocks of 128 input features
     int stages;
-    int a_bufs;        // W4: unpacked operand tiles
+    int a_bufs;        // W4: operand tiles in TMEM, behind the accumulators
     int split;         // S
     int list_bytes;    // shared memory of the groups' tile list
     int ctiles;        // channel tiles
@@ -47,16 +49,16 @@ template <int CG, int TN, bool W4, bool GATED>
 struct TcShape {
     static constexpr int H = GATED ? 2 : 1;
     static constexpr int XR = TN / CG;                     // token rows loaded by one CTA
-    static constexpr int kTile = H * 128 * 128;            // operand bytes of the weights, unpacked
-    static constexpr int kPacked = H * 128 * 64;
-    static constexpr int kW = W4 ? kPacked : kTile;        // what a stage holds of them
+    static constexpr int kW = H * 128 * (W4 ? 64 : 128);   // bytes of the weights' rows in a stage
     static constexpr int kX = XR * 128;
     static constexpr int kStage = kW + kX;
-    static constexpr int kEpi = TN >= 128 ? 8 : 4;         // epilogue warps
+    static constexpr int kEpi = TN >= 96 ? 8 : 4;          // epilogue warps
     static constexpr int kCW = TN / (kEpi / 4);            // accumulator columns of one warp
-    static constexpr int kThreads = 128 + 32 * kEpi + (W4 ? 128 : 0);
+    static constexpr int kUnpack = W4 ? 8 : 0;             // unpacking warps
+    static constexpr int kThreads = 128 + 32 * (kEpi + kUnpack);
     static constexpr int kCols = H * TN;                   // accumulator columns of a tile
-    static constexpr int kPerSm = TN <= 64 && !(W4 && GATED) ? 2 : 1;   // CTAs that share an SM
+    static constexpr int kACols = 32 * H;                  // W4: columns of an operand tile
+    static constexpr int kPerSm = TN <= (W4 && GATED ? 32 : 64) ? 2 : 1;   // CTAs that share an SM
 };
 
 // ---- cluster-wide pieces
@@ -74,39 +76,16 @@ __device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// Arrive on a barrier of any CTA of the cluster (address from mapa, or of the own CTA).
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-// The same without release: frees an accumulator (see mbar_arrive_relaxed).
+// Arrive on a barrier of any CTA of the cluster (address from mapa, or of the own CTA) without release:
+// what it orders are tcgen05 accesses, completed by tcgen05.wait and ordered by tcgen05.fence, and loads
+// whose values have been used.  (With .release.cluster the unpackers took over 1000 cycles a block.)
 __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t bar) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ bool mbar_try_cluster(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}\n"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-// A converged warp's bounded wait that also acquires what other CTAs released.
-__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, long long limit) {
-    bool ok = mbar_try_cluster(bar, parity);
-    if (!ok) {
-        const long long t0 = clock64();
-        while (!ok && clock64() - t0 <= limit) {
-#pragma unroll
-            for (int k = 0; k < 8 && !ok; ++k) ok = mbar_try_cluster(bar, parity);
-        }
-    }
-    return __all_sync(0xffffffffu, ok);
-}
-__device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t v) {
-    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+// Store to a CTA of the cluster; its barrier there counts the bytes when they have arrived.
+__device__ __forceinline__ void st_async(uint32_t addr, uint32_t v, uint32_t bar) {
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.u32 [%0], %1, [%2];" ::"r"(addr), "r"(v), "r"(bar)
+                 : "memory");
 }
 
 template <int CG>
@@ -154,6 +133,38 @@ __device__ __forceinline__ void mma_pair_chunk_elect(uint32_t d, uint64_t da, ui
         "l"(da), "l"(db), "r"(idesc), "r"(acc)
         : "memory");
 }
+// The same with the M operand in TMEM: a K slice of 32 codes is 8 columns.
+template <int CG>
+__device__ __forceinline__ void mma_tmem_chunk_elect(uint32_t d, uint32_t a, uint64_t db, uint32_t idesc, uint32_t acc) {
+#define PTQ8_TMEM_CHUNK(G)                                                          \
+    asm volatile(                                                                   \
+        "{\n\t.reg .pred e, p;\n\t.reg .b64 b1, b2, b3;\n\t.reg .b32 a1, a2, a3;\n\t" \
+        "elect.sync _|e, 0xffffffff;\n\t"                                          \
+        "setp.ne.b32 p, %4, 0;\n\t"                                                \
+        "@e tcgen05.mma.cta_group::" G ".kind::i8 [%0], [%1], %2, %3, p;\n\t"       \
+        "add.s32 a1, %1, 8;\n\tadd.s64 b1, %2, 2;\n\t"                             \
+        "@e tcgen05.mma.cta_group::" G ".kind::i8 [%0], [a1], b1, %3, 1;\n\t"       \
+        "add.s32 a2, %1, 16;\n\tadd.s64 b2, %2, 4;\n\t"                            \
+        "@e tcgen05.mma.cta_group::" G ".kind::i8 [%0], [a2], b2, %3, 1;\n\t"       \
+        "add.s32 a3, %1, 24;\n\tadd.s64 b3, %2, 6;\n\t"                            \
+        "@e tcgen05.mma.cta_group::" G ".kind::i8 [%0], [a3], b3, %3, 1;\n\t}\n" ::"r"(d), \
+        "r"(a), "l"(db), "r"(idesc), "r"(acc)                                       \
+        : "memory")
+    if constexpr (CG == 2)
+        PTQ8_TMEM_CHUNK("2");
+    else
+        PTQ8_TMEM_CHUNK("1");
+#undef PTQ8_TMEM_CHUNK
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0],"
+        " {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // Arrive on `bar` (the pair's: in both CTAs) when the MMAs issued so far have completed.
 template <int CG>
 __device__ __forceinline__ void commit_elect(uint32_t bar) {
@@ -286,10 +297,9 @@ __device__ __forceinline__ void store_partials(T* y, size_t ldy, const int* recv
     }
 }
 
-// 16 packed bytes (32 codes) -> two 16-byte granules of 16 times the codes.
-__device__ __forceinline__ void widen(const uint4& p, uint4& lo, uint4& hi) {
+// 16 packed bytes -> 8 words of 16 times the 32 codes, in order.
+__device__ __forceinline__ void widen(const uint4& p, uint32_t* o) {
     const uint32_t m = 0xF0F0F0F0u;
-    uint32_t o[8];
     const uint32_t w[4] = {p.x, p.y, p.z, p.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -297,8 +307,6 @@ __device__ __forceinline__ void widen(const uint4& p, uint4& lo, uint4& hi) {
         o[2 * i] = __byte_perm(even, odd, 0x5140);
         o[2 * i + 1] = __byte_perm(even, odd, 0x7362);
     }
-    lo = make_uint4(o[0], o[1], o[2], o[3]);
-    hi = make_uint4(o[4], o[5], o[6], o[7]);
 }
 
 template <int CG, int TN, bool W4, bool GATED>
@@ -320,8 +328,7 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
 
     const uint32_t base = (smem_u32(dyn) + 1023u) & ~1023u;
     uint8_t* const base_p = dyn + (base - smem_u32(dyn));
-    const uint32_t a_ring = base + p.stages * Sh::kStage;                       // W4: unpacked tiles
-    const uint32_t after = a_ring + (W4 ? p.a_bufs * Sh::kTile : 0);            // tile list, or partial sums
+    const uint32_t after = base + p.stages * Sh::kStage;   // tile list, partial sums
     int* const list = reinterpret_cast<int*>(base_p + (after - base));
     const uint32_t recv = after + p.list_bytes;
     const uint32_t b0 = smem_u32(bars);
@@ -329,6 +336,7 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
     const uint32_t afull = b0 + 8 * 3 * kMaxLinStages, aempty = afull + 32, accfull = aempty + 32, accempty = accfull + 16,
                    partial = accempty + 16, drain = partial + 8;
 
+    griddep_launch();
     if (warp == 0 && elect_one()) {
         tma_prefetch(&map_x);
         tma_prefetch(&map_w);
@@ -340,14 +348,14 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
             mbar_init(pfull + 8 * s, 1);
         }
         for (int a = 0; a < 4; ++a) {
-            mbar_init(afull + 8 * a, 4 * CG);
+            mbar_init(afull + 8 * a, 4 * H * CG);
             mbar_init(aempty + 8 * a, 1);
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(accfull + 8 * a, 1);
             mbar_init(accempty + 8 * a, Sh::kEpi * CG);
         }
-        mbar_init(partial, S * Sh::kEpi);
+        mbar_init(partial, 1);
         mbar_init(drain, 1);
         fence_mbar_init();
     }
@@ -362,8 +370,10 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
             tmem_relinquish();
         }
     }
-    griddep_launch();
-    griddep_wait();   // nothing above reads or writes global memory
+    __syncwarp();
+    tc_fence_before();
+    if (clustered) cluster_sync();   // the peers' barriers exist
+    griddep_wait();                  // nothing above reads or writes global memory
     const bool listed = p.l.offsets != nullptr;
     if (listed && warp == 2) {   // first tile of each group
         int sum = 0;
@@ -386,11 +396,9 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
         if (lane == 0) list[p.l.groups] = sum;
     }
     __syncwarp();
-    tc_fence_before();
     __syncthreads();
-    if (clustered) cluster_sync();
     tc_fence_after();
-    const uint32_t tmem = tmem_slot;
+    const uint32_t tmem = tmem_slot, a_tiles = tmem + p.acc_bufs * Sh::kCols;
 
     Tiles<TN> tiles(p.l, listed ? list : nullptr, p.ctiles);
     const int per = CG == 2 ? 2 : S;
@@ -425,7 +433,7 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
                 if (elect_one()) {
                     const uint32_t wdst = base + s * Sh::kStage, xdst = wdst + Sh::kW;
                     if (leader) mbar_expect_tx(full + 8 * s, CG * (W4 ? Sh::kX : Sh::kStage));
-                    if (W4) mbar_expect_tx(pfull + 8 * s, Sh::kPacked);
+                    if (W4) mbar_expect_tx(pfull + 8 * s, Sh::kW);
                     if (!(p.stall && blockIdx.x == 0 && issued == 0)) {
 #pragma unroll
                         for (int h = 0; h < H; ++h) {
@@ -475,27 +483,28 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
             const int nn = columns_of<CG, TN>(tile);
             const uint32_t idesc = (make_idesc_i8(nn) & ~(0x1Fu << 24)) | (static_cast<uint32_t>(128 * CG >> 4) << 24);
             const uint32_t d = tmem + buf * Sh::kCols;
-            if (!mbar_wait_cluster(accempty + 8 * buf, accph, limit)) {
+            if (!mbar_wait_warp(accempty + 8 * buf, accph, limit)) {
                 give_up(ERR_WAIT_ACC);
                 ok = false;
                 break;
             }
             tc_fence_after();
             for (int kb = kb0; kb < kb1; ++kb) {
-                bool there = mbar_wait_cluster(full + 8 * s, ph, limit);
-                if (W4 && there) there = mbar_wait_cluster(afull + 8 * ab, aph, limit);
+                bool there = mbar_wait_warp(full + 8 * s, ph, limit);
+                if (W4 && there) there = mbar_wait_warp(afull + 8 * ab, aph, limit);
                 if (!there) {
                     give_up(ERR_WAIT_FULL);
                     ok = false;
                     break;
                 }
                 tc_fence_after();
-                const uint32_t wsrc = W4 ? a_ring + ab * Sh::kTile : base + s * Sh::kStage;
                 const uint64_t db = make_sdesc(base + s * Sh::kStage + Sh::kW, 128);
 #pragma unroll
                 for (int h = 0; h < H; ++h) {
-                    const uint64_t da = make_sdesc(wsrc + h * 16384, 128);
-                    if constexpr (CG == 2)
+                    const uint64_t da = make_sdesc(base + s * Sh::kStage + h * 16384, 128);
+                    if constexpr (W4)
+                        mma_tmem_chunk_elect<CG>(d + h * TN, a_tiles + ab * Sh::kACols + h * 32, db, idesc, kb > kb0);
+                    else if constexpr (CG == 2)
                         mma_pair_chunk_elect(d + h * TN, da, db, idesc, kb > kb0);
                     else
                         mma_chunk_elect<4>(d + h * TN, da, db, idesc, kb > kb0);
@@ -545,7 +554,7 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
             __syncwarp();
             for (int i = lane; c0 + i < c1; i += 32) sxs[i] = __ldg(p.l.xs + tile.row0 + c0 + i);
             __syncwarp();
-            if (!mbar_wait_cluster(accfull + 8 * buf, accph, limit)) {
+            if (!mbar_wait_warp(accfull + 8 * buf, accph, limit)) {
                 give_up(ERR_WAIT_ACC);
                 break;
             }
@@ -568,6 +577,8 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
                 }
             } else {
                 const int tokens = TN / S, shift = 31 - __clz(tokens);   // S is a power of two
+                const int first = rank * tokens, mine = min(max(tile.valid - first, 0), tokens);
+                if (warp == 4 && lane == 0) mbar_expect_tx(partial, S * mine * H * 128 * 4);
                 for (int cc = c0; cc < c1; cc += 16) {
                     uint32_t v[H][16];
 #pragma unroll
@@ -580,20 +591,18 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
                         if (cc + j < c1) {
                             const int to = (cc + j) >> shift, tk = (cc + j) & (tokens - 1);
                             const uint32_t dst = mapa(recv + (((rank * tokens + tk) * H) * 128 + lane_c) * 4, to);
+                            const uint32_t bar = mapa(partial, to);
 #pragma unroll
-                            for (int h = 0; h < H; ++h) st_cluster(dst + h * 512, v[h][j]);
+                            for (int h = 0; h < H; ++h) st_async(dst + h * 512, v[h][j], bar);
                         }
                     }
                 }
-                __syncwarp();
-                if (lane < S) mbar_arrive_cluster(mapa(partial, lane));
-                if (!mbar_wait_cluster(partial, 0, limit)) {
+                if (!mbar_wait_warp(partial, 0, limit)) {
                     give_up(ERR_WAIT_PARTIAL);
                     break;
                 }
                 const int* got = reinterpret_cast<const int*>(base_p + (recv - base));
-                const int first = rank * tokens;
-                if (part == 0) {
+                {
                     if (p.l.y_type == Y_F32)
                         store_partials<float, H>(static_cast<float*>(p.l.y) + at, p.l.ldy, got, S, tokens, sxs, ch, lane_c, first, tile.valid);
                     else if (p.l.y_type == Y_F16)
@@ -606,32 +615,42 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
         }
     } else if (W4 && warp >= 4 + Sh::kEpi) {
         // ---------------------------------------------------------------- unpackers
-        const int u = tid - 32 * (4 + Sh::kEpi);   // 0..127
+        // Gated: the first four warps widen the gate tile, the others the up tile; otherwise the two
+        // sets of four take every other block.
+        const int quad = warp & 3, set = (warp - 4 - Sh::kEpi) >> 2, row = quad * 32 + lane;
         const uint32_t afull_at = CG == 2 ? mapa(afull, 0) : afull;
-        int s = 0, ab = 0;
+        const uint32_t lanes = a_tiles + (GATED ? set * 32 : 0) + (static_cast<uint32_t>(quad * 32) << 16);
+        const uint8_t* src = base_p + (GATED ? set * 8192 : 0) + row * 64;
+        const int turn = (row >> 1) & 3;   // the 64-byte TMA swizzle of this row
+        int s = 0, ab = 0, mine = 0;
         uint32_t ph = 0, aph = 1;
         bool ok = true;
         for (int t = t0; ok && tiles.get(t, tile); t += dt) {
             for (int kb = kb0; kb < kb1; ++kb) {
-                if (!mbar_wait_warp(pfull + 8 * s, ph, limit) || !mbar_wait_cluster(aempty + 8 * ab, aph, limit)) {
-                    give_up(ERR_WAIT_UNPACK);
-                    ok = false;
-                    break;
+                if (GATED || mine == set) {
+                    if (!mbar_wait_warp(pfull + 8 * s, ph, limit)) {
+                        give_up(ERR_WAIT_UNPACK);
+                        ok = false;
+                        break;
+                    }
+                    uint32_t o[16];
+                    widen(*reinterpret_cast<const uint4*>(src + s * Sh::kStage + ((0 ^ turn) << 4)), o);
+                    widen(*reinterpret_cast<const uint4*>(src + s * Sh::kStage + ((1 ^ turn) << 4)), o + 8);
+                    if (!mbar_wait_warp(aempty + 8 * ab, aph, limit)) {
+                        give_up(ERR_WAIT_UNPACK);
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    tmem_st16(lanes + ab * Sh::kACols, o);
+                    widen(*reinterpret_cast<const uint4*>(src + s * Sh::kStage + ((2 ^ turn) << 4)), o);
+                    widen(*reinterpret_cast<const uint4*>(src + s * Sh::kStage + ((3 ^ turn) << 4)), o + 8);
+                    tmem_st16(lanes + ab * Sh::kACols + 16, o);
+                    tmem_wait_st();
+                    tc_fence_before();
+                    if (lane == 0) mbar_arrive_cluster_relaxed(afull_at + 8 * ab);
                 }
-                const uint8_t* src = base_p + s * Sh::kStage;
-                uint8_t* dst = base_p + (a_ring - base) + ab * Sh::kTile;
-#pragma unroll
-                for (int i = 0; i < 4 * H; ++i) {
-                    const int item = i * 128 + u, r = item >> 2, q = item & 3;   // row, 16-byte granule of the packed row
-                    uint4 lo, hi;
-                    widen(*reinterpret_cast<const uint4*>(src + item * 16), lo, hi);
-                    uint8_t* row = dst + r * 128;
-                    *reinterpret_cast<uint4*>(row + (((2 * q) ^ (r & 7)) << 4)) = lo;
-                    *reinterpret_cast<uint4*>(row + (((2 * q + 1) ^ (r & 7)) << 4)) = hi;
-                }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(afull_at + 8 * ab);
+                mine ^= 1;
                 if (++ab == p.a_bufs) {
                     ab = 0;
                     aph ^= 1;

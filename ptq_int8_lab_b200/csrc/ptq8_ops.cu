@@ -185,22 +185,22 @@ struct Variant {
     int cg, tn;            // CTAs per tile, tokens per tile
     bool w4, gated;
     TcKernel kernel;
-    int threads, stage, tile, cols, x_rows, per_sm;
+    int threads, stage, cols, a_cols, x_rows, per_sm;
 };
 
 template <int CG, int TN, bool W4, bool GATED>
 Variant variant() {
     using Sh = TcShape<CG, TN, W4, GATED>;
-    return {CG, TN, W4, GATED, linear_tc_kernel<CG, TN, W4, GATED>, Sh::kThreads, Sh::kStage, Sh::kTile, Sh::kCols, Sh::XR, Sh::kPerSm};
+    return {CG, TN, W4, GATED, linear_tc_kernel<CG, TN, W4, GATED>, Sh::kThreads, Sh::kStage, Sh::kCols, W4 ? Sh::kACols : 0, Sh::XR, Sh::kPerSm};
 }
 
 const Variant kVariants[] = {
     variant<1, 16, false, false>(),  variant<1, 16, false, true>(),  variant<1, 16, true, false>(),  variant<1, 16, true, true>(),
     variant<1, 32, false, false>(),  variant<1, 32, false, true>(),  variant<1, 32, true, false>(),  variant<1, 32, true, true>(),
     variant<1, 64, false, false>(),  variant<1, 64, false, true>(),  variant<1, 64, true, false>(),  variant<1, 64, true, true>(),
-    variant<1, 128, false, false>(), variant<1, 128, false, true>(), variant<1, 128, true, false>(), variant<1, 128, true, true>(),
-    variant<2, 128, false, false>(), variant<2, 128, false, true>(), variant<2, 128, true, false>(), variant<2, 128, true, true>(),
-    variant<2, 256, false, false>(), variant<2, 256, true, false>(),
+    variant<1, 128, false, false>(), variant<1, 128, false, true>(), variant<1, 128, true, false>(), variant<1, 96, true, true>(),
+    variant<2, 128, false, false>(), variant<2, 128, false, true>(), variant<2, 256, false, false>(),
+    variant<2, 192, true, false>(),  variant<2, 96, true, true>(),
 };
 
 // Dynamic shared memory of a CTA that shares its SM with another, or not.
@@ -213,9 +213,11 @@ struct Choice {
 Choice choose(const ptq8_ops* o, const ptq8_linear_args& a, int groups, bool gated) {
     const long long m = (a.rows + groups - 1) / groups;   // rows that a group has on average
     const int kblocks = (a.in_features + 127) / 128;
-    Choice c{1, m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128, 1};
+    const bool w4 = a.w_bits == 4;
+    const int big = w4 && gated ? 96 : 128;
+    Choice c{1, m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : big, 1};
     const long long tiles = (a.out_features + 127) / 128 * std::max<long long>(groups > 1 ? std::min<long long>(groups, a.rows) : 1, (a.rows + c.tn - 1) / c.tn);
-    if (c.tn == 128 && tiles > 2 * o->sms) c = {2, gated ? 128 : 256, 1};
+    if (c.tn == big && tiles > 2 * o->sms) c = {2, w4 ? (gated ? 96 : 192) : (gated ? 128 : 256), 1};
     if (c.tn <= 32)
         while (c.split < 8 && tiles * c.split * 2 <= 2 * o->sms && kblocks >= 4 * c.split) c.split *= 2;
     return c;
@@ -260,7 +262,7 @@ int run_tc(ptq8_ops* o, const ptq8_linear_args& a, const LinearParams& l, cudaSt
         const cuuint64_t dims[3] = {static_cast<cuuint64_t>(wide), static_cast<cuuint64_t>(channels), static_cast<cuuint64_t>(l.groups)};
         const cuuint64_t pitch[2] = {ldw, l.groups > 1 ? static_cast<cuuint64_t>(l.gstride) : ldw};
         const cuuint32_t box[3] = {w4 ? 64u : 128u, 128, 1};
-        if (const int rc = encode(o, &mw, 3, a.w, dims, pitch, box, w4 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B))
+        if (const int rc = encode(o, &mw, 3, a.w, dims, pitch, box, w4 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B))
             return rc;
     }
     TcParams p{};
@@ -269,14 +271,14 @@ int run_tc(ptq8_ops* o, const ptq8_linear_args& a, const LinearParams& l, cudaSt
     p.split = c.split;
     p.ctiles = (a.out_features + 128 * c.cg - 1) / (128 * c.cg);
     p.list_bytes = l.offsets ? ((l.groups + 1) * 4 + 127) / 128 * 128 : 0;
-    p.a_bufs = w4 ? 2 : 0;
+    p.a_bufs = w4 ? 128 / v->a_cols : 0;
     p.acc_bufs = c.split > 1 ? 1 : 2;
     p.tmem_cols = 32;
-    while (static_cast<int>(p.tmem_cols) < v->cols * p.acc_bufs) p.tmem_cols *= 2;
+    while (static_cast<int>(p.tmem_cols) < v->cols * p.acc_bufs + v->a_cols * p.a_bufs) p.tmem_cols *= 2;
     p.wait_limit = o->wait_limit;
     p.err = o->error_dev;
     p.stall = o->stall;
-    const int extra = 1024 + p.a_bufs * v->tile + p.list_bytes + (c.split > 1 ? v->cols * 128 * 4 : 0);
+    const int extra = 1024 + p.list_bytes + (c.split > 1 ? v->cols * 128 * 4 : 0);
     p.stages = std::min(kMaxLinStages, ((v->per_sm == 2 ? kSmemTwo : kSmemOne) - extra) / v->stage);
     if (p.stages < 2) return fail(o, PTQ8_ERR_INVALID, "linear: %d stages", p.stages);
     const int smem = extra + p.stages * v->stage;
