@@ -114,57 +114,56 @@ __device__ __forceinline__ void load_rows_3d(uint32_t dst, const CUtensorMap* m,
             : "memory");
 }
 
-// The four K slices of one 128-byte block; the pair's form of mma_chunk_elect<4>.
-__device__ __forceinline__ void mma_pair_chunk_elect(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) {
-    asm volatile(
-        "{\n\t.reg .pred e, p;\n\t.reg .b64 a1, b1, a2, b2, a3, b3;\n\t"
-        "elect.sync _|e, 0xffffffff;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "@e tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t"
-        "add.s64 a1, %1, 2;\n\t"
-        "add.s64 b1, %2, 2;\n\t"
-        "@e tcgen05.mma.cta_group::2.kind::i8 [%0], a1, b1, %3, 1;\n\t"
-        "add.s64 a2, %1, 4;\n\t"
-        "add.s64 b2, %2, 4;\n\t"
-        "@e tcgen05.mma.cta_group::2.kind::i8 [%0], a2, b2, %3, 1;\n\t"
-        "add.s64 a3, %1, 6;\n\t"
-        "add.s64 b3, %2, 6;\n\t"
-        "@e tcgen05.mma.cta_group::2.kind::i8 [%0], a3, b3, %3, 1;\n\t}\n" ::"r"(d),
-        "l"(da), "l"(db), "r"(idesc), "r"(acc)
-        : "memory");
-}
-// The same with the M operand in TMEM: a K slice of 32 codes is 8 columns.
-template <int CG>
-__device__ __forceinline__ void mma_tmem_chunk_elect(uint32_t d, uint32_t a, uint64_t db, uint32_t idesc, uint32_t acc) {
-#define PTQ8_TMEM_CHUNK(G)                                                          \
-    asm volatile(                                                                   \
-        "{\n\t.reg .pred e, p;\n\t.reg .b64 b1, b2, b3;\n\t.reg .b32 a1, a2, a3;\n\t" \
-        "elect.sync _|e, 0xffffffff;\n\t"                                          \
-        "setp.ne.b32 p, %4, 0;\n\t"                                                \
-        "@e tcgen05.mma.cta_group::" G ".kind::i8 [%0], [%1], %2, %3, p;\n\t"       \
-        "add.s32 a1, %1, 8;\n\tadd.s64 b1, %2, 2;\n\t"                             \
-        "@e tcgen05.mma.cta_group::" G ".kind::i8 [%0], [a1], b1, %3, 1;\n\t"       \
-        "add.s32 a2, %1, 16;\n\tadd.s64 b2, %2, 4;\n\t"                            \
-        "@e tcgen05.mma.cta_group::" G ".kind::i8 [%0], [a2], b2, %3, 1;\n\t"       \
-        "add.s32 a3, %1, 24;\n\tadd.s64 b3, %2, 6;\n\t"                            \
-        "@e tcgen05.mma.cta_group::" G ".kind::i8 [%0], [a3], b3, %3, 1;\n\t}\n" ::"r"(d), \
-        "r"(a), "l"(db), "r"(idesc), "r"(acc)                                       \
+// One block of 128 input features: the H tiles' four K slices each (D columns d and d + step), then the
+// commit that releases the block -- in one asm block with one election, and descriptors advanced in their
+// low words only (the start address, 14 bits that never carry inside shared memory): with an election per
+// K chunk and 64-bit adds the issuing warp, not the tensor core, set the pace.
+// M operand: shared-memory descriptor (a K slice of 32 codes is 2 units of 16 bytes, the second tile 1024
+// units further), or TMEM (8 columns, 32 columns further).
+#define PTQ8_MMA(G, D, A, P) "@e tcgen05.mma.cta_group::" G ".kind::i8 [" D "], " A ", B, %5, " P ";\n\t"
+#define PTQ8_S(G, D, AO, BO, P)                                                                             \
+    "add.u32 ta, %2, " AO ";\n\tadd.u32 tb, %3, " BO ";\n\tmov.b64 A, {ta, %4};\n\tmov.b64 B, {tb, %4};\n\t" \
+    PTQ8_MMA(G, D, "A", P)
+#define PTQ8_T(G, D, AO, BO, P)                                                                             \
+    "add.u32 ta, %2, " AO ";\n\tadd.u32 tb, %3, " BO ";\n\tmov.b64 B, {tb, %4};\n\t" PTQ8_MMA(G, D, "[ta]", P)
+#define PTQ8_S4(G) PTQ8_S(G, "%0", "0", "0", "p") PTQ8_S(G, "%0", "2", "2", "1") PTQ8_S(G, "%0", "4", "4", "1") PTQ8_S(G, "%0", "6", "6", "1")
+#define PTQ8_S8(G) PTQ8_S4(G) PTQ8_S(G, "%1", "1024", "0", "p") PTQ8_S(G, "%1", "1026", "2", "1") PTQ8_S(G, "%1", "1028", "4", "1") PTQ8_S(G, "%1", "1030", "6", "1")
+#define PTQ8_T4(G) PTQ8_T(G, "%0", "0", "0", "p") PTQ8_T(G, "%0", "8", "2", "1") PTQ8_T(G, "%0", "16", "4", "1") PTQ8_T(G, "%0", "24", "6", "1")
+#define PTQ8_T8(G) PTQ8_T4(G) PTQ8_T(G, "%1", "32", "0", "p") PTQ8_T(G, "%1", "40", "2", "1") PTQ8_T(G, "%1", "48", "4", "1") PTQ8_T(G, "%1", "56", "6", "1")
+#define PTQ8_COMMIT1 "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%7];\n\t}\n"
+#define PTQ8_COMMIT2                                                                                        \
+    "mov.u16 m, 3;\n\t@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%7], m;\n\t}\n"
+#define PTQ8_BLOCK(BODY)                                                                                    \
+    asm volatile(                                                                                           \
+        "{\n\t.reg .pred e, p;\n\t.reg .b64 A, B;\n\t.reg .b32 ta, tb;\n\t.reg .b16 m;\n\t"                  \
+        "elect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %6, 0;\n\t" BODY ::"r"(d), "r"(d + step), "r"(a),     \
+        "r"(b), "r"(hi), "r"(idesc), "r"(acc), "r"(bar)                                                     \
         : "memory")
-    if constexpr (CG == 2)
-        PTQ8_TMEM_CHUNK("2");
-    else
-        PTQ8_TMEM_CHUNK("1");
-#undef PTQ8_TMEM_CHUNK
+
+// a: TMEM address (TMEM_A) or low word of the descriptor; b: low word; hi: the descriptors' high word.
+template <int CG, int H, bool TMEM_A>
+__device__ __forceinline__ void mma_block(uint32_t d, uint32_t step, uint32_t a, uint32_t b, uint32_t hi, uint32_t idesc,
+                                          uint32_t acc, uint32_t bar) {
+    if constexpr (CG == 1 && H == 1 && !TMEM_A) PTQ8_BLOCK(PTQ8_S4("1") PTQ8_COMMIT1);
+    if constexpr (CG == 1 && H == 2 && !TMEM_A) PTQ8_BLOCK(PTQ8_S8("1") PTQ8_COMMIT1);
+    if constexpr (CG == 2 && H == 1 && !TMEM_A) PTQ8_BLOCK(PTQ8_S4("2") PTQ8_COMMIT2);
+    if constexpr (CG == 2 && H == 2 && !TMEM_A) PTQ8_BLOCK(PTQ8_S8("2") PTQ8_COMMIT2);
+    if constexpr (CG == 1 && H == 1 && TMEM_A) PTQ8_BLOCK(PTQ8_T4("1") PTQ8_COMMIT1);
+    if constexpr (CG == 1 && H == 2 && TMEM_A) PTQ8_BLOCK(PTQ8_T8("1") PTQ8_COMMIT1);
+    if constexpr (CG == 2 && H == 1 && TMEM_A) PTQ8_BLOCK(PTQ8_T4("2") PTQ8_COMMIT2);
+    if constexpr (CG == 2 && H == 2 && TMEM_A) PTQ8_BLOCK(PTQ8_T8("2") PTQ8_COMMIT2);
 }
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0],"
-        " {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
-        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
-        : "memory");
-}
-__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+#undef PTQ8_MMA
+#undef PTQ8_S
+#undef PTQ8_T
+#undef PTQ8_S4
+#undef PTQ8_S8
+#undef PTQ8_T4
+#undef PTQ8_T8
+#undef PTQ8_COMMIT1
+#undef PTQ8_COMMIT2
+#undef PTQ8_BLOCK
+
 // Arrive on `bar` (the pair's: in both CTAs) when the MMAs issued so far have completed.
 template <int CG>
 __device__ __forceinline__ void commit_elect(uint32_t bar) {
@@ -177,6 +176,19 @@ __device__ __forceinline__ void commit_elect(uint32_t bar) {
     else
         mma_commit_elect(bar);
 }
+
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0],"
+        " {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16,"
+        " %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+        "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+        "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // ---- tiles
 
@@ -209,8 +221,8 @@ struct Tiles {
             i = t - start[g];
         }
         const int tt = static_cast<int>((end - beg + TN - 1) / TN);
+        if (!start && i >= tt * ctiles) return false;
         const int full = kBand * ctiles, band = i / full, rest = i - band * full;
-        if (band * kBand >= tt) return false;
         const int wide = min(kBand, tt - band * kBand);
         o.ct = rest / wide;
         const int k = band * kBand + (rest - o.ct * wide);
@@ -316,7 +328,7 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
     using Sh = TcShape<CG, TN, W4, GATED>;
     constexpr int H = Sh::H;
     extern __shared__ uint8_t dyn[];
-    __shared__ __align__(8) uint64_t bars[3 * kMaxLinStages + 16];
+    __shared__ __align__(8) uint64_t bars[2 * kMaxLinStages + 10];
     __shared__ uint32_t tmem_slot;
     __shared__ __align__(16) float sxs_all[Sh::kEpi][Sh::kCW];   // token scales, each epilogue warp its own columns
 
@@ -332,8 +344,8 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
     int* const list = reinterpret_cast<int*>(base_p + (after - base));
     const uint32_t recv = after + p.list_bytes;
     const uint32_t b0 = smem_u32(bars);
-    const uint32_t full = b0, empty = full + 8 * p.stages, pfull = empty + 8 * p.stages;
-    const uint32_t afull = b0 + 8 * 3 * kMaxLinStages, aempty = afull + 32, accfull = aempty + 32, accempty = accfull + 16,
+    const uint32_t full = b0, empty = full + 8 * p.stages;
+    const uint32_t afull = b0 + 8 * 2 * kMaxLinStages, accfull = afull + 32, accempty = accfull + 16,
                    partial = accempty + 16, drain = partial + 8;
 
     griddep_launch();
@@ -345,12 +357,8 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
         for (int s = 0; s < p.stages; ++s) {
             mbar_init(full + 8 * s, 1);
             mbar_init(empty + 8 * s, 1);
-            mbar_init(pfull + 8 * s, 1);
         }
-        for (int a = 0; a < 4; ++a) {
-            mbar_init(afull + 8 * a, 4 * H * CG);
-            mbar_init(aempty + 8 * a, 1);
-        }
+        for (int a = 0; a < 4; ++a) mbar_init(afull + 8 * a, 4 * H * CG);
         for (int a = 0; a < 2; ++a) {
             mbar_init(accfull + 8 * a, 1);
             mbar_init(accempty + 8 * a, Sh::kEpi * CG);
@@ -416,7 +424,9 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
 
     if (warp == 0) {
         // ---------------------------------------------------------------- producer
-        const uint32_t full_at = CG == 2 ? mapa(full, 0) : full;   // the pair's loads all count at the leader
+        // The pair's loads all count at the leader; with int4 weights at the own CTA, whose unpackers
+        // pass it on.
+        const uint32_t full_at = CG == 2 && !W4 ? mapa(full, 0) : full;
         int s = 0, issued = 0;
         uint32_t ph = 1;
         bool ok = true;
@@ -432,17 +442,16 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
                 }
                 if (elect_one()) {
                     const uint32_t wdst = base + s * Sh::kStage, xdst = wdst + Sh::kW;
-                    if (leader) mbar_expect_tx(full + 8 * s, CG * (W4 ? Sh::kX : Sh::kStage));
-                    if (W4) mbar_expect_tx(pfull + 8 * s, Sh::kW);
+                    if (leader || W4) mbar_expect_tx(full + 8 * s, (W4 ? 1 : CG) * Sh::kStage);
                     if (!(p.stall && blockIdx.x == 0 && issued == 0)) {
 #pragma unroll
                         for (int h = 0; h < H; ++h) {
                             if constexpr (W4)
-                                load_rows_3d<1>(wdst + h * 8192, &map_w, pfull + 8 * s, kb * 64, h * p.l.n + c, tile.group);
+                                load_rows_3d<1>(wdst + h * 8192, &map_w, full_at + 8 * s, kb * 64, h * p.l.n + c, tile.group);
                             else
                                 load_rows_3d<CG>(wdst + h * 16384, &map_w, full_at + 8 * s, kb * 128, h * p.l.n + c, tile.group);
                         }
-                        load_rows_2d<CG>(xdst, &map_x, full_at + 8 * s, kb * 128, r);
+                        load_rows_2d<W4 ? 1 : CG>(xdst, &map_x, full_at + 8 * s, kb * 128, r);
                     }
                 }
                 __syncwarp();
@@ -470,14 +479,15 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
             const int n = min(issued, p.stages);
             for (int i = 1; i <= n; ++i) {
                 const int back = issued - i;
-                if (leader) mbar_wait_warp(full + 8 * (back % p.stages), (back / p.stages) & 1, limit);
-                if (W4) mbar_wait_warp(pfull + 8 * (back % p.stages), (back / p.stages) & 1, limit);
+                if (leader || W4) mbar_wait_warp(full + 8 * (back % p.stages), (back / p.stages) & 1, limit);
             }
         }
     } else if (warp == 1) {
         // ---------------------------------------------------------------- MMA issuer (the pair's leader)
         int s = 0, ab = 0, buf = 0;
         uint32_t ph = 0, aph = 0, accph = 1;
+        const uint64_t desc = make_sdesc(base, 128);
+        const uint32_t desc0 = static_cast<uint32_t>(desc), desc_hi = static_cast<uint32_t>(desc >> 32);
         bool ok = leader;
         for (int t = t0; ok && tiles.get(t, tile); t += dt) {
             const int nn = columns_of<CG, TN>(tile);
@@ -490,33 +500,20 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
             }
             tc_fence_after();
             for (int kb = kb0; kb < kb1; ++kb) {
-                bool there = mbar_wait_warp(full + 8 * s, ph, limit);
-                if (W4 && there) there = mbar_wait_warp(afull + 8 * ab, aph, limit);
-                if (!there) {
+                // W4: the unpackers saw the stage's loads arrive, the tokens' rows among them
+                if (!mbar_wait_warp(W4 ? afull + 8 * ab : full + 8 * s, W4 ? aph : ph, limit)) {
                     give_up(ERR_WAIT_FULL);
                     ok = false;
                     break;
                 }
                 tc_fence_after();
-                const uint64_t db = make_sdesc(base + s * Sh::kStage + Sh::kW, 128);
-#pragma unroll
-                for (int h = 0; h < H; ++h) {
-                    const uint64_t da = make_sdesc(base + s * Sh::kStage + h * 16384, 128);
-                    if constexpr (W4)
-                        mma_tmem_chunk_elect<CG>(d + h * TN, a_tiles + ab * Sh::kACols + h * 32, db, idesc, kb > kb0);
-                    else if constexpr (CG == 2)
-                        mma_pair_chunk_elect(d + h * TN, da, db, idesc, kb > kb0);
-                    else
-                        mma_chunk_elect<4>(d + h * TN, da, db, idesc, kb > kb0);
+                const uint32_t st = desc0 + s * (Sh::kStage >> 4);
+                mma_block<CG, H, W4>(d, TN, W4 ? a_tiles + ab * Sh::kACols : st, st + (Sh::kW >> 4), desc_hi, idesc, kb > kb0,
+                                     empty + 8 * s);
+                if (W4 && ++ab == p.a_bufs) {
+                    ab = 0;
+                    aph ^= 1;
                 }
-                if (W4) {
-                    commit_elect<CG>(aempty + 8 * ab);
-                    if (++ab == p.a_bufs) {
-                        ab = 0;
-                        aph ^= 1;
-                    }
-                }
-                commit_elect<CG>(empty + 8 * s);
                 if (++s == p.stages) {
                     s = 0;
                     ph ^= 1;
@@ -622,45 +619,54 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
         const uint32_t lanes = a_tiles + (GATED ? set * 32 : 0) + (static_cast<uint32_t>(quad * 32) << 16);
         const uint8_t* src = base_p + (GATED ? set * 8192 : 0) + row * 64;
         const int turn = (row >> 1) & 3;   // the 64-byte TMA swizzle of this row
-        int s = 0, ab = 0, mine = 0;
-        uint32_t ph = 0, aph = 1;
-        bool ok = true;
-        for (int t = t0; ok && tiles.get(t, tile); t += dt) {
-            for (int kb = kb0; kb < kb1; ++kb) {
-                if (GATED || mine == set) {
-                    if (!mbar_wait_warp(pfull + 8 * s, ph, limit)) {
-                        give_up(ERR_WAIT_UNPACK);
-                        ok = false;
-                        break;
-                    }
-                    uint32_t o[16];
-                    widen(*reinterpret_cast<const uint4*>(src + s * Sh::kStage + ((0 ^ turn) << 4)), o);
-                    widen(*reinterpret_cast<const uint4*>(src + s * Sh::kStage + ((1 ^ turn) << 4)), o + 8);
-                    if (!mbar_wait_warp(aempty + 8 * ab, aph, limit)) {
-                        give_up(ERR_WAIT_UNPACK);
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    tmem_st16(lanes + ab * Sh::kACols, o);
-                    widen(*reinterpret_cast<const uint4*>(src + s * Sh::kStage + ((2 ^ turn) << 4)), o);
-                    widen(*reinterpret_cast<const uint4*>(src + s * Sh::kStage + ((3 ^ turn) << 4)), o + 8);
-                    tmem_st16(lanes + ab * Sh::kACols + 16, o);
-                    tmem_wait_st();
-                    tc_fence_before();
-                    if (lane == 0) mbar_arrive_cluster_relaxed(afull_at + 8 * ab);
+        // This CTA's blocks, tile after tile.  The operand tile of block i is free when block i - a_bufs is
+        // released: its stage's barrier (its next phase cannot end before block i itself is unpacked).
+        const int total = listed ? list[p.l.groups] : static_cast<int>((p.l.rows + TN - 1) / TN) * p.ctiles;
+        const int tiles_here = t0 >= total ? 0 : S > 1 ? 1 : (total - t0 + dt - 1) / dt;
+        const long long blocks = static_cast<long long>(tiles_here) * (kb1 - kb0);
+        constexpr int step = GATED ? 1 : 2;
+        int s = GATED ? 0 : set, ab = s, old = s;   // a_bufs is even: block set + a_bufs is this set's too
+        uint32_t ph = 0, oldph = 0;
+        for (long long i = GATED ? 0 : set; i < blocks; i += step) {
+            if (!mbar_wait_warp(full + 8 * s, ph, limit)) {
+                give_up(ERR_WAIT_UNPACK);
+                break;
+            }
+            // all of the block in registers before the operand tile is free: what follows the MMAs'
+            // release of it is the store alone
+            uint32_t o[32];
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                widen(*reinterpret_cast<const uint4*>(src + s * Sh::kStage + ((q ^ turn) << 4)), o + 8 * q);
+            if (i >= p.a_bufs) {
+                if (!mbar_wait_warp(empty + 8 * old, oldph, limit)) {
+                    give_up(ERR_WAIT_UNPACK);
+                    break;
                 }
-                mine ^= 1;
-                if (++ab == p.a_bufs) {
-                    ab = 0;
-                    aph ^= 1;
-                }
-                if (++s == p.stages) {
-                    s = 0;
-                    ph ^= 1;
+                old += step;
+                if (old >= p.stages) {
+                    old -= p.stages;
+                    oldph ^= 1;
                 }
             }
-            if (S > 1) break;
+            tc_fence_after();
+            tmem_st32(lanes + ab * Sh::kACols, o);
+            tmem_wait_st();
+            tc_fence_before();
+            // the pair's leader learns of both CTAs' rows here: their copies have landed (seen above)
+            if (lane == 0) {
+                if (CG == 1)
+                    mbar_arrive(afull_at + 8 * ab);
+                else
+                    mbar_arrive_cluster_relaxed(afull_at + 8 * ab);
+            }
+            ab += step;
+            if (ab >= p.a_bufs) ab -= p.a_bufs;
+            s += step;
+            if (s >= p.stages) {
+                s -= p.stages;
+                ph ^= 1;
+            }
         }
     }
 

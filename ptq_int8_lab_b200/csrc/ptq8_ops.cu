@@ -280,7 +280,7 @@ int run_tc(ptq8_ops* o, const ptq8_linear_args& a, const LinearParams& l, cudaSt
     p.stall = o->stall;
     const int extra = 1024 + p.list_bytes + (c.split > 1 ? v->cols * 128 * 4 : 0);
     p.stages = std::min(kMaxLinStages, ((v->per_sm == 2 ? kSmemTwo : kSmemOne) - extra) / v->stage);
-    if (p.stages < 2) return fail(o, PTQ8_ERR_INVALID, "linear: %d stages", p.stages);
+    if (p.stages < std::max(2, p.a_bufs)) return fail(o, PTQ8_ERR_INVALID, "linear: %d stages", p.stages);
     const int smem = extra + p.stages * v->stage;
     // tiles at most: each group's last tile may be partly filled
     const long long row_tiles = l.offsets ? a.rows / c.tn + std::min<long long>(l.groups, a.rows) : (a.rows + c.tn - 1) / c.tn;
