@@ -52,7 +52,7 @@ struct TcShape {
     static constexpr int kW = H * 128 * (W4 ? 64 : 128);   // bytes of the weights' rows in a stage
     static constexpr int kX = XR * 128;
     static constexpr int kStage = kW + kX;
-    static constexpr int kEpi = TN >= 96 ? 8 : 4;          // epilogue warps
+    static constexpr int kEpi = TN >= 128 ? 8 : 4;          // epilogue warps
     static constexpr int kCW = TN / (kEpi / 4);            // accumulator columns of one warp
     static constexpr int kUnpack = W4 ? 8 : 0;             // unpacking warps
     static constexpr int kThreads = 128 + 32 * (kEpi + kUnpack);

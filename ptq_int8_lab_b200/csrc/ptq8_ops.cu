@@ -198,9 +198,9 @@ const Variant kVariants[] = {
     variant<1, 16, false, false>(),  variant<1, 16, false, true>(),  variant<1, 16, true, false>(),  variant<1, 16, true, true>(),
     variant<1, 32, false, false>(),  variant<1, 32, false, true>(),  variant<1, 32, true, false>(),  variant<1, 32, true, true>(),
     variant<1, 64, false, false>(),  variant<1, 64, false, true>(),  variant<1, 64, true, false>(),  variant<1, 64, true, true>(),
-    variant<1, 128, false, false>(), variant<1, 128, false, true>(), variant<1, 128, true, false>(), variant<1, 96, true, true>(),
-    variant<2, 128, false, false>(), variant<2, 128, false, true>(), variant<2, 256, false, false>(),
-    variant<2, 192, true, false>(),  variant<2, 96, true, true>(),
+    variant<1, 128, false, false>(), variant<1, 128, false, true>(), variant<1, 128, true, false>(), variant<1, 128, true, true>(),
+    variant<2, 128, false, false>(), variant<2, 128, false, true>(), variant<2, 128, true, true>(),
+    variant<2, 256, false, false>(), variant<2, 256, true, false>(),
 };
 
 // Dynamic shared memory of a CTA that shares its SM with another, or not.
@@ -213,11 +213,9 @@ struct Choice {
 Choice choose(const ptq8_ops* o, const ptq8_linear_args& a, int groups, bool gated) {
     const long long m = (a.rows + groups - 1) / groups;   // rows that a group has on average
     const int kblocks = (a.in_features + 127) / 128;
-    const bool w4 = a.w_bits == 4;
-    const int big = w4 && gated ? 96 : 128;
-    Choice c{1, m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : big, 1};
+    Choice c{1, m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128, 1};
     const long long tiles = (a.out_features + 127) / 128 * std::max<long long>(groups > 1 ? std::min<long long>(groups, a.rows) : 1, (a.rows + c.tn - 1) / c.tn);
-    if (c.tn == big && tiles > 2 * o->sms) c = {2, w4 ? (gated ? 96 : 192) : (gated ? 128 : 256), 1};
+    if (c.tn == 128 && tiles > 2 * o->sms) c = {2, gated ? 128 : 256, 1};
     if (c.tn <= 32)
         while (c.split < 8 && tiles * c.split * 2 <= 2 * o->sms && kblocks >= 4 * c.split) c.split *= 2;
     return c;
@@ -271,8 +269,11 @@ int run_tc(ptq8_ops* o, const ptq8_linear_args& a, const LinearParams& l, cudaSt
     p.split = c.split;
     p.ctiles = (a.out_features + 128 * c.cg - 1) / (128 * c.cg);
     p.list_bytes = l.offsets ? ((l.groups + 1) * 4 + 127) / 128 * 128 : 0;
-    p.a_bufs = w4 ? 128 / v->a_cols : 0;
-    p.acc_bufs = c.split > 1 ? 1 : 2;
+    // Two accumulators where TMEM holds them; with int4 weights four operand tiles come first, which hide
+    // the way from the MMAs' release of a tile to its next use (4096 x 4096 x 4096 gated: 112 us, with
+    // tiles of 96 tokens, two accumulators and two operand tiles 150 us).
+    p.acc_bufs = c.split > 1 || 2 * v->cols + (w4 ? 128 : 0) > 512 ? 1 : 2;
+    p.a_bufs = w4 ? std::min(4, (512 / v->per_sm - p.acc_bufs * v->cols) / v->a_cols) & ~1 : 0;
     p.tmem_cols = 32;
     while (static_cast<int>(p.tmem_cols) < v->cols * p.acc_bufs + v->a_cols * p.a_bufs) p.tmem_cols *= 2;
     p.wait_limit = o->wait_limit;
