@@ -147,22 +147,31 @@ using RowsKernel = void (*)(RowsParams);
 struct RowsVariant {
     int tpr;      // threads per row
     int vecs;     // vectors of 16 bytes that they hold (0: any number, read twice)
-    RowsKernel aligned, shifted;
+    RowsKernel plain, any;
 };
 
 template <typename T, int TPR, int NV>
 RowsVariant rows_variant() {
-    return {TPR, TPR * NV, rows_kernel<T, TPR, NV, false>, rows_kernel<T, TPR, NV, true>};
+    return {TPR, TPR * NV, rows_kernel<T, TPR, NV, true>, rows_kernel<T, TPR, NV, false>};
 }
 
-// By row length, four vectors a thread at most: 64 KB of loads in flight on an SM full of threads.
+// By row length.  With much to read four vectors a thread, which share the row's statistics (16384 rows of
+// 2048 f16: 15.8 us, with two vectors a thread 18.8); with less more threads a row, which finish sooner
+// (2000 rows of 2048 bf16: 4.5 us, with four vectors 6.1; 300 of 4096: 2.7 and 3.5).
+constexpr long long kManyVectors = 1LL << 20;
+
 template <typename T>
-const RowsVariant& rows_for(int vecs) {
-    static const RowsVariant k[] = {rows_variant<T, 32, 1>(),  rows_variant<T, 32, 2>(),  rows_variant<T, 32, 4>(),
-                                    rows_variant<T, 128, 2>(), rows_variant<T, 128, 4>(), rows_variant<T, 256, 4>(),
-                                    rows_variant<T, 512, 4>(), rows_variant<T, 1024, 4>()};
+const RowsVariant& rows_for(int vecs, bool many) {
+    static const RowsVariant most[] = {rows_variant<T, 32, 1>(),  rows_variant<T, 32, 2>(),  rows_variant<T, 32, 4>(),
+                                       rows_variant<T, 64, 4>(),  rows_variant<T, 128, 4>(), rows_variant<T, 256, 4>(),
+                                       rows_variant<T, 512, 4>(), rows_variant<T, 1024, 4>()};
+    static const RowsVariant soon[] = {rows_variant<T, 32, 1>(),  rows_variant<T, 64, 1>(),  rows_variant<T, 128, 1>(),
+                                       rows_variant<T, 128, 2>(), rows_variant<T, 256, 2>(), rows_variant<T, 512, 2>()};
     static const RowsVariant any = rows_variant<T, 512, 0>();
-    for (const RowsVariant& v : k)
+    if (!many)
+        for (const RowsVariant& v : soon)
+            if (vecs <= v.vecs) return v;
+    for (const RowsVariant& v : most)
         if (vecs <= v.vecs) return v;
     return any;
 }
@@ -170,10 +179,15 @@ const RowsVariant& rows_for(int vecs) {
 int run_rows(ptq8_ops* o, const ptq8_rows_args& a, cudaStream_t st) {
     const RowsParams p{a.x, a.codes, a.scale, a.rows, static_cast<size_t>(a.ldx), static_cast<size_t>(a.ldc), a.x_rows, a.n_rows, a.width};
     const int size = static_cast<int>(type_size(a.x_type)), vecs = (a.width + 16 / size - 1) / (16 / size);
-    const RowsVariant& v = a.x_type == PTQ8_F32 ? rows_for<float>(vecs) : a.x_type == PTQ8_F16 ? rows_for<__half>(vecs) : rows_for<__nv_bfloat16>(vecs);
-    const bool aligned = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && (a.x_rows <= 1 || a.ldx * size % 16 == 0);
-    const int block = std::max(256, v.tpr), per = block / v.tpr;
-    const cudaError_t e = launch(aligned ? v.aligned : v.shifted, dim3(static_cast<unsigned>((a.n_rows + per - 1) / per)), dim3(block), 0, 1, st, p);
+    const bool many = vecs * a.n_rows >= kManyVectors;
+    const RowsVariant& v = a.x_type == PTQ8_F32   ? rows_for<float>(vecs, many)
+                           : a.x_type == PTQ8_F16 ? rows_for<__half>(vecs, many)
+                                                  : rows_for<__nv_bfloat16>(vecs, many);
+    const int lanes = 16 / size;   // elements of a vector
+    const bool plain = a.width % lanes == 0 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && (a.x_rows <= 1 || a.ldx % lanes == 0) &&
+                       reinterpret_cast<uintptr_t>(a.codes) % lanes == 0 && (a.n_rows <= 1 || a.ldc % lanes == 0);
+    const int block = std::max(128, v.tpr), per = block / v.tpr;
+    const cudaError_t e = launch(plain ? v.plain : v.any, dim3(static_cast<unsigned>((a.n_rows + per - 1) / per)), dim3(block), 0, 1, st, p);
     return e == cudaSuccess ? PTQ8_OK : cuda_fail(o, "quantize_rows", e);
 }
 

@@ -18,15 +18,7 @@ struct RowsParams {
     int width;
 };
 
-// Exact code of y for the 32-bit scale s: round_half_away(y / s).  double(y) / double(s) never
-// rounds onto a half-integer that it is not: the quotient of two 24-bit numbers differs from
-// k + 1/2 by more than 2^-33 relative, or not at all.
-__device__ __forceinline__ int row_code_exact(float y, float s) {
-    const double v = static_cast<double>(y) / static_cast<double>(s);
-    return static_cast<int>(v >= 0.0 ? floor(v + 0.5) : ceil(v - 0.5));
-}
-
-// How one 16-byte vector of T is read: its largest magnitude as a bit pattern (NaN above infinity
+// How one 16-byte vector of T is read: its largest magnitude as a 32-bit pattern (NaN above infinity
 // above every number, so a maximum of patterns loses neither), and its values.
 template <typename T>
 struct Vec;
@@ -42,7 +34,10 @@ struct Vec<float> {
 template <>
 struct Vec<__nv_bfloat16> {
     static constexpr int V = 8;
-    static __device__ __forceinline__ uint32_t join(uint32_t m, uint32_t w) { return __vmaxu2(m, w & 0x7FFF7FFFu); }
+    static __device__ __forceinline__ uint32_t join(uint32_t m, uint32_t w) {
+        const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&m), __habs2(*reinterpret_cast<__nv_bfloat162*>(&w)));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
     static __device__ __forceinline__ uint32_t top(uint32_t m) { return max(m & 0xFFFFu, m >> 16) << 16; }
     static __device__ __forceinline__ void values(const uint4& v, float (&f)[8]) {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -56,7 +51,10 @@ struct Vec<__nv_bfloat16> {
 template <>
 struct Vec<__half> {
     static constexpr int V = 8;
-    static __device__ __forceinline__ uint32_t join(uint32_t m, uint32_t w) { return __vmaxu2(m, w & 0x7FFF7FFFu); }
+    static __device__ __forceinline__ uint32_t join(uint32_t m, uint32_t w) {
+        const __half2 r = __hmax2_nan(*reinterpret_cast<__half2*>(&m), __habs2(*reinterpret_cast<__half2*>(&w)));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
     static __device__ __forceinline__ uint32_t top(uint32_t m) {
         return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(max(m & 0xFFFFu, m >> 16)))));
     }
@@ -79,7 +77,7 @@ __device__ __forceinline__ uint4 load16(const void* p) {
 
 // The first n (>= 1) elements of a vector one by one; the others are zero (code 0, no part in the maximum).
 template <typename T>
-__device__ __forceinline__ uint4 load_part(const T* p, int n) {
+__device__ __noinline__ uint4 load_part(const T* p, int n) {
     uint4 v = make_uint4(0, 0, 0, 0);
     uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
@@ -118,46 +116,61 @@ __device__ __forceinline__ uint4 load_shifted(const T* p, const char* lo, const 
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Codes of one vector.  Multipliers that bracket 1/s, each in one FMA with 1.5 * 2^23 added: the sum
-// lies in [2^23, 2^24) where floats are 1 apart, so it is rounded to the nearest integer and its low
-// byte is the code (|y / s| <= 127 (1 + 2^-23): s is the row's own).  Where both agree, every number
-// between y * inv_lo and y * inv_hi rounds to that integer, and so does the exact quotient, which lies
-// strictly inside; where they do not, a half-integer lies between them and the exact form decides.
+// Codes of one vector: round_half_away(f / s), the exact quotient.  Multipliers that bracket 1/s, each in
+// one FMA with 1.5 * 2^23 added: the sum lies in [2^23, 2^24) where floats are 1 apart, so it is rounded to
+// the nearest integer and its low byte is the code (|f / s| <= 127 (1 + 2^-23): s is the row's own).  Where
+// both agree, every number between f * inv_lo and f * inv_hi rounds to that integer, and so does the exact
+// quotient, which lies strictly inside.  Where they do not (`flag`), a half-integer t lies between them, and
+// the sign of f - t s decides: one FMA, whose rounding keeps the sign of the exact value.
+// Codes of a vector that cannot be stored as a word: n bytes of c, one by one.
+__device__ __noinline__ void store_bytes(int8_t* out, uint2 c, int n) {
+    for (int i = 0; i < n; ++i) out[i] = static_cast<int8_t>((i < 4 ? c.x : c.y) >> (8 * (i & 3)));
+}
+
+constexpr float kRowMagic = 12582912.0f;
+
 template <int V>
-__device__ __forceinline__ void codes_of(const float (&f)[V], float inv_lo, float inv_hi, float s, uint32_t (&out)[V / 4]) {
-    constexpr float kMagic = 12582912.0f;
-    const float2 lo = make_float2(inv_lo, inv_lo), hi = make_float2(inv_hi, inv_hi), mg = make_float2(kMagic, kMagic);
-    uint32_t m[V], flag = 0;
-#pragma unroll
-    for (int i = 0; i < V; i += 2) {
-        const float2 y = make_float2(f[i], f[i + 1]);
-        const float2 a = __ffma2_rn(y, lo, mg), b = __ffma2_rn(y, hi, mg);
-        flag |= (__float_as_uint(a.x) ^ __float_as_uint(b.x)) | (__float_as_uint(a.y) ^ __float_as_uint(b.y));
-        m[i] = __float_as_uint(a.x);
-        m[i + 1] = __float_as_uint(a.y);
-    }
-    if (flag) {
-#pragma unroll 1
-        for (int i = 0; i < V; ++i) {
-            float y = f[0];
-#pragma unroll
-            for (int j = 1; j < V; ++j) y = i == j ? f[j] : y;
-            const uint32_t c = static_cast<uint32_t>(row_code_exact(y, s));
-#pragma unroll
-            for (int j = 0; j < V; ++j) m[j] = i == j ? c : m[j];
-        }
-    }
+__device__ __forceinline__ void pack_codes(const uint32_t (&m)[V], uint32_t (&out)[V / 4]) {
 #pragma unroll
     for (int k = 0; k < V / 4; ++k)
         out[k] = __byte_perm(__byte_perm(m[4 * k], m[4 * k + 1], 0x0040), __byte_perm(m[4 * k + 2], m[4 * k + 3], 0x0040), 0x5410);
 }
 
+template <int V>
+__device__ __forceinline__ void codes_of(const float (&f)[V], float inv_lo, float inv_hi, uint32_t (&out)[V / 4], uint32_t& flag) {
+    const float2 lo = make_float2(inv_lo, inv_lo), hi = make_float2(inv_hi, inv_hi), mg = make_float2(kRowMagic, kRowMagic);
+    uint32_t m[V];
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+        const float2 y = make_float2(f[i], f[i + 1]);
+        const float2 a = __ffma2_rn(y, lo, mg), b = __ffma2_rn(y, hi, mg);
+        flag |= __float_as_uint(a.x) ^ __float_as_uint(b.x);
+        flag |= __float_as_uint(a.y) ^ __float_as_uint(b.y);
+        m[i] = __float_as_uint(a.x);
+        m[i + 1] = __float_as_uint(a.y);
+    }
+    pack_codes<V>(m, out);
+}
+
+template <int V>
+__device__ __forceinline__ void codes_exact(const float (&f)[V], float inv_lo, float inv_hi, float s, uint32_t (&out)[V / 4]) {
+    uint32_t m[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const float a = __fmaf_rn(f[i], inv_lo, kRowMagic) - kRowMagic, b = __fmaf_rn(f[i], inv_hi, kRowMagic) - kRowMagic;
+        const float k = fminf(a, b), d = __fmaf_rn(-(k + 0.5f), s, f[i]);
+        m[i] = __float_as_uint((a == b ? a : (d > 0.0f || (d == 0.0f && f[i] > 0.0f)) ? k + 1.0f : k) + kRowMagic);
+    }
+    pack_codes<V>(m, out);
+}
+
 // One pass over the data: TPR threads per row hold it in registers, NV vectors of 16 bytes each,
 // between its maximum and its codes.  (NV 0, for rows longer than that: a loop that reads them twice.)
-// SHIFT: rows that do not start at multiples of 16 bytes.
-template <typename T, int TPR, int NV, bool SHIFT>
-__global__ void __launch_bounds__(TPR > 256 ? TPR : 256) rows_kernel(RowsParams p) {
-    constexpr int V = Vec<T>::V, kBlock = TPR > 256 ? TPR : 256, kWarps = TPR / 32;
+// PLAIN: rows of whole vectors that start at multiples of 16 bytes, codes that can be stored in words.
+// Instructions bound it, not memory, so that the common form has no other case in it.
+template <typename T, int TPR, int NV, bool PLAIN>
+__global__ void __launch_bounds__(TPR > 128 ? TPR : 128) rows_kernel(RowsParams p) {
+    constexpr int V = Vec<T>::V, kBlock = TPR > 128 ? TPR : 128, kWarps = TPR / 32, kHeld = NV ? NV : 1;
     __shared__ uint32_t part[kBlock / 32];
     griddep_launch();
     griddep_wait();
@@ -168,22 +181,28 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) rows_kernel(RowsParams 
     const bool read = src >= 0 && src < p.x_rows;
     const T* x = static_cast<const T*>(p.x) + static_cast<size_t>(read ? src : 0) * p.ldx;
     const char* lo = static_cast<const char*>(p.x);
-    const char* hi = SHIFT ? lo + (static_cast<size_t>(p.x_rows - 1) * p.ldx + p.width) * sizeof(T) : nullptr;
+    const char* hi = PLAIN ? nullptr : lo + (static_cast<size_t>(p.x_rows - 1) * p.ldx + p.width) * sizeof(T);
+    const int vecs = (p.width + V - 1) / V, readable = read ? vecs : 0;
     auto fetch = [&](int v) {
-        const int k = v * V;
-        if (!read || k >= p.width) return make_uint4(0, 0, 0, 0);
-        if (k + V > p.width) return load_part(x + k, p.width - k);
-        return SHIFT ? load_shifted(x + k, lo, hi) : load16(x + k);
+        uint4 q = make_uint4(0, 0, 0, 0);
+        if (v < readable) {
+            if (PLAIN)
+                q = load16(x + v * V);
+            else if ((v + 1) * V > p.width)
+                q = load_part(x + v * V, p.width - v * V);
+            else
+                q = load_shifted(x + v * V, lo, hi);
+        }
+        return q;
     };
-    uint4 d[NV ? NV : 1];
     uint32_t top = 0;
     auto join = [&](const uint4& q) { top = Vec<T>::join(Vec<T>::join(Vec<T>::join(Vec<T>::join(top, q.x), q.y), q.z), q.w); };
-    const int vecs = (p.width + V - 1) / V;
+    uint4 d[kHeld];
     if (NV) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) d[i] = fetch(lane + i * TPR);
+        for (int i = 0; i < kHeld; ++i) d[i] = fetch(lane + i * TPR);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) join(d[i]);
+        for (int i = 0; i < kHeld; ++i) join(d[i]);
     } else {
         for (int v = lane; v < vecs; v += TPR) join(fetch(v));
     }
@@ -207,28 +226,27 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) rows_kernel(RowsParams 
     }
     if (lane == 0) p.scale[r] = read ? s : 0.0f;
     int8_t* out = p.codes + r * p.ldc;
-    const bool whole = (reinterpret_cast<uintptr_t>(out) & (V - 1)) == 0;
+    const bool words = PLAIN || (reinterpret_cast<uintptr_t>(out) & (V - 1)) == 0;
     auto emit = [&](int v, const uint4& q) {
-        const int k = v * V;
-        if (k >= p.width) return;
+        if (v >= vecs) return;
         float f[V];
-        uint32_t c[V / 4] = {};
+        uint32_t c[V / 4], flag = 0;
         Vec<T>::values(q, f);
-        if (finite) codes_of<V>(f, inv_lo, inv_hi, s, c);
-        if (whole && k + V <= p.width) {
+        codes_of<V>(f, inv_lo, inv_hi, c, flag);
+        if (flag) codes_exact<V>(f, inv_lo, inv_hi, s, c);
+        if (!finite) c[0] = c[V / 4 - 1] = 0;
+        if (PLAIN || (words && (v + 1) * V <= p.width)) {
             if (V == 8)
-                *reinterpret_cast<uint2*>(out + k) = make_uint2(c[0], c[V / 4 - 1]);
+                *reinterpret_cast<uint2*>(out + v * V) = make_uint2(c[0], c[V / 4 - 1]);
             else
-                *reinterpret_cast<uint32_t*>(out + k) = c[0];
+                *reinterpret_cast<uint32_t*>(out + v * V) = c[0];
         } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (k + i < p.width) out[k + i] = static_cast<int8_t>(c[i / 4] >> (8 * (i & 3)));
+            store_bytes(out + v * V, make_uint2(c[0], c[V / 4 - 1]), min(V, p.width - v * V));
         }
     };
     if (NV) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) emit(lane + i * TPR, d[i]);
+        for (int i = 0; i < kHeld; ++i) emit(lane + i * TPR, d[i]);
     } else {
         for (int v = lane; v < vecs; v += TPR) emit(v, fetch(v));
     }

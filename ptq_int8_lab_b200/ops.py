@@ -36,32 +36,31 @@ except AttributeError:   # a torch without CUDA
         return torch.cuda.current_stream(device).cuda_stream
 
 
-def _matrix(name: str, t: torch.Tensor, dtypes, device: int) -> Tuple[int, int, int]:
-    """(rows, columns, row pitch) of a 2-D tensor with consecutive columns."""
+# Calls check their tensors with inline conditions; where one fails, these say what is wrong (or return:
+# a single column has no pitch to be consecutive).
+
+def _check_matrix(name: str, t: torch.Tensor, dtypes, dims: int, device: int):
+    if t.dim() != dims:
+        raise Ptq8Error(f"{name}: shape {tuple(t.shape)}, {'two dimensions are' if dims == 2 else '[groups, channels, in] is'} wanted")
     if t.dtype not in dtypes:
         raise Ptq8Error(f"{name}: dtype {t.dtype}")
     if t.get_device() != device:
         raise Ptq8Error(f"{name}: on {t.device}, not on cuda:{device}")
-    if t.dim() != 2:
-        raise Ptq8Error(f"{name}: shape {tuple(t.shape)}, two dimensions are wanted")
-    rows, cols = t.shape
-    pitch, step = t.stride()
-    if step != 1 and cols > 1:
-        raise Ptq8Error(f"{name}: columns {step} elements apart, not consecutive")
-    return rows, cols, (pitch if rows > 1 else max(cols, 1))
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise Ptq8Error(f"{name}: columns {t.stride(-1)} elements apart, not consecutive")
 
 
-def _vector(name: str, t: torch.Tensor, dtype, shape, device: int) -> int:
-    if t.dtype != dtype or t.shape != shape:
-        raise Ptq8Error(f"{name}: {t.dtype} {tuple(t.shape)}, {dtype} {tuple(shape)} is wanted")
+def _check_vector(name: str, t: torch.Tensor, dtype, values: int, device: int):
+    if t.dtype != dtype or t.numel() != values:
+        raise Ptq8Error(f"{name}: {t.dtype} {tuple(t.shape)}, {values} values of {dtype} are wanted")
     if t.get_device() != device:
         raise Ptq8Error(f"{name}: on {t.device}, not on cuda:{device}")
     if not t.is_contiguous():
         raise Ptq8Error(f"{name}: not contiguous")
-    return t.data_ptr()
 
 
-_F32, _I32, _I8, _BYTES = torch.float32, torch.int32, (torch.int8,), (torch.uint8, torch.int8)
+_F32, _I32, _INT8 = torch.float32, torch.int32, torch.int8
+_CODES = {8: (torch.int8,), 4: (torch.uint8, torch.int8)}
 
 
 class Int8Ops:
@@ -71,6 +70,7 @@ class Int8Ops:
         self._h = None
         err = ctypes.create_string_buffer(1024)
         self._lib = lib()
+        self._linear, self._grouped = self._lib.ptq8_linear, self._lib.ptq8_linear_grouped
         self._h = self._lib.ptq8_ops_create(device, err, len(err))
         if not self._h:
             raise Ptq8Error(err.value.decode(errors="replace"), 3)
@@ -96,73 +96,111 @@ class Int8Ops:
 
         rows (int32 [R]): output row r is token rows[r]; an index outside [0, T) gives codes 0
         and scale 0.  Codes made here have rows that start at multiples of 16 bytes."""
-        n, width, ldx = _matrix("x", x, _TYPES, self.device)
+        d = self.device
+        x_type = _TYPES.get(x.dtype)
+        if x.dim() != 2:
+            _check_matrix("x", x, _TYPES, 2, d)
+        n, width = x.shape
+        ldx, step = x.stride()
+        if x_type is None or x.get_device() != d or step != 1:
+            _check_matrix("x", x, _TYPES, 2, d)
         at, r = 0, n
         if rows is not None:
             r = rows.numel()
-            at = _vector("rows", rows, _I32, (r,), self.device)
+            if rows.dtype is not _I32 or not rows.is_contiguous() or rows.get_device() != d:
+                _check_vector("rows", rows, _I32, r, d)
+            at = rows.data_ptr()
+        stream = self._stream(stream, out is not None)
         if out is None:
-            stream = self._stream(stream, False)
-            codes = torch.empty((r, (width + 15) // 16 * 16), dtype=torch.int8, device=x.device)[:, :width]
+            codes = torch.empty((r, (width + 15) // 16 * 16), dtype=_INT8, device=x.device)[:, :width]
             scale = torch.empty(r, dtype=_F32, device=x.device)
         else:
-            stream = self._stream(stream, True)
             codes, scale = out
-        cr, cw, ldc = _matrix("codes", codes, _I8, self.device)
-        if cr != r or cw != width:
-            raise Ptq8Error(f"codes: shape {(cr, cw)}, {(r, width)} is wanted")
-        if r == 0:
-            return codes, scale
-        _ROWS.pack_into(self._rows_args, 0, x.data_ptr(), ldx, n, at, r, codes.data_ptr(), ldc,
-                        _vector("scale", scale, _F32, (r,), self.device), width, _TYPES[x.dtype])
-        self._check(self._lib.ptq8_quantize_rows(self._h, self._rows_args, stream))
+            if codes.dim() != 2:
+                _check_matrix("codes", codes, (_INT8,), 2, d)
+            c_rows, c_cols = codes.shape
+            if c_rows != r or c_cols != width:
+                raise Ptq8Error(f"codes: shape {tuple(codes.shape)}, {(r, width)} is wanted")
+            if scale.dtype is not _F32 or scale.numel() != r or not scale.is_contiguous() or scale.get_device() != d:
+                _check_vector("scale", scale, _F32, r, d)
+        ldc, step = codes.stride()
+        if codes.dtype is not _INT8 or codes.get_device() != d or step != 1:
+            _check_matrix("codes", codes, (_INT8,), 2, d)
+        if r:
+            _ROWS.pack_into(self._rows_args, 0, x.data_ptr(), ldx, n, at, r, codes.data_ptr(), ldc,
+                            scale.data_ptr(), width, x_type)
+            rc = self._lib.ptq8_quantize_rows(self._h, self._rows_args, stream)
+            if rc:
+                self._check(rc)
         return codes, scale
 
     def _product(self, call, x, x_scale, offsets, w, w_scale, bias, bits, act, dtype, out, stream):
         d = self.device
-        rows, k, ldx = _matrix("x", x, _I8, d)
-        if bits != 8 and bits != 4:
+        codes = _CODES.get(bits)
+        if codes is None:
             raise Ptq8Error(f"bits {bits}: 8 or 4")
         if act != EPI_NONE and act != EPI_SWIGLU:
             raise Ptq8Error(f"act {act}: EPI_NONE or EPI_SWIGLU")
+        if x.dim() != 2:
+            _check_matrix("x", x, (_INT8,), 2, d)
+        rows, k = x.shape
+        ldx, step = x.stride()
+        if x.dtype is not _INT8 or x.get_device() != d or step != 1:
+            _check_matrix("x", x, (_INT8,), 2, d)
+        groups = gstride = at = 0
+        dims = 2 if offsets is None else 3
+        if w.dim() != dims:
+            _check_matrix("w", w, codes, dims, d)
         if offsets is None:
-            channels, wide, ldw = _matrix("w", w, _I8 if bits == 8 else _BYTES, d)
-            groups = gstride = at = 0
-            shape = (channels,)
+            channels, wide = w.shape
+            ldw, step = w.stride()
         else:
-            if w.dim() != 3:
-                raise Ptq8Error(f"w: shape {tuple(w.shape)}, [groups, channels, in] is wanted")
-            groups = w.shape[0]
+            groups, channels, wide = w.shape
+            gstride, ldw, step = w.stride()
             if groups == 0:
                 raise Ptq8Error("w: no groups")
-            gstride = w.stride(0)
-            channels, wide, ldw = _matrix("w", w[0], _I8 if bits == 8 else _BYTES, d)
-            if groups == 1:
-                gstride = ldw * channels
-            shape = (groups, channels)
-            at = _vector("offsets", offsets, _I32, (groups + 1,), d)
+            if offsets.dtype is not _I32 or offsets.numel() != groups + 1 or not offsets.is_contiguous() or offsets.get_device() != d:
+                _check_vector("offsets", offsets, _I32, groups + 1, d)
+            at = offsets.data_ptr()
+        if w.dtype not in codes or w.get_device() != d or step != 1:
+            _check_matrix("w", w, codes, dims, d)
         if wide != (k if bits == 8 else (k + 1) // 2):
             raise Ptq8Error(f"w: rows of {wide} bytes for {k} input features at {bits} bits")
+        if x_scale.dtype is not _F32 or x_scale.numel() != rows or not x_scale.is_contiguous() or x_scale.get_device() != d:
+            _check_vector("x_scale", x_scale, _F32, rows, d)
+        values = groups * channels if groups else channels
+        if w_scale.dtype is not _F32 or w_scale.numel() != values or not w_scale.is_contiguous() or w_scale.get_device() != d:
+            _check_vector("w_scale", w_scale, _F32, values, d)
+        b = 0
+        if bias is not None:
+            if bias.dtype is not _F32 or bias.numel() != values or not bias.is_contiguous() or bias.get_device() != d:
+                _check_vector("bias", bias, _F32, values, d)
+            b = bias.data_ptr()
         n = channels
         if act == EPI_SWIGLU:
             if channels % 2:
                 raise Ptq8Error(f"w: {channels} channels do not split into gate and up")
             n = channels // 2
+        stream = self._stream(stream, out is not None)
         if out is None:
-            stream = self._stream(stream, False)
             if dtype not in _TYPES:
                 raise Ptq8Error(f"dtype {dtype}: f32, f16 or bf16")
             out = torch.empty((rows, n), dtype=dtype, device=x.device)
-        else:
-            stream = self._stream(stream, True)
-        yr, yc, ldy = _matrix("out", out, _TYPES, d)
-        if yr != rows or yc != n:
-            raise Ptq8Error(f"out: shape {(yr, yc)}, {(rows, n)} is wanted")
-        _LINEAR.pack_into(self._linear_args, 0, x.data_ptr(), ldx, _vector("x_scale", x_scale, _F32, (rows,), d),
-                          w.data_ptr(), ldw, gstride, _vector("w_scale", w_scale, _F32, shape, d),
-                          0 if bias is None else _vector("bias", bias, _F32, shape, d), out.data_ptr(), ldy, at, rows,
-                          k, n, groups, bits, act, _TYPES[out.dtype])
-        self._check(call(self._h, self._linear_args, stream))
+        elif out.dim() != 2:
+            _check_matrix("out", out, _TYPES, 2, d)
+        y_type = _TYPES.get(out.dtype)
+        y_rows, y_cols = out.shape
+        ldy, step = out.stride()
+        if y_type is None or step != 1 or out.get_device() != d:
+            _check_matrix("out", out, _TYPES, 2, d)
+        if y_rows != rows or y_cols != n:
+            raise Ptq8Error(f"out: shape {tuple(out.shape)}, {(rows, n)} is wanted")
+        _LINEAR.pack_into(self._linear_args, 0, x.data_ptr(), ldx, x_scale.data_ptr(), w.data_ptr(), ldw, gstride,
+                          w_scale.data_ptr(), b, out.data_ptr(), ldy, at, rows, k, n, groups, bits, act,
+                          y_type)
+        rc = call(self._h, self._linear_args, stream)
+        if rc:
+            self._check(rc)
         return out
 
     def linear(self, x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
@@ -171,7 +209,7 @@ class Int8Ops:
         """y [T, out] of codes x [T, in] (scale x_scale [T]) and weight codes w [channels, in] (bits 8) or
         [channels, (in + 1) // 2] (bits 4: code k in the low half of byte k // 2 for even k), scale w_scale
         [channels].  act EPI_SWIGLU: channels = 2 * out, gate then up.  dtype: of y where out is not given."""
-        return self._product(self._lib.ptq8_linear, x, x_scale, None, w, w_scale, bias, bits, act, dtype, out, stream)
+        return self._product(self._linear, x, x_scale, None, w, w_scale, bias, bits, act, dtype, out, stream)
 
     def linear_grouped(self, x: torch.Tensor, x_scale: torch.Tensor, offsets: torch.Tensor, w: torch.Tensor,
                        w_scale: torch.Tensor, bias: Optional[torch.Tensor] = None, bits: int = 8,
@@ -181,7 +219,7 @@ class Int8Ops:
         w[g] [channels, in], w_scale[g] and bias[g].  Rows of no group are not written."""
         if offsets is None:
             raise Ptq8Error("offsets: None")
-        return self._product(self._lib.ptq8_linear_grouped, x, x_scale, offsets, w, w_scale, bias, bits, act, dtype,
+        return self._product(self._grouped, x, x_scale, offsets, w, w_scale, bias, bits, act, dtype,
                              out, stream)
 
     def check_device_error(self, stream=None):
