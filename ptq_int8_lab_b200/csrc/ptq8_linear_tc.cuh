@@ -11,7 +11,7 @@
 //         of 1/S of the tokens to the CTA that finishes them.  Integer sums: the order of
 //         arrival changes nothing.
 //   GATED: two accumulators per tile, gate and up channels, joined in the epilogue.
-//   W4: weights arrive packed; eight warps widen them as 16 times the code (the nibble moved to
+//   W4: weights arrive packed; eight or sixteen warps widen them as 16 times the code (the nibble moved to
 //       its byte's high half: no sign extension; the channel's scale carries the exact factor
 //       1/16) and write them to TMEM, from where the MMA takes its M operand.  A thread owns
 //       a channel, which is a TMEM lane.  Through shared memory the same took twice the time:
@@ -28,13 +28,13 @@ namespace ptq8 {
 enum : int { ERR_WAIT_UNPACK = 5, ERR_WAIT_PARTIAL = 6 };
 
 constexpr int kMaxLinStages = 12;
+constexpr long long kLandCycles = 200000;   // about 0.1 ms: far more than a store to a peer takes
 constexpr int kBand = 8;   // token tiles per band of the tile order: a band's operands stay in L2
 
 struct TcParams {
     LinearParams l;
     int kblocks;       // blocks of 128 input features
     int stages;
-    int a_bufs;        // W4: operand tiles in TMEM, behind the accumulators
     int split;         // S
     int list_bytes;    // shared memory of the groups' tile list
     int ctiles;        // channel tiles
@@ -54,11 +54,22 @@ struct TcShape {
     static constexpr int kStage = kW + kX;
     static constexpr int kEpi = TN >= 128 ? 8 : 4;          // epilogue warps
     static constexpr int kCW = TN / (kEpi / 4);            // accumulator columns of one warp
-    static constexpr int kUnpack = W4 ? 8 : 0;             // unpacking warps
-    static constexpr int kThreads = 128 + 32 * (kEpi + kUnpack);
     static constexpr int kCols = H * TN;                   // accumulator columns of a tile
     static constexpr int kACols = 32 * H;                  // W4: columns of an operand tile
-    static constexpr int kPerSm = TN <= (W4 && GATED ? 32 : 64) ? 2 : 1;   // CTAs that share an SM
+    // CTAs that share an SM (the next launch's, too: its set-up then overlaps this one's end)
+    static constexpr int kPerSm = TN <= (W4 && GATED ? 32 : 64) ? 2 : 1;
+    static constexpr int kColumns = 512 / kPerSm;          // of TMEM
+    static constexpr int kUnpack = !W4 ? 0 : kPerSm == 2 ? 8 : 16;   // unpacking warps
+    static constexpr int kTurns = kUnpack / (4 * H);       // sets of them that take turns at the blocks
+    // Two accumulators where TMEM holds them.  With int4 weights the operand tiles have half of it (what two
+    // accumulators leave, where CTAs share an SM): they hide the way from the MMAs' release of a tile to its
+    // next use.  4096 x 4096 x 4096 gated: 99 us with one accumulator and four operand tiles, 150 us with
+    // tiles of 96 tokens, two and two.
+    static constexpr int kAccBufs = 2 * kCols > (W4 ? (kPerSm == 2 ? kColumns - kACols : 256) : kColumns) ? 1 : 2;
+    static constexpr int kABufs = !W4 ? 0 : kPerSm == 2 ? (kColumns - 2 * kCols) / kACols / kTurns * kTurns : 256 / kACols;
+    static constexpr int kACol0 = kPerSm == 2 ? 2 * kCols : 256;     // W4: first column of the operand tiles
+    static constexpr int kThreads = 128 + 32 * (kEpi + kUnpack);
+    static_assert(!W4 || (kABufs >= 2 && kABufs <= 8), "operand tiles");
 };
 
 // ---- cluster-wide pieces
@@ -73,9 +84,19 @@ __device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// Brings a box of the weights into L2.  Harmless where an earlier kernel of the stream still writes it: L2 is
+// where both meet, and the copies that read it come after the wait for that kernel.
+__device__ __forceinline__ void prefetch_3d(const CUtensorMap* m, int c0, int c1, int c2) {
+    asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(reinterpret_cast<uint64_t>(m)),
+                 "r"(c0), "r"(c1), "r"(c2)
+                 : "memory");
+}
+
 // Arrive on a barrier of any CTA of the cluster (address from mapa, or of the own CTA) without release:
 // what it orders are tcgen05 accesses, completed by tcgen05.wait and ordered by tcgen05.fence, and loads
 // whose values have been used.  (With .release.cluster the unpackers took over 1000 cycles a block.)
@@ -328,7 +349,7 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
     using Sh = TcShape<CG, TN, W4, GATED>;
     constexpr int H = Sh::H;
     extern __shared__ uint8_t dyn[];
-    __shared__ __align__(8) uint64_t bars[2 * kMaxLinStages + 10];
+    __shared__ __align__(8) uint64_t bars[2 * kMaxLinStages + 14];
     __shared__ uint32_t tmem_slot;
     __shared__ __align__(16) float sxs_all[Sh::kEpi][Sh::kCW];   // token scales, each epilogue warp its own columns
 
@@ -345,7 +366,7 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
     const uint32_t recv = after + p.list_bytes;
     const uint32_t b0 = smem_u32(bars);
     const uint32_t full = b0, empty = full + 8 * p.stages;
-    const uint32_t afull = b0 + 8 * 2 * kMaxLinStages, accfull = afull + 32, accempty = accfull + 16,
+    const uint32_t afull = b0 + 8 * 2 * kMaxLinStages, accfull = afull + 64, accempty = accfull + 16,
                    partial = accempty + 16, drain = partial + 8;
 
     griddep_launch();
@@ -358,7 +379,7 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
             mbar_init(full + 8 * s, 1);
             mbar_init(empty + 8 * s, 1);
         }
-        for (int a = 0; a < 4; ++a) mbar_init(afull + 8 * a, 4 * H * CG);
+        for (int a = 0; a < 8; ++a) mbar_init(afull + 8 * a, 4 * H * CG);
         for (int a = 0; a < 2; ++a) {
             mbar_init(accfull + 8 * a, 1);
             mbar_init(accempty + 8 * a, Sh::kEpi * CG);
@@ -378,11 +399,23 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
             tmem_relinquish();
         }
     }
+    const bool listed = p.l.offsets != nullptr;
+    Tiles<TN> tiles(p.l, listed ? list : nullptr, p.ctiles);
+    const int per = CG == 2 ? 2 : S;
+    const int t0 = blockIdx.x / per, dt = gridDim.x / per;
+    const int kb0 = static_cast<int>(static_cast<long long>(p.kblocks) * (S > 1 ? rank : 0) / S);
+    const int kb1 = static_cast<int>(static_cast<long long>(p.kblocks) * (S > 1 ? rank + 1 : 1) / S);
+    Tile tile;
+    if (warp == 0 && !listed && tiles.get(t0, tile) && elect_one()) {
+        // while the kernel before this one drains: the weights of the first stages
+        const int c = (tile.ct * CG + static_cast<int>(CG == 2 ? rank : 0)) * 128;
+        for (int kb = kb0; kb < min(kb1, kb0 + p.stages); ++kb)
+            for (int h = 0; h < H; ++h) prefetch_3d(&map_w, kb * (W4 ? 64 : 128), h * p.l.n + c, 0);
+    }
     __syncwarp();
     tc_fence_before();
     if (clustered) cluster_sync();   // the peers' barriers exist
-    griddep_wait();                  // nothing above reads or writes global memory
-    const bool listed = p.l.offsets != nullptr;
+    griddep_wait();                  // nothing above reads or writes global memory (but for prefetches)
     if (listed && warp == 2) {   // first tile of each group
         int sum = 0;
         for (int g0 = 0; g0 < p.l.groups; g0 += 32) {
@@ -406,21 +439,17 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
     __syncwarp();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = tmem_slot, a_tiles = tmem + p.acc_bufs * Sh::kCols;
+    const uint32_t tmem = tmem_slot, a_tiles = tmem + Sh::kACol0;
 
-    Tiles<TN> tiles(p.l, listed ? list : nullptr, p.ctiles);
-    const int per = CG == 2 ? 2 : S;
-    const int t0 = blockIdx.x / per, dt = gridDim.x / per;
-    const int kb0 = static_cast<int>(static_cast<long long>(p.kblocks) * (S > 1 ? rank : 0) / S);
-    const int kb1 = static_cast<int>(static_cast<long long>(p.kblocks) * (S > 1 ? rank + 1 : 1) / S);
     const long long limit = p.wait_limit;
+    bool arrived = false, failed = false;
     auto give_up = [&](int code) {
+        failed = true;
         if (lane == 0) {
             *static_cast<volatile int*>(p.err) = code;
             __threadfence_system();
         }
     };
-    Tile tile;
 
     if (warp == 0) {
         // ---------------------------------------------------------------- producer
@@ -510,7 +539,7 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
                 const uint32_t st = desc0 + s * (Sh::kStage >> 4);
                 mma_block<CG, H, W4>(d, TN, W4 ? a_tiles + ab * Sh::kACols : st, st + (Sh::kW >> 4), desc_hi, idesc, kb > kb0,
                                      empty + 8 * s);
-                if (W4 && ++ab == p.a_bufs) {
+                if (W4 && ++ab == Sh::kABufs) {
                     ab = 0;
                     aph ^= 1;
                 }
@@ -594,6 +623,9 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
                         }
                     }
                 }
+                __syncwarp();
+                cluster_arrive();   // nothing more goes to the peers
+                arrived = true;
                 if (!mbar_wait_warp(partial, 0, limit)) {
                     give_up(ERR_WAIT_PARTIAL);
                     break;
@@ -612,22 +644,23 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
         }
     } else if (W4 && warp >= 4 + Sh::kEpi) {
         // ---------------------------------------------------------------- unpackers
-        // Gated: the first four warps widen the gate tile, the others the up tile; otherwise the two
-        // sets of four take every other block.
+        // Sets of four warps: gated, every other one works on the up tile; sets with the same tile take turns
+        // at the blocks.  A block takes a set over 700 cycles from end to end, the MMAs 250 to 600.
         const int quad = warp & 3, set = (warp - 4 - Sh::kEpi) >> 2, row = quad * 32 + lane;
+        const int half = GATED ? set & 1 : 0, first = GATED ? set >> 1 : set;
         const uint32_t afull_at = CG == 2 ? mapa(afull, 0) : afull;
-        const uint32_t lanes = a_tiles + (GATED ? set * 32 : 0) + (static_cast<uint32_t>(quad * 32) << 16);
-        const uint8_t* src = base_p + (GATED ? set * 8192 : 0) + row * 64;
+        const uint32_t lanes = a_tiles + half * 32 + (static_cast<uint32_t>(quad * 32) << 16);
+        const uint8_t* src = base_p + half * 8192 + row * 64;
         const int turn = (row >> 1) & 3;   // the 64-byte TMA swizzle of this row
         // This CTA's blocks, tile after tile.  The operand tile of block i is free when block i - a_bufs is
         // released: its stage's barrier (its next phase cannot end before block i itself is unpacked).
         const int total = listed ? list[p.l.groups] : static_cast<int>((p.l.rows + TN - 1) / TN) * p.ctiles;
         const int tiles_here = t0 >= total ? 0 : S > 1 ? 1 : (total - t0 + dt - 1) / dt;
         const long long blocks = static_cast<long long>(tiles_here) * (kb1 - kb0);
-        constexpr int step = GATED ? 1 : 2;
-        int s = GATED ? 0 : set, ab = s, old = s;   // a_bufs is even: block set + a_bufs is this set's too
+        constexpr int step = Sh::kTurns;
+        int s = first, ab = first, old = first;   // kABufs is a multiple of the turns: block first + kABufs is this set's too
         uint32_t ph = 0, oldph = 0;
-        for (long long i = GATED ? 0 : set; i < blocks; i += step) {
+        for (long long i = first; i < blocks; i += step) {
             if (!mbar_wait_warp(full + 8 * s, ph, limit)) {
                 give_up(ERR_WAIT_UNPACK);
                 break;
@@ -638,7 +671,7 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
 #pragma unroll
             for (int q = 0; q < 4; ++q)
                 widen(*reinterpret_cast<const uint4*>(src + s * Sh::kStage + ((q ^ turn) << 4)), o + 8 * q);
-            if (i >= p.a_bufs) {
+            if (i >= Sh::kABufs) {
                 if (!mbar_wait_warp(empty + 8 * old, oldph, limit)) {
                     give_up(ERR_WAIT_UNPACK);
                     break;
@@ -661,7 +694,7 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
                     mbar_arrive_cluster_relaxed(afull_at + 8 * ab);
             }
             ab += step;
-            if (ab >= p.a_bufs) ab -= p.a_bufs;
+            if (ab >= Sh::kABufs) ab -= Sh::kABufs;
             s += step;
             if (s >= p.stages) {
                 s -= p.stages;
@@ -670,11 +703,18 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
         }
     }
 
-    // No CTA of a cluster ends, and no TMEM is freed, while a peer may still reach it.
+    // No CTA of a cluster ends, and no TMEM is freed, while a peer may still reach it.  Partial sums sent to
+    // this CTA have all arrived (it waited for them; if that wait ran out, the pause lets them land).
     __syncwarp();
+    if (clustered && !arrived) cluster_arrive();
+    if (clustered) cluster_wait();
+    if (S > 1 && failed) {
+        const long long c0 = clock64();
+        while (clock64() - c0 < kLandCycles) {
+        }
+    }
     tc_fence_before();
     __syncthreads();
-    if (clustered) cluster_sync();
     if (warp == 2) {
         tc_fence_after();
         if constexpr (CG == 2)

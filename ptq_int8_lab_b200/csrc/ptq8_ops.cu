@@ -199,13 +199,13 @@ struct Variant {
     int cg, tn;            // CTAs per tile, tokens per tile
     bool w4, gated;
     TcKernel kernel;
-    int threads, stage, cols, a_cols, x_rows, per_sm;
+    int threads, stage, cols, acc_bufs, a_bufs, x_rows, per_sm;
 };
 
 template <int CG, int TN, bool W4, bool GATED>
 Variant variant() {
     using Sh = TcShape<CG, TN, W4, GATED>;
-    return {CG, TN, W4, GATED, linear_tc_kernel<CG, TN, W4, GATED>, Sh::kThreads, Sh::kStage, Sh::kCols, W4 ? Sh::kACols : 0, Sh::XR, Sh::kPerSm};
+    return {CG, TN, W4, GATED, linear_tc_kernel<CG, TN, W4, GATED>, Sh::kThreads, Sh::kStage, Sh::kCols, Sh::kAccBufs, Sh::kABufs, Sh::XR, Sh::kPerSm};
 }
 
 const Variant kVariants[] = {
@@ -283,19 +283,16 @@ int run_tc(ptq8_ops* o, const ptq8_linear_args& a, const LinearParams& l, cudaSt
     p.split = c.split;
     p.ctiles = (a.out_features + 128 * c.cg - 1) / (128 * c.cg);
     p.list_bytes = l.offsets ? ((l.groups + 1) * 4 + 127) / 128 * 128 : 0;
-    // Two accumulators where TMEM holds them; with int4 weights four operand tiles come first, which hide
-    // the way from the MMAs' release of a tile to its next use (4096 x 4096 x 4096 gated: 112 us, with
-    // tiles of 96 tokens, two accumulators and two operand tiles 150 us).
-    p.acc_bufs = c.split > 1 || 2 * v->cols + (w4 ? 128 : 0) > 512 ? 1 : 2;
-    p.a_bufs = w4 ? std::min(4, (512 / v->per_sm - p.acc_bufs * v->cols) / v->a_cols) & ~1 : 0;
+    p.acc_bufs = c.split > 1 ? 1 : v->acc_bufs;
     p.tmem_cols = 32;
-    while (static_cast<int>(p.tmem_cols) < v->cols * p.acc_bufs + v->a_cols * p.a_bufs) p.tmem_cols *= 2;
+    while (static_cast<int>(p.tmem_cols) < v->cols * p.acc_bufs) p.tmem_cols *= 2;
+    if (w4) p.tmem_cols = 512 / v->per_sm;
     p.wait_limit = o->wait_limit;
     p.err = o->error_dev;
     p.stall = o->stall;
     const int extra = 1024 + p.list_bytes + (c.split > 1 ? v->cols * 128 * 4 : 0);
     p.stages = std::min(kMaxLinStages, ((v->per_sm == 2 ? kSmemTwo : kSmemOne) - extra) / v->stage);
-    if (p.stages < std::max(2, p.a_bufs)) return fail(o, PTQ8_ERR_INVALID, "linear: %d stages", p.stages);
+    if (p.stages < std::max(2, v->a_bufs)) return fail(o, PTQ8_ERR_INVALID, "linear: %d stages", p.stages);
     const int smem = extra + p.stages * v->stage;
     // tiles at most: each group's last tile may be partly filled
     const long long row_tiles = l.offsets ? a.rows / c.tn + std::min<long long>(l.groups, a.rows) : (a.rows + c.tn - 1) / c.tn;
