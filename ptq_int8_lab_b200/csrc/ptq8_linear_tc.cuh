@@ -316,16 +316,18 @@ __device__ __forceinline__ void store_columns(T* y, size_t ldy, uint32_t acc, co
     }
 }
 
-// The finishing half of a split tile: the S partial sums of this CTA's tokens.
+// The finishing half of a split tile: the S partial sums of tokens t0 .. t0 + tokens - 1 of the tile, every
+// step-th of them from `part` on.
 template <typename T, int H>
 __device__ __forceinline__ void store_partials(T* y, size_t ldy, const int* recv, int S, int tokens, const float* xs,
-                                               const Channel<H>& ch, int lane_c, int t0, int valid) {
-    for (int t = 0; t < tokens && t0 + t < valid; ++t) {
+                                               const Channel<H>& ch, int lane_c, int t0, int mine, int part, int step) {
+    for (int t = part; t < mine; t += step) {
+        const float x = __ldg(xs + t0 + t);
         int a[2] = {0, 0};
         for (int s = 0; s < S; ++s)
 #pragma unroll
             for (int h = 0; h < H; ++h) a[h] += recv[((s * tokens + t) * H + h) * 128 + lane_c];
-        const float r = finish<H>(ch, xs[t0 + t], a[0], a[1]);
+        const float r = finish<H>(ch, x, a[0], a[1]);
         if (ch.ok) y[static_cast<size_t>(t0 + t) * ldy] = from_f32<T>(r);
     }
 }
@@ -631,14 +633,14 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
                     break;
                 }
                 const int* got = reinterpret_cast<const int*>(base_p + (recv - base));
-                {
-                    if (p.l.y_type == Y_F32)
-                        store_partials<float, H>(static_cast<float*>(p.l.y) + at, p.l.ldy, got, S, tokens, sxs, ch, lane_c, first, tile.valid);
-                    else if (p.l.y_type == Y_F16)
-                        store_partials<__half, H>(static_cast<__half*>(p.l.y) + at, p.l.ldy, got, S, tokens, sxs, ch, lane_c, first, tile.valid);
-                    else
-                        store_partials<__nv_bfloat16, H>(static_cast<__nv_bfloat16*>(p.l.y) + at, p.l.ldy, got, S, tokens, sxs, ch, lane_c, first, tile.valid);
-                }
+                const float* xs = p.l.xs + tile.row0;
+                constexpr int step = Sh::kEpi / 4;
+                if (p.l.y_type == Y_F32)
+                    store_partials<float, H>(static_cast<float*>(p.l.y) + at, p.l.ldy, got, S, tokens, xs, ch, lane_c, first, mine, part, step);
+                else if (p.l.y_type == Y_F16)
+                    store_partials<__half, H>(static_cast<__half*>(p.l.y) + at, p.l.ldy, got, S, tokens, xs, ch, lane_c, first, mine, part, step);
+                else
+                    store_partials<__nv_bfloat16, H>(static_cast<__nv_bfloat16*>(p.l.y) + at, p.l.ldy, got, S, tokens, xs, ch, lane_c, first, mine, part, step);
                 break;
             }
         }
