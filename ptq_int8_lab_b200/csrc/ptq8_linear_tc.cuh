@@ -33,7 +33,7 @@ constexpr int kBand = 8;   // token tiles per band of the tile order: a band's o
 
 struct TcParams {
     LinearParams l;
-    int kblocks;       // blocks of 128 input features
+    int kblocks;       // stages of input features: KD blocks of 128
     int stages;
     int split;         // S
     int list_bytes;    // shared memory of the groups' tile list
@@ -49,8 +49,12 @@ template <int CG, int TN, bool W4, bool GATED>
 struct TcShape {
     static constexpr int H = GATED ? 2 : 1;
     static constexpr int XR = TN / CG;                     // token rows loaded by one CTA
-    static constexpr int kW = H * 128 * (W4 ? 64 : 128);   // bytes of the weights' rows in a stage
-    static constexpr int kX = XR * 128;
+    // Blocks of 128 input features in a stage: two where one leaves the MMA warp's wait uncovered (4096 x 4096
+    // x 8192: 121 -> 99 us; elsewhere loads bound it, and two only make it wait for more).
+    static constexpr int KD = CG == 2 && TN == 128 && !W4 && !GATED ? 2 : 1;
+    static constexpr int kW = KD * H * 128 * (W4 ? 64 : 128);   // bytes of the weights' rows in a stage
+    static constexpr int kXBlock = XR * 128;
+    static constexpr int kX = KD * kXBlock;
     static constexpr int kStage = kW + kX;
     static constexpr int kEpi = TN >= 128 ? 8 : 4;          // epilogue warps
     static constexpr int kCW = TN / (kEpi / 4);            // accumulator columns of one warp
@@ -151,6 +155,10 @@ __device__ __forceinline__ void load_rows_3d(uint32_t dst, const CUtensorMap* m,
 #define PTQ8_S8(G) PTQ8_S4(G) PTQ8_S(G, "%1", "1024", "0", "p") PTQ8_S(G, "%1", "1026", "2", "1") PTQ8_S(G, "%1", "1028", "4", "1") PTQ8_S(G, "%1", "1030", "6", "1")
 #define PTQ8_T4(G) PTQ8_T(G, "%0", "0", "0", "p") PTQ8_T(G, "%0", "8", "2", "1") PTQ8_T(G, "%0", "16", "4", "1") PTQ8_T(G, "%0", "24", "6", "1")
 #define PTQ8_T8(G) PTQ8_T4(G) PTQ8_T(G, "%1", "32", "0", "p") PTQ8_T(G, "%1", "40", "2", "1") PTQ8_T(G, "%1", "48", "4", "1") PTQ8_T(G, "%1", "56", "6", "1")
+#define PTQ8_D(G, AO, BO)                                                                                   \
+    "add.u32 ta, %2, " AO ";\n\tadd.u32 tb, %8, " BO ";\n\tmov.b64 A, {ta, %4};\n\tmov.b64 B, {tb, %4};\n\t" \
+    PTQ8_MMA(G, "%0", "A", "1")
+#define PTQ8_D8(G) PTQ8_S4(G) PTQ8_D(G, "1024", "0") PTQ8_D(G, "1026", "2") PTQ8_D(G, "1028", "4") PTQ8_D(G, "1030", "6")
 #define PTQ8_COMMIT1 "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%7];\n\t}\n"
 #define PTQ8_COMMIT2                                                                                        \
     "mov.u16 m, 3;\n\t@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%7], m;\n\t}\n"
@@ -158,13 +166,18 @@ __device__ __forceinline__ void load_rows_3d(uint32_t dst, const CUtensorMap* m,
     asm volatile(                                                                                           \
         "{\n\t.reg .pred e, p;\n\t.reg .b64 A, B;\n\t.reg .b32 ta, tb;\n\t.reg .b16 m;\n\t"                  \
         "elect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %6, 0;\n\t" BODY ::"r"(d), "r"(d + step), "r"(a),     \
-        "r"(b), "r"(hi), "r"(idesc), "r"(acc), "r"(bar)                                                     \
+        "r"(b), "r"(hi), "r"(idesc), "r"(acc), "r"(bar), "r"(b2)                                            \
         : "memory")
 
 // a: TMEM address (TMEM_A) or low word of the descriptor; b: low word; hi: the descriptors' high word.
-template <int CG, int H, bool TMEM_A>
-__device__ __forceinline__ void mma_block(uint32_t d, uint32_t step, uint32_t a, uint32_t b, uint32_t hi, uint32_t idesc,
-                                          uint32_t acc, uint32_t bar) {
+// KD 2: two blocks, the second one's M operand 1024 units further and its tokens at b2.
+template <int CG, int H, bool TMEM_A, int KD>
+__device__ __forceinline__ void mma_block(uint32_t d, uint32_t step, uint32_t a, uint32_t b, uint32_t b2, uint32_t hi,
+                                          uint32_t idesc, uint32_t acc, uint32_t bar) {
+    static_assert(KD == 1 || (H == 1 && !TMEM_A), "two blocks of one int8 tile");
+    if constexpr (CG == 1 && KD == 2) PTQ8_BLOCK(PTQ8_D8("1") PTQ8_COMMIT1);
+    if constexpr (CG == 2 && KD == 2) PTQ8_BLOCK(PTQ8_D8("2") PTQ8_COMMIT2);
+    if constexpr (KD == 2) return;
     if constexpr (CG == 1 && H == 1 && !TMEM_A) PTQ8_BLOCK(PTQ8_S4("1") PTQ8_COMMIT1);
     if constexpr (CG == 1 && H == 2 && !TMEM_A) PTQ8_BLOCK(PTQ8_S8("1") PTQ8_COMMIT1);
     if constexpr (CG == 2 && H == 1 && !TMEM_A) PTQ8_BLOCK(PTQ8_S4("2") PTQ8_COMMIT2);
@@ -179,6 +192,8 @@ __device__ __forceinline__ void mma_block(uint32_t d, uint32_t step, uint32_t a,
 #undef PTQ8_T
 #undef PTQ8_S4
 #undef PTQ8_S8
+#undef PTQ8_D
+#undef PTQ8_D8
 #undef PTQ8_T4
 #undef PTQ8_T8
 #undef PTQ8_COMMIT1
@@ -411,7 +426,7 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
     if (warp == 0 && !listed && tiles.get(t0, tile) && elect_one()) {
         // while the kernel before this one drains: the weights of the first stages
         const int c = (tile.ct * CG + static_cast<int>(CG == 2 ? rank : 0)) * 128;
-        for (int kb = kb0; kb < min(kb1, kb0 + p.stages); ++kb)
+        for (int kb = kb0 * Sh::KD; kb < min(kb1, kb0 + p.stages) * Sh::KD; ++kb)
             for (int h = 0; h < H; ++h) prefetch_3d(&map_w, kb * (W4 ? 64 : 128), h * p.l.n + c, 0);
     }
     __syncwarp();
@@ -476,13 +491,18 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
                     if (leader || W4) mbar_expect_tx(full + 8 * s, (W4 ? 1 : CG) * Sh::kStage);
                     if (!(p.stall && blockIdx.x == 0 && issued == 0)) {
 #pragma unroll
-                        for (int h = 0; h < H; ++h) {
-                            if constexpr (W4)
-                                load_rows_3d<1>(wdst + h * 8192, &map_w, full_at + 8 * s, kb * 64, h * p.l.n + c, tile.group);
-                            else
-                                load_rows_3d<CG>(wdst + h * 16384, &map_w, full_at + 8 * s, kb * 128, h * p.l.n + c, tile.group);
+                        for (int b = 0; b < Sh::KD; ++b) {
+                            const int k = kb * Sh::KD + b;
+#pragma unroll
+                            for (int h = 0; h < H; ++h) {
+                                if constexpr (W4)
+                                    load_rows_3d<1>(wdst + h * 8192, &map_w, full_at + 8 * s, k * 64, h * p.l.n + c, tile.group);
+                                else
+                                    load_rows_3d<CG>(wdst + (b * H + h) * 16384, &map_w, full_at + 8 * s, k * 128, h * p.l.n + c,
+                                                     tile.group);
+                            }
+                            load_rows_2d<W4 ? 1 : CG>(xdst + b * Sh::kXBlock, &map_x, full_at + 8 * s, k * 128, r);
                         }
-                        load_rows_2d<W4 ? 1 : CG>(xdst, &map_x, full_at + 8 * s, kb * 128, r);
                     }
                 }
                 __syncwarp();
@@ -539,8 +559,8 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
                 }
                 tc_fence_after();
                 const uint32_t st = desc0 + s * (Sh::kStage >> 4);
-                mma_block<CG, H, W4>(d, TN, W4 ? a_tiles + ab * Sh::kACols : st, st + (Sh::kW >> 4), desc_hi, idesc, kb > kb0,
-                                     empty + 8 * s);
+                mma_block<CG, H, W4, Sh::KD>(d, TN, W4 ? a_tiles + ab * Sh::kACols : st, st + (Sh::kW >> 4),
+                                             st + ((Sh::kW + Sh::kXBlock) >> 4), desc_hi, idesc, kb > kb0, empty + 8 * s);
                 if (W4 && ++ab == Sh::kABufs) {
                     ab = 0;
                     aph ^= 1;

@@ -199,13 +199,13 @@ struct Variant {
     int cg, tn;            // CTAs per tile, tokens per tile
     bool w4, gated;
     TcKernel kernel;
-    int threads, stage, cols, acc_bufs, a_bufs, x_rows, per_sm;
+    int threads, stage, depth, cols, acc_bufs, a_bufs, x_rows, per_sm;
 };
 
 template <int CG, int TN, bool W4, bool GATED>
 Variant variant() {
     using Sh = TcShape<CG, TN, W4, GATED>;
-    return {CG, TN, W4, GATED, linear_tc_kernel<CG, TN, W4, GATED>, Sh::kThreads, Sh::kStage, Sh::kCols, Sh::kAccBufs, Sh::kABufs, Sh::XR, Sh::kPerSm};
+    return {CG, TN, W4, GATED, linear_tc_kernel<CG, TN, W4, GATED>, Sh::kThreads, Sh::kStage, 128 * Sh::KD, Sh::kCols, Sh::kAccBufs, Sh::kABufs, Sh::XR, Sh::kPerSm};
 }
 
 const Variant kVariants[] = {
@@ -255,7 +255,7 @@ int encode(ptq8_ops* o, CUtensorMap* m, int rank, const void* base, const cuuint
 
 int run_tc(ptq8_ops* o, const ptq8_linear_args& a, const LinearParams& l, cudaStream_t st) {
     const bool gated = a.epilogue == PTQ8_EPI_SWIGLU, w4 = a.w_bits == 4;
-    const Choice c = choose(o, a, l.groups, gated);
+    Choice c = choose(o, a, l.groups, gated);
     const Variant* v = nullptr;
     for (const Variant& k : kVariants)
         if (k.cg == c.cg && k.tn == c.tn && k.w4 == w4 && k.gated == gated) v = &k;
@@ -279,7 +279,8 @@ int run_tc(ptq8_ops* o, const ptq8_linear_args& a, const LinearParams& l, cudaSt
     }
     TcParams p{};
     p.l = l;
-    p.kblocks = (a.in_features + 127) / 128;
+    p.kblocks = (a.in_features + v->depth - 1) / v->depth;
+    while (c.split > p.kblocks) c.split /= 2;
     p.split = c.split;
     p.ctiles = (a.out_features + 128 * c.cg - 1) / (128 * c.cg);
     p.list_bytes = l.offsets ? ((l.groups + 1) * 4 + 127) / 128 * 128 : 0;
