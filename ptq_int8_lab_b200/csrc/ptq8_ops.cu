@@ -5,6 +5,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -220,19 +221,69 @@ const Variant kVariants[] = {
 // Dynamic shared memory of a CTA that shares its SM with another, or not.
 constexpr int kSmemTwo = 110 * 1024, kSmemOne = 222 * 1024;
 
-struct Choice {
-    int cg, tn, split;
-};
+// Shared memory beside the stages: their alignment, the tile list, a split's partial sums.
+int smem_beside(const Variant& v, int split, int list_bytes) { return 1024 + list_bytes + (split > 1 ? v.cols * 128 * 4 : 0); }
 
-Choice choose(const ptq8_ops* o, const ptq8_linear_args& a, int groups, bool gated) {
-    const long long m = (a.rows + groups - 1) / groups;   // rows that a group has on average
-    const int kblocks = (a.in_features + 127) / 128;
-    Choice c{1, m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128, 1};
-    const long long tiles = (a.out_features + 127) / 128 * std::max<long long>(groups > 1 ? std::min<long long>(groups, a.rows) : 1, (a.rows + c.tn - 1) / c.tn);
-    if (c.tn == 128 && tiles > 2 * o->sms) c = {2, gated ? 128 : 256, 1};
-    if (c.tn <= 32)
-        while (c.split < 8 && tiles * c.split * 2 <= 2 * o->sms && kblocks >= 4 * c.split) c.split *= 2;
-    return c;
+int stages_of(const Variant& v, int split, int list_bytes) {
+    return std::min(kMaxLinStages, ((v.per_sm == 2 ? kSmemTwo : kSmemOne) - smem_beside(v, split, list_bytes)) / v.stage);
+}
+
+int list_bytes_of(const ptq8_linear_args& a, bool listed) { return listed ? ((a.groups + 1) * 4 + 127) / 128 * 128 : 0; }
+
+// A launch's time in cycles, up to what all variants share.  Per stage a CTA takes the longest of its chain (the
+// MMAs and the wait before them) and, for the CTAs that share an SM, their MMAs, their loads at what an SM draws
+// from L2, and the widening of int4 weights.  Few tiles are worth a cluster each: a split pays for sending and
+// joining its sums, and clusters of 4 and 8 do not fill every GPC.  The constants are fitted to 7200 timings of
+// 508 calls (1 to 8192 tokens, 512 to 16384 features, 1 to 64 groups, both types, gated or not) under every
+// variant: the variant of the least estimate is 2.4 % slower than the fastest one on average, 35 % at most.
+float estimate(const ptq8_ops* o, const ptq8_linear_args& a, int groups, const Variant& v, int split) {
+    constexpr float kMma = 70, kMmaTmem = 84;        // least cycles of an MMA, M operand in shared memory or TMEM
+    constexpr float kWait = 145, kWaitTwo = 50;      // wait of the MMA warp per block (two blocks a stage)
+    constexpr float kLoad = 64;                      // bytes per cycle into an SM
+    constexpr float kWiden = 175;                    // int4: cycles of an SM per tile of 128 x 128 codes
+    constexpr float kColumn = 17.5f, kPush = 16;     // epilogue per accumulator column; sending one to a peer
+    constexpr float kSplit = 1400, kWave = 1900;     // a split tile's joining; a further wave of clusters
+    constexpr float kCluster = 570;                  // start of a launch with clusters
+    constexpr float kRagged = 0.56f;                 // part of a row tile that uneven groups waste each
+    constexpr float kFill4 = 0.92f, kFill8 = 0.82f;  // share of the SMs that clusters of 4 and of 8 can take
+    constexpr float kPacked = 0.75f;                 // CTAs per SM from which two come to share one
+    const float h = v.gated ? 2 : 1, rows = static_cast<float>(a.rows);
+    const float used = static_cast<float>(std::min<long long>(groups, a.rows)), mean = rows / used;
+    const float row_tiles = groups > 1 ? std::max(used, std::ceil(used * (mean / v.tn + kRagged))) : std::ceil(rows / v.tn);
+    const float tiles = row_tiles * static_cast<float>((a.out_features + 128 * v.cg - 1) / (128 * v.cg));
+    const float blocks = std::ceil(std::ceil(a.in_features / 128.0f) / split);
+    const float columns = std::min<float>(v.tn, std::ceil(std::ceil(mean) / (16 * v.cg)) * (16 * v.cg));
+    const float share = v.per_sm == 2 && tiles * v.cg * split > kPacked * o->sms ? 2 : 1;
+    const float mma = 4 * h * std::max(v.w4 ? kMmaTmem : kMma, columns / 2);
+    const float load = (h * 128 * (v.w4 ? 64 : 128) + v.x_rows * 128) / kLoad;
+    const float block = std::max({mma + (v.depth > 128 ? kWaitTwo : kWait), share * mma, share * load, share * (v.w4 ? kWiden * h : 0)});
+    const float fill = split == 8 ? kFill8 : split == 4 ? kFill4 : 1;
+    const float slots = std::max(1.0f, std::floor(std::floor(o->sms * v.per_sm * fill) / (v.cg * split)));
+    const float waves = std::ceil(tiles / slots);
+    float out = kColumn * columns * h / (v.tn >= 128 ? 2 : 1);
+    if (split > 1) out += kSplit + kPush * columns * h;
+    const float start = v.cg * split > 1 ? kCluster : 0;
+    if (split == 1 && waves > 1) return start + waves * std::max(blocks * block, out) + out;
+    return start + waves * (blocks * block + out + (split > 1 ? kWave : 0));
+}
+
+// The variant of the least estimate, among tiles not much longer than the rows of a group.
+const Variant* choose(const ptq8_ops* o, const ptq8_linear_args& a, bool listed, int& split) {
+    const int groups = listed ? a.groups : 1;
+    const bool gated = a.epilogue == PTQ8_EPI_SWIGLU, w4 = a.w_bits == 4;
+    const float mean = static_cast<float>(a.rows) / std::min<long long>(groups, a.rows);
+    const Variant* best = nullptr;
+    float least = 0;
+    for (const Variant& v : kVariants) {
+        if (v.w4 != w4 || v.gated != gated || (v.tn > 16 && v.tn >= 4 * v.cg * mean)) continue;
+        for (int s = 1; s <= (v.cg == 2 ? 1 : 8) && s * v.depth < a.in_features + v.depth; s *= 2) {
+            // the operand tile of a block is free when its stage is
+            if (stages_of(v, s, list_bytes_of(a, listed)) < std::max(2, v.a_bufs)) continue;
+            const float t = estimate(o, a, groups, v, s);
+            if (!best || t < least) best = &v, split = s, least = t;
+        }
+    }
+    return best;
 }
 
 bool aligned16(long long v) { return v % 16 == 0; }
@@ -255,11 +306,8 @@ int encode(ptq8_ops* o, CUtensorMap* m, int rank, const void* base, const cuuint
 
 int run_tc(ptq8_ops* o, const ptq8_linear_args& a, const LinearParams& l, cudaStream_t st) {
     const bool gated = a.epilogue == PTQ8_EPI_SWIGLU, w4 = a.w_bits == 4;
-    Choice c = choose(o, a, l.groups, gated);
-    const Variant* v = nullptr;
-    for (const Variant& k : kVariants)
-        if (k.cg == c.cg && k.tn == c.tn && k.w4 == w4 && k.gated == gated) v = &k;
-    if (!v) return fail(o, PTQ8_ERR_INVALID, "linear: no kernel for %d CTAs, %d tokens", c.cg, c.tn);
+    int split = 1;
+    const Variant* v = choose(o, a, l.offsets != nullptr, split);
     const long long channels = static_cast<long long>(a.out_features) * (gated ? 2 : 1);
     const int wide = w4 ? (a.in_features + 1) / 2 : a.in_features;
     CUtensorMap mx, mw;
@@ -280,27 +328,24 @@ int run_tc(ptq8_ops* o, const ptq8_linear_args& a, const LinearParams& l, cudaSt
     TcParams p{};
     p.l = l;
     p.kblocks = (a.in_features + v->depth - 1) / v->depth;
-    while (c.split > p.kblocks) c.split /= 2;
-    p.split = c.split;
-    p.ctiles = (a.out_features + 128 * c.cg - 1) / (128 * c.cg);
-    p.list_bytes = l.offsets ? ((l.groups + 1) * 4 + 127) / 128 * 128 : 0;
-    p.acc_bufs = c.split > 1 ? 1 : v->acc_bufs;
+    p.split = split;
+    p.ctiles = (a.out_features + 128 * v->cg - 1) / (128 * v->cg);
+    p.list_bytes = list_bytes_of(a, l.offsets != nullptr);
+    p.acc_bufs = split > 1 ? 1 : v->acc_bufs;
     p.tmem_cols = 32;
     while (static_cast<int>(p.tmem_cols) < v->cols * p.acc_bufs) p.tmem_cols *= 2;
     if (w4) p.tmem_cols = 512 / v->per_sm;
     p.wait_limit = o->wait_limit;
     p.err = o->error_dev;
     p.stall = o->stall;
-    const int extra = 1024 + p.list_bytes + (c.split > 1 ? v->cols * 128 * 4 : 0);
-    p.stages = std::min(kMaxLinStages, ((v->per_sm == 2 ? kSmemTwo : kSmemOne) - extra) / v->stage);
-    if (p.stages < std::max(2, v->a_bufs)) return fail(o, PTQ8_ERR_INVALID, "linear: %d stages", p.stages);
-    const int smem = extra + p.stages * v->stage;
+    p.stages = stages_of(*v, split, p.list_bytes);
+    const int smem = smem_beside(*v, split, p.list_bytes) + p.stages * v->stage;
     // tiles at most: each group's last tile may be partly filled
-    const long long row_tiles = l.offsets ? a.rows / c.tn + std::min<long long>(l.groups, a.rows) : (a.rows + c.tn - 1) / c.tn;
+    const long long row_tiles = l.offsets ? a.rows / v->tn + std::min<long long>(l.groups, a.rows) : (a.rows + v->tn - 1) / v->tn;
     const long long tiles = row_tiles * p.ctiles;
     if (tiles > 0x3FFFFFFF / 8) return fail(o, PTQ8_ERR_INVALID, "linear: %lld tiles", tiles);
-    const int per = c.cg * c.split, slots = o->sms * v->per_sm / per;
-    const long long clusters = c.split > 1 ? tiles : std::min<long long>(tiles, slots);
+    const int per = v->cg * split, slots = o->sms * v->per_sm / per;
+    const long long clusters = split > 1 ? tiles : std::min<long long>(tiles, slots);
     const cudaError_t e = launch(v->kernel, dim3(static_cast<unsigned>(clusters * per)), dim3(v->threads), smem, per, st, mx, mw, p);
     return e == cudaSuccess ? PTQ8_OK : cuda_fail(o, "linear", e);
 }
