@@ -237,11 +237,14 @@ def test_linear_shapes(ops, rows, k, n, bits, gated):
     check(lambda t: ops.linear(*a, bits=bits, act=1 if gated else 0, dtype=t), plain_product(x, xs, w, ws, b), n, gated, dtype)
 
 
-@pytest.mark.parametrize("rows,k,n", [(2500, 272, 2100), (5000, 130, 1111), (4097, 640, 1290), (9000, 48, 530)])
+@pytest.mark.parametrize("rows,k,n", [(2500, 272, 2100), (5000, 130, 1111), (4097, 640, 1290), (9000, 48, 530),
+                                      (700, 8192, 500), (130, 16384, 260), (48, 8200, 1000), (300, 300, 5000),
+                                      (20, 4096, 9000), (1000, 2000, 130)])
 @pytest.mark.parametrize("bits", [8, 4])
 @pytest.mark.parametrize("gated", [False, True])
 def test_linear_many_tiles(ops, rows, k, n, bits, gated):
-    """More tiles than the device runs at once: every CTA takes several."""
+    """More tiles than the device runs at once, so that every CTA takes several; and few tiles with long sums, which
+    clusters share."""
     rng = np.random.default_rng(rows)
     x, xs, w, ws, b = case(rng, rows, k, n, bits, gated, True)
     a = (laid(x), dev(xs), laid(w if bits == 8 else pack4(w)), dev(ws), dev(b))
