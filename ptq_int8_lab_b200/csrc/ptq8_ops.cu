@@ -15,6 +15,7 @@
 
 #include "ptq8.h"
 #include "ptq8_linear.cuh"
+#include "ptq8_linear_few.cuh"
 #include "ptq8_linear_tc.cuh"
 #include "ptq8_rows.cuh"
 
@@ -288,8 +289,8 @@ const Variant* choose(const ptq8_ops* o, const ptq8_linear_args& a, bool listed,
 
 bool aligned16(long long v) { return v % 16 == 0; }
 
-// What TMA needs of the operands' layout (a pitch that no second row uses does not count).
-bool tc_layout(const ptq8_linear_args& a, bool grouped) {
+// What TMA and 16-byte loads need of the operands' layout (a pitch that no second row uses does not count).
+bool vector_layout(const ptq8_linear_args& a, bool grouped) {
     return aligned16(reinterpret_cast<uintptr_t>(a.x)) && aligned16(reinterpret_cast<uintptr_t>(a.w)) &&
            (aligned16(a.ldx) || a.rows == 1) && (aligned16(a.ldw) || a.out_features == 1 && a.epilogue == PTQ8_EPI_NONE) &&
            (!grouped || a.groups == 1 || aligned16(a.w_group_stride)) && a.ldx < (1LL << 39) && a.ldw < (1LL << 39);
@@ -350,6 +351,42 @@ int run_tc(ptq8_ops* o, const ptq8_linear_args& a, const LinearParams& l, cudaSt
     return e == cudaSuccess ? PTQ8_OK : cuda_fail(o, "linear", e);
 }
 
+using FewKernel = void (*)(FewParams);
+
+template <int MT>
+FewKernel few_kernel(bool w4, bool gated) {
+    return w4 ? (gated ? linear_few_kernel<MT, true, true> : linear_few_kernel<MT, true, false>)
+              : (gated ? linear_few_kernel<MT, false, true> : linear_few_kernel<MT, false, false>);
+}
+
+// Up to four tokens, or one a group on average, while the weights that they read stay small: one token x 4096 x
+// 4096 takes 5.3 us here and 6.1 us as a tensor-core tile (int4 4.1 and 6.9), four tokens 6.0 and 6.6 (5.0 and
+// 7.5); six tokens 8.8 and 6.6.  From 32 MB on (4096 x 8192 int8: 10.9 and 8.8 us) bulk copies into shared memory
+// keep more bytes in flight.  Rows that are not whole vectors of 16 bytes of weights go to the tensor cores too: at
+// 2001 x 1270 joining single bytes made four tokens 1.2 (int4 1.6) times slower than a tile.
+bool few_rows(const ptq8_linear_args& a, int groups) {
+    constexpr long long kMostBytes = 24LL << 20;
+    const long long channels = static_cast<long long>(a.out_features) * (a.epilogue == PTQ8_EPI_SWIGLU ? 2 : 1);
+    const long long bytes = std::min<long long>(groups, a.rows) * channels * a.in_features * a.w_bits / 8;
+    return (groups > 1 ? a.rows <= groups : a.rows <= 4) && bytes <= kMostBytes && a.in_features % (a.w_bits == 4 ? 32 : 16) == 0;
+}
+
+int run_few(ptq8_ops* o, const ptq8_linear_args& a, const LinearParams& l, cudaStream_t st) {
+    const bool gated = a.epilogue == PTQ8_EPI_SWIGLU, w4 = a.w_bits == 4;
+    const int channels = kFewRows / (gated ? 2 : 1);   // of a warp
+    const long long sets = (static_cast<long long>(a.out_features) + channels - 1) / channels;
+    const long long used = std::min<long long>(l.groups, a.rows);
+    FewParams p{l, 1};
+    while (p.ks < kFewWarps && sets * used * p.ks < 1LL * kFewWarps * o->sms) p.ks *= 2;
+    // groups differ in their rows: room for two of them at least
+    const long long rows = l.groups > 1 ? std::max(2LL, a.rows / used) : a.rows;
+    const FewKernel kernel = rows == 1 ? few_kernel<1>(w4, gated) : rows == 2 ? few_kernel<2>(w4, gated) : few_kernel<4>(w4, gated);
+    const int per = kFewWarps / p.ks;
+    const cudaError_t e = launch(kernel, dim3(static_cast<unsigned>((sets + per - 1) / per), static_cast<unsigned>(l.groups)),
+                                 dim3(32 * kFewWarps), 0, 1, st, p);
+    return e == cudaSuccess ? PTQ8_OK : cuda_fail(o, "linear", e);
+}
+
 int run_linear(ptq8_ops* o, const ptq8_linear_args& a, bool grouped, cudaStream_t st) {
     LinearParams p{};
     p.x = a.x;
@@ -369,7 +406,7 @@ int run_linear(ptq8_ops* o, const ptq8_linear_args& a, bool grouped, cudaStream_
     p.groups = grouped ? a.groups : 1;
     p.y_type = a.y_type;
     const bool gated = a.epilogue == PTQ8_EPI_SWIGLU, w4 = a.w_bits == 4;
-    if (tc_layout(a, grouped)) return run_tc(o, a, p, st);
+    if (vector_layout(a, grouped)) return few_rows(a, p.groups) ? run_few(o, a, p, st) : run_tc(o, a, p, st);
     const long long row_tiles = (a.rows + kAnyTile - 1) / kAnyTile;
     // blocks stride over the channel tiles (x) and over a group's row tiles (y)
     const dim3 grid(static_cast<unsigned>((a.out_features + kAnyTile - 1) / kAnyTile),

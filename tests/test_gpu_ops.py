@@ -590,3 +590,26 @@ def test_handles(ops):
     assert L.ptq8_linear(None, None, None) == 1 and L.ptq8_quantize_rows(None, None, None) == 1
     assert L.ptq8_linear(ops._h, None, None) == 1 and L.ptq8_linear_grouped(ops._h, None, None) == 1
     assert L.ptq8_quantize_rows(ops._h, None, None) == 1
+
+
+@pytest.mark.parametrize("rows", [1, 2, 3, 4])
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("k,n,pitch", [(2001, 130, 2016), (1023, 33, 1024), (511, 3, 512), (4112, 66, 4112), (1024, 1, 1024),
+                                       (17, 7, 32), (2016, 130, 2016), (4096, 50, 8192)])
+def test_few_tokens_row_ends(ops, rows, bits, gated, k, n, pitch):
+    """Weights and codes whose last row ends with its buffer, and rows followed by bytes that must not count."""
+    rng = np.random.default_rng(k + rows)
+    x, xs, w, ws, b = case(rng, rows, k, n, bits, gated, True)
+
+    def exact_end(a, p):
+        """A device copy with pitch p whose buffer ends where its last row does."""
+        a = torch.from_numpy(np.ascontiguousarray(a))
+        buf = torch.full(((a.shape[0] - 1) * p + a.shape[1],), 85, dtype=a.dtype, device="cuda")
+        t = buf.as_strided(a.shape, (p, 1))
+        t.copy_(a)
+        return t
+
+    wc = w if bits == 8 else pack4(w)
+    a = (exact_end(x, pitch), dev(xs), exact_end(wc, pitch if bits == 8 else (pitch // 2 + 15) // 16 * 16), dev(ws), dev(b))
+    check(lambda t: ops.linear(*a, bits=bits, act=1 if gated else 0, dtype=t), plain_product(x, xs, w, ws, b), n, gated, "bf16")

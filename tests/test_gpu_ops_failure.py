@@ -13,7 +13,7 @@ pytestmark = pytest.mark.gpu
 TIMEOUT = 4   # PTQ8_ERR_TIMEOUT
 
 
-@pytest.mark.parametrize("rows,k,n,bits,act", [(1, 1024, 256, 8, 0), (16, 4096, 4096, 8, 0), (16, 4096, 512, 4, 1),
+@pytest.mark.parametrize("rows,k,n,bits,act", [(5, 1024, 256, 8, 0), (16, 4096, 4096, 8, 0), (16, 4096, 512, 4, 1),
                                                (100, 512, 300, 8, 1), (600, 1024, 512, 4, 0), (6000, 512, 2048, 8, 0),
                                                (6000, 512, 2048, 4, 1)])
 def test_wait_runs_out(rows, k, n, bits, act):
@@ -42,7 +42,7 @@ def test_wait_runs_out(rows, k, n, bits, act):
 def test_calls_refused_until_reported():
     from ptq_int8_lab_b200.ops import Int8Ops
     ops = Int8Ops(0)
-    x, xs = torch.zeros((4, 64), dtype=torch.int8, device="cuda"), torch.ones(4, device="cuda")
+    x, xs = torch.zeros((6, 64), dtype=torch.int8, device="cuda"), torch.ones(6, device="cuda")
     w, ws = torch.zeros((32, 64), dtype=torch.int8, device="cuda"), torch.ones(32, device="cuda")
     ops.set_wait_test(10_000_000, True)
     ops.linear(x, xs, w, ws)
