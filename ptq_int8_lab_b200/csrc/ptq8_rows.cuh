@@ -78,42 +78,46 @@ __device__ __forceinline__ uint4 load16(const void* p) {
 // The first n (>= 1) elements of a vector one by one; the others are zero (code 0, no part in the maximum).
 template <typename T>
 __device__ __noinline__ uint4 load_part(const T* p, int n) {
-    uint4 v = make_uint4(0, 0, 0, 0);
     uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < Vec<T>::V; ++i) {
-        if (i >= n) break;
-        if (sizeof(T) == 4)
-            w[i] = reinterpret_cast<const uint32_t*>(p)[i];
-        else
-            w[i / 2] |= static_cast<uint32_t>(reinterpret_cast<const unsigned short*>(p)[i]) << (16 * (i & 1));
-    }
-    v = make_uint4(w[0], w[1], w[2], w[3]);
-    return v;
-}
-
-// A whole vector that starts at any element: two aligned loads joined, where both lie inside the
-// tensor [lo, hi); one by one at its very ends.
-template <typename T>
-__device__ __forceinline__ uint4 load_shifted(const T* p, const char* lo, const char* hi) {
-    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
-    const uint32_t off = at & 15;
-    const char* a = reinterpret_cast<const char*>(at - off);
-    if (a < lo || a + 32 > hi) return load_part(p, Vec<T>::V);
-    const uint4 x = load16(a), y = load16(a + 16);
-    uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-    if (off & 8)
-#pragma unroll
-        for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
-    if (off & 4)
-#pragma unroll
-        for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
-    if (sizeof(T) == 2) {
-        const uint32_t bits = (off & 2) * 8;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], bits);
+        if (i < n) {
+            if (sizeof(T) == 4)
+                w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+            else
+                w[i / 2] |= static_cast<uint32_t>(reinterpret_cast<const unsigned short*>(p)[i]) << (16 * (i & 1));
+        }
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// The first n elements of a vector, zero in the others' place.
+template <typename T>
+__device__ __forceinline__ uint4 first_of(uint4 q, int n) {
+    if (n >= Vec<T>::V) return q;
+    uint32_t* w = &q.x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int here = (n * static_cast<int>(sizeof(T)) - 4 * i);   // bytes of this word that count
+        w[i] = here >= 4 ? w[i] : here <= 0 ? 0u : w[i] & 0xFFFFu;
+    }
+    return q;
+}
+
+// A whole vector that starts `off` bytes past a multiple of 16 (off: the same for a row's vectors, so for a
+// warp): two aligned loads joined.  Both lie inside the tensor, or the caller loads one by one.
+__device__ __forceinline__ uint4 load_shifted(const void* p, uint32_t off) {
+    const char* a = static_cast<const char*>(p) - off;
+    const uint4 x = load16(a);
+    if (off == 0) return x;
+    const uint4 y = load16(a + 16);
+    const uint32_t bits = (off & 3) * 8;
+    switch (off >> 2) {
+        case 0: return make_uint4(__funnelshift_r(x.x, x.y, bits), __funnelshift_r(x.y, x.z, bits), __funnelshift_r(x.z, x.w, bits), __funnelshift_r(x.w, y.x, bits));
+        case 1: return make_uint4(__funnelshift_r(x.y, x.z, bits), __funnelshift_r(x.z, x.w, bits), __funnelshift_r(x.w, y.x, bits), __funnelshift_r(y.x, y.y, bits));
+        case 2: return make_uint4(__funnelshift_r(x.z, x.w, bits), __funnelshift_r(x.w, y.x, bits), __funnelshift_r(y.x, y.y, bits), __funnelshift_r(y.y, y.z, bits));
+        default: return make_uint4(__funnelshift_r(x.w, y.x, bits), __funnelshift_r(y.x, y.y, bits), __funnelshift_r(y.y, y.z, bits), __funnelshift_r(y.z, y.w, bits));
+    }
 }
 
 // Codes of one vector: round_half_away(f / s), the exact quotient.  Multipliers that bracket 1/s, each in
@@ -122,8 +126,17 @@ __device__ __forceinline__ uint4 load_shifted(const T* p, const char* lo, const 
 // both agree, every number between f * inv_lo and f * inv_hi rounds to that integer, and so does the exact
 // quotient, which lies strictly inside.  Where they do not (`flag`), a half-integer t lies between them, and
 // the sign of f - t s decides: one FMA, whose rounding keeps the sign of the exact value.
-// Codes of a vector that cannot be stored as a word: n bytes of c, one by one.
-__device__ __noinline__ void store_bytes(int8_t* out, uint2 c, int n) {
+// The first n < 8 codes of a vector, in the largest pieces that their place allows.
+__device__ __forceinline__ void store_first(int8_t* out, uint2 c, int n, bool words) {
+    if (words) {   // out is a multiple of the vector's codes
+        if (n & 4) *reinterpret_cast<uint32_t*>(out) = c.x;
+        const uint32_t rest = n & 4 ? c.y : c.x;
+        out += n & 4;
+        if (n & 2) *reinterpret_cast<unsigned short*>(out) = static_cast<unsigned short>(rest);
+        if (n & 1) out[n & 2] = static_cast<int8_t>(rest >> (n & 2 ? 16 : 0));
+        return;
+    }
+#pragma unroll 1
     for (int i = 0; i < n; ++i) out[i] = static_cast<int8_t>((i < 4 ? c.x : c.y) >> (8 * (i & 3)));
 }
 
@@ -180,18 +193,20 @@ __global__ void __launch_bounds__(TPR > 128 ? TPR : 128) rows_kernel(RowsParams 
     const long long src = !there ? -1 : p.rows ? p.rows[r] : static_cast<long long>(r);
     const bool read = src >= 0 && src < p.x_rows;
     const T* x = static_cast<const T*>(p.x) + static_cast<size_t>(read ? src : 0) * p.ldx;
-    const char* lo = static_cast<const char*>(p.x);
-    const char* hi = PLAIN ? nullptr : lo + (static_cast<size_t>(p.x_rows - 1) * p.ldx + p.width) * sizeof(T);
+    // Not PLAIN: where the row starts, and whether aligned loads around its vectors stay inside the tensor (they
+    // may leave it in its first and last row).
+    const uint32_t off = PLAIN ? 0 : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(x) & 15);
+    const bool inner = PLAIN || (src > 0 && src + 1 < p.x_rows && p.ldx >= 16);
     const int vecs = (p.width + V - 1) / V, readable = read ? vecs : 0;
     auto fetch = [&](int v) {
         uint4 q = make_uint4(0, 0, 0, 0);
         if (v < readable) {
             if (PLAIN)
                 q = load16(x + v * V);
-            else if ((v + 1) * V > p.width)
-                q = load_part(x + v * V, p.width - v * V);
+            else if (inner)
+                q = first_of<T>(load_shifted(x + v * V, off), p.width - v * V);
             else
-                q = load_shifted(x + v * V, lo, hi);
+                q = load_part(x + v * V, min(V, p.width - v * V));
         }
         return q;
     };
@@ -241,7 +256,7 @@ __global__ void __launch_bounds__(TPR > 128 ? TPR : 128) rows_kernel(RowsParams 
             else
                 *reinterpret_cast<uint32_t*>(out + v * V) = c[0];
         } else {
-            store_bytes(out + v * V, make_uint2(c[0], c[V / 4 - 1]), min(V, p.width - v * V));
+            store_first(out + v * V, make_uint2(c[0], c[V / 4 - 1]), min(V, p.width - v * V), words);
         }
     };
     if (NV) {
