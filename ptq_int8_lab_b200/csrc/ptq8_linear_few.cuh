@@ -17,7 +17,8 @@ struct FewParams {
     int ks;   // warps that share four rows' sum: a power of two
 };
 
-__device__ __forceinline__ uint4 ld16(const void* p) { return __ldg(static_cast<const uint4*>(p)); }
+// Plain loads, not read-only ones: with programmatic launch the tensors may be written while this kernel has started.
+__device__ __forceinline__ uint4 ld16(const void* p) { return *static_cast<const uint4*>(p); }
 
 // acc += the products of 4 words of weights with 4 words of codes.
 __device__ __forceinline__ int dot16(const uint4& w, const uint4& x, int acc) {
@@ -88,12 +89,12 @@ __global__ void __launch_bounds__(32 * kFewWarps, MT == 4 ? 2 : 4) linear_few_ke
     const int r_lane = lane / MT, t_lane = lane % MT, c = c0 + r_lane % C;
     const bool mine_ok = part == 0 && lane < kFewRows * MT && c < l.n && beg < end;
     const size_t at = static_cast<size_t>(g) * (l.n * H) + (r_lane / C) * l.n + c;
-    const float ws = mine_ok ? __ldg(l.ws + at) * (W4 ? 0.0625f : 1.0f) : 0.0f;
-    const float bias = mine_ok && l.bias ? __ldg(l.bias + at) : 0.0f;
+    const float ws = mine_ok ? l.ws[at] * (W4 ? 0.0625f : 1.0f) : 0.0f;
+    const float bias = mine_ok && l.bias ? l.bias[at] : 0.0f;
     for (long long t0 = beg; t0 < end; t0 += MT) {
         const int tokens = static_cast<int>(min(static_cast<long long>(MT), end - t0));
         const bool here = mine_ok && t_lane < tokens;
-        const float xs = here ? __ldg(l.xs + t0 + t_lane) : 0.0f;
+        const float xs = here ? l.xs[t0 + t_lane] : 0.0f;
         int acc[kFewRows][MT] = {};
         const uint8_t* x[MT];
 #pragma unroll

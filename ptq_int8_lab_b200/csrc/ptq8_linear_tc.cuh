@@ -292,8 +292,8 @@ __device__ __forceinline__ Channel<H> channel_of(const LinearParams& l, int grou
 #pragma unroll
     for (int h = 0; h < H; ++h) {
         const size_t at = static_cast<size_t>(group) * (l.n * H) + h * l.n + c;
-        ch.ws[h] = ch.ok ? __ldg(l.ws + at) * (W4 ? 0.0625f : 1.0f) : 0.0f;
-        ch.b[h] = ch.ok && l.bias ? __ldg(l.bias + at) : 0.0f;
+        ch.ws[h] = ch.ok ? l.ws[at] * (W4 ? 0.0625f : 1.0f) : 0.0f;
+        ch.b[h] = ch.ok && l.bias ? l.bias[at] : 0.0f;
     }
     return ch;
 }
@@ -337,7 +337,7 @@ template <typename T, int H>
 __device__ __forceinline__ void store_partials(T* y, size_t ldy, const int* recv, int S, int tokens, const float* xs,
                                                const Channel<H>& ch, int lane_c, int t0, int mine, int part, int step) {
     for (int t = part; t < mine; t += step) {
-        const float x = __ldg(xs + t0 + t);
+        const float x = xs[t0 + t];
         int a[2] = {0, 0};
         for (int s = 0; s < S; ++s)
 #pragma unroll
@@ -600,7 +600,7 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
             const Channel<H> ch = channel_of<H, W4>(p.l, tile.group, c);
             const int c0 = part * Sh::kCW, c1 = min(c0 + Sh::kCW, tile.valid);
             __syncwarp();
-            for (int i = lane; c0 + i < c1; i += 32) sxs[i] = __ldg(p.l.xs + tile.row0 + c0 + i);
+            for (int i = lane; c0 + i < c1; i += 32) sxs[i] = p.l.xs[tile.row0 + c0 + i];
             __syncwarp();
             if (!mbar_wait_warp(accfull + 8 * buf, accph, limit)) {
                 give_up(ERR_WAIT_ACC);

@@ -239,6 +239,7 @@ int list_bytes_of(const ptq8_linear_args& a, bool listed) { return listed ? ((a.
 // variant: the variant of the least estimate is 2.4 % slower than the fastest one on average, 35 % at most.
 float estimate(const ptq8_ops* o, const ptq8_linear_args& a, int groups, const Variant& v, int split) {
     constexpr float kMma = 70, kMmaTmem = 84;        // least cycles of an MMA, M operand in shared memory or TMEM
+    constexpr float kMmaTmemPair = 78;               // the latter for a pair: 4096 x 4096 x 4096 gated 100 us, one CTA a tile 105
     constexpr float kWait = 145, kWaitTwo = 50;      // wait of the MMA warp per block (two blocks a stage)
     constexpr float kLoad = 64;                      // bytes per cycle into an SM
     constexpr float kWiden = 175;                    // int4: cycles of an SM per tile of 128 x 128 codes
@@ -255,7 +256,7 @@ float estimate(const ptq8_ops* o, const ptq8_linear_args& a, int groups, const V
     const float blocks = std::ceil(std::ceil(a.in_features / 128.0f) / split);
     const float columns = std::min<float>(v.tn, std::ceil(std::ceil(mean) / (16 * v.cg)) * (16 * v.cg));
     const float share = v.per_sm == 2 && tiles * v.cg * split > kPacked * o->sms ? 2 : 1;
-    const float mma = 4 * h * std::max(v.w4 ? kMmaTmem : kMma, columns / 2);
+    const float mma = 4 * h * std::max(!v.w4 ? kMma : v.cg == 2 ? kMmaTmemPair : kMmaTmem, columns / 2);
     const float load = (h * 128 * (v.w4 ? 64 : 128) + v.x_rows * 128) / kLoad;
     const float block = std::max({mma + (v.depth > 128 ? kWaitTwo : kWait), share * mma, share * load, share * (v.w4 ? kWiden * h : 0)});
     const float fill = split == 8 ? kFill8 : split == 4 ? kFill4 : 1;
