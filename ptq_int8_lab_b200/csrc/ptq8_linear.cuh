@@ -56,8 +56,19 @@ __device__ __forceinline__ void group_rows(const LinearParams& p, int g, long lo
     end = min(max(static_cast<long long>(p.offsets[g + 1]), beg), p.rows);
 }
 
-// The kernel for every layout (any pitch, any alignment): 64 tokens x 64 channels per block, both
-// operands' chunks of 64 codes copied byte by byte into shared memory, dp4a on 4x4 outputs a thread.
+// Up to four bytes that start anywhere, zero past the n-th.
+__device__ __forceinline__ uint32_t join4(const uint8_t* p, int n) {
+    uint32_t v = 0;
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+        if (b < n) v |= static_cast<uint32_t>(p[b]) << (8 * b);
+    return v;
+}
+
+// The kernel for layouts that neither TMA nor 16-byte loads can read (rows at any byte): 64 tokens x 64 channels
+// per block, chunks of 64 codes of both operands joined byte by byte in shared memory, dp4a on 4x4 outputs a
+// thread.  The byte loads bound it: 1024 tokens x 1001 -> 1024 takes 72 us, 6.7 us where rows start at
+// multiples of 16 bytes (as quantize_rows lays codes, and weights are laid once).
 constexpr int kAnyTile = 64;
 
 template <bool W4, bool GATED>
@@ -75,25 +86,24 @@ __global__ void __launch_bounds__(256) linear_any_kernel(LinearParams p) {
          t0 += static_cast<long long>(gridDim.y) * kAnyTile) {
         int acc[H][4][4] = {};
         for (int k0 = 0; k0 < p.k; k0 += 64) {
-            for (int i = tid; i < kAnyTile * 64; i += 256) {
-                const int r = i >> 6, k = k0 + (i & 63);
-                int8_t v = 0;
-                if (t0 + r < end && k < p.k) v = p.x[static_cast<size_t>(t0 + r) * p.ldx + k];
-                reinterpret_cast<int8_t*>(sx[r])[i & 63] = v;
+            // a thread joins four codes of one row at a time
+            for (int i = tid; i < kAnyTile * 16; i += 256) {
+                const int r = i >> 4, k = k0 + (i & 15) * 4;
+                uint32_t v = 0;
+                if (t0 + r < end) v = join4(reinterpret_cast<const uint8_t*>(p.x) + static_cast<size_t>(t0 + r) * p.ldx + k, p.k - k);
+                sx[r][i & 15] = v;
             }
-            for (int i = tid; i < H * kAnyTile * 64; i += 256) {
-                const int h = i / (kAnyTile * 64), r = (i >> 6) % kAnyTile, k = k0 + (i & 63), c = c0 + r;
-                int8_t v = 0;
-                if (c < p.n && k < p.k) {
+            for (int i = tid; i < H * kAnyTile * 16; i += 256) {
+                const int h = i / (kAnyTile * 16), r = (i >> 4) % kAnyTile, k = k0 + (i & 15) * 4, c = c0 + r;
+                uint32_t v = 0, rest;
+                if (c < p.n) {
                     const uint8_t* row = w + static_cast<size_t>(h * p.n + c) * p.ldw;
-                    if (W4) {
-                        const uint8_t b = row[k >> 1];
-                        v = static_cast<int8_t>(static_cast<int8_t>((k & 1) ? b & 0xF0 : b << 4) >> 4);
-                    } else {
-                        v = static_cast<int8_t>(row[k]);
-                    }
+                    if (W4)
+                        unpack_w4(join4(row + k / 2, min(2, (p.k + 1) / 2 - k / 2)), v, rest);   // x has zeros past its end
+                    else
+                        v = join4(row + k, p.k - k);
                 }
-                reinterpret_cast<int8_t*>(sw[h][r])[i & 63] = v;
+                sw[h][r][i & 15] = v;
             }
             __syncthreads();
 #pragma unroll 4

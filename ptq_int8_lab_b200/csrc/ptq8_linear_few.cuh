@@ -4,6 +4,9 @@
 // partial sums between CTAs) costs more than the arithmetic.  Here a warp owns four weight rows (gated: two
 // gate and two up rows), a lane 16 bytes of each at a time, and the only exchange is the warp's sum at the
 // end.  Where rows are few and long, KS warps of a block share four rows' input features.
+//
+// Bound by the weights' way from DRAM and the launch: one token x 4096 x 4096 takes 5.2 us (int4 4.0 us) with
+// weights from DRAM, 3.8 us (3.6 us) from L2; 1024 x 1024 takes 2.0 us, of which a launch after another is 1.3.
 #pragma once
 
 #include "ptq8_linear.cuh"

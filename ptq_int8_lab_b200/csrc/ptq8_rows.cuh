@@ -1,4 +1,8 @@
 // Per-token quantization: one symmetric int8 scale per row, from the row itself.
+//
+// One read, one write: 8192 x 4096 bf16 in 17.3 us (100.7 MB at 5.8 TB/s, 90 % of a plain copy), f32 in 25.7 us
+// (98 %).  Instructions come next (11 M warp instructions for the former, issue slots 70 % busy): they bound
+// the gathered form, which reads a token from L2 once per row that asks for it (16384 rows of 2048 f16 15.7 us).
 #pragma once
 
 #include <cuda_bf16.h>
