@@ -341,7 +341,8 @@ int ptq8_quantize_rows(ptq8_ops* ops, const ptq8_rows_args* args, void* stream);
  * The tensor-core kernels need x, w (and a group's weights) to start at multiples of 16 bytes and row pitches that
  * are multiples of 16 bytes; any other layout runs on a slower kernel.
  * ptq8_linear_grouped: rows offsets[g] .. offsets[g+1]-1 meet group g's weights (offsets: device memory, groups+1
- * values, not decreasing, within [0, rows]; values outside are clamped); rows of no group are not written. */
+ * values, not decreasing, within [0, rows]; values outside are clamped, and where they decrease no access leaves the
+ * tensors, but rows of two groups may hold either's product); rows of no group are not written. */
 typedef struct {
     const int8_t* x;       /* [rows][in_features], pitch ldx */
     long long ldx;

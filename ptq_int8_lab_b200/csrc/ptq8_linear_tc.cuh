@@ -252,27 +252,28 @@ template <int TN>
 struct Tiles {
     const LinearParams& l;
     const int* start;   // shared memory: first tile of each group, and the end; null: one group of all rows
+    const int* row;     // and first row
     int ctiles;
     int g = 0;          // cursor: tiles are asked for in increasing order
-    __device__ Tiles(const LinearParams& lp, const int* s, int c) : l(lp), start(s), ctiles(c) {}
+    __device__ Tiles(const LinearParams& lp, const int* s, const int* r, int c) : l(lp), start(s), row(r), ctiles(c) {}
     __device__ bool get(int t, Tile& o) {
-        long long beg = 0, end = l.rows;
-        int i = t;
+        int beg = 0, end = static_cast<int>(l.rows), i = t;
         if (start) {
             while (g < l.groups && t >= start[g + 1]) ++g;
             if (g >= l.groups) return false;
-            group_rows(l, g, beg, end);
+            beg = row[g];
+            end = row[g + 1];
             i = t - start[g];
         }
-        const int tt = static_cast<int>((end - beg + TN - 1) / TN);
+        const int tt = (end - beg + TN - 1) / TN;   // rows + TN fits: the host limits rows
         if (!start && i >= tt * ctiles) return false;
         const int full = kBand * ctiles, band = i / full, rest = i - band * full;
         const int wide = min(kBand, tt - band * kBand);
         o.ct = rest / wide;
         const int k = band * kBand + (rest - o.ct * wide);
         o.group = g;
-        o.row0 = static_cast<int>(beg) + k * TN;
-        o.valid = min(TN, static_cast<int>(end) - o.row0);
+        o.row0 = beg + k * TN;
+        o.valid = min(TN, end - o.row0);
         return true;
     }
 };
@@ -387,7 +388,8 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
     const uint32_t base = (smem_u32(dyn) + 1023u) & ~1023u;
     uint8_t* const base_p = dyn + (base - smem_u32(dyn));
     const uint32_t after = base + p.stages * Sh::kStage;   // tile list, partial sums
-    int* const list = reinterpret_cast<int*>(base_p + (after - base));
+    int* const list = reinterpret_cast<int*>(base_p + (after - base));   // first tile of each group, and the end
+    int* const first_row = list + p.l.groups + 1;                        // and first row
     const uint32_t recv = after + p.list_bytes;
     const uint32_t b0 = smem_u32(bars);
     const uint32_t full = b0, empty = full + 8 * p.stages;
@@ -425,7 +427,7 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
         }
     }
     const bool listed = p.l.offsets != nullptr;
-    Tiles<TN> tiles(p.l, listed ? list : nullptr, p.ctiles);
+    Tiles<TN> tiles(p.l, listed ? list : nullptr, first_row, p.ctiles);
     const int per = CG == 2 ? 2 : S;
     const int t0 = blockIdx.x / per, dt = gridDim.x / per;
     const int kb0 = static_cast<int>(static_cast<long long>(p.kblocks) * (S > 1 ? rank : 0) / S);
@@ -441,15 +443,27 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
     tc_fence_before();
     if (clustered) cluster_sync();   // the peers' barriers exist
     griddep_wait();                  // nothing above reads or writes global memory (but for prefetches)
-    if (listed && warp == 2) {   // first tile of each group
+    if (listed && warp == 2) {
+        // The groups' first rows, clamped into [0, rows] and never decreasing, then their first tiles: what the
+        // offsets hold, the tiles are no more than the launch was made for.
+        const int most = static_cast<int>(p.l.rows);
+        int row = 0;
+        for (int g0 = 0; g0 <= p.l.groups; g0 += 32) {
+            int v = g0 + lane <= p.l.groups ? min(max(p.l.offsets[g0 + lane], 0), most) : 0;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int o = __shfl_up_sync(0xffffffffu, v, d);
+                if (lane >= d) v = max(v, o);
+            }
+            v = max(v, row);
+            if (g0 + lane <= p.l.groups) first_row[g0 + lane] = v;
+            row = __shfl_sync(0xffffffffu, v, 31);
+        }
+        __syncwarp();
         int sum = 0;
         for (int g0 = 0; g0 < p.l.groups; g0 += 32) {
             int n = 0;
-            if (g0 + lane < p.l.groups) {
-                long long beg, end;
-                group_rows(p.l, g0 + lane, beg, end);
-                n = static_cast<int>((end - beg + TN - 1) / TN) * p.ctiles;
-            }
+            if (g0 + lane < p.l.groups) n = (first_row[g0 + lane + 1] - first_row[g0 + lane] + TN - 1) / TN * p.ctiles;
             int incl = n;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {

@@ -21,6 +21,9 @@
 
 using namespace ptq8;
 
+// what the Python mirror packs
+static_assert(sizeof(ptq8_rows_args) == 72 && sizeof(ptq8_linear_args) == 120, "argument structs");
+
 struct ptq8_ops {
     int device = 0;
     int sms = 0;
@@ -229,7 +232,7 @@ int stages_of(const Variant& v, int split, int list_bytes) {
     return std::min(kMaxLinStages, ((v.per_sm == 2 ? kSmemTwo : kSmemOne) - smem_beside(v, split, list_bytes)) / v.stage);
 }
 
-int list_bytes_of(const ptq8_linear_args& a, bool listed) { return listed ? ((a.groups + 1) * 4 + 127) / 128 * 128 : 0; }
+int list_bytes_of(const ptq8_linear_args& a, bool listed) { return listed ? ((a.groups + 1) * 8 + 127) / 128 * 128 : 0; }
 
 // A launch's time in cycles, up to what all variants share.  Per stage a CTA takes the longest of its chain (the
 // MMAs and the wait before them) and, for the CTAs that share an SM, their MMAs, their loads at what an SM draws
@@ -294,7 +297,7 @@ bool aligned16(long long v) { return v % 16 == 0; }
 bool vector_layout(const ptq8_linear_args& a, bool grouped) {
     return aligned16(reinterpret_cast<uintptr_t>(a.x)) && aligned16(reinterpret_cast<uintptr_t>(a.w)) &&
            (aligned16(a.ldx) || a.rows == 1) && (aligned16(a.ldw) || a.out_features == 1 && a.epilogue == PTQ8_EPI_NONE) &&
-           (!grouped || a.groups == 1 || aligned16(a.w_group_stride)) && a.ldx < (1LL << 39) && a.ldw < (1LL << 39);
+           (!grouped || a.groups == 1 || (aligned16(a.w_group_stride) && a.w_group_stride < (1LL << 39))) && a.ldx < (1LL << 39) && a.ldw < (1LL << 39);
 }
 
 int encode(ptq8_ops* o, CUtensorMap* m, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
