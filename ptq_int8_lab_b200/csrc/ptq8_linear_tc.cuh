@@ -36,7 +36,7 @@ namespace ptq8 {
 enum : int { ERR_WAIT_UNPACK = 5, ERR_WAIT_PARTIAL = 6 };
 
 constexpr int kMaxLinStages = 12;
-constexpr long long kLandCycles = 200000;   // about 0.1 ms: far more than a store to a peer takes
+constexpr long long kLandCycles = 200000;   // about 0.1 ms: far more than a copy to a peer takes
 constexpr int kBand = 8;   // token tiles per band of the tile order: a band's operands stay in L2
 
 struct TcParams {
@@ -115,9 +115,10 @@ __device__ __forceinline__ void prefetch_3d(const CUtensorMap* m, int c0, int c1
 __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t bar) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// Store to a CTA of the cluster; its barrier there counts the bytes when they have arrived.
-__device__ __forceinline__ void st_async(uint32_t addr, uint32_t v, uint32_t bar) {
-    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.u32 [%0], %1, [%2];" ::"r"(addr), "r"(v), "r"(bar)
+// Copy from the own shared memory to a CTA's of the cluster; its barrier there counts the bytes.
+__device__ __forceinline__ void copy_to_peer(uint32_t dst, uint32_t src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "r"(src), "r"(bytes), "r"(bar)
                  : "memory");
 }
 
@@ -340,19 +341,20 @@ __device__ __forceinline__ void store_columns(T* y, size_t ldy, uint32_t acc, co
     }
 }
 
-// The finishing half of a split tile: the S partial sums of tokens t0 .. t0 + tokens - 1 of the tile, every
-// step-th of them from `part` on.
+// The finishing half of a split tile: the S partial sums of this CTA's tokens, every step-th of them from `part`
+// on.  got: this lane's channel of the first token of the first CTA; a token is H * 32 words further, a CTA `cta`
+// words.  xs: the scales of the tokens that this warp finishes, in order.
 template <typename T, int H>
-__device__ __forceinline__ void store_partials(T* y, size_t ldy, const int* recv, int S, int tokens, const float* xs,
-                                               const Channel<H>& ch, int lane_c, int t0, int mine, int part, int step) {
-    for (int t = part; t < mine; t += step) {
-        const float x = xs[t0 + t];
+__device__ __forceinline__ void store_partials(T* y, size_t ldy, const int* got, int S, int cta, const float* xs, const Channel<H>& ch,
+                                               int mine, int part, int step) {
+#pragma unroll 4
+    for (int t = part, i = 0; t < mine; t += step, ++i) {
         int a[2] = {0, 0};
         for (int s = 0; s < S; ++s)
 #pragma unroll
-            for (int h = 0; h < H; ++h) a[h] += recv[((s * tokens + t) * H + h) * 128 + lane_c];
-        const float r = finish<H>(ch, x, a[0], a[1]);
-        if (ch.ok) y[static_cast<size_t>(t0 + t) * ldy] = from_f32<T>(r);
+            for (int h = 0; h < H; ++h) a[h] += got[s * cta + (t * H + h) * 32];
+        const float r = finish<H>(ch, xs[i], a[0], a[1]);
+        if (ch.ok) y[static_cast<size_t>(t) * ldy] = from_f32<T>(r);
     }
 }
 
@@ -621,8 +623,15 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
             const int c = (tile.ct * CG + static_cast<int>(CG == 2 ? rank : 0)) * 128 + lane_c;
             const Channel<H> ch = channel_of<H, W4>(p.l, tile.group, c);
             const int c0 = part * Sh::kCW, c1 = min(c0 + Sh::kCW, tile.valid);
+            // split: this CTA's tokens of the tile
+            const int tokens = TN / S, first = S > 1 ? static_cast<int>(rank) * tokens : 0, mine = min(max(tile.valid - first, 0), tokens);
             __syncwarp();
-            for (int i = lane; c0 + i < c1; i += 32) sxs[i] = p.l.xs[tile.row0 + c0 + i];
+            if (S == 1) {
+                for (int i = lane; c0 + i < c1; i += 32) sxs[i] = p.l.xs[tile.row0 + c0 + i];
+            } else {   // of the tokens that this warp finishes
+                constexpr int step = Sh::kEpi / 4;
+                for (int t = part + lane * step; t < mine; t += 32 * step) sxs[t / step] = p.l.xs[tile.row0 + first + t];
+            }
             __syncwarp();
             if (!mbar_wait_warp(accfull + 8 * buf, accph, limit)) {
                 give_up(ERR_WAIT_ACC);
@@ -646,9 +655,12 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
                     accph ^= 1;
                 }
             } else {
-                const int tokens = TN / S, shift = 31 - __clz(tokens);   // S is a power of two
-                const int first = rank * tokens, mine = min(max(tile.valid - first, 0), tokens);
-                if (warp == 4 && lane == 0) mbar_expect_tx(partial, S * mine * H * 128 * 4);
+                // Partial sums by receiver, then quadrant, token, tile: what this warp sends to one of them is one copy
+                // from the stages' memory (every load into it has been used).  Storing single words to the peers
+                // took 60 cycles a column.
+                const int shift = 31 - __clz(tokens);   // S is a power of two
+                const int piece = tokens * H * 128, slot = 4 * piece;   // bytes of a quadrant's sums, and of all
+                if (warp == 4 && lane == 0) mbar_expect_tx(partial, S * mine * H * 512);
                 for (int cc = c0; cc < c1; cc += 16) {
                     uint32_t v[H][16];
 #pragma unroll
@@ -658,31 +670,34 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
                     for (int h = 0; h < H; ++h) pin_after(v[h]);
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
-                        if (cc + j < c1) {
-                            const int to = (cc + j) >> shift, tk = (cc + j) & (tokens - 1);
-                            const uint32_t dst = mapa(recv + (((rank * tokens + tk) * H) * 128 + lane_c) * 4, to);
-                            const uint32_t bar = mapa(partial, to);
+                        const int to = (cc + j) >> shift, tk = (cc + j) & (tokens - 1);
 #pragma unroll
-                            for (int h = 0; h < H; ++h) st_async(dst + h * 512, v[h][j], bar);
-                        }
+                        for (int h = 0; h < H; ++h)
+                            *reinterpret_cast<uint32_t*>(base_p + to * slot + quad * piece + (tk * H + h) * 128 + lane * 4) = v[h][j];
                     }
                 }
+                fence_proxy_async_smem();
                 __syncwarp();
-                cluster_arrive();   // nothing more goes to the peers
+                const int to = (c0 >> shift) + lane, there = min(max(tile.valid - to * tokens, 0), tokens);
+                if (to << shift < c0 + Sh::kCW && there > 0)
+                    copy_to_peer(mapa(recv + rank * slot + quad * piece, to), base + to * slot + quad * piece, there * H * 128, mapa(partial, to));
+                __syncwarp();
+                const bool joined = mbar_wait_warp(partial, 0, limit);
+                cluster_arrive();   // what the peers sent here has left their memory
                 arrived = true;
-                if (!mbar_wait_warp(partial, 0, limit)) {
+                if (!joined) {
                     give_up(ERR_WAIT_PARTIAL);
                     break;
                 }
-                const int* got = reinterpret_cast<const int*>(base_p + (recv - base));
-                const float* xs = p.l.xs + tile.row0;
+                const int* got = reinterpret_cast<const int*>(base_p + (recv - base) + quad * piece) + lane;
+                const size_t own = at + static_cast<size_t>(first) * p.l.ldy;
                 constexpr int step = Sh::kEpi / 4;
                 if (p.l.y_type == Y_F32)
-                    store_partials<float, H>(static_cast<float*>(p.l.y) + at, p.l.ldy, got, S, tokens, xs, ch, lane_c, first, mine, part, step);
+                    store_partials<float, H>(static_cast<float*>(p.l.y) + own, p.l.ldy, got, S, slot / 4, sxs, ch, mine, part, step);
                 else if (p.l.y_type == Y_F16)
-                    store_partials<__half, H>(static_cast<__half*>(p.l.y) + at, p.l.ldy, got, S, tokens, xs, ch, lane_c, first, mine, part, step);
+                    store_partials<__half, H>(static_cast<__half*>(p.l.y) + own, p.l.ldy, got, S, slot / 4, sxs, ch, mine, part, step);
                 else
-                    store_partials<__nv_bfloat16, H>(static_cast<__nv_bfloat16*>(p.l.y) + at, p.l.ldy, got, S, tokens, xs, ch, lane_c, first, mine, part, step);
+                    store_partials<__nv_bfloat16, H>(static_cast<__nv_bfloat16*>(p.l.y) + own, p.l.ldy, got, S, slot / 4, sxs, ch, mine, part, step);
                 break;
             }
         }
@@ -747,8 +762,8 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
         }
     }
 
-    // No CTA of a cluster ends, and no TMEM is freed, while a peer may still reach it.  Partial sums sent to
-    // this CTA have all arrived (it waited for them; if that wait ran out, the pause lets them land).
+    // No CTA of a cluster ends, and no TMEM is freed, while a peer may still reach it.  Partial sums sent by this
+    // CTA have arrived when its peers have; if a wait for them ran out, the pause lets the copies land.
     __syncwarp();
     if (clustered && !arrived) cluster_arrive();
     if (clustered) cluster_wait();

@@ -282,8 +282,9 @@ const Variant* choose(const ptq8_ops* o, const ptq8_linear_args& a, bool listed,
     for (const Variant& v : kVariants) {
         if (v.w4 != w4 || v.gated != gated || (v.tn > 16 && v.tn >= 4 * v.cg * mean)) continue;
         for (int s = 1; s <= (v.cg == 2 ? 1 : 8) && s * v.depth < a.in_features + v.depth; s *= 2) {
-            // the operand tile of a block is free when its stage is
-            if (stages_of(v, s, list_bytes_of(a, listed)) < std::max(2, v.a_bufs)) continue;
+            // the operand tile of a block is free when its stage is; a split's sums leave from the stages' memory
+            const int stages = stages_of(v, s, list_bytes_of(a, listed));
+            if (stages < std::max(2, v.a_bufs) || (s > 1 && stages * v.stage < v.cols * 128 * 4)) continue;
             const float t = estimate(o, a, groups, v, s);
             if (!best || t < least) best = &v, split = s, least = t;
         }
