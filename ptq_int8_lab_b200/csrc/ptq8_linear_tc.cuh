@@ -96,11 +96,11 @@ __device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
+// A relaxed arrival where no data of the thread has to be seen by the peers (a releasing one first waits for its
+// stores): barrier set-up, which fence.mbarrier_init orders, and the end of a split tile.
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 // Brings a box of the weights into L2.  Harmless where an earlier kernel of the stream still writes it: L2 is
 // where both meet, and the copies that read it come after the wait for that kernel.
 __device__ __forceinline__ void prefetch_3d(const CUtensorMap* m, int c0, int c1, int c2) {
@@ -115,6 +115,20 @@ __device__ __forceinline__ void prefetch_3d(const CUtensorMap* m, int c0, int c1
 __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t bar) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// Shared-memory accesses by address: the compiler would keep loads through a pointer behind every store to y, which
+// it has to think may overlap.
+__device__ __forceinline__ int lds32(uint32_t a) {
+    int v;
+    asm volatile("ld.shared.s32 %0, [%1];" : "=r"(v) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ float4 lds128f(uint32_t a) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ void sts32(uint32_t a, uint32_t v) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory"); }
+
 // Copy from the own shared memory to a CTA's of the cluster; its barrier there counts the bytes.
 __device__ __forceinline__ void copy_to_peer(uint32_t dst, uint32_t src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
@@ -314,14 +328,14 @@ __device__ __forceinline__ float finish(const Channel<H>& ch, float xs, int a0, 
     return H == 2 ? swiglu(v, dequant(a1, xs, ch.ws[H - 1], ch.b[H - 1])) : v;
 }
 
-// Columns [c0, c1) of a warp's 32 accumulator lanes -> y.  xs: their token scales, from column c0 on.
+// Columns [c0, c1) of a warp's 32 accumulator lanes -> y.  xs: shared address of their token scales, from column c0 on.
 template <typename T, int H, int TN>
-__device__ __forceinline__ void store_columns(T* y, size_t ldy, uint32_t acc, const float* xs, const Channel<H>& ch, int c0,
-                                              int c1) {
-    for (int c = c0; c < c1; c += 16) {
+__device__ __forceinline__ void store_columns(T* y, size_t ldy, uint32_t acc, uint32_t xs, const Channel<H>& ch, int c0, int c1) {
+    for (int c = c0; c < c1; c += 16, xs += 64) {
         uint32_t v[16], u[16];
         tmem_ld16(acc + c, v);
         if (H == 2) tmem_ld16(acc + TN + c, u);
+        const float4 x4[4] = {lds128f(xs), lds128f(xs + 16), lds128f(xs + 32), lds128f(xs + 48)};
         tmem_wait_ld();
         pin_after(v);
         if (H == 2) pin_after(u);
@@ -329,12 +343,14 @@ __device__ __forceinline__ void store_columns(T* y, size_t ldy, uint32_t acc, co
         const int left = c1 - c;
 #pragma unroll
         for (int j = 0; j < 16; j += 4) {
-            const float4 x4 = *reinterpret_cast<const float4*>(xs + (c - c0) + j);
-            const float xf[4] = {x4.x, x4.y, x4.z, x4.w};
+            const float xf[4] = {x4[j / 4].x, x4[j / 4].y, x4[j / 4].z, x4[j / 4].w};
+            float r[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                r[i] = finish<H>(ch, xf[i], static_cast<int>(v[j + i]), H == 2 ? static_cast<int>(u[j + i]) : 0);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float r = finish<H>(ch, xf[i], static_cast<int>(v[j + i]), H == 2 ? static_cast<int>(u[j + i]) : 0);
-                if (ch.ok && j + i < left) *out = from_f32<T>(r);
+                if (ch.ok && j + i < left) *out = from_f32<T>(r[i]);
                 out += ldy;
             }
         }
@@ -342,19 +358,25 @@ __device__ __forceinline__ void store_columns(T* y, size_t ldy, uint32_t acc, co
 }
 
 // The finishing half of a split tile: the S partial sums of this CTA's tokens, every step-th of them from `part`
-// on.  got: this lane's channel of the first token of the first CTA; a token is H * 32 words further, a CTA `cta`
-// words.  xs: the scales of the tokens that this warp finishes, in order.
+// on, four at a time.  got: shared address of this lane's channel of the first token of the first CTA; a token is
+// H * 128 bytes further, a CTA `cta` bytes.  xs: shared address of the scales of the tokens that this warp finishes.
 template <typename T, int H>
-__device__ __forceinline__ void store_partials(T* y, size_t ldy, const int* got, int S, int cta, const float* xs, const Channel<H>& ch,
+__device__ __forceinline__ void store_partials(T* y, size_t ldy, uint32_t got, int S, int cta, uint32_t xs, const Channel<H>& ch,
                                                int mine, int part, int step) {
-#pragma unroll 4
-    for (int t = part, i = 0; t < mine; t += step, ++i) {
-        int a[2] = {0, 0};
+    for (int t = part; t < mine; t += 4 * step, xs += 16) {
+        int a[4][H] = {};
         for (int s = 0; s < S; ++s)
 #pragma unroll
-            for (int h = 0; h < H; ++h) a[h] += got[s * cta + (t * H + h) * 32];
-        const float r = finish<H>(ch, xs[i], a[0], a[1]);
-        if (ch.ok) y[static_cast<size_t>(t) * ldy] = from_f32<T>(r);
+            for (int i = 0; i < 4; ++i)   // tokens past the end: what lies there is not used
+#pragma unroll
+                for (int h = 0; h < H; ++h) a[i][h] += lds32(got + s * cta + (min(t + i * step, mine - 1) * H + h) * 128);
+        const float4 x4 = lds128f(xs);
+        const float xf[4] = {x4.x, x4.y, x4.z, x4.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float r = finish<H>(ch, xf[i], a[i][0], a[i][H - 1]);
+            if (ch.ok && t + i * step < mine) y[static_cast<size_t>(t + i * step) * ldy] = from_f32<T>(r);
+        }
     }
 }
 
@@ -443,7 +465,10 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
     }
     __syncwarp();
     tc_fence_before();
-    if (clustered) cluster_sync();   // the peers' barriers exist
+    if (clustered) {   // the peers' barriers exist
+        cluster_arrive_relaxed();
+        cluster_wait();
+    }
     griddep_wait();                  // nothing above reads or writes global memory (but for prefetches)
     if (listed && warp == 2) {
         // The groups' first rows, clamped into [0, rows] and never decreasing, then their first tiles: what the
@@ -615,6 +640,7 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
         // ---------------------------------------------------------------- epilogue
         const int quad = warp & 3, part = (warp - 4) >> 2;
         float* const sxs = sxs_all[warp - 4];
+        const uint32_t xs_at = smem_u32(sxs);
         const int lane_c = quad * 32 + lane;
         const uint32_t accempty_at = CG == 2 ? mapa(accempty, 0) : accempty;
         int buf = 0;
@@ -642,11 +668,11 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
             const size_t at = static_cast<size_t>(tile.row0) * p.l.ldy + c;
             if (CG == 2 || S == 1) {
                 if (p.l.y_type == Y_F32)
-                    store_columns<float, H, TN>(static_cast<float*>(p.l.y) + at, p.l.ldy, acc, sxs, ch, c0, c1);
+                    store_columns<float, H, TN>(static_cast<float*>(p.l.y) + at, p.l.ldy, acc, xs_at, ch, c0, c1);
                 else if (p.l.y_type == Y_F16)
-                    store_columns<__half, H, TN>(static_cast<__half*>(p.l.y) + at, p.l.ldy, acc, sxs, ch, c0, c1);
+                    store_columns<__half, H, TN>(static_cast<__half*>(p.l.y) + at, p.l.ldy, acc, xs_at, ch, c0, c1);
                 else
-                    store_columns<__nv_bfloat16, H, TN>(static_cast<__nv_bfloat16*>(p.l.y) + at, p.l.ldy, acc, sxs, ch, c0, c1);
+                    store_columns<__nv_bfloat16, H, TN>(static_cast<__nv_bfloat16*>(p.l.y) + at, p.l.ldy, acc, xs_at, ch, c0, c1);
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cluster_relaxed(accempty_at + 8 * buf);
@@ -669,11 +695,14 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
 #pragma unroll
                     for (int h = 0; h < H; ++h) pin_after(v[h]);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
+                    for (int j = 0; j < 16; j += 2) {   // two tokens at least go to the same CTA
                         const int to = (cc + j) >> shift, tk = (cc + j) & (tokens - 1);
+                        const uint32_t at_j = base + to * slot + quad * piece + tk * (H * 128) + lane * 4;
 #pragma unroll
-                        for (int h = 0; h < H; ++h)
-                            *reinterpret_cast<uint32_t*>(base_p + to * slot + quad * piece + (tk * H + h) * 128 + lane * 4) = v[h][j];
+                        for (int h = 0; h < H; ++h) {
+                            sts32(at_j + h * 128, v[h][j]);
+                            sts32(at_j + (H + h) * 128, v[h][j + 1]);
+                        }
                     }
                 }
                 fence_proxy_async_smem();
@@ -683,21 +712,21 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
                     copy_to_peer(mapa(recv + rank * slot + quad * piece, to), base + to * slot + quad * piece, there * H * 128, mapa(partial, to));
                 __syncwarp();
                 const bool joined = mbar_wait_warp(partial, 0, limit);
-                cluster_arrive();   // what the peers sent here has left their memory
+                cluster_arrive_relaxed();   // what the peers sent here has left their memory
                 arrived = true;
                 if (!joined) {
                     give_up(ERR_WAIT_PARTIAL);
                     break;
                 }
-                const int* got = reinterpret_cast<const int*>(base_p + (recv - base) + quad * piece) + lane;
+                const uint32_t got = recv + quad * piece + lane * 4;
                 const size_t own = at + static_cast<size_t>(first) * p.l.ldy;
                 constexpr int step = Sh::kEpi / 4;
                 if (p.l.y_type == Y_F32)
-                    store_partials<float, H>(static_cast<float*>(p.l.y) + own, p.l.ldy, got, S, slot / 4, sxs, ch, mine, part, step);
+                    store_partials<float, H>(static_cast<float*>(p.l.y) + own, p.l.ldy, got, S, slot, xs_at, ch, mine, part, step);
                 else if (p.l.y_type == Y_F16)
-                    store_partials<__half, H>(static_cast<__half*>(p.l.y) + own, p.l.ldy, got, S, slot / 4, sxs, ch, mine, part, step);
+                    store_partials<__half, H>(static_cast<__half*>(p.l.y) + own, p.l.ldy, got, S, slot, xs_at, ch, mine, part, step);
                 else
-                    store_partials<__nv_bfloat16, H>(static_cast<__nv_bfloat16*>(p.l.y) + own, p.l.ldy, got, S, slot / 4, sxs, ch, mine, part, step);
+                    store_partials<__nv_bfloat16, H>(static_cast<__nv_bfloat16*>(p.l.y) + own, p.l.ldy, got, S, slot, xs_at, ch, mine, part, step);
                 break;
             }
         }
