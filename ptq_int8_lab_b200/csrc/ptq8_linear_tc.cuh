@@ -81,7 +81,7 @@ struct TcShape {
     static constexpr int kABufs = !W4 ? 0 : kPerSm == 2 ? (kColumns - 2 * kCols) / kACols / kTurns * kTurns : 256 / kACols;
     static constexpr int kACol0 = kPerSm == 2 ? 2 * kCols : 256;     // W4: first column of the operand tiles
     static constexpr int kThreads = 128 + 32 * (kEpi + kUnpack);
-    static_assert(!W4 || (kABufs >= 2 && kABufs <= 8), "operand tiles");
+    static_assert(!W4 || (kABufs >= 2 && kABufs <= 8 && kABufs % kTurns == 0), "operand tiles");
 };
 
 // ---- cluster-wide pieces
@@ -740,13 +740,14 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
         const uint32_t lanes = a_tiles + half * 32 + (static_cast<uint32_t>(quad * 32) << 16);
         const uint8_t* src = base_p + half * 8192 + row * 64;
         const int turn = (row >> 1) & 3;   // the 64-byte TMA swizzle of this row
-        // This CTA's blocks, tile after tile.  The operand tile of block i is free when block i - a_bufs is
+        // This CTA's blocks, tile after tile.  Stages and operand tiles are multiples of the turns, so that each has
+        // one set, which sees every phase of its barriers in order.  The operand tile of block i is free when block i - a_bufs is
         // released: its stage's barrier (its next phase cannot end before block i itself is unpacked).
         const int total = listed ? list[p.l.groups] : static_cast<int>((p.l.rows + TN - 1) / TN) * p.ctiles;
         const int tiles_here = t0 >= total ? 0 : S > 1 ? 1 : (total - t0 + dt - 1) / dt;
         const long long blocks = static_cast<long long>(tiles_here) * (kb1 - kb0);
         constexpr int step = Sh::kTurns;
-        int s = first, ab = first, old = first;   // kABufs is a multiple of the turns: block first + kABufs is this set's too
+        int s = first, ab = first, old = first;
         uint32_t ph = 0, oldph = 0;
         for (long long i = first; i < blocks; i += step) {
             if (!mbar_wait_warp(full + 8 * s, ph, limit)) {

@@ -204,13 +204,13 @@ struct Variant {
     int cg, tn;            // CTAs per tile, tokens per tile
     bool w4, gated;
     TcKernel kernel;
-    int threads, stage, depth, cols, acc_bufs, a_bufs, x_rows, per_sm;
+    int threads, stage, depth, cols, acc_bufs, a_bufs, turns, x_rows, per_sm;
 };
 
 template <int CG, int TN, bool W4, bool GATED>
 Variant variant() {
     using Sh = TcShape<CG, TN, W4, GATED>;
-    return {CG, TN, W4, GATED, linear_tc_kernel<CG, TN, W4, GATED>, Sh::kThreads, Sh::kStage, 128 * Sh::KD, Sh::kCols, Sh::kAccBufs, Sh::kABufs, Sh::XR, Sh::kPerSm};
+    return {CG, TN, W4, GATED, linear_tc_kernel<CG, TN, W4, GATED>, Sh::kThreads, Sh::kStage, 128 * Sh::KD, Sh::kCols, Sh::kAccBufs, Sh::kABufs, W4 ? Sh::kTurns : 1, Sh::XR, Sh::kPerSm};
 }
 
 const Variant kVariants[] = {
@@ -228,8 +228,13 @@ constexpr int kSmemTwo = 110 * 1024, kSmemOne = 222 * 1024;
 // Shared memory beside the stages: their alignment, the tile list, a split's partial sums.
 int smem_beside(const Variant& v, int split, int list_bytes) { return 1024 + list_bytes + (split > 1 ? v.cols * 128 * 4 : 0); }
 
+// Unpacking sets take turns at the blocks, and a barrier's parity tells two phases apart: each set has to wait for
+// every phase of the stages that it waits for.  So the stages are a multiple of the turns, which gives each stage
+// one set.  (Otherwise a set could ask for a stage while the load before, another set's, is still on its way, and
+// take the phase before that for the one it asks for.)
 int stages_of(const Variant& v, int split, int list_bytes) {
-    return std::min(kMaxLinStages, ((v.per_sm == 2 ? kSmemTwo : kSmemOne) - smem_beside(v, split, list_bytes)) / v.stage);
+    const int most = std::min(kMaxLinStages, ((v.per_sm == 2 ? kSmemTwo : kSmemOne) - smem_beside(v, split, list_bytes)) / v.stage);
+    return most / v.turns * v.turns;
 }
 
 int list_bytes_of(const ptq8_linear_args& a, bool listed) { return listed ? ((a.groups + 1) * 8 + 127) / 128 * 128 : 0; }
@@ -239,19 +244,19 @@ int list_bytes_of(const ptq8_linear_args& a, bool listed) { return listed ? ((a.
 // from L2, and the widening of int4 weights.  Few tiles are worth a cluster each: a split pays for sending and
 // joining its sums, and clusters of 4 and 8 do not fill every GPC.  The constants are fitted to 7200 timings of
 // 508 calls (1 to 8192 tokens, 512 to 16384 features, 1 to 64 groups, both types, gated or not) under every
-// variant: the variant of the least estimate is 2.4 % slower than the fastest one on average, 35 % at most.
+// variant: the variant of the least estimate is 1.6 % slower than the fastest one on average, 22 % at most.
 float estimate(const ptq8_ops* o, const ptq8_linear_args& a, int groups, const Variant& v, int split) {
-    constexpr float kMma = 70, kMmaTmem = 84;        // least cycles of an MMA, M operand in shared memory or TMEM
-    constexpr float kMmaTmemPair = 78;               // the latter for a pair: 4096 x 4096 x 4096 gated 100 us, one CTA a tile 105
-    constexpr float kWait = 145, kWaitTwo = 50;      // wait of the MMA warp per block (two blocks a stage)
-    constexpr float kLoad = 64;                      // bytes per cycle into an SM
-    constexpr float kWiden = 175;                    // int4: cycles of an SM per tile of 128 x 128 codes
-    constexpr float kColumn = 17.5f, kPush = 16;     // epilogue per accumulator column; sending one to a peer
-    constexpr float kSplit = 1400, kWave = 1900;     // a split tile's joining; a further wave of clusters
-    constexpr float kCluster = 570;                  // start of a launch with clusters
-    constexpr float kRagged = 0.56f;                 // part of a row tile that uneven groups waste each
-    constexpr float kFill4 = 0.92f, kFill8 = 0.82f;  // share of the SMs that clusters of 4 and of 8 can take
-    constexpr float kPacked = 0.75f;                 // CTAs per SM from which two come to share one
+    constexpr float kMma = 77.5f, kMmaTmem = 104;    // least cycles of an MMA, M operand in shared memory or TMEM
+    constexpr float kMmaTmemPair = 102;              // the latter for a pair: 4096 x 4096 x 4096 gated 100 us, one CTA a tile 105
+    constexpr float kWait = 144, kWaitTwo = 47;      // wait of the MMA warp per block (two blocks a stage)
+    constexpr float kLoad = 61;                      // bytes per cycle into an SM
+    constexpr float kWiden = 225;                    // int4: cycles of an SM per tile of 128 x 128 codes
+    constexpr float kColumn = 12, kPush = 54;        // epilogue per accumulator column; sending one to a peer
+    constexpr float kSplit = 645, kWave = 1055;      // a split tile's joining; a further wave of clusters
+    constexpr float kCluster = 430;                  // start of a launch with clusters
+    constexpr float kRagged = 0.62f;                 // part of a row tile that uneven groups waste each
+    constexpr float kFill4 = 0.96f, kFill8 = 0.82f;  // share of the SMs that clusters of 4 and of 8 can take
+    constexpr float kPacked = 0.47f;                 // CTAs per SM from which two come to share one
     const float h = v.gated ? 2 : 1, rows = static_cast<float>(a.rows);
     const float used = static_cast<float>(std::min<long long>(groups, a.rows)), mean = rows / used;
     const float row_tiles = groups > 1 ? std::max(used, std::ceil(used * (mean / v.tn + kRagged))) : std::ceil(rows / v.tn);
