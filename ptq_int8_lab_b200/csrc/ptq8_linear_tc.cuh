@@ -19,10 +19,10 @@
 //
 // What bounds it (B200; device time in a graph, operands from DRAM):
 //   many tokens        4096 x 4096 x 8192 int8 88 us: 3.1 POP/s, the tensor pipe active 87 % of the time, at
-//                      the clock that the power limit leaves (int4 92 us; gated 92 and 100 us: two weight tiles
+//                      the clock that the power limit leaves (int4 92 us; gated 92 and 104 us: two weight tiles
 //                      to one of tokens, bound by the 64 bytes a cycle that an SM draws from L2)
 //   hundreds           512 x 4096 x 4096 12 us: again L2 to SM, and too few tiles to share them more
-//   few                16 x 4096 x 4096 7 us: latency (set-up 1, first bytes 1, partial sums 1 us), then an MMA
+//   few                16 x 4096 x 4096 6.5 us: latency (set-up 1, first bytes 1, partial sums 0.7 us), then an MMA
 //                      of 16 columns, which takes 55 to 75 cycles instead of 8
 //
 // Warps: 0 TMA producer, 1 MMA issuer, 2 TMEM and the groups' tile list, 4.. epilogue, then
@@ -72,7 +72,7 @@ struct TcShape {
     static constexpr int kPerSm = TN <= (W4 && GATED ? 32 : 64) ? 2 : 1;
     static constexpr int kColumns = 512 / kPerSm;          // of TMEM
     static constexpr int kUnpack = !W4 ? 0 : kPerSm == 2 ? 8 : 16;   // unpacking warps
-    static constexpr int kTurns = kUnpack / (4 * H);       // sets of them that take turns at the blocks
+    static constexpr int kTurns = W4 ? kUnpack / (4 * H) : 1;   // sets of them that take turns at the blocks
     // Two accumulators where TMEM holds them.  With int4 weights the operand tiles have half of it (what two
     // accumulators leave, where CTAs share an SM): they hide the way from the MMAs' release of a tile to its
     // next use.  4096 x 4096 x 4096 gated: 99 us with one accumulator and four operand tiles, 150 us with

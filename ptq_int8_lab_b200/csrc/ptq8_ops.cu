@@ -210,7 +210,7 @@ struct Variant {
 template <int CG, int TN, bool W4, bool GATED>
 Variant variant() {
     using Sh = TcShape<CG, TN, W4, GATED>;
-    return {CG, TN, W4, GATED, linear_tc_kernel<CG, TN, W4, GATED>, Sh::kThreads, Sh::kStage, 128 * Sh::KD, Sh::kCols, Sh::kAccBufs, Sh::kABufs, W4 ? Sh::kTurns : 1, Sh::XR, Sh::kPerSm};
+    return {CG, TN, W4, GATED, linear_tc_kernel<CG, TN, W4, GATED>, Sh::kThreads, Sh::kStage, 128 * Sh::KD, Sh::kCols, Sh::kAccBufs, Sh::kABufs, Sh::kTurns, Sh::XR, Sh::kPerSm};
 }
 
 const Variant kVariants[] = {

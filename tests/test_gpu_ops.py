@@ -507,6 +507,26 @@ def test_same_outputs_every_time(ops):
             assert torch.equal(first, ops.linear(*a, bias=dev(b), act=int(gated)))
 
 
+@pytest.mark.parametrize("rows,k,n,gated", [(3000, 8192, 80, False), (2000, 4096, 600, False), (500, 4096, 512, True),
+                                            (48, 8192, 1024, False)])
+def test_int4_many_launches(ops, rows, k, n, gated):
+    """int4 tiles whose loads come from cold memory, over and over: the stages that the unpacking warps share in turns
+    hold each launch's own weights.  Four weight sets in turn, each output equal to its first."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    ch = 2 * n if gated else n
+    x = torch.randint(-128, 128, (rows, k), generator=g, device="cuda", dtype=torch.int8)
+    xs, ws = torch.rand(rows, generator=g, device="cuda") + 0.1, torch.rand(ch, generator=g, device="cuda") * 1e-5
+    w = [torch.randint(0, 256, (ch, k // 2), generator=g, device="cuda", dtype=torch.uint8) for _ in range(4)]
+    first = [ops.linear(x, xs, v, ws, bits=4, act=int(gated)) for v in w]
+    flush = torch.empty(160 << 20, dtype=torch.uint8, device="cuda")
+    wrong = torch.zeros((), dtype=torch.int64, device="cuda")
+    for i in range(160):
+        flush.fill_(i & 1)
+        wrong += (ops.linear(x, xs, w[i % 4], ws, bits=4, act=int(gated)) != first[i % 4]).sum()
+    assert int(wrong) == 0
+    ops.check_device_error()
+
+
 def _ok():
     z = lambda *s, t=torch.int8: torch.zeros(s, dtype=t, device="cuda")   # noqa: E731
     return dict(x=z(4, 64), x_scale=z(4, t=torch.float32), w=z(32, 64), w_scale=z(32, t=torch.float32))
