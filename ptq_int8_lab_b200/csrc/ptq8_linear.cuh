@@ -42,8 +42,54 @@ __device__ __forceinline__ float dequant(int acc, float xs, float ws, float bias
     return __fadd_rn(__fmul_rn(__int2float_rn(acc), __fmul_rn(xs, ws)), bias);
 }
 
-// silu(g) * u.  exp(-g) overflows to infinity below g = -88, where the quotient is -0.
-__device__ __forceinline__ float swiglu(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
+// silu(g) * u = g / (1 + exp(-g)) * u.
+//
+// exp(-g) = 2^t, t = -g log2(e): t's rounding alone would cost |g| units in the last place, so the rest that it leaves
+// (exact in one FMA, plus log2(e)'s own rest) goes into the result as 1 + rest * ln 2.  Errors in units of 2^-23:
+// exponential 2.5, sum 1/2, reciprocal 1, two products 1/2 each.  (With expf and an IEEE quotient 4096 tokens of 4096 ->
+// 2 x 8192 int4 took 272 us instead of 204: the next tile waits for the epilogue's instructions.)
+//
+// Beyond |g| = 64, which is rare, exp(-g) leaves a float's range before the quotient does (a normal number down to
+// g = -91.8), and the rest of an infinite t is not a number.  There, far below zero, the quotient is g exp(g) to the last
+// place, exp(g) in two factors: exp(g + 64), the sum exact, and exp(-64).
+constexpr float kSiluNear = 64.0f;
+constexpr float kLog2e = 0x1.715476p+0f, kLog2eRest = 0x1.4ae0cp-26f, kLn2 = 0x1.62e43p-1f;
+
+__device__ __forceinline__ float ex2_approx(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float rcp_approx(float v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float silu_far(float g) {
+    if (g > 0.0f) return g;   // 1 + exp(-g) is 1
+    return g * expf(g + 64.0f) * 1.6038108905486378e-28f;
+}
+__device__ __forceinline__ float swiglu(float g, float u) {
+    if (fabsf(g) > kSiluNear) return silu_far(g) * u;
+    const float t = __fmul_rn(g, -kLog2e);
+    const float rest = __fmaf_rn(g, kLog2eRest, __fmaf_rn(g, kLog2e, t));   // what t leaves, its sign turned
+    const float e = ex2_approx(t);
+    const float d = __fmaf_rn(e, __fmul_rn(rest, -kLn2), __fadd_rn(e, 1.0f));
+    return __fmul_rn(__fmul_rn(g, rcp_approx(d)), u);
+}
+
+// The near steps of swiglu() for two outputs at once.  `most` takes in the denominators: below 2^92 at the end, every gate
+// was one that these steps serve (above -63.8; far above zero they give g too).
+constexpr float kSwigluMost = 0x1p92f;
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 swiglu2(float2 g, float2 u, float2& most) {
+    const float2 t = __fmul2_rn(g, both(-kLog2e));
+    const float2 rest = __ffma2_rn(g, both(kLog2eRest), __ffma2_rn(g, both(kLog2e), t));
+    const float2 e = make_float2(ex2_approx(t.x), ex2_approx(t.y));
+    const float2 d = __ffma2_rn(e, __fmul2_rn(rest, both(-kLn2)), __fadd2_rn(e, both(1.0f)));
+    most = __fadd2_rn(most, d);
+    return __fmul2_rn(__fmul2_rn(g, make_float2(rcp_approx(d.x), rcp_approx(d.y))), u);
+}
 
 // Rows of group g, clamped into [0, rows].
 __device__ __forceinline__ void group_rows(const LinearParams& p, int g, long long& beg, long long& end) {

@@ -12,10 +12,10 @@
 //         arrival changes nothing.
 //   GATED: two accumulators per tile, gate and up channels, joined in the epilogue.
 //   W4: weights arrive packed; eight or sixteen warps widen them as 16 times the code (the nibble moved to
-//       its byte's high half: no sign extension; the channel's scale carries the exact factor
-//       1/16) and write them to TMEM, from where the MMA takes its M operand.  A thread owns
-//       a channel, which is a TMEM lane.  Through shared memory the same took twice the time:
-//       writing the widened tile and the MMA's reads of it filled shared memory's bandwidth.
+//       its byte's high half: no sign extension; the channel's scale carries 1/16) and write them to TMEM,
+//       from where the MMA takes its M operand.  A thread owns a channel, which is a TMEM lane.  Through
+//       shared memory the same took twice the time: writing the widened tile and the MMA's reads of it
+//       filled shared memory's bandwidth.
 //
 // What bounds it (B200; device time in a graph, operands from DRAM):
 //   many tokens        4096 x 4096 x 8192 int8 88 us: 3.1 POP/s, the tensor pipe active 87 % of the time, at
@@ -247,6 +247,26 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32
         "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
         : "memory");
 }
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&v)[16]) { tmem_ld16(taddr, v); }
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&v)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                 : "r"(taddr));
+}
+__device__ __forceinline__ void pin(uint32_t (&v)[16]) { pin_after(v); }
+__device__ __forceinline__ void pin(uint32_t (&v)[8]) {
+    asm volatile("" : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]));
+}
+// One column; read through pinned() once it has been waited for.
+__device__ __forceinline__ uint32_t tmem_ld1(uint32_t taddr) {
+    uint32_t v;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(v) : "r"(taddr));
+    return v;
+}
+__device__ __forceinline__ int pinned(uint32_t v) {
+    asm volatile("" : "+r"(v));
+    return static_cast<int>(v);
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // ---- tiles
@@ -322,36 +342,66 @@ __device__ __forceinline__ Channel<H> channel_of(const LinearParams& l, int grou
     return ch;
 }
 
+// A lane's outputs for two tokens, each step on both at once.  With SwiGLU: right where `most` stays below kSwigluMost.
 template <int H>
-__device__ __forceinline__ float finish(const Channel<H>& ch, float xs, int a0, int a1) {
-    const float v = dequant(a0, xs, ch.ws[0], ch.b[0]);
-    return H == 2 ? swiglu(v, dequant(a1, xs, ch.ws[H - 1], ch.b[H - 1])) : v;
+__device__ __forceinline__ float2 finish2(const Channel<H>& ch, float2 xs, const int2 (&a)[H], float2& most) {
+    float2 v[H];
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+        float2 acc = make_float2(__int2float_rn(a[h].x), __int2float_rn(a[h].y));
+        // dequant(); the last sum one by one, since the compiler fuses a packed product and sum
+        acc = __fmul2_rn(acc, __fmul2_rn(xs, both(ch.ws[h])));
+        v[h] = make_float2(__fadd_rn(acc.x, ch.b[h]), __fadd_rn(acc.y, ch.b[h]));
+    }
+    return H == 2 ? swiglu2(v[0], v[H - 1], most) : v[0];
+}
+// One output, whatever its gate.
+__device__ __forceinline__ float finish_far(const Channel<2>& ch, float xs, int a0, int a1) {
+    return swiglu(dequant(a0, xs, ch.ws[0], ch.b[0]), dequant(a1, xs, ch.ws[1], ch.b[1]));
 }
 
-// Columns [c0, c1) of a warp's 32 accumulator lanes -> y.  xs: shared address of their token scales, from column c0 on.
-template <typename T, int H, int TN>
+// Columns [c0, c1) of a warp's 32 accumulator lanes -> y.  xs: shared address of their token scales, from column c0 on
+// (zero past the end).
+template <typename T, int H, bool W4, int TN>
 __device__ __forceinline__ void store_columns(T* y, size_t ldy, uint32_t acc, uint32_t xs, const Channel<H>& ch, int c0, int c1) {
-    for (int c = c0; c < c1; c += 16, xs += 64) {
-        uint32_t v[16], u[16];
-        tmem_ld16(acc + c, v);
-        if (H == 2) tmem_ld16(acc + TN + c, u);
-        const float4 x4[4] = {lds128f(xs), lds128f(xs + 16), lds128f(xs + 32), lds128f(xs + 48)};
+    // Columns at a time: eight where the unpackers leave few registers (4096 x 4096 -> 2 x 8192: 204 us, with sixteen 209).
+    constexpr int N = W4 && H == 2 ? 8 : 16;
+    for (int c = c0; c < c1; c += N, xs += 4 * N) {
+        uint32_t v[N], u[N];
+        tmem_ld(acc + c, v);
+        if (H == 2) tmem_ld(acc + TN + c, u);
         tmem_wait_ld();
-        pin_after(v);
-        if (H == 2) pin_after(u);
-        T* out = y + static_cast<size_t>(c) * ldy;
+        pin(v);
+        if (H == 2) pin(u);
+        T* const out = y + static_cast<size_t>(c) * ldy;
         const int left = c1 - c;
+        float2 most = both(0.0f);
+        T* o = out;
 #pragma unroll
-        for (int j = 0; j < 16; j += 4) {
-            const float xf[4] = {x4[j / 4].x, x4[j / 4].y, x4[j / 4].z, x4[j / 4].w};
-            float r[4];
+        for (int j = 0; j < N; j += 4) {
+            const float4 x4 = lds128f(xs + 4 * j);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                r[i] = finish<H>(ch, xf[i], static_cast<int>(v[j + i]), H == 2 ? static_cast<int>(u[j + i]) : 0);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (ch.ok && j + i < left) *out = from_f32<T>(r[i]);
-                out += ldy;
+            for (int i = j; i < j + 4; i += 2) {
+                int2 a[H];
+                a[0] = make_int2(v[i], v[i + 1]);
+                if (H == 2) a[H - 1] = make_int2(u[i], u[i + 1]);
+                const float2 r = finish2<H>(ch, i & 2 ? make_float2(x4.z, x4.w) : make_float2(x4.x, x4.y), a, most);
+                if (ch.ok && i < left) *o = from_f32<T>(r.x);
+                o += ldy;
+                if (ch.ok && i + 1 < left) *o = from_f32<T>(r.y);
+                o += ldy;
+            }
+        }
+        if constexpr (H == 2) {
+            if (__any_sync(0xffffffffu, !(most.x + most.y < kSwigluMost))) {   // rare: once more, one by one
+                o = out;
+#pragma unroll 1
+                for (int j = 0; j < min(left, N); ++j, o += ldy) {
+                    const uint32_t g1 = tmem_ld1(acc + c + j), u1 = tmem_ld1(acc + TN + c + j);
+                    tmem_wait_ld();
+                    const float r = finish_far(ch, __int_as_float(lds32(xs + 4 * j)), pinned(g1), pinned(u1));
+                    if (ch.ok) *o = from_f32<T>(r);
+                }
             }
         }
     }
@@ -371,11 +421,29 @@ __device__ __forceinline__ void store_partials(T* y, size_t ldy, uint32_t got, i
 #pragma unroll
                 for (int h = 0; h < H; ++h) a[i][h] += lds32(got + s * cta + (min(t + i * step, mine - 1) * H + h) * 128);
         const float4 x4 = lds128f(xs);
-        const float xf[4] = {x4.x, x4.y, x4.z, x4.w};
+        float2 most = both(0.0f);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float r = finish<H>(ch, xf[i], a[i][0], a[i][H - 1]);
-            if (ch.ok && t + i * step < mine) y[static_cast<size_t>(t + i * step) * ldy] = from_f32<T>(r);
+        for (int i = 0; i < 4; i += 2) {
+            int2 b[H];
+#pragma unroll
+            for (int h = 0; h < H; ++h) b[h] = make_int2(a[i][h], a[i + 1][h]);
+            const float2 r = finish2<H>(ch, i ? make_float2(x4.z, x4.w) : make_float2(x4.x, x4.y), b, most);
+            if (ch.ok && t + i * step < mine) y[static_cast<size_t>(t + i * step) * ldy] = from_f32<T>(r.x);
+            if (ch.ok && t + (i + 1) * step < mine) y[static_cast<size_t>(t + (i + 1) * step) * ldy] = from_f32<T>(r.y);
+        }
+        if constexpr (H == 2) {
+            if (!(most.x + most.y < kSwigluMost)) {   // rare: once more, one by one
+#pragma unroll 1
+                for (int i = t, k = 0; i < min(mine, t + 4 * step); i += step, ++k) {
+                    int g1 = 0, u1 = 0;
+                    for (int s = 0; s < S; ++s) {
+                        g1 += lds32(got + s * cta + i * 256);
+                        u1 += lds32(got + s * cta + i * 256 + 128);
+                    }
+                    const float r = finish_far(ch, __int_as_float(lds32(xs + 4 * k)), g1, u1);
+                    if (ch.ok) y[static_cast<size_t>(i) * ldy] = from_f32<T>(r);
+                }
+            }
         }
     }
 }
@@ -653,10 +721,11 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
             const int tokens = TN / S, first = S > 1 ? static_cast<int>(rank) * tokens : 0, mine = min(max(tile.valid - first, 0), tokens);
             __syncwarp();
             if (S == 1) {
-                for (int i = lane; c0 + i < c1; i += 32) sxs[i] = p.l.xs[tile.row0 + c0 + i];
+                for (int i = lane; i < (max(c1 - c0, 0) + 15) / 16 * 16; i += 32) sxs[i] = c0 + i < c1 ? p.l.xs[tile.row0 + c0 + i] : 0.0f;
             } else {   // of the tokens that this warp finishes
                 constexpr int step = Sh::kEpi / 4;
-                for (int t = part + lane * step; t < mine; t += 32 * step) sxs[t / step] = p.l.xs[tile.row0 + first + t];
+                for (int t = part + lane * step; t < (mine + 4 * step - 1) / (4 * step) * 4 * step; t += 32 * step)
+                    sxs[t / step] = t < mine ? p.l.xs[tile.row0 + first + t] : 0.0f;
             }
             __syncwarp();
             if (!mbar_wait_warp(accfull + 8 * buf, accph, limit)) {
@@ -668,11 +737,11 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
             const size_t at = static_cast<size_t>(tile.row0) * p.l.ldy + c;
             if (CG == 2 || S == 1) {
                 if (p.l.y_type == Y_F32)
-                    store_columns<float, H, TN>(static_cast<float*>(p.l.y) + at, p.l.ldy, acc, xs_at, ch, c0, c1);
+                    store_columns<float, H, W4, TN>(static_cast<float*>(p.l.y) + at, p.l.ldy, acc, xs_at, ch, c0, c1);
                 else if (p.l.y_type == Y_F16)
-                    store_columns<__half, H, TN>(static_cast<__half*>(p.l.y) + at, p.l.ldy, acc, xs_at, ch, c0, c1);
+                    store_columns<__half, H, W4, TN>(static_cast<__half*>(p.l.y) + at, p.l.ldy, acc, xs_at, ch, c0, c1);
                 else
-                    store_columns<__nv_bfloat16, H, TN>(static_cast<__nv_bfloat16*>(p.l.y) + at, p.l.ldy, acc, xs_at, ch, c0, c1);
+                    store_columns<__nv_bfloat16, H, W4, TN>(static_cast<__nv_bfloat16*>(p.l.y) + at, p.l.ldy, acc, xs_at, ch, c0, c1);
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cluster_relaxed(accempty_at + 8 * buf);
