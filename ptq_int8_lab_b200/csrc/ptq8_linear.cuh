@@ -36,8 +36,9 @@ __device__ __forceinline__ void store_y(void* y, size_t at, float v, int type) {
         static_cast<__nv_bfloat16*>(y)[at] = __float2bfloat16_rn(v);
 }
 
-// Two roundings, then one more for the bias: the engine's dequantization.  A packed int4 code
-// stands in the high half of its byte wherever `f` carries the exact factor 1/16.
+// Two roundings, then one more for the bias: the engine's dequantization.  (Where packed int4 codes are multiplied as
+// 16 times the code, `acc` is the sum shifted back: with 1/16 in the scale the product of scales could lose places
+// near the smallest normal number.)
 __device__ __forceinline__ float dequant(int acc, float xs, float ws, float bias) {
     return __fadd_rn(__fmul_rn(__int2float_rn(acc), __fmul_rn(xs, ws)), bias);
 }

@@ -53,7 +53,7 @@ __device__ __forceinline__ FewCodes<W4> few_codes(const uint4& a, const uint4& b
 template <bool W4>
 __device__ __forceinline__ int few_dot(const uint4& w, const FewCodes<W4>& c, int acc) {
     if (!W4) return dot16(w, c.even, acc);
-    // 16 times each code, in its byte's high half
+    // 16 times each code, in its byte's high half (the sum is shifted back)
     const uint32_t m = 0xF0F0F0F0u;
     acc = dot16(make_uint4((w.x << 4) & m, (w.y << 4) & m, (w.z << 4) & m, (w.w << 4) & m), c.even, acc);
     return dot16(make_uint4(w.x & m, w.y & m, w.z & m, w.w & m), c.odd, acc);
@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, MT == 4 ? 2 : 4) linear_few_ke
     const int r_lane = lane / MT, t_lane = lane % MT, c = c0 + r_lane % C;
     const bool mine_ok = part == 0 && lane < kFewRows * MT && c < l.n && beg < end;
     const size_t at = static_cast<size_t>(g) * (l.n * H) + (r_lane / C) * l.n + c;
-    const float ws = mine_ok ? l.ws[at] * (W4 ? 0.0625f : 1.0f) : 0.0f;
+    const float ws = mine_ok ? l.ws[at] : 0.0f;
     const float bias = mine_ok && l.bias ? l.bias[at] : 0.0f;
     for (long long t0 = beg; t0 < end; t0 += MT) {
         const int tokens = static_cast<int>(min(static_cast<long long>(MT), end - t0));
@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, MT == 4 ? 2 : 4) linear_few_ke
             if (part == 0 && lane < kFewRows * MT)
                 for (int i = 1; i < p.ks; ++i) mine += sums[warp + i][lane];
         }
-        float v = here ? dequant(mine, xs, ws, bias) : 0.0f;
+        float v = here ? dequant(W4 ? mine >> 4 : mine, xs, ws, bias) : 0.0f;
         if (GATED) v = swiglu(v, __shfl_down_sync(0xffffffffu, v, C * MT));
         if (here && r_lane < C) store_y(l.y, static_cast<size_t>(t0 + t_lane) * l.ldy + c, v, l.y_type);
         if (p.ks > 1) __syncthreads();

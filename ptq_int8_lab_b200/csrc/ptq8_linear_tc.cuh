@@ -12,7 +12,7 @@
 //         arrival changes nothing.
 //   GATED: two accumulators per tile, gate and up channels, joined in the epilogue.
 //   W4: weights arrive packed; eight or sixteen warps widen them as 16 times the code (the nibble moved to
-//       its byte's high half: no sign extension; the channel's scale carries 1/16) and write them to TMEM,
+//       its byte's high half: no sign extension; the epilogue takes the factor out) and write them to TMEM,
 //       from where the MMA takes its M operand.  A thread owns a channel, which is a TMEM lane.  Through
 //       shared memory the same took twice the time: writing the widened tile and the MMA's reads of it
 //       filled shared memory's bandwidth.
@@ -329,26 +329,27 @@ struct Channel {
     bool ok;
 };
 
-template <int H, bool W4>
+template <int H>
 __device__ __forceinline__ Channel<H> channel_of(const LinearParams& l, int group, int c) {
     Channel<H> ch;
     ch.ok = c < l.n;
 #pragma unroll
     for (int h = 0; h < H; ++h) {
         const size_t at = static_cast<size_t>(group) * (l.n * H) + h * l.n + c;
-        ch.ws[h] = ch.ok ? l.ws[at] * (W4 ? 0.0625f : 1.0f) : 0.0f;
+        ch.ws[h] = ch.ok ? l.ws[at] : 0.0f;
         ch.b[h] = ch.ok && l.bias ? l.bias[at] : 0.0f;
     }
     return ch;
 }
 
 // A lane's outputs for two tokens, each step on both at once.  With SwiGLU: right where `most` stays below kSwigluMost.
-template <int H>
+template <int H, bool W4>
 __device__ __forceinline__ float2 finish2(const Channel<H>& ch, float2 xs, const int2 (&a)[H], float2& most) {
     float2 v[H];
 #pragma unroll
     for (int h = 0; h < H; ++h) {
         float2 acc = make_float2(__int2float_rn(a[h].x), __int2float_rn(a[h].y));
+        if (W4) acc = __fmul2_rn(acc, both(0.0625f));   // the codes were multiplied as 16 times their value
         // dequant(); the last sum one by one, since the compiler fuses a packed product and sum
         acc = __fmul2_rn(acc, __fmul2_rn(xs, both(ch.ws[h])));
         v[h] = make_float2(__fadd_rn(acc.x, ch.b[h]), __fadd_rn(acc.y, ch.b[h]));
@@ -356,8 +357,10 @@ __device__ __forceinline__ float2 finish2(const Channel<H>& ch, float2 xs, const
     return H == 2 ? swiglu2(v[0], v[H - 1], most) : v[0];
 }
 // One output, whatever its gate.
+template <bool W4>
 __device__ __forceinline__ float finish_far(const Channel<2>& ch, float xs, int a0, int a1) {
-    return swiglu(dequant(a0, xs, ch.ws[0], ch.b[0]), dequant(a1, xs, ch.ws[1], ch.b[1]));
+    constexpr int shift = W4 ? 4 : 0;
+    return swiglu(dequant(a0 >> shift, xs, ch.ws[0], ch.b[0]), dequant(a1 >> shift, xs, ch.ws[1], ch.b[1]));
 }
 
 // Columns [c0, c1) of a warp's 32 accumulator lanes -> y.  xs: shared address of their token scales, from column c0 on
@@ -385,7 +388,7 @@ __device__ __forceinline__ void store_columns(T* y, size_t ldy, uint32_t acc, ui
                 int2 a[H];
                 a[0] = make_int2(v[i], v[i + 1]);
                 if (H == 2) a[H - 1] = make_int2(u[i], u[i + 1]);
-                const float2 r = finish2<H>(ch, i & 2 ? make_float2(x4.z, x4.w) : make_float2(x4.x, x4.y), a, most);
+                const float2 r = finish2<H, W4>(ch, i & 2 ? make_float2(x4.z, x4.w) : make_float2(x4.x, x4.y), a, most);
                 if (ch.ok && i < left) *o = from_f32<T>(r.x);
                 o += ldy;
                 if (ch.ok && i + 1 < left) *o = from_f32<T>(r.y);
@@ -399,7 +402,7 @@ __device__ __forceinline__ void store_columns(T* y, size_t ldy, uint32_t acc, ui
                 for (int j = 0; j < min(left, N); ++j, o += ldy) {
                     const uint32_t g1 = tmem_ld1(acc + c + j), u1 = tmem_ld1(acc + TN + c + j);
                     tmem_wait_ld();
-                    const float r = finish_far(ch, __int_as_float(lds32(xs + 4 * j)), pinned(g1), pinned(u1));
+                    const float r = finish_far<W4>(ch, __int_as_float(lds32(xs + 4 * j)), pinned(g1), pinned(u1));
                     if (ch.ok) *o = from_f32<T>(r);
                 }
             }
@@ -410,7 +413,7 @@ __device__ __forceinline__ void store_columns(T* y, size_t ldy, uint32_t acc, ui
 // The finishing half of a split tile: the S partial sums of this CTA's tokens, every step-th of them from `part`
 // on, four at a time.  got: shared address of this lane's channel of the first token of the first CTA; a token is
 // H * 128 bytes further, a CTA `cta` bytes.  xs: shared address of the scales of the tokens that this warp finishes.
-template <typename T, int H>
+template <typename T, int H, bool W4>
 __device__ __forceinline__ void store_partials(T* y, size_t ldy, uint32_t got, int S, int cta, uint32_t xs, const Channel<H>& ch,
                                                int mine, int part, int step) {
     for (int t = part; t < mine; t += 4 * step, xs += 16) {
@@ -427,7 +430,7 @@ __device__ __forceinline__ void store_partials(T* y, size_t ldy, uint32_t got, i
             int2 b[H];
 #pragma unroll
             for (int h = 0; h < H; ++h) b[h] = make_int2(a[i][h], a[i + 1][h]);
-            const float2 r = finish2<H>(ch, i ? make_float2(x4.z, x4.w) : make_float2(x4.x, x4.y), b, most);
+            const float2 r = finish2<H, W4>(ch, i ? make_float2(x4.z, x4.w) : make_float2(x4.x, x4.y), b, most);
             if (ch.ok && t + i * step < mine) y[static_cast<size_t>(t + i * step) * ldy] = from_f32<T>(r.x);
             if (ch.ok && t + (i + 1) * step < mine) y[static_cast<size_t>(t + (i + 1) * step) * ldy] = from_f32<T>(r.y);
         }
@@ -440,7 +443,7 @@ __device__ __forceinline__ void store_partials(T* y, size_t ldy, uint32_t got, i
                         g1 += lds32(got + s * cta + i * 256);
                         u1 += lds32(got + s * cta + i * 256 + 128);
                     }
-                    const float r = finish_far(ch, __int_as_float(lds32(xs + 4 * k)), g1, u1);
+                    const float r = finish_far<W4>(ch, __int_as_float(lds32(xs + 4 * k)), g1, u1);
                     if (ch.ok) y[static_cast<size_t>(i) * ldy] = from_f32<T>(r);
                 }
             }
@@ -715,7 +718,7 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
         uint32_t accph = 0;
         for (int t = t0; tiles.get(t, tile); t += dt) {
             const int c = (tile.ct * CG + static_cast<int>(CG == 2 ? rank : 0)) * 128 + lane_c;
-            const Channel<H> ch = channel_of<H, W4>(p.l, tile.group, c);
+            const Channel<H> ch = channel_of<H>(p.l, tile.group, c);
             const int c0 = part * Sh::kCW, c1 = min(c0 + Sh::kCW, tile.valid);
             // split: this CTA's tokens of the tile
             const int tokens = TN / S, first = S > 1 ? static_cast<int>(rank) * tokens : 0, mine = min(max(tile.valid - first, 0), tokens);
@@ -791,11 +794,11 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
                 const size_t own = at + static_cast<size_t>(first) * p.l.ldy;
                 constexpr int step = Sh::kEpi / 4;
                 if (p.l.y_type == Y_F32)
-                    store_partials<float, H>(static_cast<float*>(p.l.y) + own, p.l.ldy, got, S, slot, xs_at, ch, mine, part, step);
+                    store_partials<float, H, W4>(static_cast<float*>(p.l.y) + own, p.l.ldy, got, S, slot, xs_at, ch, mine, part, step);
                 else if (p.l.y_type == Y_F16)
-                    store_partials<__half, H>(static_cast<__half*>(p.l.y) + own, p.l.ldy, got, S, slot, xs_at, ch, mine, part, step);
+                    store_partials<__half, H, W4>(static_cast<__half*>(p.l.y) + own, p.l.ldy, got, S, slot, xs_at, ch, mine, part, step);
                 else
-                    store_partials<__nv_bfloat16, H>(static_cast<__nv_bfloat16*>(p.l.y) + own, p.l.ldy, got, S, slot, xs_at, ch, mine, part, step);
+                    store_partials<__nv_bfloat16, H, W4>(static_cast<__nv_bfloat16*>(p.l.y) + own, p.l.ldy, got, S, slot, xs_at, ch, mine, part, step);
                 break;
             }
         }

@@ -48,3 +48,31 @@ def test_swiglu_over_the_range(ops, rows, k, pad, bits, up):
     tol = np.abs(want) * 5 * 2.0 ** -23 * (1 + 1e-6) + 2.0 ** -149 * (1 + abs(u))
     assert np.all(np.abs(y.astype(np.float64) - want)[:, inside] <= tol[inside])
     assert np.all(y[:, ~inside] == np.where(want[~inside] > 0, np.inf, -np.inf).astype(np.float32))
+
+
+def pack4(c):
+    """int8 codes in [-8, 7] -> two per byte, the even one in the low half."""
+    if c.shape[-1] % 2:
+        c = np.concatenate([c, np.zeros((*c.shape[:-1], 1), np.int8)], axis=-1)
+    return ((c[..., 0::2] & 15) | ((c[..., 1::2] & 15) << 4)).astype(np.uint8)
+
+
+@pytest.mark.parametrize("rows,k,pad", PATHS)
+@pytest.mark.parametrize("bits", [8, 4])
+def test_scales_near_the_smallest_normal_number(ops, rows, k, pad, bits):
+    """Products of scales from 2^-150 to 2^-120, so normal, subnormal and zero ones: bit for bit the definition's two
+    roundings in numpy's 32 bits, on every kernel."""
+    rng = np.random.default_rng(rows + bits)
+    n = 300
+    x = rng.integers(-128, 128, (rows, k), dtype=np.int8)
+    w = rng.integers(-8, 8, (n, k), dtype=np.int8)
+    xs = np.exp2(rng.uniform(-65, -60, rows)).astype(np.float32)
+    ws = np.exp2(rng.uniform(-85, -60, n)).astype(np.float32)
+    xd, wc = strided(rows, k, pad), w if bits == 8 else pack4(w)
+    xd.copy_(torch.from_numpy(x))
+    wd = strided(*wc.shape, pad, torch.int8 if bits == 8 else torch.uint8)
+    wd.copy_(torch.from_numpy(wc))
+    y = ops.linear(xd, torch.from_numpy(xs).cuda(), wd, torch.from_numpy(ws).cuda(), bits=bits, dtype=torch.float32).cpu().numpy()
+    acc = (x.astype(np.int64) @ w.astype(np.int64).T).astype(np.float32)
+    want = acc * (xs[:, None] * ws[None, :])
+    assert np.array_equal(y.view(np.int32), (want + np.float32(0)).view(np.int32))
