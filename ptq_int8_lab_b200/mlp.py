@@ -93,7 +93,7 @@ class Int8Experts:
         h = o.linear_grouped(codes, scale, offsets, *self.gate_up, bits=self.bits, act=EPI_SWIGLU, dtype=x.dtype)
         codes, scale = o.quantize_rows(h)
         y = o.linear_grouped(codes, scale, offsets, *self.down, bits=self.bits, dtype=torch.float32)
-        y = y[where].view(x.shape[0], self.top, -1)
+        y = y[where].view(x.shape[0], self.top, y.shape[1])
         return (y * weight[..., None]).sum(dim=1).to(x.dtype)
 
 
