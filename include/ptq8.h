@@ -306,6 +306,8 @@ typedef struct ptq8_ops ptq8_ops;
 /* int32 sums of in_features products of codes of magnitude <= 128 never overflow up to here */
 #define PTQ8_MAX_IN_FEATURES 131071
 #define PTQ8_MAX_GROUPS 1024
+/* widest row of quantize_rows: its vectors of 4 or 8 values end within an int */
+#define PTQ8_MAX_ROW_WIDTH 0x7FFFFFF0
 
 ptq8_ops* ptq8_ops_create(int device, char* err, size_t errlen);
 void ptq8_ops_destroy(ptq8_ops* ops); /* the caller has synchronised the streams it used */

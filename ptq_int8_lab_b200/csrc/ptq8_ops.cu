@@ -103,7 +103,8 @@ int cuda_fail(ptq8_ops* o, const char* what, cudaError_t e) {
 int check_rows(ptq8_ops* o, const ptq8_rows_args& a) {
     const char* w = "quantize_rows";
     if (a.x_type < PTQ8_F32 || a.x_type > PTQ8_BF16) return fail(o, PTQ8_ERR_INVALID, "%s: x_type %d", w, a.x_type);
-    if (a.width <= 0) return fail(o, PTQ8_ERR_INVALID, "%s: width %d", w, a.width);
+    if (a.width <= 0 || a.width > PTQ8_MAX_ROW_WIDTH)
+        return fail(o, PTQ8_ERR_INVALID, "%s: width %d (1 to %d)", w, a.width, PTQ8_MAX_ROW_WIDTH);
     if (a.x_rows < 0 || a.n_rows < 0 || a.n_rows > 0x7FFFFFFFLL)
         return fail(o, PTQ8_ERR_INVALID, "%s: x_rows %lld, n_rows %lld", w, a.x_rows, a.n_rows);
     if (!a.rows && a.n_rows != a.x_rows)
