@@ -289,7 +289,8 @@ const char* ptq8_last_error(const ptq8_engine* e);
  * static activation ranges).  All tensors are device memory of the handle's device;
  * every call only enqueues work on `stream` (a cudaStream_t, NULL: the legacy default
  * stream), allocates nothing and may be captured in a CUDA graph.  Row pitches are in
- * elements of the tensor, and may exceed the row's width.  One handle per device per
+ * elements of the tensor, and may exceed the row's width.  A tensor is aligned to its
+ * element type, or the call is refused.  One handle per device per
  * host thread; handles are independent of engines. */
 
 typedef struct ptq8_ops ptq8_ops;

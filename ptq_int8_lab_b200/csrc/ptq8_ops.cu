@@ -87,6 +87,8 @@ cudaError_t launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, int
 
 size_t type_size(int t) { return t == PTQ8_F32 ? 4 : 2; }
 
+bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
 // What every call checks first: a wait of an earlier call that ran out, until it is cleared.
 int ready(ptq8_ops* o) {
     if (*static_cast<volatile int*>(o->error))
@@ -113,8 +115,8 @@ int check_rows(ptq8_ops* o, const ptq8_rows_args& a) {
     if (a.ldc < a.width && a.n_rows > 1) return fail(o, PTQ8_ERR_INVALID, "%s: ldc %lld < width %d", w, a.ldc, a.width);
     if (a.n_rows == 0) return PTQ8_OK;
     if ((!a.x && a.x_rows) || !a.codes || !a.scale) return fail(o, PTQ8_ERR_INVALID, "%s: null pointer", w);
-    if (reinterpret_cast<uintptr_t>(a.x) % type_size(a.x_type))
-        return fail(o, PTQ8_ERR_INVALID, "%s: x is not aligned to its element type", w);
+    if (!aligned(a.x, type_size(a.x_type))) return fail(o, PTQ8_ERR_INVALID, "%s: x is not aligned to its element type", w);
+    if (!aligned(a.rows, 4) || !aligned(a.scale, 4)) return fail(o, PTQ8_ERR_INVALID, "%s: rows or scale not aligned to 4 bytes", w);
     return PTQ8_OK;
 }
 
@@ -143,8 +145,9 @@ int check_linear(ptq8_ops* o, const ptq8_linear_args& a, bool grouped) {
     }
     if (a.rows == 0) return PTQ8_OK;
     if (!a.x || !a.x_scale || !a.w || !a.w_scale || !a.y) return fail(o, PTQ8_ERR_INVALID, "%s: null pointer", w);
-    if (reinterpret_cast<uintptr_t>(a.y) % type_size(a.y_type))
-        return fail(o, PTQ8_ERR_INVALID, "%s: y is not aligned to its element type", w);
+    if (!aligned(a.y, type_size(a.y_type))) return fail(o, PTQ8_ERR_INVALID, "%s: y is not aligned to its element type", w);
+    if (!aligned(a.x_scale, 4) || !aligned(a.w_scale, 4) || !aligned(a.bias, 4) || (grouped && !aligned(a.offsets, 4)))
+        return fail(o, PTQ8_ERR_INVALID, "%s: x_scale, w_scale, bias or offsets not aligned to 4 bytes", w);
     return PTQ8_OK;
 }
 

@@ -1,5 +1,6 @@
 """Arguments that the C entries refuse before any launch."""
 import pytest
+import torch
 
 from ptq_int8_lab_b200 import engine as E
 
@@ -26,3 +27,35 @@ def test_row_width(ops, width, rc):
     """Rows whose last vector would end past an int are refused.  (No rows: nothing is launched either way.)"""
     got, text = rows_call(ops, width=width, ldx=1 << 31, ldc=1 << 31)
     assert got == rc and (rc == 0 or "width" in text)
+
+
+def linear_call(ops, grouped=False, **change):
+    from ptq_int8_lab_b200.ops import _LINEAR
+    a = dict(x=0, ldx=64, x_scale=0, w=0, ldw=64, w_group_stride=64 * 32, w_scale=0, bias=0, y=0, ldy=32, offsets=0, rows=2,
+             in_features=64, out_features=32, groups=1, w_bits=8, epilogue=0, y_type=0)
+    assert not set(change) - set(a)
+    a.update(change)
+    call = E.lib().ptq8_linear_grouped if grouped else E.lib().ptq8_linear
+    rc = call(ops._h, _LINEAR.pack(*a.values()), None)
+    return rc, E.lib().ptq8_ops_last_error(ops._h).decode()
+
+
+def test_misaligned_tensors(ops):
+    """A pointer that is no multiple of its element's size: refused, one operand at a time."""
+    buf = torch.zeros(1 << 16, dtype=torch.uint8, device="cuda")
+    at = [buf.data_ptr() + i * 8192 for i in range(8)]
+    good = dict(x=at[0], x_rows=2, n_rows=2, codes=at[1], scale=at[2], ldx=64, ldc=64, width=64)
+    assert rows_call(ops, **good)[0] == 0 and rows_call(ops, **good, rows=at[3])[0] == 0
+    for change in (dict(scale=at[2] + 2), dict(rows=at[3] + 1), dict(x=at[0] + 2), dict(x=at[0] + 1, x_type=2)):
+        rc, text = rows_call(ops, **{**good, **change})
+        assert rc == INVALID and "aligned" in text
+    good = dict(x=at[0], x_scale=at[1], w=at[2], w_scale=at[3], bias=at[4], y=at[5])
+    assert linear_call(ops, **good)[0] == 0 and linear_call(ops, True, **good, offsets=at[6])[0] == 0
+    for change in (dict(x_scale=at[1] + 2), dict(w_scale=at[3] + 1), dict(bias=at[4] + 2), dict(y=at[5] + 2), dict(y=at[5] + 1, y_type=2)):
+        for grouped in (False, True):
+            rc, text = linear_call(ops, grouped, **{**good, "offsets": at[6], **change})
+            assert rc == INVALID and "aligned" in text
+    rc, text = linear_call(ops, True, **good, offsets=at[6] + 2)
+    assert rc == INVALID and "aligned" in text
+    assert linear_call(ops, False, **good, offsets=at[6] + 2)[0] == 0   # not looked at there
+    torch.cuda.synchronize()
