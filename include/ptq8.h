@@ -311,7 +311,9 @@ typedef struct ptq8_ops ptq8_ops;
 #define PTQ8_MAX_ROW_WIDTH 0x7FFFFFF0
 
 ptq8_ops* ptq8_ops_create(int device, char* err, size_t errlen);
-void ptq8_ops_destroy(ptq8_ops* ops); /* the caller has synchronised the streams it used */
+/* Waits for nothing: kernels of the handle may still run, and graphs that hold them may be replayed.  What a device
+ * wait of theirs that runs out would report is lost with the handle; ptq8_ops_check_device_error comes before. */
+void ptq8_ops_destroy(ptq8_ops* ops);
 const char* ptq8_ops_last_error(const ptq8_ops* ops);
 /* Waits for `stream`, then reports (and clears) a bounded device wait that ran out: PTQ8_ERR_TIMEOUT.
  * Until it is cleared here, every further call on the handle returns PTQ8_ERR_TIMEOUT too. */

@@ -10,6 +10,7 @@
 #include <cstdio>
 #include <cstring>
 #include <exception>
+#include <mutex>
 #include <new>
 #include <string>
 
@@ -27,7 +28,7 @@ static_assert(sizeof(ptq8_rows_args) == 72 && sizeof(ptq8_linear_args) == 120, "
 struct ptq8_ops {
     int device = 0;
     int sms = 0;
-    int* error = nullptr;       // pinned host word that a kernel whose bounded wait ran out sets
+    int* error = nullptr;       // pinned host word that a kernel whose bounded wait ran out sets (error_word())
     int* error_dev = nullptr;   // its device address
     long long wait_limit = kWaitLimitCycles;
     int stall = 0;
@@ -83,6 +84,31 @@ cudaError_t launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, int
     cfg.attrs = at;
     cfg.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// A handle's error word, zero.  Words come from pinned blocks that stay with the process and no word is used again: a
+// kernel of a destroyed handle that is still running, or a graph that holds one, may write its word at any time after.
+cudaError_t error_word(int** host, int** dev) {
+    constexpr int kWords = 1024;
+    static std::mutex lock;
+    static int* block = nullptr;
+    static int used = kWords;
+    std::lock_guard<std::mutex> hold(lock);
+    if (used == kWords) {
+        int* fresh = nullptr;
+        const cudaError_t e = cudaHostAlloc(&fresh, kWords * sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable);
+        if (e != cudaSuccess) return e;
+        std::memset(fresh, 0, kWords * sizeof(int));
+        block = fresh;
+        used = 0;
+    }
+    void* at = nullptr;
+    const cudaError_t e = cudaHostGetDevicePointer(&at, block, 0);
+    if (e != cudaSuccess) return e;
+    *host = block + used;
+    *dev = static_cast<int*>(at) + used;
+    ++used;
+    return cudaSuccess;
 }
 
 size_t type_size(int t) { return t == PTQ8_F32 ? 4 : 2; }
@@ -460,36 +486,24 @@ ptq8_ops* ptq8_ops_create(int device, char* err, size_t errlen) {
         }
         OnDevice on(device);
         if (e == cudaSuccess) e = on.rc;
-        int* host = nullptr;
-        int* dev = nullptr;
-        if (e == cudaSuccess) e = cudaHostAlloc(&host, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable);
-        if (e == cudaSuccess) {
-            *host = 0;
-            e = cudaHostGetDevicePointer(&dev, host, 0);
-        }
-        if (e != cudaSuccess) {
-            if (host) cudaFreeHost(host);
-            cudaGetLastError();   // reported here: the process's next check must not find it again
-            say(err, errlen, std::string("ptq8_ops_create: ") + cudaGetErrorString(e));
-            return nullptr;
-        }
         void* encode = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &encode, cudaEnableDefault, &q);
+        cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSuccess;
+        if (e == cudaSuccess) e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &encode, cudaEnableDefault, &q);
         if (e == cudaSuccess && q != cudaDriverEntryPointSuccess) e = cudaErrorNotSupported;
         for (const Variant& v : kVariants)
             if (e == cudaSuccess)
                 e = cudaFuncSetAttribute(reinterpret_cast<const void*>(v.kernel), cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          v.per_sm == 2 ? kSmemTwo : kSmemOne);
+        int* host = nullptr;
+        int* dev = nullptr;
+        if (e == cudaSuccess) e = error_word(&host, &dev);
         if (e != cudaSuccess) {
-            cudaFreeHost(host);
-            cudaGetLastError();
+            cudaGetLastError();   // reported here: the process's next check must not find it again
             say(err, errlen, std::string("ptq8_ops_create: ") + cudaGetErrorString(e));
             return nullptr;
         }
         auto* o = new (std::nothrow) ptq8_ops();
         if (!o) {
-            cudaFreeHost(host);
             say(err, errlen, "ptq8_ops_create: out of host memory");
             return nullptr;
         }
@@ -506,11 +520,7 @@ ptq8_ops* ptq8_ops_create(int device, char* err, size_t errlen) {
     }
 }
 
-void ptq8_ops_destroy(ptq8_ops* o) {
-    if (!o) return;
-    cudaFreeHost(o->error);
-    delete o;
-}
+void ptq8_ops_destroy(ptq8_ops* o) { delete o; }
 
 const char* ptq8_ops_last_error(const ptq8_ops* o) { return o ? o->err.c_str() : "null handle"; }
 

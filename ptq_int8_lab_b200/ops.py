@@ -64,7 +64,8 @@ _CODES = {8: (torch.int8,), 4: (torch.uint8, torch.int8)}
 
 
 class Int8Ops:
-    """Handle of the token operators; one per device per host thread."""
+    """Handle of the token operators; one per device per host thread.  close() (or a with block) ends it with a last check
+    for device waits that ran out."""
 
     def __init__(self, device: int = 0):
         self._h = None
@@ -230,7 +231,25 @@ class Int8Ops:
         """Failure-detection test hook (see ptq8_ops_set_wait_test)."""
         self._check(self._lib.ptq8_ops_set_wait_test(self._h, int(wait_limit_cycles), 1 if stall_first_load else 0))
 
-    def __del__(self):
+    def _destroy(self):
         h, self._h = getattr(self, "_h", None), None
         if h:
             self._lib.ptq8_ops_destroy(h)
+
+    def close(self, stream=None):
+        """check_device_error(), then give the handle up.  (Without it nothing is waited for: calls in flight finish, but
+        a device wait of theirs that runs out is not reported.)"""
+        try:
+            if self._h:
+                self.check_device_error(stream)
+        finally:
+            self._destroy()
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()
+
+    def __del__(self):
+        self._destroy()
