@@ -9,10 +9,8 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
-#include <exception>
 #include <mutex>
 #include <new>
-#include <string>
 
 #include "ptq8.h"
 #include "ptq8_linear.cuh"
@@ -33,23 +31,22 @@ struct ptq8_ops {
     long long wait_limit = kWaitLimitCycles;
     int stall = 0;
     PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
-    std::string err;
+    char err[512] = "";         // message of the last refusal: a fixed buffer, since refusing must not throw
 };
 
 namespace {
 
 int fail(ptq8_ops* o, int status, const char* f, ...) {
-    char buf[512];
     va_list ap;
     va_start(ap, f);
-    std::vsnprintf(buf, sizeof buf, f, ap);
+    std::vsnprintf(o->err, sizeof o->err, f, ap);
     va_end(ap);
-    o->err = buf;
     return status;
 }
 
-void say(char* err, size_t n, const std::string& m) {
-    if (err && n) std::snprintf(err, n, "%s", m.c_str());
+// A message for a caller who has no handle yet.
+void say(char* err, size_t n, const char* f, const char* more = "") {
+    if (err && n) std::snprintf(err, n, f, more);
 }
 
 // The device becomes current for the call and is given back: a process may drive several.
@@ -459,17 +456,13 @@ int run_linear(ptq8_ops* o, const ptq8_linear_args& a, bool grouped, cudaStream_
 
 int product(ptq8_ops* o, const ptq8_linear_args* a, bool grouped, void* stream) {
     if (!o) return PTQ8_ERR_INVALID;
-    try {
-        if (!a) return fail(o, PTQ8_ERR_INVALID, "null arguments");
-        if (const int rc = check_linear(o, *a, grouped)) return rc;
-        if (const int rc = ready(o)) return rc;
-        if (a->rows == 0) return PTQ8_OK;
-        OnDevice on(o->device);
-        if (on.rc != cudaSuccess) return cuda_fail(o, "cudaSetDevice", on.rc);
-        return run_linear(o, *a, grouped, static_cast<cudaStream_t>(stream));
-    } catch (const std::exception& ex) {
-        return PTQ8_ERR_INVALID;
-    }
+    if (!a) return fail(o, PTQ8_ERR_INVALID, "null arguments");
+    if (const int rc = check_linear(o, *a, grouped)) return rc;
+    if (const int rc = ready(o)) return rc;
+    if (a->rows == 0) return PTQ8_OK;
+    OnDevice on(o->device);
+    if (on.rc != cudaSuccess) return cuda_fail(o, "cudaSetDevice", on.rc);
+    return run_linear(o, *a, grouped, static_cast<cudaStream_t>(stream));
 }
 
 }  // namespace
@@ -481,7 +474,7 @@ ptq8_ops* ptq8_ops_create(int device, char* err, size_t errlen) {
         cudaDeviceProp prop;
         cudaError_t e = cudaGetDeviceProperties(&prop, device);
         if (e == cudaSuccess && prop.major != 10) {
-            say(err, errlen, std::string("device is not sm_100: ") + prop.name);
+            say(err, errlen, "device is not sm_100: %s", prop.name);
             return nullptr;
         }
         OnDevice on(device);
@@ -499,7 +492,7 @@ ptq8_ops* ptq8_ops_create(int device, char* err, size_t errlen) {
         if (e == cudaSuccess) e = error_word(&host, &dev);
         if (e != cudaSuccess) {
             cudaGetLastError();   // reported here: the process's next check must not find it again
-            say(err, errlen, std::string("ptq8_ops_create: ") + cudaGetErrorString(e));
+            say(err, errlen, "ptq8_ops_create: %s", cudaGetErrorString(e));
             return nullptr;
         }
         auto* o = new (std::nothrow) ptq8_ops();
@@ -514,29 +507,25 @@ ptq8_ops* ptq8_ops_create(int device, char* err, size_t errlen) {
         o->encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(encode);
         say(err, errlen, "");
         return o;
-    } catch (const std::exception& ex) {
-        say(err, errlen, ex.what());
+    } catch (...) {   // std::mutex may throw
+        say(err, errlen, "ptq8_ops_create: a host lock failed");
         return nullptr;
     }
 }
 
 void ptq8_ops_destroy(ptq8_ops* o) { delete o; }
 
-const char* ptq8_ops_last_error(const ptq8_ops* o) { return o ? o->err.c_str() : "null handle"; }
+const char* ptq8_ops_last_error(const ptq8_ops* o) { return o ? o->err : "null handle"; }
 
 int ptq8_ops_check_device_error(ptq8_ops* o, void* stream) {
     if (!o) return PTQ8_ERR_INVALID;
-    try {
-        OnDevice on(o->device);
-        cudaError_t e = on.rc;
-        if (e == cudaSuccess) e = cudaStreamSynchronize(static_cast<cudaStream_t>(stream));
-        if (e != cudaSuccess) return cuda_fail(o, "cudaStreamSynchronize", e);
-        const int rc = ready(o);
-        *static_cast<volatile int*>(o->error) = 0;
-        return rc;
-    } catch (const std::exception& ex) {
-        return PTQ8_ERR_INVALID;
-    }
+    OnDevice on(o->device);
+    cudaError_t e = on.rc;
+    if (e == cudaSuccess) e = cudaStreamSynchronize(static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(o, "cudaStreamSynchronize", e);
+    const int rc = ready(o);
+    *static_cast<volatile int*>(o->error) = 0;
+    return rc;
 }
 
 int ptq8_ops_set_wait_test(ptq8_ops* o, long long wait_limit_cycles, int stall_first_load) {
@@ -548,17 +537,13 @@ int ptq8_ops_set_wait_test(ptq8_ops* o, long long wait_limit_cycles, int stall_f
 
 int ptq8_quantize_rows(ptq8_ops* o, const ptq8_rows_args* a, void* stream) {
     if (!o) return PTQ8_ERR_INVALID;
-    try {
-        if (!a) return fail(o, PTQ8_ERR_INVALID, "null arguments");
-        if (const int rc = check_rows(o, *a)) return rc;
-        if (const int rc = ready(o)) return rc;
-        if (a->n_rows == 0) return PTQ8_OK;
-        OnDevice on(o->device);
-        if (on.rc != cudaSuccess) return cuda_fail(o, "cudaSetDevice", on.rc);
-        return run_rows(o, *a, static_cast<cudaStream_t>(stream));
-    } catch (const std::exception& ex) {
-        return PTQ8_ERR_INVALID;
-    }
+    if (!a) return fail(o, PTQ8_ERR_INVALID, "null arguments");
+    if (const int rc = check_rows(o, *a)) return rc;
+    if (const int rc = ready(o)) return rc;
+    if (a->n_rows == 0) return PTQ8_OK;
+    OnDevice on(o->device);
+    if (on.rc != cudaSuccess) return cuda_fail(o, "cudaSetDevice", on.rc);
+    return run_rows(o, *a, static_cast<cudaStream_t>(stream));
 }
 
 int ptq8_linear(ptq8_ops* o, const ptq8_linear_args* a, void* stream) { return product(o, a, false, stream); }
