@@ -26,7 +26,9 @@
 //                      of 16 columns, which takes 55 to 75 cycles instead of 8
 //
 // Warps: 0 TMA producer, 1 MMA issuer, 2 TMEM and the groups' tile list, 4.. epilogue, then
-// (W4) the unpackers.  All waits are bounded.
+// (W4) the unpackers.  Waits for data are bounded.  The TMEM allocation and the cluster's barriers have no limit to give;
+// they end because what they wait for does: columns are held by kernels that need nothing more of this SM (each lets its
+// successor start only once it holds its own), and every thread of a cluster reaches its barriers.
 #pragma once
 
 #include "ptq8_linear.cuh"
@@ -491,7 +493,6 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
     const uint32_t afull = b0 + 8 * 2 * kMaxLinStages, accfull = afull + 64, accempty = accfull + 16,
                    partial = accempty + 16, drain = partial + 8;
 
-    griddep_launch();
     if (warp == 0 && elect_one()) {
         tma_prefetch(&map_x);
         tma_prefetch(&map_w);
@@ -539,7 +540,12 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
     if (clustered) {   // the peers' barriers exist
         cluster_arrive_relaxed();
         cluster_wait();
+    } else {
+        __syncthreads();
     }
+    // Only now, with this CTA's TMEM allocated, may the next kernel start: a CTA of it that took the columns first would wait
+    // for this kernel, and this kernel's allocation, which has no limit, for that CTA.
+    griddep_launch();
     griddep_wait();                  // nothing above reads or writes global memory (but for prefetches)
     if (listed && warp == 2) {
         // The groups' first rows, clamped into [0, rows] and never decreasing, then their first tiles: what the
