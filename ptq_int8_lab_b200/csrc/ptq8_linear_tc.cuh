@@ -111,9 +111,10 @@ __device__ __forceinline__ void prefetch_3d(const CUtensorMap* m, int c0, int c1
                  : "memory");
 }
 
-// Arrive on a barrier of any CTA of the cluster (address from mapa, or of the own CTA) without release:
-// what it orders are tcgen05 accesses, completed by tcgen05.wait and ordered by tcgen05.fence, and loads
-// whose values have been used.  (With .release.cluster the unpackers took over 1000 cycles a block.)
+// Arrive on a barrier of any CTA of the cluster (address from mapa, or of the own CTA) without release: what it orders are
+// the thread's tcgen05 accesses, completed by tcgen05.wait, ordered before the arrival by tcgen05.fence::before_thread_sync
+// and, at the waiting side, by tcgen05.fence::after_thread_sync.  No data that other instructions wrote may depend on it.
+// (With .release.cluster the unpackers took over 1000 cycles a block.)
 __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t bar) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -596,9 +597,9 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
 
     if (warp == 0) {
         // ---------------------------------------------------------------- producer
-        // The pair's loads all count at the leader; with int4 weights at the own CTA, whose unpackers
-        // pass it on.
-        const uint32_t full_at = CG == 2 && !W4 ? mapa(full, 0) : full;
+        // The pair's loads all count at the leader, which issues the MMAs; but packed weights at the own CTA, whose
+        // unpackers read them.
+        const uint32_t x_at = CG == 2 ? mapa(full, 0) : full, w_at = W4 ? full : x_at;
         int s = 0, issued = 0;
         uint32_t ph = 1;
         bool ok = true;
@@ -614,7 +615,7 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
                 }
                 if (elect_one()) {
                     const uint32_t wdst = base + s * Sh::kStage, xdst = wdst + Sh::kW;
-                    if (leader || W4) mbar_expect_tx(full + 8 * s, (W4 ? 1 : CG) * Sh::kStage);
+                    if (leader || W4) mbar_expect_tx(full + 8 * s, (W4 ? 1 : CG) * Sh::kW + (leader ? CG : 0) * Sh::kX);
                     if (!(p.stall && blockIdx.x == 0 && issued == 0)) {
 #pragma unroll
                         for (int b = 0; b < Sh::KD; ++b) {
@@ -622,12 +623,12 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
 #pragma unroll
                             for (int h = 0; h < H; ++h) {
                                 if constexpr (W4)
-                                    load_rows_3d<1>(wdst + h * 8192, &map_w, full_at + 8 * s, k * 64, h * p.l.n + c, tile.group);
+                                    load_rows_3d<1>(wdst + h * 8192, &map_w, w_at + 8 * s, k * 64, h * p.l.n + c, tile.group);
                                 else
-                                    load_rows_3d<CG>(wdst + (b * H + h) * 16384, &map_w, full_at + 8 * s, k * 128, h * p.l.n + c,
+                                    load_rows_3d<CG>(wdst + (b * H + h) * 16384, &map_w, w_at + 8 * s, k * 128, h * p.l.n + c,
                                                      tile.group);
                             }
-                            load_rows_2d<W4 ? 1 : CG>(xdst + b * Sh::kXBlock, &map_x, full_at + 8 * s, k * 128, r);
+                            load_rows_2d<CG>(xdst + b * Sh::kXBlock, &map_x, x_at + 8 * s, k * 128, r);
                         }
                     }
                 }
@@ -652,7 +653,8 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
             if (!ok) give_up(ERR_WAIT_EMPTY);
         }
         if (!ok) {
-            // own copies in flight must land before the CTA ends
+            // own copies in flight must land before the CTA ends (what a pair's second CTA loads counts at the leader, which
+            // waits for it: no CTA ends before both have given up)
             const int n = min(issued, p.stages);
             for (int i = 1; i <= n; ++i) {
                 const int back = issued - i;
@@ -677,7 +679,7 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
             }
             tc_fence_after();
             for (int kb = kb0; kb < kb1; ++kb) {
-                // W4: the unpackers saw the stage's loads arrive, the tokens' rows among them
+                // W4: this CTA's unpackers saw the stage's loads arrive, the tokens' rows of both CTAs among them
                 if (!mbar_wait_warp(W4 ? afull + 8 * ab : full + 8 * s, W4 ? aph : ph, limit)) {
                     give_up(ERR_WAIT_FULL);
                     ok = false;
@@ -853,10 +855,11 @@ __global__ void __launch_bounds__(TcShape<CG, TN, W4, GATED>::kThreads, TcShape<
             tmem_st32(lanes + ab * Sh::kACols, o);
             tmem_wait_st();
             tc_fence_before();
-            // the pair's leader learns of both CTAs' rows here: their copies have landed (seen above)
+            // In the leader the arrival also passes on what the wait above saw: the tokens' rows.  From the second CTA it
+            // stands for the TMEM stores alone.
             if (lane == 0) {
-                if (CG == 1)
-                    mbar_arrive(afull_at + 8 * ab);
+                if (leader)
+                    mbar_arrive(afull + 8 * ab);
                 else
                     mbar_arrive_cluster_relaxed(afull_at + 8 * ab);
             }
