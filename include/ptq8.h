@@ -371,6 +371,29 @@ typedef struct {
 int ptq8_linear(ptq8_ops* ops, const ptq8_linear_args* args, void* stream);
 int ptq8_linear_grouped(ptq8_ops* ops, const ptq8_linear_args* args, void* stream);
 
+/* Which kernel a product runs on.  Host only: no handle, no device, and the tensors are not read (their addresses'
+ * alignment counts).  The answer is the one that a call with these arguments takes on a device of `sms` SMs. */
+#define PTQ8_KERNEL_ANY 0   /* any layout */
+#define PTQ8_KERNEL_FEW 1   /* a few tokens, weights streamed to registers */
+#define PTQ8_KERNEL_TILES 2 /* tensor-core tiles: the fields below */
+typedef struct {
+    int kernel;             /* PTQ8_KERNEL_* */
+    int variant;            /* index of the tile variant, 0 up to ptq8_linear_variants() - 1 */
+    int ctas, tokens;       /* CTAs and tokens of a tile */
+    int w_bits, epilogue;   /* what the variant serves */
+    int split;              /* CTAs that share a tile's sum */
+    int stages, turns;      /* shared-memory stages of a CTA; sets of int4 unpacking warps that take turns at them */
+    int operand_tiles;      /* int4: widened weight tiles in TMEM */
+    int smem_bytes;         /* dynamic shared memory of a CTA */
+} ptq8_linear_choice;
+int ptq8_linear_variants(void);
+int ptq8_linear_choose(int sms, const ptq8_linear_args* args, int grouped, ptq8_linear_choice* choice);
+/* The same for one variant and split, whatever the call would choose: PTQ8_ERR_INVALID where that pair cannot serve it. */
+int ptq8_linear_choose_as(int sms, const ptq8_linear_args* args, int grouped, int variant, int split, ptq8_linear_choice* choice);
+/* Test hook: products of this handle run as `variant` with `split` (-1: as they choose), or are refused where that pair
+ * cannot serve them. */
+int ptq8_ops_set_choice_test(ptq8_ops* ops, int variant, int split);
+
 #ifdef __cplusplus
 }
 #endif

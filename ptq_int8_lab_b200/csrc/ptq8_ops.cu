@@ -9,6 +9,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <iterator>
 #include <mutex>
 #include <new>
 
@@ -30,6 +31,7 @@ struct ptq8_ops {
     int* error_dev = nullptr;   // its device address
     long long wait_limit = kWaitLimitCycles;
     int stall = 0;
+    int variant = -1, split = 1;   // test hook: the tile variant of every product
     PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
     char err[512] = "";         // message of the last refusal: a fixed buffer, since refusing must not throw
 };
@@ -272,7 +274,7 @@ int list_bytes_of(const ptq8_linear_args& a, bool listed) { return listed ? ((a.
 // joining its sums, and clusters of 4 and 8 do not fill every GPC.  The constants are fitted to 7200 timings of
 // 508 calls (1 to 8192 tokens, 512 to 16384 features, 1 to 64 groups, both types, gated or not) under every
 // variant: the variant of the least estimate is 1.6 % slower than the fastest one on average, 22 % at most.
-float estimate(const ptq8_ops* o, const ptq8_linear_args& a, int groups, const Variant& v, int split) {
+float estimate(int sms, const ptq8_linear_args& a, int groups, const Variant& v, int split) {
     constexpr float kMma = 77.5f, kMmaTmem = 104;    // least cycles of an MMA, M operand in shared memory or TMEM
     constexpr float kMmaTmemPair = 102;              // the latter for a pair: 4096 x 4096 x 4096 gated 100 us, one CTA a tile 105
     constexpr float kWait = 144, kWaitTwo = 47;      // wait of the MMA warp per block (two blocks a stage)
@@ -290,12 +292,12 @@ float estimate(const ptq8_ops* o, const ptq8_linear_args& a, int groups, const V
     const float tiles = row_tiles * static_cast<float>((a.out_features + 128 * v.cg - 1) / (128 * v.cg));
     const float blocks = std::ceil(std::ceil(a.in_features / 128.0f) / split);
     const float columns = std::min<float>(v.tn, std::ceil(std::ceil(mean) / (16 * v.cg)) * (16 * v.cg));
-    const float share = v.per_sm == 2 && tiles * v.cg * split > kPacked * o->sms ? 2 : 1;
+    const float share = v.per_sm == 2 && tiles * v.cg * split > kPacked * sms ? 2 : 1;
     const float mma = 4 * h * std::max(!v.w4 ? kMma : v.cg == 2 ? kMmaTmemPair : kMmaTmem, columns / 2);
     const float load = (h * 128 * (v.w4 ? 64 : 128) + v.x_rows * 128) / kLoad;
     const float block = std::max({mma + (v.depth > 128 ? kWaitTwo : kWait), share * mma, share * load, share * (v.w4 ? kWiden * h : 0)});
     const float fill = split == 8 ? kFill8 : split == 4 ? kFill4 : 1;
-    const float slots = std::max(1.0f, std::floor(std::floor(o->sms * v.per_sm * fill) / (v.cg * split)));
+    const float slots = std::max(1.0f, std::floor(std::floor(sms * v.per_sm * fill) / (v.cg * split)));
     const float waves = std::ceil(tiles / slots);
     float out = kColumn * columns * h / (v.tn >= 128 ? 2 : 1);
     if (split > 1) out += kSplit + kPush * columns * h;
@@ -304,20 +306,26 @@ float estimate(const ptq8_ops* o, const ptq8_linear_args& a, int groups, const V
     return start + waves * (blocks * block + out + (split > 1 ? kWave : 0));
 }
 
+// Whether a call can run as variant v with the sum over input features split s ways.
+bool serves(const ptq8_linear_args& a, bool listed, const Variant& v, int s) {
+    if (v.w4 != (a.w_bits == 4) || v.gated != (a.epilogue == PTQ8_EPI_SWIGLU)) return false;
+    if (s < 1 || s > (v.cg == 2 ? 1 : 8) || (s & (s - 1)) || static_cast<long long>(s - 1) * v.depth >= a.in_features) return false;
+    // the operand tile of a block is free when its stage is; a split's sums leave from the stages' memory
+    const int stages = stages_of(v, s, list_bytes_of(a, listed));
+    return stages >= std::max(2, v.a_bufs) && (s == 1 || stages * v.stage >= v.cols * 128 * 4);
+}
+
 // The variant of the least estimate, among tiles not much longer than the rows of a group.
-const Variant* choose(const ptq8_ops* o, const ptq8_linear_args& a, bool listed, int& split) {
+const Variant* choose(int sms, const ptq8_linear_args& a, bool listed, int& split) {
     const int groups = listed ? a.groups : 1;
-    const bool gated = a.epilogue == PTQ8_EPI_SWIGLU, w4 = a.w_bits == 4;
     const float mean = static_cast<float>(a.rows) / std::min<long long>(groups, a.rows);
     const Variant* best = nullptr;
     float least = 0;
     for (const Variant& v : kVariants) {
-        if (v.w4 != w4 || v.gated != gated || (v.tn > 16 && v.tn >= 4 * v.cg * mean)) continue;
-        for (int s = 1; s <= (v.cg == 2 ? 1 : 8) && s * v.depth < a.in_features + v.depth; s *= 2) {
-            // the operand tile of a block is free when its stage is; a split's sums leave from the stages' memory
-            const int stages = stages_of(v, s, list_bytes_of(a, listed));
-            if (stages < std::max(2, v.a_bufs) || (s > 1 && stages * v.stage < v.cols * 128 * 4)) continue;
-            const float t = estimate(o, a, groups, v, s);
+        if (v.tn > 16 && v.tn >= 4 * v.cg * mean) continue;
+        for (int s = 1; s <= 8; s *= 2) {
+            if (!serves(a, listed, v, s)) continue;
+            const float t = estimate(sms, a, groups, v, s);
             if (!best || t < least) best = &v, split = s, least = t;
         }
     }
@@ -345,7 +353,12 @@ int encode(ptq8_ops* o, CUtensorMap* m, int rank, const void* base, const cuuint
 int run_tc(ptq8_ops* o, const ptq8_linear_args& a, const LinearParams& l, cudaStream_t st) {
     const bool gated = a.epilogue == PTQ8_EPI_SWIGLU, w4 = a.w_bits == 4;
     int split = 1;
-    const Variant* v = choose(o, a, l.offsets != nullptr, split);
+    const Variant* v = nullptr;
+    if (o->variant < 0)
+        v = choose(o->sms, a, l.offsets != nullptr, split);
+    else if (serves(a, l.offsets != nullptr, kVariants[o->variant], o->split))
+        v = &kVariants[o->variant], split = o->split;
+    if (!v) return fail(o, PTQ8_ERR_INVALID, "linear: variant %d with split %d does not serve this call", o->variant, o->split);
     const long long channels = static_cast<long long>(a.out_features) * (gated ? 2 : 1);
     const int wide = w4 ? (a.in_features + 1) / 2 : a.in_features;
     CUtensorMap mx, mw;
@@ -443,7 +456,9 @@ int run_linear(ptq8_ops* o, const ptq8_linear_args& a, bool grouped, cudaStream_
     p.groups = grouped ? a.groups : 1;
     p.y_type = a.y_type;
     const bool gated = a.epilogue == PTQ8_EPI_SWIGLU, w4 = a.w_bits == 4;
-    if (vector_layout(a, grouped)) return few_rows(a, p.groups) ? run_few(o, a, p, st) : run_tc(o, a, p, st);
+    const bool vectors = vector_layout(a, grouped);
+    if (o->variant >= 0 && !vectors) return fail(o, PTQ8_ERR_INVALID, "linear: variant %d does not serve this layout", o->variant);
+    if (vectors) return few_rows(a, p.groups) && o->variant < 0 ? run_few(o, a, p, st) : run_tc(o, a, p, st);
     const long long row_tiles = (a.rows + kAnyTile - 1) / kAnyTile;
     // blocks stride over the channel tiles (x) and over a group's row tiles (y)
     const dim3 grid(static_cast<unsigned>((a.out_features + kAnyTile - 1) / kAnyTile),
@@ -463,6 +478,27 @@ int product(ptq8_ops* o, const ptq8_linear_args* a, bool grouped, void* stream) 
     OnDevice on(o->device);
     if (on.rc != cudaSuccess) return cuda_fail(o, "cudaSetDevice", on.rc);
     return run_linear(o, *a, grouped, static_cast<cudaStream_t>(stream));
+}
+
+// ptq8_linear_choose and ptq8_linear_choose_as (variant >= 0).
+int choice_of(int sms, const ptq8_linear_args* args, bool grouped, int variant, int split, ptq8_linear_choice* c) {
+    ptq8_ops none;   // takes the message of a refusal
+    if (!args || !c || sms < 1 || variant >= static_cast<int>(std::size(kVariants))) return PTQ8_ERR_INVALID;
+    const ptq8_linear_args& a = *args;
+    if (const int rc = check_linear(&none, a, grouped)) return rc;
+    if (a.rows == 0) return PTQ8_ERR_INVALID;   // runs on no kernel
+    *c = ptq8_linear_choice{};
+    const bool vectors = vector_layout(a, grouped);
+    if (variant < 0 && (!vectors || few_rows(a, grouped ? a.groups : 1))) {
+        c->kernel = vectors ? PTQ8_KERNEL_FEW : PTQ8_KERNEL_ANY;
+        return PTQ8_OK;
+    }
+    const Variant* v = variant < 0 ? choose(sms, a, grouped, split) : &kVariants[variant];
+    if (!vectors || !serves(a, grouped, *v, split)) return PTQ8_ERR_INVALID;
+    const int list = list_bytes_of(a, grouped), stages = stages_of(*v, split, list);
+    *c = {PTQ8_KERNEL_TILES, static_cast<int>(v - kVariants), v->cg, v->tn, a.w_bits, a.epilogue, split, stages, v->turns, v->a_bufs,
+          smem_beside(*v, split, list) + stages * v->stage};
+    return PTQ8_OK;
 }
 
 }  // namespace
@@ -532,6 +568,24 @@ int ptq8_ops_set_wait_test(ptq8_ops* o, long long wait_limit_cycles, int stall_f
     if (!o) return PTQ8_ERR_INVALID;
     o->wait_limit = wait_limit_cycles > 0 ? wait_limit_cycles : kWaitLimitCycles;
     o->stall = stall_first_load != 0;
+    return PTQ8_OK;
+}
+
+int ptq8_linear_variants(void) { return static_cast<int>(std::size(kVariants)); }
+
+int ptq8_linear_choose(int sms, const ptq8_linear_args* a, int grouped, ptq8_linear_choice* c) {
+    return choice_of(sms, a, grouped != 0, -1, 1, c);
+}
+
+int ptq8_linear_choose_as(int sms, const ptq8_linear_args* a, int grouped, int variant, int split, ptq8_linear_choice* c) {
+    return variant < 0 ? PTQ8_ERR_INVALID : choice_of(sms, a, grouped != 0, variant, split, c);
+}
+
+int ptq8_ops_set_choice_test(ptq8_ops* o, int variant, int split) {
+    if (!o) return PTQ8_ERR_INVALID;
+    if (variant >= ptq8_linear_variants()) return fail(o, PTQ8_ERR_INVALID, "variant %d of %d", variant, ptq8_linear_variants());
+    o->variant = variant < 0 ? -1 : variant;
+    o->split = split;
     return PTQ8_OK;
 }
 

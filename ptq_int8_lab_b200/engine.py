@@ -54,6 +54,7 @@ EXPORTS = (
     "ptq8_load", "ptq8_forward", "ptq8_forward_debug", "ptq8_capture_graph", "ptq8_destroy", "ptq8_last_error",
     "ptq8_ops_create", "ptq8_ops_destroy", "ptq8_ops_last_error", "ptq8_ops_check_device_error",
     "ptq8_ops_set_wait_test", "ptq8_quantize_rows", "ptq8_linear", "ptq8_linear_grouped",
+    "ptq8_linear_variants", "ptq8_linear_choose", "ptq8_linear_choose_as", "ptq8_ops_set_choice_test",
 )
 
 
@@ -147,6 +148,10 @@ def lib() -> ctypes.CDLL:
         "ptq8_quantize_rows": (c_int, [c_void_p, c_void_p, c_void_p]),
         "ptq8_linear": (c_int, [c_void_p, c_void_p, c_void_p]),
         "ptq8_linear_grouped": (c_int, [c_void_p, c_void_p, c_void_p]),
+        "ptq8_linear_variants": (c_int, []),
+        "ptq8_linear_choose": (c_int, [c_int, c_void_p, c_int, c_void_p]),
+        "ptq8_linear_choose_as": (c_int, [c_int, c_void_p, c_int, c_int, c_int, c_void_p]),
+        "ptq8_ops_set_choice_test": (c_int, [c_void_p, c_int, c_int]),
     }
     for name, (res, args) in sig.items():
         f = getattr(L, name)

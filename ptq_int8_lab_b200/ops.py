@@ -16,7 +16,7 @@ from __future__ import annotations
 
 import ctypes
 import struct
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -61,6 +61,48 @@ def _check_vector(name: str, t: torch.Tensor, dtype, values: int, device: int):
 
 _F32, _I32, _INT8 = torch.float32, torch.int32, torch.int8
 _CODES = {8: (torch.int8,), 4: (torch.uint8, torch.int8)}
+
+
+KERNEL_ANY, KERNEL_FEW, KERNEL_TILES = 0, 1, 2
+
+
+class LinearChoice(NamedTuple):
+    """What a product runs on (ptq8_linear_choice); the fields after kernel are those of KERNEL_TILES."""
+    kernel: int
+    variant: int
+    ctas: int
+    tokens: int
+    w_bits: int
+    epilogue: int
+    split: int
+    stages: int
+    turns: int
+    operand_tiles: int
+    smem_bytes: int
+
+
+def linear_variants() -> int:
+    return lib().ptq8_linear_variants()
+
+
+def linear_choice(rows: int, in_features: int, out_features: int, bits: int = 8, act: int = EPI_NONE, groups: int = 0,
+                  variant: Optional[int] = None, split: int = 1, sms: int = 148, pitch: int = 16) -> Optional[LinearChoice]:
+    """What linear() (groups 0) or linear_grouped() runs on, for rows laid at multiples of `pitch` bytes; or, with `variant`,
+    that variant's launch (None: it cannot serve the call).  Needs no device."""
+    wide = (in_features + 1) // 2 if bits == 4 else in_features
+    ldx, ldw = (-(-v // pitch) * pitch for v in (in_features, wide))
+    channels = out_features * (2 if act == EPI_SWIGLU else 1)
+    at = 1 << 12   # an address that no one reads
+    args = _LINEAR.pack(at, ldx, at, at, ldw, ldw * channels, at, 0, at, out_features, at if groups else 0, rows, in_features,
+                        out_features, groups, bits, act, 2)
+    out = (ctypes.c_int * len(LinearChoice._fields))()
+    if variant is None:
+        rc = lib().ptq8_linear_choose(sms, args, 1 if groups else 0, out)
+    else:
+        rc = lib().ptq8_linear_choose_as(sms, args, 1 if groups else 0, variant, split, out)
+    if rc and variant is None:
+        raise Ptq8Error("linear_choice: not a product", rc)
+    return None if rc else LinearChoice(*out)
 
 
 class Int8Ops:
@@ -230,6 +272,10 @@ class Int8Ops:
     def set_wait_test(self, wait_limit_cycles: int = 0, stall_first_load: bool = False):
         """Failure-detection test hook (see ptq8_ops_set_wait_test)."""
         self._check(self._lib.ptq8_ops_set_wait_test(self._h, int(wait_limit_cycles), 1 if stall_first_load else 0))
+
+    def set_choice_test(self, variant: int = -1, split: int = 1):
+        """Test hook: products run as one tile variant (see ptq8_ops_set_choice_test)."""
+        self._check(self._lib.ptq8_ops_set_choice_test(self._h, int(variant), int(split)))
 
     def _destroy(self):
         h, self._h = getattr(self, "_h", None), None
