@@ -254,6 +254,11 @@ const Variant kVariants[] = {
 // Dynamic shared memory of a CTA that shares its SM with another, or not.
 constexpr int kSmemTwo = 110 * 1024, kSmemOne = 222 * 1024;
 
+// And at least: TMEM is allocated for as many CTAs as are meant to share an SM, so that a further one's allocation would
+// wait, and clusters whose CTAs wait so on two SMs for each other's would wait for good.  78 KB keep a third CTA from two
+// that share, 160 KB any other from one that has its SM's columns to itself (the SM's 228 KB hold 1 KB more per CTA).
+constexpr int kLeastTwo = 78 * 1024, kLeastOne = 160 * 1024;
+
 // Shared memory beside the stages: their alignment, the tile list, a split's partial sums.
 int smem_beside(const Variant& v, int split, int list_bytes) { return 1024 + list_bytes + (split > 1 ? v.cols * 128 * 4 : 0); }
 
@@ -264,6 +269,10 @@ int smem_beside(const Variant& v, int split, int list_bytes) { return 1024 + lis
 int stages_of(const Variant& v, int split, int list_bytes) {
     const int most = std::min(kMaxLinStages, ((v.per_sm == 2 ? kSmemTwo : kSmemOne) - smem_beside(v, split, list_bytes)) / v.stage);
     return most / v.turns * v.turns;
+}
+
+int smem_of(const Variant& v, int split, int list_bytes) {
+    return std::max(v.per_sm == 2 ? kLeastTwo : kLeastOne, smem_beside(v, split, list_bytes) + stages_of(v, split, list_bytes) * v.stage);
 }
 
 int list_bytes_of(const ptq8_linear_args& a, bool listed) { return listed ? ((a.groups + 1) * 8 + 127) / 128 * 128 : 0; }
@@ -390,7 +399,7 @@ int run_tc(ptq8_ops* o, const ptq8_linear_args& a, const LinearParams& l, cudaSt
     p.err = o->error_dev;
     p.stall = o->stall;
     p.stages = stages_of(*v, split, p.list_bytes);
-    const int smem = smem_beside(*v, split, p.list_bytes) + p.stages * v->stage;
+    const int smem = smem_of(*v, split, p.list_bytes);
     // tiles at most: each group's last tile may be partly filled
     const long long row_tiles = l.offsets ? a.rows / v->tn + std::min<long long>(l.groups, a.rows) : (a.rows + v->tn - 1) / v->tn;
     const long long tiles = row_tiles * p.ctiles;
@@ -497,7 +506,7 @@ int choice_of(int sms, const ptq8_linear_args* args, bool grouped, int variant, 
     if (!vectors || !serves(a, grouped, *v, split)) return PTQ8_ERR_INVALID;
     const int list = list_bytes_of(a, grouped), stages = stages_of(*v, split, list);
     *c = {PTQ8_KERNEL_TILES, static_cast<int>(v - kVariants), v->cg, v->tn, a.w_bits, a.epilogue, split, stages, v->turns, v->a_bufs,
-          smem_beside(*v, split, list) + stages * v->stage};
+          smem_of(*v, split, list)};
     return PTQ8_OK;
 }
 

@@ -34,6 +34,16 @@ def test_stages_are_multiples_of_the_turns():
     assert seen == set(range(O.linear_variants()))
 
 
+def test_shared_memory_keeps_tmem_apart():
+    """CTAs that share an SM take half of its TMEM columns each, so three of them must not fit; the others take all of
+    them, so none of them may stand beside another.  1 KB of each CTA is the system's."""
+    sizes = {c.smem_bytes for *_, c in every_launch()}
+    two, one = {s for s in sizes if s <= 113 * 1024}, {s for s in sizes if s > 113 * 1024}
+    assert two and one and max(one) <= 227 * 1024
+    assert 3 * (min(two) + 1024) > 228 * 1024 >= 2 * (max(two) + 1024)
+    assert min(one) + min(two) + 2048 > 228 * 1024
+
+
 def test_some_variant_serves_every_call():
     rng = random.Random(0)
     for _ in range(3000):
