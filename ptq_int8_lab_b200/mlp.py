@@ -102,7 +102,8 @@ def _float_mlp(x, gate_up, down):
     return (torch.nn.functional.silu(g) * u) @ down.t()
 
 
-def main(argv=None):
+def main(argv=None) -> Tuple[float, float]:
+    """Runs both; returns the relative differences from float (dense, experts)."""
     ap = argparse.ArgumentParser(description="Dense and expert MLPs with int8 activations, against float.")
     for name, value in (("tokens", 16), ("hidden", 1024), ("width", 2048), ("experts", 8), ("top", 2), ("bits", 8), ("seed", 0)):
         ap.add_argument("--" + name, type=int, default=value)
@@ -116,8 +117,9 @@ def main(argv=None):
     got = Int8MLP(w1[0], w2[0], a.bits, ops=ops)(x)
     f1, f2 = torch.from_numpy(w1).cuda(), torch.from_numpy(w2).cuda()
     want = _float_mlp(x, f1[0], f2[0])
+    dense = float((got - want).norm() / want.norm())
     print(f"dense: {a.tokens} tokens, {a.hidden} -> 2 x {a.width} -> {a.hidden}, W{a.bits}A8: "
-          f"relative difference from float {float((got - want).norm() / want.norm()):.4f}")
+          f"relative difference from float {dense:.4f}")
     moe = Int8Experts(router, w1, w2, a.top, a.bits, ops=ops)
     got = moe(x)
     p, ids = torch.topk(x @ moe.router.t(), a.top, dim=1)
@@ -125,7 +127,9 @@ def main(argv=None):
     want = torch.stack([sum(p[t, j] * _float_mlp(x[t:t + 1], f1[e], f2[e])[0] for j, e in enumerate(ids[t].tolist()))
                         for t in range(a.tokens)])
     ops.check_device_error()
-    print(f"experts: top {a.top} of {a.experts}: relative difference from float {float((got - want).norm() / want.norm()):.4f}")
+    experts = float((got - want).norm() / want.norm())
+    print(f"experts: top {a.top} of {a.experts}: relative difference from float {experts:.4f}")
+    return dense, experts
 
 
 if __name__ == "__main__":

@@ -81,3 +81,11 @@ def test_experts_with_routing_of_its_own(bits, tokens, experts, top):
             ch, sh = _codes((g / (1 + np.exp(-g)) * u).astype(np.float32))
             want[t] += weight * ((c2 @ ch) * sh * s2)
     assert np.linalg.norm(got - want) <= 1e-2 * np.linalg.norm(want)
+
+
+def test_command_returns_what_it_prints(capsys):
+    from ptq_int8_lab_b200 import mlp
+    far = mlp.main(["--tokens", "9", "--hidden", "128", "--width", "160", "--experts", "4"])
+    printed = [float(line.rsplit(" ", 1)[1]) for line in capsys.readouterr().out.splitlines()]
+    assert len(far) == 2 and all(0 < d < 0.05 for d in far)
+    assert all(abs(d - p) <= 5.1e-5 for d, p in zip(far, printed))
