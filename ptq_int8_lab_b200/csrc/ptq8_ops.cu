@@ -418,16 +418,24 @@ FewKernel few_kernel(bool w4, bool gated) {
               : (gated ? linear_few_kernel<MT, false, true> : linear_few_kernel<MT, false, false>);
 }
 
-// Up to four tokens, or one a group on average, while the weights that they read stay small: one token x 4096 x
-// 4096 takes 5.3 us here and 6.1 us as a tensor-core tile (int4 4.1 and 6.9), four tokens 6.0 and 6.6 (5.0 and
-// 7.5); six tokens 8.8 and 6.6.  From 32 MB on (4096 x 8192 int8: 10.9 and 8.8 us) bulk copies into shared memory
-// keep more bytes in flight.  Rows that are not whole vectors of 16 bytes of weights go to the tensor cores too: at
-// 2001 x 1270 joining single bytes made four tokens 1.2 (int4 1.6) times slower than a tile.
+// Up to four tokens, or one a group on average, while the weights that they read stay small.  Weights from DRAM, us here
+// and as the best tensor-core tile of 16:
+//   tokens x 4096 x channels     4096 int8   4608 int8   5120 int8    6144 int8   8192 int4   10240 int4   12288 int4
+//   1                            5.2   5.9   5.9   6.8   9.7    7.2   10.2  7.5   5.9   7.5   7.2    9.6   7.4   10.0
+//   2                            6.0   5.9   6.7   6.8   11.0   7.2   11.5  7.5   8.5   7.6   9.4    9.6   9.3   10.0
+//   4                            5.9   6.0   6.6   7.0   8.8    7.4   9.0   7.5   7.6   7.7   11.4   9.8   12.1  10.0
+// Above 18 MB rows are no longer shared by two warps, so that a few blocks more than there are SMs make a second turn, and
+// bulk copies into shared memory keep more bytes in flight (2048 x 10240 int8, one token, is the other way: 6.6 and 7.4 us).
+// One token on int4 codes goes further, since its tiles wait for the unpacking.
+// Rows that are not whole vectors of 16 bytes of weights go to the tensor cores too: at 2001 x 1270 joining single bytes
+// made four tokens 1.2 (int4 1.6) times slower than a tile.
+// The host does not know how ragged groups are.  64 rows of 64 experts, 1024 -> 256: one each or at random 5.8 us (a tile 8.4),
+// half of them in one group 20 us (7.2), all of them 34 us (6.7): a group's rows pass over its weights two at a time.
 bool few_rows(const ptq8_linear_args& a, int groups) {
-    constexpr long long kMostBytes = 24LL << 20;
+    const long long most = a.w_bits == 4 && a.rows == 1 ? 24LL << 20 : 18LL << 20;
     const long long channels = static_cast<long long>(a.out_features) * (a.epilogue == PTQ8_EPI_SWIGLU ? 2 : 1);
     const long long bytes = std::min<long long>(groups, a.rows) * channels * a.in_features * a.w_bits / 8;
-    return (groups > 1 ? a.rows <= groups : a.rows <= 4) && bytes <= kMostBytes && a.in_features % (a.w_bits == 4 ? 32 : 16) == 0;
+    return (groups > 1 ? a.rows <= groups : a.rows <= 4) && bytes <= most && a.in_features % (a.w_bits == 4 ? 32 : 16) == 0;
 }
 
 int run_few(ptq8_ops* o, const ptq8_linear_args& a, const LinearParams& l, cudaStream_t st) {

@@ -74,3 +74,17 @@ def test_refusals():
             O.linear_choice(**bad)
     assert E.lib().ptq8_linear_choose(148, None, 0, None) == 1 and E.lib().ptq8_linear_choose_as(148, None, 0, 0, 1, None) == 1
     assert E.lib().ptq8_ops_set_choice_test(None, 0, 1) == 1
+
+
+def test_weights_that_the_few_token_kernel_takes():
+    """Up to 18 MB of weights, 24 MB for one token on int4 codes: above, tiles were faster (4096 x 5632 int8 from DRAM:
+    9.9 and 7.4 us)."""
+    few, tiles = O.KERNEL_FEW, O.KERNEL_TILES
+    for rows in (1, 2, 4):
+        for act in (0, 1):
+            for n, kernel in ((4096, few), (4608, few), (4624, tiles), (5632, tiles), (8192, tiles)):
+                assert O.linear_choice(rows, 4096, n // (1 + act), 8, act).kernel == kernel
+            for n, kernel in ((9216, few), (9248, few if rows == 1 else tiles), (12288, few if rows == 1 else tiles), (12320, tiles)):
+                assert O.linear_choice(rows, 4096, n // (1 + act), 4, act).kernel == kernel
+    assert O.linear_choice(5, 4096, 64).kernel == tiles and O.linear_choice(4, 4096, 64).kernel == few
+    assert O.linear_choice(8, 1024, 1024, groups=8).kernel == few and O.linear_choice(9, 1024, 1024, groups=8).kernel == tiles
