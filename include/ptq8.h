@@ -291,7 +291,7 @@ const char* ptq8_last_error(const ptq8_engine* e);
  * stream), allocates nothing and may be captured in a CUDA graph.  Row pitches are in
  * elements of the tensor, and may exceed the row's width.  A tensor is aligned to its
  * element type, or the call is refused.  One handle per device per
- * host thread; handles are independent of engines. */
+ * host thread; handles are independent of engines.  Forward only. */
 
 typedef struct ptq8_ops ptq8_ops;
 

@@ -114,7 +114,7 @@ __device__ __forceinline__ uint32_t join4(const uint8_t* p, int n) {
 
 // The kernel for layouts that neither TMA nor 16-byte loads can read (rows at any byte): 64 tokens x 64 channels
 // per block, chunks of 64 codes of both operands joined byte by byte in shared memory, dp4a on 4x4 outputs a
-// thread.  The byte loads bound it: 1024 tokens x 1001 -> 1024 takes 72 us, 6.7 us where rows start at
+// thread.  The byte loads bound it: 1024 tokens x 1001 -> 1024 takes 90 us, 6.5 us where rows start at
 // multiples of 16 bytes (as quantize_rows lays codes, and weights are laid once).
 constexpr int kAnyTile = 64;
 

@@ -18,10 +18,10 @@
 //       filled shared memory's bandwidth.
 //
 // What bounds it (B200; device time in a graph, operands from DRAM):
-//   many tokens        4096 x 4096 x 8192 int8 88 us: 3.1 POP/s, the tensor pipe active 87 % of the time, at
-//                      the clock that the power limit leaves (int4 92 us; gated 92 and 104 us: two weight tiles
+//   many tokens        4096 x 4096 x 8192 int8 86 us: 3.2 POP/s, the tensor pipe active 89 % of the time, at
+//                      the clock that the power limit leaves (int4 90 us; gated 90 and 102 us: two weight tiles
 //                      to one of tokens, bound by the 64 bytes a cycle that an SM draws from L2)
-//   hundreds           512 x 4096 x 4096 12 us: again L2 to SM, and too few tiles to share them more
+//   hundreds           512 x 4096 x 4096 11 us: again L2 to SM, and too few tiles to share them more
 //   few                16 x 4096 x 4096 6.5 us: latency (set-up 1, first bytes 1, partial sums 0.7 us), then an MMA
 //                      of 16 columns, which takes 55 to 75 cycles instead of 8
 //

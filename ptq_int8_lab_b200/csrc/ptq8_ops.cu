@@ -280,12 +280,17 @@ int list_bytes_of(const ptq8_linear_args& a, bool listed) { return listed ? ((a.
 // A launch's time in cycles, up to what all variants share.  Per stage a CTA takes the longest of its chain (the
 // MMAs and the wait before them) and, for the CTAs that share an SM, their MMAs, their loads at what an SM draws
 // from L2, and the widening of int4 weights.  Few tiles are worth a cluster each: a split pays for sending and
-// joining its sums, and clusters of 4 and 8 do not fill every GPC.  The constants are fitted to 7200 timings of
-// 508 calls (1 to 8192 tokens, 512 to 16384 features, 1 to 64 groups, both types, gated or not) under every
-// variant: the variant of the least estimate is 1.6 % slower than the fastest one on average, 22 % at most.
+// joining its sums, and clusters of 4 and 8 do not fill every GPC.
+//
+// How well it chooses: 902 calls (1 to 8192 tokens, 512 to 16384 features, 1 to 64 groups; int8 and int4, with and
+// without SwiGLU) were timed as every variant and split not far too long for them, 6711 in all, each with operands from DRAM,
+// with operands in L2, and called from Python in a loop.  The choice is 2.5, 2.3 and 2.8 % slower than the fastest
+// variant on average, 14 to 19 % at the 95th percentile, and 64 % at most: tiles of 64 tokens with SwiGLU, which hold two
+// stages, are rated too well where the weights come from DRAM (128 tokens, 4096 -> 2 x 4096 int8: 25.7 us, a pair of 128
+// tokens 16.4).  Constants fitted to half of the calls did no better on the other half than these.
 float estimate(int sms, const ptq8_linear_args& a, int groups, const Variant& v, int split) {
     constexpr float kMma = 77.5f, kMmaTmem = 104;    // least cycles of an MMA, M operand in shared memory or TMEM
-    constexpr float kMmaTmemPair = 102;              // the latter for a pair: 4096 x 4096 x 4096 gated 100 us, one CTA a tile 105
+    constexpr float kMmaTmemPair = 102;              // the latter for a pair: 4096 x 4096 x 4096 gated 102 us, one CTA a tile 107
     constexpr float kWait = 144, kWaitTwo = 47;      // wait of the MMA warp per block (two blocks a stage)
     constexpr float kLoad = 61;                      // bytes per cycle into an SM
     constexpr float kWiden = 225;                    // int4: cycles of an SM per tile of 128 x 128 codes

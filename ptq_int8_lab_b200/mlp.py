@@ -9,7 +9,7 @@ states and prints how far they are from the same MLPs in float.
 Weights are quantized on the host with the engine's own quantizer (one scale per output
 channel, int8 or int4) and laid out once; activations are quantized per token on the way.
 A dense layer is four launches, one with experts the same four between its routing and the
-weighted sum of its rows.
+weighted sum of its rows.  No gradient passes through them.
 """
 from __future__ import annotations
 

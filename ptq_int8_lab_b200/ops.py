@@ -10,7 +10,8 @@ token, int8 or packed int4 weights with one scale per output channel, exact int3
 
 Calls enqueue on the current torch stream (or the one given) and return; nothing
 synchronises or allocates except outputs that the caller does not pass.  What is refused
-raises ``Ptq8Error``; tensors on the CPU are refused too.
+raises ``Ptq8Error``; tensors on the CPU are refused too.  There are no gradients: outputs
+never require one, also where an input does.
 """
 from __future__ import annotations
 
