@@ -59,3 +59,15 @@ def test_misaligned_tensors(ops):
     assert rc == INVALID and "aligned" in text
     assert linear_call(ops, False, **good, offsets=at[6] + 2)[0] == 0   # not looked at there
     torch.cuda.synchronize()
+
+
+def test_outputs_never_require_gradients(ops):
+    """Inputs may (weights kept as parameters, hidden states of a layer before): the outputs are those without, and say so."""
+    x = torch.randn((6, 64), device="cuda", requires_grad=True)
+    codes, scale = ops.quantize_rows(x)
+    again = ops.quantize_rows(x.detach())
+    assert not scale.requires_grad and torch.equal(codes, again[0]) and torch.equal(scale, again[1])
+    w = torch.randint(-128, 128, (32, 64), device="cuda", dtype=torch.int8)
+    ws = torch.nn.Parameter(torch.rand(32, device="cuda"))
+    y = ops.linear(codes, scale, w, ws, bias=ws)
+    assert not y.requires_grad and torch.equal(y, ops.linear(codes, scale, w, ws.detach(), bias=ws.detach()))
