@@ -394,6 +394,86 @@ int ptq8_linear_choose_as(int sms, const ptq8_linear_args* args, int grouped, in
  * cannot serve them. */
 int ptq8_ops_set_choice_test(ptq8_ops* ops, int variant, int split);
 
+/* ---- the cache of keys and values in 4 bits --------------------------------------
+ *
+ * A row (one token, one head; of the keys or the values) is head_dim codes of 4 bits, code 2 i in the low and 2 i + 1 in the
+ * high half of byte i, and a pair of bf16 numbers: step, then least.  Code c stands for least + step * c.  The rows of a
+ * head lie one after another in pages of `page` tokens.  A sequence's positions 0, 1, .. lie in the pages that its row of
+ * the table names, one after another; its length counts its positions, those of the new tokens among them, which are the
+ * last ones: of n new tokens, token i has position length - n + i.  New tokens of all sequences lie one after another:
+ * sequence b's are starts[b] .. starts[b + 1] - 1, or token b alone where starts is NULL.
+ *
+ * Table, lengths and starts are device memory and read on the device.  starts must not decrease; values outside
+ * [0, tokens] are clamped, and where they decrease no access leaves the tensors, but a token may be taken for another
+ * sequence's.  A position without a page (behind the table's row, before 0, or where the table names no page of the cache)
+ * is not written, reads as zeros and is not attended to.  Codes and pairs, and all of their page and head strides, are
+ * aligned to 16 bytes. */
+#define PTQ8_MAX_SEQUENCES 1024
+typedef struct {
+    uint8_t* k;             /* codes [pages][kv_heads][page][head_dim / 2] */
+    uint8_t* v;
+    uint16_t* k_scale;      /* bf16 (step, least) [pages][kv_heads][page][2] */
+    uint16_t* v_scale;
+    long long k_page, k_head, v_page, v_head;                                 /* strides in bytes */
+    long long k_scale_page, k_scale_head, v_scale_page, v_scale_head;
+    const int* table;       /* [sequences][table_width], pitch table_pitch elements */
+    long long table_pitch;
+    const int* lengths;     /* [sequences] */
+    const int* starts;      /* [sequences + 1] or NULL (then tokens == sequences) */
+    long long pages;
+    int table_width;
+    int page;               /* tokens of a page: 16, 32, 64, .. 4096 */
+    int kv_heads;
+    int head_dim;           /* 64, 128 or 256 */
+    int sequences;          /* up to PTQ8_MAX_SEQUENCES */
+    int reserved;
+} ptq8_cache;
+
+/* ptq8_cache_write: the new tokens' keys and values into the cache, for each row x
+ *   least = the largest bf16 number <= min x
+ *   step = max(the smallest bf16 number >= fl32(fl32(max x - least) / 15), 2^-100)
+ *   code = rint(fl32(fl32(x - least) * fl32(1 / step))) (halves to even), within 0 .. 15
+ * A row that holds NaN or an infinity, or whose spread no float holds, gets codes 0 and NaN for both: whatever attends to
+ * it is NaN.  A page that is written belongs to one sequence; where two write the same row it holds a mixture of theirs.
+ * ptq8_cache_read: what the cache holds at the new tokens' positions, fl32(least + step * code), rounded once more to
+ * `type`.  Tokens of no sequence are left as they were. */
+typedef struct {
+    ptq8_cache cache;
+    void* k;                /* [tokens][kv_heads][head_dim], head_dim consecutive; read by ptq8_cache_write, */
+    void* v;                /* written by ptq8_cache_read */
+    long long k_token, k_head, v_token, v_head;   /* strides in elements */
+    long long tokens;
+    int type;               /* PTQ8_F32 / F16 / BF16 */
+    int reserved;
+} ptq8_cache_rows_args;
+int ptq8_cache_write(ptq8_ops* ops, const ptq8_cache_rows_args* args, void* stream);
+int ptq8_cache_read(ptq8_ops* ops, const ptq8_cache_rows_args* args, void* stream);
+
+/* out[token][h] = sum_j p_j v_j, p = softmax_j(scale * q[token][h] . k_j), over the positions j up to the token's own, keys and
+ * values of head h / (heads / kv_heads).  A token that sees no position gets zeros; tokens of no sequence are left as they
+ * were.  Queries are f16 or bf16, the output has their type; sums and the softmax are f32, p (times the value's step) is rounded
+ * to f16's 11 bits for its product with the codes.  Rows of keys or values that a token does not see have no part in its
+ * output, whatever they hold.
+ * workspace: device memory of ptq8_cache_attention_workspace() bytes, aligned to 16 bytes, which this call alone uses until its
+ * kernels have run: calls on one stream may share it, calls on two streams or of two graphs that may run at once may not. */
+typedef struct {
+    ptq8_cache cache;
+    const void* q;          /* [tokens][heads][head_dim], head_dim consecutive */
+    void* out;              /* the same shape; must not overlap the inputs */
+    long long q_token, q_head, out_token, out_head;   /* strides in elements */
+    long long tokens;
+    void* workspace;
+    long long workspace_bytes;
+    float scale;
+    int heads;              /* a multiple of kv_heads */
+    int type;               /* PTQ8_F16 / BF16 */
+    int reserved;
+} ptq8_cache_attention_args;
+int ptq8_cache_attention(ptq8_ops* ops, const ptq8_cache_attention_args* args, void* stream);
+/* Bytes that a call with these arguments needs (0: it needs none), or -1 where it is refused (see ptq8_ops_last_error).
+ * Neither the tensors' addresses nor their contents count. */
+long long ptq8_cache_attention_workspace(ptq8_ops* ops, const ptq8_cache_attention_args* args);
+
 #ifdef __cplusplus
 }
 #endif

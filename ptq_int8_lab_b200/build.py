@@ -23,6 +23,7 @@ SOURCES = (
     ("ptq8_model.cpp", "ptq8_model.o", ["-x", "c++"]),
     ("ptq8_engine.cu", "ptq8_engine.o", ["-lineinfo"]),
     ("ptq8_ops.cu", "ptq8_ops.o", ["-lineinfo"]),
+    ("ptq8_cache.cu", "ptq8_cache.o", ["-lineinfo"]),
 )
 
 

@@ -1,22 +1,18 @@
 // Token operators: host side of ptq8_quantize_rows, ptq8_linear and ptq8_linear_grouped
 // (argument checks, kernel choice, launches) and their extern "C" boundary.
-#include <cuda.h>
-#include <cuda_runtime.h>
-#include <cudaTypedefs.h>
 
 #include <algorithm>
 #include <cmath>
-#include <cstdarg>
 #include <cstdio>
 #include <cstring>
 #include <iterator>
 #include <mutex>
 #include <new>
 
-#include "ptq8.h"
 #include "ptq8_linear.cuh"
 #include "ptq8_linear_few.cuh"
 #include "ptq8_linear_tc.cuh"
+#include "ptq8_ops.cuh"
 #include "ptq8_rows.cuh"
 
 using namespace ptq8;
@@ -24,66 +20,7 @@ using namespace ptq8;
 // what the Python mirror packs
 static_assert(sizeof(ptq8_rows_args) == 72 && sizeof(ptq8_linear_args) == 120, "argument structs");
 
-struct ptq8_ops {
-    int device = 0;
-    int sms = 0;
-    int* error = nullptr;       // pinned host word that a kernel whose bounded wait ran out sets (error_word())
-    int* error_dev = nullptr;   // its device address
-    long long wait_limit = kWaitLimitCycles;
-    int stall = 0;
-    int variant = -1, split = 1;   // test hook: the tile variant of every product
-    PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
-    char err[512] = "";         // message of the last refusal: a fixed buffer, since refusing must not throw
-};
-
 namespace {
-
-int fail(ptq8_ops* o, int status, const char* f, ...) {
-    va_list ap;
-    va_start(ap, f);
-    std::vsnprintf(o->err, sizeof o->err, f, ap);
-    va_end(ap);
-    return status;
-}
-
-// A message for a caller who has no handle yet.
-void say(char* err, size_t n, const char* f, const char* more = "") {
-    if (err && n) std::snprintf(err, n, f, more);
-}
-
-// The device becomes current for the call and is given back: a process may drive several.
-struct OnDevice {
-    int before = -1;
-    cudaError_t rc;
-    explicit OnDevice(int device) {
-        rc = cudaGetDevice(&before);
-        if (rc == cudaSuccess && before != device) rc = cudaSetDevice(device);
-        if (before == device) before = -1;
-    }
-    ~OnDevice() {
-        if (before >= 0) cudaSetDevice(before);
-    }
-};
-
-// One launch with programmatic stream serialization: the kernel may be scheduled while the kernel
-// before it on the stream drains, and waits (griddepcontrol.wait) before it touches global memory.
-template <typename... P, typename... A>
-cudaError_t launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, int cluster, cudaStream_t stream, const A&... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute at[2];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    at[1].id = cudaLaunchAttributeClusterDimension;
-    at[1].val.clusterDim.x = cluster;
-    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = cluster > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
 
 // A handle's error word, zero.  Words come from pinned blocks that stay with the process and no word is used again: a
 // kernel of a destroyed handle that is still running, or a graph that holds one, may write its word at any time after.
@@ -108,23 +45,6 @@ cudaError_t error_word(int** host, int** dev) {
     *dev = static_cast<int*>(at) + used;
     ++used;
     return cudaSuccess;
-}
-
-size_t type_size(int t) { return t == PTQ8_F32 ? 4 : 2; }
-
-bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
-
-// What every call checks first: a wait of an earlier call that ran out, until it is cleared.
-int ready(ptq8_ops* o) {
-    if (*static_cast<volatile int*>(o->error))
-        return fail(o, PTQ8_ERR_TIMEOUT, "a device wait of an earlier call ran out (code %d); its outputs are invalid",
-                    *o->error);
-    return PTQ8_OK;
-}
-
-int cuda_fail(ptq8_ops* o, const char* what, cudaError_t e) {
-    cudaGetLastError();   // reported here: the process's next check must not find it again
-    return fail(o, PTQ8_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
 int check_rows(ptq8_ops* o, const ptq8_rows_args& a) {
@@ -545,6 +465,7 @@ ptq8_ops* ptq8_ops_create(int device, char* err, size_t errlen) {
             if (e == cudaSuccess)
                 e = cudaFuncSetAttribute(reinterpret_cast<const void*>(v.kernel), cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          v.per_sm == 2 ? kSmemTwo : kSmemOne);
+        if (e == cudaSuccess) e = cache_attributes();
         int* host = nullptr;
         int* dev = nullptr;
         if (e == cudaSuccess) e = error_word(&host, &dev);

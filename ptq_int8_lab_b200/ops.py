@@ -29,6 +29,9 @@ EPI_SWIGLU = 1   # weights hold gate channels, then up channels: y = silu(gate) 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _ROWS = struct.Struct("QqqQqQqQii")           # ptq8_rows_args
 _LINEAR = struct.Struct("QqQQqqQQQqQqiiiiii")  # ptq8_linear_args
+_CACHE = "QQQQqqqqqqqqQqQQqiiiiii"             # ptq8_cache
+_CACHE_ROWS = struct.Struct(_CACHE + "QQqqqqqii")       # ptq8_cache_rows_args
+_ATTENTION = struct.Struct(_CACHE + "QQqqqqqQqfiii")    # ptq8_cache_attention_args
 
 try:
     _raw_stream = torch._C._cuda_getCurrentRawStream
@@ -60,8 +63,47 @@ def _check_vector(name: str, t: torch.Tensor, dtype, values: int, device: int):
         raise Ptq8Error(f"{name}: not contiguous")
 
 
-_F32, _I32, _INT8 = torch.float32, torch.int32, torch.int8
+_F32, _I32, _INT8, _U8, _BF16 = torch.float32, torch.int32, torch.int8, torch.uint8, torch.bfloat16
+_WORKSPACE = struct.Struct("Qq")
+_WORKSPACE_AT = struct.calcsize("@" + _CACHE + "QQqqqqq")   # its place in ptq8_cache_attention_args
 _CODES = {8: (torch.int8,), 4: (torch.uint8, torch.int8)}
+
+
+class Cache4(NamedTuple):
+    """Keys and values of one layer in 4 bits: pages of `page` tokens, for each head of a page its rows one after another.
+
+    Codes are two per byte, the even one low; scales are (step, least) pairs: code c stands for least + step * c."""
+    k: torch.Tensor         # uint8 [pages, kv_heads, page, head_dim // 2]
+    k_scale: torch.Tensor   # bf16 [pages, kv_heads, page, 2]
+    v: torch.Tensor
+    v_scale: torch.Tensor
+
+
+def new_cache(pages: int, kv_heads: int, head_dim: int, page: int = 64, device: int = 0) -> Cache4:
+    """An empty Cache4: zeros stand for zeros."""
+    def part(n, dtype):
+        return torch.zeros((pages, kv_heads, page, n), dtype=dtype, device=f"cuda:{device}")
+    return Cache4(part(head_dim // 2, torch.uint8), part(2, torch.bfloat16), part(head_dim // 2, torch.uint8), part(2, torch.bfloat16))
+
+
+def _check_part(name: str, t: torch.Tensor, dtype, shape, device: int):
+    if t.dtype != dtype or tuple(t.shape) != shape:
+        raise Ptq8Error(f"cache.{name}: {t.dtype} {tuple(t.shape)}, {dtype} {shape} is wanted")
+    if t.get_device() != device:
+        raise Ptq8Error(f"cache.{name}: on {t.device}, not on cuda:{device}")
+    if t.stride(3) != 1 or t.stride(2) != shape[3]:
+        raise Ptq8Error(f"cache.{name}: a head's rows of a page are not consecutive")
+
+
+def _check_rows(name: str, t: torch.Tensor, dtypes, shape, device: int):
+    if t.dtype not in dtypes:
+        raise Ptq8Error(f"{name}: dtype {t.dtype}")
+    if tuple(t.shape) != shape:
+        raise Ptq8Error(f"{name}: shape {tuple(t.shape)}, {shape} is wanted")
+    if t.get_device() != device:
+        raise Ptq8Error(f"{name}: on {t.device}, not on cuda:{device}")
+    if t.stride(2) != 1:
+        raise Ptq8Error(f"{name}: columns {t.stride(2)} elements apart, not consecutive")
 
 
 KERNEL_ANY, KERNEL_FEW, KERNEL_TILES = 0, 1, 2
@@ -121,6 +163,8 @@ class Int8Ops:
         self.device = device
         self._rows_args = ctypes.create_string_buffer(_ROWS.size)
         self._linear_args = ctypes.create_string_buffer(_LINEAR.size)
+        self._cache_args = ctypes.create_string_buffer(_CACHE_ROWS.size)
+        self._attention_args = ctypes.create_string_buffer(_ATTENTION.size)
 
     def _check(self, rc: int):
         if rc:
@@ -265,6 +309,136 @@ class Int8Ops:
             raise Ptq8Error("offsets: None")
         return self._product(self._grouped, x, x_scale, offsets, w, w_scale, bias, bits, act, dtype,
                              out, stream)
+
+    def _cache(self, cache, table, lengths, starts, tokens):
+        """The fields of ptq8_cache.  tokens: the new tokens, or None where starts is None (one per sequence)."""
+        k, ks, v, vs = cache
+        d = self.device
+        if k.dim() != 4:
+            raise Ptq8Error(f"cache.k: shape {tuple(k.shape)}, [pages, kv_heads, page, head_dim // 2] is wanted")
+        shape = tuple(k.shape)
+        pairs = (*shape[:3], 2)
+        # one look at what calls have in common; where it fails, _check_part says what is wrong
+        if (k.dtype is not _U8 or v.dtype is not _U8 or ks.dtype is not _BF16 or vs.dtype is not _BF16 or v.shape != k.shape
+                or tuple(ks.shape) != pairs or vs.shape != ks.shape):
+            for name, t, dtype, want in (("k", k, _U8, shape), ("v", v, _U8, shape), ("k_scale", ks, _BF16, pairs), ("v_scale", vs, _BF16, pairs)):
+                _check_part(name, t, dtype, want, d)
+        (kp, kh, kr, k1), (vp, vh, vr, v1) = k.stride(), v.stride()
+        (ksp, ksh, ksr, ks1), (vsp, vsh, vsr, vs1) = ks.stride(), vs.stride()
+        half = shape[3]
+        if (k1 != 1 or v1 != 1 or ks1 != 1 or vs1 != 1 or kr != half or vr != half or ksr != 2 or vsr != 2 or k.get_device() != d
+                or v.get_device() != d or ks.get_device() != d or vs.get_device() != d):
+            for name, t, dtype, want in (("k", k, _U8, shape), ("v", v, _U8, shape), ("k_scale", ks, _BF16, pairs), ("v_scale", vs, _BF16, pairs)):
+                _check_part(name, t, dtype, want, d)
+        if table.dim() != 2 or table.dtype is not _I32 or table.get_device() != d or (table.stride(1) != 1 and table.shape[1] > 1):
+            _check_matrix("table", table, (_I32,), 2, d)
+        seqs, wide = table.shape
+        if lengths.dtype is not _I32 or lengths.numel() != seqs or not lengths.is_contiguous() or lengths.get_device() != d:
+            _check_vector("lengths", lengths, _I32, seqs, d)
+        at = 0
+        if starts is not None:
+            if starts.dtype is not _I32 or starts.numel() != seqs + 1 or not starts.is_contiguous() or starts.get_device() != d:
+                _check_vector("starts", starts, _I32, seqs + 1, d)
+            at = starts.data_ptr()
+        elif tokens != seqs:
+            raise Ptq8Error(f"{tokens} tokens without starts, but {seqs} sequences")
+        return (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), kp, kh, vp, vh, 2 * ksp, 2 * ksh, 2 * vsp, 2 * vsh,
+                table.data_ptr(), table.stride(0), lengths.data_ptr(), at, shape[0], wide, shape[2], shape[1], 2 * half, seqs, 0)
+
+    def _cache_rows(self, call, cache, k, v, table, lengths, starts, stream):
+        if k.dim() != 3:
+            raise Ptq8Error(f"k: shape {tuple(k.shape)}, [tokens, kv_heads, head_dim] is wanted")
+        fields = self._cache(cache, table, lengths, starts, k.shape[0])
+        dtype = _TYPES.get(k.dtype)
+        want = (k.shape[0], fields[19], fields[20])
+        if dtype is None or tuple(k.shape) != want or k.get_device() != self.device or k.stride(2) != 1:
+            _check_rows("k", k, _TYPES, want, self.device)
+        if v.dtype is not k.dtype or tuple(v.shape) != want or v.get_device() != self.device or v.stride(2) != 1:
+            _check_rows("v", v, (k.dtype,), want, self.device)
+        _CACHE_ROWS.pack_into(self._cache_args, 0, *fields, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+                              want[0], dtype, 0)
+        rc = call(self._h, self._cache_args, self._stream(stream, True))
+        if rc:
+            self._check(rc)
+
+    def cache_write(self, cache: Cache4, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
+                    starts: Optional[torch.Tensor] = None, stream=None) -> None:
+        """Keys and values k, v [T, kv_heads, head_dim] (f32 / f16 / bf16) of new tokens into the cache, in 4 bits.
+
+        table int32 [sequences, n]: the pages of each sequence; lengths int32 [sequences]: its positions, the new tokens (its
+        last ones) among them; starts int32 [sequences + 1]: sequence b's new tokens are starts[b] .. starts[b + 1] - 1, without
+        it token b alone.  Positions without a page are skipped.  A page that is written belongs to one sequence."""
+        self._cache_rows(self._lib.ptq8_cache_write, cache, k, v, table, lengths, starts, stream)
+
+    def cache_read(self, cache: Cache4, table: torch.Tensor, lengths: torch.Tensor, starts: Optional[torch.Tensor] = None,
+                   tokens: Optional[int] = None, dtype: torch.dtype = torch.bfloat16, out=None, stream=None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """(k, v) [T, kv_heads, head_dim] that the cache holds at the positions where cache_write with the same arguments
+        writes; zeros where a position has no page.  With starts and without out, tokens is T.  Rows of no sequence are not
+        written."""
+        stream = self._stream(stream, out is not None)
+        if out is None:
+            if dtype not in _TYPES:
+                raise Ptq8Error(f"dtype {dtype}: f32, f16 or bf16")
+            if tokens is None:
+                if starts is not None:
+                    raise Ptq8Error("tokens: None; with starts and without out it tells how many there are")
+                tokens = table.shape[0]
+            shape = (tokens, cache[0].shape[1], 2 * cache[0].shape[3])
+            out = tuple(torch.empty(shape, dtype=dtype, device=f"cuda:{self.device}") for _ in range(2))
+        k, v = out
+        self._cache_rows(self._lib.ptq8_cache_read, cache, k, v, table, lengths, starts, stream)
+        return k, v
+
+    def cache_attention(self, q: torch.Tensor, cache: Cache4, table: torch.Tensor, lengths: torch.Tensor,
+                        starts: Optional[torch.Tensor] = None, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                        workspace: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+        """softmax(scale * q k^T) v of queries q [T, heads, head_dim] (f16 / bf16) over the cache, causal: a token sees the positions
+        of its sequence up to its own.  table, lengths, starts as in cache_write (which comes first: the new tokens attend to
+        themselves too).  heads is a multiple of the cache's kv_heads; scale: head_dim ** -0.5 where not given.  A token that sees
+        nothing gets zeros; tokens of no sequence are not written.
+
+        workspace: uint8, cache_attention_workspace() bytes; one is made where it is not given, which with stream it has to be."""
+        stream = self._stream(stream, out is not None and workspace is not None)
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        args, need = self._attention(q, cache, table, lengths, starts, scale, out)
+        if workspace is None:
+            if need:
+                workspace = torch.empty(need, dtype=_U8, device=q.device)
+        elif workspace.dtype is not _U8 or not workspace.is_contiguous() or workspace.get_device() != self.device:
+            raise Ptq8Error(f"workspace: {workspace.dtype} on {workspace.device}, consecutive uint8 on cuda:{self.device} is wanted")
+        at, size = (workspace.data_ptr(), workspace.numel()) if workspace is not None else (0, 0)
+        _WORKSPACE.pack_into(args, _WORKSPACE_AT, at, size)
+        rc = self._lib.ptq8_cache_attention(self._h, args, stream)
+        if rc:
+            self._check(rc)
+        return out
+
+    def _attention(self, q, cache, table, lengths, starts, scale, out):
+        if q.dim() != 3:
+            raise Ptq8Error(f"q: shape {tuple(q.shape)}, [tokens, heads, head_dim] is wanted")
+        d = self.device
+        tokens, heads, dim = q.shape
+        fields = self._cache(cache, table, lengths, starts, tokens)
+        kind = _TYPES.get(q.dtype)
+        if not kind or dim != fields[20] or q.get_device() != d or q.stride(2) != 1:
+            _check_rows("q", q, (torch.float16, _BF16), (tokens, heads, fields[20]), d)
+        if out.dtype is not q.dtype or out.shape != q.shape or out.get_device() != d or out.stride(2) != 1:
+            if out.dim() != 3:
+                raise Ptq8Error(f"out: shape {tuple(out.shape)}, {tuple(q.shape)} is wanted")
+            _check_rows("out", out, (q.dtype,), tuple(q.shape), d)
+        args = self._attention_args
+        _ATTENTION.pack_into(args, 0, *fields, q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1), tokens,
+                             0, 0, dim ** -0.5 if scale is None else scale, heads, kind, 0)
+        need = self._lib.ptq8_cache_attention_workspace(self._h, args)
+        if need < 0:
+            self._check(1)
+        return args, need
+
+    def cache_attention_workspace(self, q: torch.Tensor, cache: Cache4, table: torch.Tensor, lengths: torch.Tensor,
+                                  starts: Optional[torch.Tensor] = None) -> int:
+        """Bytes of workspace that cache_attention() needs for tensors of these shapes.  A workspace serves one call at a time."""
+        return self._attention(q, cache, table, lengths, starts, None, q)[1]
 
     def check_device_error(self, stream=None):
         """Wait for the stream; raise Ptq8Error (status PTQ8_ERR_TIMEOUT) if a bounded device wait ran out."""
