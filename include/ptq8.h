@@ -394,6 +394,33 @@ int ptq8_linear_choose_as(int sms, const ptq8_linear_args* args, int grouped, in
  * cannot serve them. */
 int ptq8_ops_set_choice_test(ptq8_ops* ops, int variant, int split);
 
+/* y[t][c] = sum_g w_scale[c][g] * (sum_{k in group g} code[c][k] * x[t][k]) + bias[c], then the epilogue, then one rounding to
+ * y's type: float activations, 4-bit weights with a scale per `group` consecutive input features (the last group may be
+ * shorter).  Codes lie as ptq8_linear's do with w_bits 4.  Sums are f32; f16 and bf16 activations are not rounded (what is less than
+ * 2^-28 of the largest among 128 beside it may lose places), f32 ones keep 22 places.  A token that holds NaN or an infinity
+ * gives NaN.
+ * Groups of a multiple of 32 features (or of all) with weights and pitches at multiples of 16 bytes run on the tensor cores;
+ * any other group and layout on a slower kernel. */
+typedef struct {
+    const void* x;         /* [rows][in_features], pitch ldx elements */
+    long long ldx;
+    const void* w;         /* [channels][in_features], two codes per byte, pitch ldw bytes */
+    long long ldw;
+    const void* w_scale;   /* [channels][groups], pitch lds elements */
+    long long lds;
+    const float* bias;     /* [channels] or NULL */
+    void* y;               /* [rows][out_features], pitch ldy elements; must not overlap the inputs */
+    long long ldy;
+    long long rows;
+    int in_features;
+    int out_features;      /* channels = out_features, or twice that with PTQ8_EPI_SWIGLU */
+    int group;
+    int epilogue;          /* PTQ8_EPI_* */
+    int x_type, scale_type, y_type;   /* PTQ8_F32 / F16 / BF16 */
+    int reserved;
+} ptq8_linear_w4_args;
+int ptq8_linear_w4(ptq8_ops* ops, const ptq8_linear_w4_args* args, void* stream);
+
 /* ---- the cache of keys and values in 4 bits --------------------------------------
  *
  * A row (one token, one head; of the keys or the values) is head_dim codes of 4 bits, code 2 i in the low and 2 i + 1 in the

@@ -24,6 +24,7 @@ SOURCES = (
     ("ptq8_engine.cu", "ptq8_engine.o", ["-lineinfo"]),
     ("ptq8_ops.cu", "ptq8_ops.o", ["-lineinfo"]),
     ("ptq8_cache.cu", "ptq8_cache.o", ["-lineinfo"]),
+    ("ptq8_w4.cu", "ptq8_w4.o", ["-lineinfo"]),
 )
 
 

@@ -466,6 +466,7 @@ ptq8_ops* ptq8_ops_create(int device, char* err, size_t errlen) {
                 e = cudaFuncSetAttribute(reinterpret_cast<const void*>(v.kernel), cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          v.per_sm == 2 ? kSmemTwo : kSmemOne);
         if (e == cudaSuccess) e = cache_attributes();
+        if (e == cudaSuccess) e = w4_attributes();
         int* host = nullptr;
         int* dev = nullptr;
         if (e == cudaSuccess) e = error_word(&host, &dev);

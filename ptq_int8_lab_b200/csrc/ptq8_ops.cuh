@@ -92,5 +92,6 @@ inline int cuda_fail(ptq8_ops* o, const char* what, cudaError_t e) {
 
 // What the kernels of the other sources need set once per device, at a handle's creation.
 cudaError_t cache_attributes();
+cudaError_t w4_attributes();
 
 }  // namespace ptq8

@@ -56,6 +56,7 @@ EXPORTS = (
     "ptq8_ops_set_wait_test", "ptq8_quantize_rows", "ptq8_linear", "ptq8_linear_grouped",
     "ptq8_linear_variants", "ptq8_linear_choose", "ptq8_linear_choose_as", "ptq8_ops_set_choice_test",
     "ptq8_cache_write", "ptq8_cache_read", "ptq8_cache_attention", "ptq8_cache_attention_workspace",
+    "ptq8_linear_w4",
 )
 
 
@@ -153,6 +154,7 @@ def lib() -> ctypes.CDLL:
         "ptq8_linear_choose": (c_int, [c_int, c_void_p, c_int, c_void_p]),
         "ptq8_linear_choose_as": (c_int, [c_int, c_void_p, c_int, c_int, c_int, c_void_p]),
         "ptq8_ops_set_choice_test": (c_int, [c_void_p, c_int, c_int]),
+        "ptq8_linear_w4": (c_int, [c_void_p, c_void_p, c_void_p]),
         "ptq8_cache_write": (c_int, [c_void_p, c_void_p, c_void_p]),
         "ptq8_cache_read": (c_int, [c_void_p, c_void_p, c_void_p]),
         "ptq8_cache_attention": (c_int, [c_void_p, c_void_p, c_void_p]),

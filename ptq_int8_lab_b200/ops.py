@@ -29,6 +29,7 @@ EPI_SWIGLU = 1   # weights hold gate channels, then up channels: y = silu(gate) 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _ROWS = struct.Struct("QqqQqQqQii")           # ptq8_rows_args
 _LINEAR = struct.Struct("QqQQqqQQQqQqiiiiii")  # ptq8_linear_args
+_W4 = struct.Struct("QqQqQqQQqqiiiiiiii")      # ptq8_linear_w4_args
 _CACHE = "QQQQqqqqqqqqQqQQqiiiiii"             # ptq8_cache
 _CACHE_ROWS = struct.Struct(_CACHE + "QQqqqqqii")       # ptq8_cache_rows_args
 _ATTENTION = struct.Struct(_CACHE + "QQqqqqqQqfiii")    # ptq8_cache_attention_args
@@ -163,6 +164,7 @@ class Int8Ops:
         self.device = device
         self._rows_args = ctypes.create_string_buffer(_ROWS.size)
         self._linear_args = ctypes.create_string_buffer(_LINEAR.size)
+        self._w4_args = ctypes.create_string_buffer(_W4.size)
         self._cache_args = ctypes.create_string_buffer(_CACHE_ROWS.size)
         self._attention_args = ctypes.create_string_buffer(_ATTENTION.size)
 
@@ -309,6 +311,53 @@ class Int8Ops:
             raise Ptq8Error("offsets: None")
         return self._product(self._grouped, x, x_scale, offsets, w, w_scale, bias, bits, act, dtype,
                              out, stream)
+
+    def linear_w4(self, x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, group: int, bias: Optional[torch.Tensor] = None,
+                  act: int = EPI_NONE, dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+        """y [T, out] of float activations x [T, in] (f32 / f16 / bf16) and 4-bit weight codes w [channels, (in + 1) // 2] (code k in the
+        low half of byte k // 2 for even k) with a scale per `group` consecutive input features: w_scale [channels,
+        ceil(in / group)] (f32 / f16 / bf16).  act EPI_SWIGLU: channels = 2 * out, gate then up.  dtype: of y where out is not given
+        (None: x's).  For generation: one to some tens of tokens."""
+        d = self.device
+        if act != EPI_NONE and act != EPI_SWIGLU:
+            raise Ptq8Error(f"act {act}: EPI_NONE or EPI_SWIGLU")
+        if not 0 < group <= 0x7FFFFFFF:
+            raise Ptq8Error(f"group {group}")
+        for name, t, dtypes in (("x", x, _TYPES), ("w", w, _CODES[4]), ("w_scale", w_scale, _TYPES)):
+            if t.dim() != 2 or t.dtype not in dtypes or t.get_device() != d or t.stride(1) != 1:
+                _check_matrix(name, t, dtypes, 2, d)
+        rows, k = x.shape
+        channels, wide = w.shape
+        if wide != (k + 1) // 2:
+            raise Ptq8Error(f"w: rows of {wide} bytes for {k} input features at 4 bits")
+        if w_scale.shape[0] != channels or w_scale.shape[1] != -(-k // group):
+            raise Ptq8Error(f"w_scale: shape {tuple(w_scale.shape)}, {(channels, -(-k // group))} is wanted")
+        b = 0
+        if bias is not None:
+            if bias.dtype is not _F32 or bias.numel() != channels or not bias.is_contiguous() or bias.get_device() != d:
+                _check_vector("bias", bias, _F32, channels, d)
+            b = bias.data_ptr()
+        n = channels
+        if act == EPI_SWIGLU:
+            if channels % 2:
+                raise Ptq8Error(f"w: {channels} channels do not split into gate and up")
+            n = channels // 2
+        stream = self._stream(stream, out is not None)
+        if out is None:
+            dtype = dtype or x.dtype
+            if dtype not in _TYPES:
+                raise Ptq8Error(f"dtype {dtype}: f32, f16 or bf16")
+            out = torch.empty((rows, n), dtype=dtype, device=x.device)
+        elif out.dim() != 2 or out.dtype not in _TYPES or out.get_device() != d or out.stride(1) != 1:
+            _check_matrix("out", out, _TYPES, 2, d)
+        if out.shape[0] != rows or out.shape[1] != n:
+            raise Ptq8Error(f"out: shape {tuple(out.shape)}, {(rows, n)} is wanted")
+        _W4.pack_into(self._w4_args, 0, x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), w_scale.data_ptr(), w_scale.stride(0), b,
+                      out.data_ptr(), out.stride(0), rows, k, n, group, act, _TYPES[x.dtype], _TYPES[w_scale.dtype], _TYPES[out.dtype], 0)
+        rc = self._lib.ptq8_linear_w4(self._h, self._w4_args, stream)
+        if rc:
+            self._check(rc)
+        return out
 
     def _cache(self, cache, table, lengths, starts, tokens):
         """The fields of ptq8_cache.  tokens: the new tokens, or None where starts is None (one per sequence)."""
