@@ -10,7 +10,7 @@
 // bf16, and what is more than 2^28 below the largest loses places only then.  p step_v is rounded to f16's 11 bits (an
 // output has 11, or bf16's 8), with 2^-24 of the largest as its finest step; everything else is f32.
 //
-// A warp takes 16 tokens at a time as the rows of its products, 8 NT query rows (query token x head of a key's group) as
+// A warp takes 16 tokens as the rows of its products, 8 NT query rows (query token x head of a key's group) as
 // the columns: keys codes [16 tokens x D] x queries [D x rows], then values codes [D x 16 tokens] x p [16 tokens x rows].
 // Which of a lane's codes stands for which place of a product is free as long as both operands agree, so a lane reads
 // its keys and values from the cache's own order, 4 D / 32 and 4 D / 64 words at a time.
@@ -18,7 +18,7 @@
 // The softmax is kept running: a row's reference is moved only when a score passes it by 8 (in powers of two), a vote of
 // the warp that fails almost always, and the sums of 8 lanes meet at the end of a segment.
 //
-// Work is units of 64 tokens of one key head and row tile.  All sequences' units lie in one order, and CTA c of N takes
+// Work is units of 128 tokens of one key head and row tile.  All sequences' units lie in one order, and CTA c of N takes
 // those from c U / N to (c + 1) U / N: equal shares whatever the lengths are, known on the device only.  A row tile cut
 // by a share's end leaves (numerators, reference, sum) in the workspace, and a second kernel joins them.
 // A producer warp keeps bulk copies of whole tiles in flight; four warps compute, RW of them on different rows, 4 / RW on
@@ -30,15 +30,17 @@
 
 namespace ptq8 {
 
-constexpr int kAttTile = 64, kAttWarps = 4, kAttThreads = 32 * (kAttWarps + 1);
+constexpr int kAttTile = 128, kAttWarps = 4, kAttThreads = 32 * (kAttWarps + 1);
 constexpr float kAttNone = -1e30f;   // reference of a row that has seen nothing
 constexpr float kAttSlack = 8.0f;
+// What a row tile costs beside its tokens (queries in, numerators joined and out), in units.
+constexpr int kAttOver = 2;
 
 struct AttDesc {
-    int slot, last;        // first partial result of the row tile, the last CTA that has one (-1: nothing to join)
-    int rows, head;        // of this tile; the key head
-    long long token0;      // of its sequence
-    int row0, pad;
+    int first, last;       // the CTAs that have parts of a row tile that is cut (last -1: it is not)
+    int rows, head, row0;  // of the sequence; the tile's key head and first row
+    int token0;            // of its sequence
+    int pad[2];
 };
 
 struct AttParams {
@@ -49,11 +51,12 @@ struct AttParams {
     float scale_log2;   // scale * log2(e)
     int per;            // query heads of a key head
     int by_item;        // 1: a CTA per row tile, none cut; 0: equal shares
+    int listed;         // descriptions by row tile (one new token per sequence, no more row tiles than CTAs), not by CTA
     int type;           // Y_F16 or Y_BF16
     int vec_q, vec_o;   // rows at multiples of 16 bytes
     float* part;        // [2 N][R][D] numerators
     float* stat;        // [2 N][R][2] reference, sum
-    AttDesc* desc;      // [N]
+    AttDesc* desc;      // [N], or by row tile
     long long wait_limit;
     int* err;
     int stall;
@@ -97,22 +100,30 @@ __device__ __forceinline__ float exp2_int(int e) { return __int_as_float((e + 12
 template <int D, int NT, int RW>
 struct AttShape {
     static constexpr int R = 8 * NT * RW, TW = kAttWarps / RW;
+    static constexpr int H = 2;   // products of 16 tokens at a time
     static constexpr int kPerSm = D * NT <= 128 ? 3 : 2;
-    static constexpr int kStages = 4;
+    static constexpr int kStages = D == 256 ? 2 : 3;
     static constexpr int kCodes = kAttTile * D / 2, kPairs = kAttTile * 4, kStage = 2 * (kCodes + kPairs);
     static constexpr int kPitch = D + 4;   // floats of a row of the joining buffer, off the banks' period
     static constexpr int kJoin = kAttWarps * 8 * NT * kPitch * 4, kStats = kAttWarps * 8 * NT * 2 * 4;
-    static constexpr int smem(int seqs) { return kStages * kStage + kJoin + kStats + (seqs + 1) * 8 + 128; }
+    // a warp's query fragments lie in its own part of the joining buffer, which it writes when it is done with them
+    static constexpr int kWarp = 8 * NT * kPitch * 4;
+    static_assert(NT * (D / 32) * 32 * 16 <= kWarp && kJoin == kAttWarps * kWarp, "query fragments fit");
+    // query rows that the producer fetches ahead (the largest tile of 256 dimensions has no room for them)
+    static constexpr bool kAhead = D < 256 || RW < 4;
+    static constexpr int kQueries = kAhead ? R * D * 2 : 0;
+    static constexpr int smem(int seqs) { return kStages * kStage + kJoin + kQueries + kStats + (seqs + 1) * 4; }
+    static_assert(kPerSm * (smem(1024) + 1024 + 256) <= 228 * 1024, "shared memory of an SM");
 };
 
 // A warp's query rows and what it has of their softmax.  Lane (g, t) = (lane / 4, lane % 4) holds, for the products,
 // row g of each tile of 8; of the sums, rows 2 t and 2 t + 1.
 template <int D, int NT>
 struct AttRows {
-    uint32_t q[NT][D / 32][4];
-    float a[NT][2], b[NT][2];            // score in powers of two = a * (step (q . codes) + least b)
-    float m[NT][2], l[NT][2], lo[NT][2]; // reference, sum of p, sum of p least_v
-    int lim[NT][2];                      // positions that the row sees
+    const uint4* q;               // fragments [NT][D / 32][32 lanes]: of a word of keys, those of its codes 0, 4; 1, 5; 2, 6; 3, 7
+    float2 a[NT], b[NT];          // score in powers of two = a * (step (q . codes) + least b)
+    float2 m[NT], l[NT], lo[NT];  // reference, sum of p, sum of p least_v
+    int lim[NT][2];               // positions that the row sees
     float o[D / 16][NT][4];
     float c;                             // what p step_v is multiplied by: a power of two
 };
@@ -121,9 +132,9 @@ __device__ __forceinline__ float att_value(const void* p, long long at, int type
     return type == Y_F16 ? __half2float(static_cast<const __half*>(p)[at]) : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[at]);
 }
 
-// The lane's part of the query rows from `row` on: D / 4 values of each tile's row g.
+// The lane's part of the query rows from `row0` on: D / 4 values of each tile's row g.  ahead: those rows in shared memory, or null.
 template <int D, int NT>
-__device__ __forceinline__ void att_queries(const AttParams& p, AttRows<D, NT>& r, long long token0, int n, int head, int row0, int rows, long long len) {
+__device__ __forceinline__ void att_queries(const AttParams& p, AttRows<D, NT>& r, uint4* q, long long token0, int n, int head, int row0, int rows, long long len, const void* ahead) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     constexpr int DL = D / 4;
     const long long cap = static_cast<long long>(p.c.width) << p.c.shift;
@@ -135,13 +146,14 @@ __device__ __forceinline__ void att_queries(const AttParams& p, AttRows<D, NT>& 
             const int i = row / p.per, j = row - i * p.per;
             const long long at = (token0 + i) * p.q_token + static_cast<long long>(head * p.per + j) * p.q_head + t * DL;
             if (p.vec_q) {
+                const char* from = ahead ? static_cast<const char*>(ahead) + ((nt * 8 + g) * D + t * DL) * 2 : static_cast<const char*>(p.q) + 2 * at;
 #pragma unroll
                 for (int k = 0; k < DL / 8; ++k) {
                     float e[8];
                     if (p.type == Y_F16)
-                        load8<__half, true>(static_cast<const __half*>(p.q) + at + 8 * k, e);
+                        load8<__half, true>(reinterpret_cast<const __half*>(from) + 8 * k, e);
                     else
-                        load8<__nv_bfloat16, true>(static_cast<const __nv_bfloat16*>(p.q) + at + 8 * k, e);
+                        load8<__nv_bfloat16, true>(reinterpret_cast<const __nv_bfloat16*>(from) + 8 * k, e);
 #pragma unroll
                     for (int z = 0; z < 8; ++z) f[8 * k + z] = e[z];
                 }
@@ -172,21 +184,19 @@ __device__ __forceinline__ void att_queries(const AttParams& p, AttRows<D, NT>& 
 #pragma unroll
         for (int w = 0; w < D / 32; ++w) {
             const float* x = f + 8 * w;
-            r.q[nt][w][0] = pair_of<__half>(x[0], x[4]);
-            r.q[nt][w][1] = pair_of<__half>(x[1] * 0.0625f, x[5] * 0.0625f);
-            r.q[nt][w][2] = pair_of<__half>(x[2], x[6]);
-            r.q[nt][w][3] = pair_of<__half>(x[3] * 0.0625f, x[7] * 0.0625f);
+            q[(nt * (D / 32) + w) * 32 + lane] = make_uint4(pair_of<__half>(x[0], x[4]), pair_of<__half>(x[1] * 0.0625f, x[5] * 0.0625f),
+                                                            pair_of<__half>(x[2], x[6]), pair_of<__half>(x[3] * 0.0625f, x[7] * 0.0625f));
         }
         // the products are 2^(e - 24) of the true ones; NaN and infinities in a row make all of its scores NaN
         const float a = isfinite(top) ? exp2_int(24 - e) * p.scale_log2 : __int_as_float(0x7FC00000);
         const float b = sum * 0x1p-24f;
+        r.a[nt] = make_float2(__shfl_sync(0xffffffffu, a, 8 * t), __shfl_sync(0xffffffffu, a, 8 * t + 4));
+        r.b[nt] = make_float2(__shfl_sync(0xffffffffu, b, 8 * t), __shfl_sync(0xffffffffu, b, 8 * t + 4));
+        r.m[nt] = both(kAttNone);
+        r.l[nt] = r.lo[nt] = both(0.0f);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int src = (2 * t + i) * 4, my = row0 + nt * 8 + 2 * t + i;
-            r.a[nt][i] = __shfl_sync(0xffffffffu, a, src);
-            r.b[nt][i] = __shfl_sync(0xffffffffu, b, src);
-            r.m[nt][i] = kAttNone;
-            r.l[nt][i] = r.lo[nt][i] = 0.0f;
+            const int my = row0 + nt * 8 + 2 * t + i;
             // query i of n sees the positions up to its own; rows past the end see all (nothing is kept of them)
             r.lim[nt][i] = my < rows ? static_cast<int>(min(max(len - n + my / p.per + 1, 0LL), cap)) : 0x7FFFFFFF;
         }
@@ -198,148 +208,175 @@ __device__ __forceinline__ void att_queries(const AttParams& p, AttRows<D, NT>& 
 #pragma unroll
             for (int i = 0; i < 4; ++i) r.o[mt][nt][i] = 0.0f;
     r.c = 0x1p120f;   // as for a bound of 2^-113 on step_v
+    r.q = q + lane;
+    __syncwarp();
 }
 
 constexpr uint32_t kLow = 0x000F000Fu, kHigh = 0x00F000F0u;
 
-// 16 tokens: tk is the first one's place in the tile, pos its position.  MASKED: some row does not see all of them, or
-// not all are there: `there` tokens from tk on, and where bit i of `pieces` is not set those of piece i (1 << shift tokens).
-template <int D, int NT, bool MASKED>
+// 16 H tokens, as H products: tk is the first one's place in the tile, pos its position.  MASKED: some row does not see
+// all of them, or not all are there: those before position `seen`, where bit i of `pieces` is set for piece i of the tile
+// (1 << piece_shift tokens).
+template <int D, int NT, int H, bool MASKED>
 __device__ __forceinline__ void att_step(AttRows<D, NT>& r, const uint8_t* K, const uint8_t* V, const uint32_t* KS, const uint32_t* VS, int tk,
                                          int pos, int seen, uint32_t pieces, int piece_shift) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     // row m of a product is token m ^ (m / 2 % 2): the lanes that read values together then meet fewer banks twice
     const int pg = g ^ ((g >> 1) & 1);
-    uint32_t ka[D / 32], kb[D / 32];
-    load_words(ka, K + (tk + pg) * (D / 2) + t * (D / 8));
-    load_words(kb, K + (tk + pg + 8) * (D / 2) + t * (D / 8));
-    uint32_t pk[2] = {KS[tk + pg], KS[tk + pg + 8]}, pv[2] = {VS[tk + pg], VS[tk + pg + 8]};
-    int at[2];
-    if constexpr (MASKED) {
+    // the lane's scores: of product h, rows pg + 8 (i / 2), query rows 2 t + i % 2
+    float x[H][NT][4] = {};
+    uint32_t pk[H][2], pv[H][2];
+    int at[H][2];
+    uint32_t keys[H][2][D / 32];
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+        const int tok = tk + 16 * h + pg;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            at[i] = pos + pg + 8 * i;
-            const bool ok = at[i] < seen && ((pieces >> ((tk + pg + 8 * i) >> piece_shift)) & 1);
-            if (!ok) pk[i] = pv[i] = 0, at[i] = 0x7FFFFFFF;   // what lies there is not looked at
+            pk[h][i] = KS[tok + 8 * i], pv[h][i] = VS[tok + 8 * i];
+            if constexpr (MASKED) {
+                at[h][i] = pos + 16 * h + pg + 8 * i;
+                const bool ok = at[h][i] < seen && ((pieces >> ((tok + 8 * i) >> piece_shift)) & 1);
+                if (!ok) pk[h][i] = pv[h][i] = 0, at[h][i] = 0x7FFFFFFF;   // what lies there is not looked at
+            }
+            load_words(keys[h][i], K + (tok + 8 * i) * (D / 2) + t * (D / 8));
         }
     }
-    float s[NT][4] = {}, s2[NT][4] = {};
 #pragma unroll
     for (int w = 0; w < D / 32; ++w) {
+        uint4 q[NT];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma_16816(s[nt], ka[w] & kLow, kb[w] & kLow, ka[w] & kHigh, kb[w] & kHigh, r.q[nt][w][0], r.q[nt][w][1]);
-        const uint32_t x = ka[w] >> 8, y = kb[w] >> 8;
+        for (int nt = 0; nt < NT; ++nt) q[nt] = r.q[(nt * (D / 32) + w) * 32];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma_16816(s2[nt], x & kLow, y & kLow, x & kHigh, y & kHigh, r.q[nt][w][2], r.q[nt][w][3]);
+        for (int z = 0; z < 2; ++z)
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                const uint32_t u = z ? keys[h][0][w] >> 8 : keys[h][0][w], v = z ? keys[h][1][w] >> 8 : keys[h][1][w];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma_16816(x[h][nt], u & kLow, v & kLow, u & kHigh, v & kHigh, z ? q[nt].z : q[nt].x, z ? q[nt].w : q[nt].y);
+            }
     }
-    float vstep[2], vleast[2];
+    // scores over a; `move`: one passes its row's reference by too much, or a value's step its bound
+    float vstep[H][2], steps = 0.0f, most = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) vstep[i] = __uint_as_float(pv[i] << 16), vleast[i] = __uint_as_float(pv[i] & 0xFFFF0000u);
-    // scores over a, then their distance to the reference in powers of two
-    bool move = fmaxf(vstep[0], vstep[1]) * r.c > 128.0f;
+    for (int h = 0; h < H; ++h)
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+        for (int i = 0; i < 2; ++i) {
+            vstep[h][i] = __uint_as_float(pv[h][i] << 16);
+            steps = fmaxf(steps, vstep[h][i]);
+            const float2 step = both(__uint_as_float(pk[h][i] << 16)), least = both(__uint_as_float(pk[h][i] & 0xFFFF0000u));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int tok = i >> 1, row = i & 1;
-            const float step = __uint_as_float(pk[tok] << 16), least = __uint_as_float(pk[tok] & 0xFFFF0000u);
-            float x = __fmaf_rn(s[nt][i] + s2[nt][i], step, least * r.b[nt][row]);
-            if (MASKED && (at[tok] == 0x7FFFFFFF || at[tok] >= r.lim[nt][row])) x = -INFINITY;
-            s[nt][i] = x;
-            s2[nt][i] = __fmaf_rn(x, r.a[nt][row], -r.m[nt][row]);
-            if (MASKED && x == -INFINITY) s2[nt][i] = -INFINITY;   // (a is NaN for a row that is not finite)
-            move = move || s2[nt][i] > kAttSlack;
+            for (int nt = 0; nt < NT; ++nt) {
+                float2 v = __ffma2_rn(make_float2(x[h][nt][2 * i], x[h][nt][2 * i + 1]), step, __fmul2_rn(least, r.b[nt]));
+                if (MASKED) {
+                    if (at[h][i] == 0x7FFFFFFF || at[h][i] >= r.lim[nt][0]) v.x = -INFINITY;
+                    if (at[h][i] == 0x7FFFFFFF || at[h][i] >= r.lim[nt][1]) v.y = -INFINITY;
+                }
+                x[h][nt][2 * i] = v.x, x[h][nt][2 * i + 1] = v.y;
+                const float2 d = __ffma2_rn(v, r.a[nt], make_float2(-r.m[nt].x, -r.m[nt].y));
+                if (!MASKED || v.x != -INFINITY) most = fmaxf(most, d.x);
+                if (!MASKED || v.y != -INFINITY) most = fmaxf(most, d.y);
+            }
         }
-    if (__any_sync(0xffffffffu, move)) {
-        float top = fmaxf(vstep[0], vstep[1]);
+    if (__any_sync(0xffffffffu, most > kAttSlack || steps * r.c > 128.0f)) {
 #pragma unroll
-        for (int d = 4; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        for (int d = 4; d < 32; d *= 2) steps = fmaxf(steps, __shfl_xor_sync(0xffffffffu, steps, d));
         // all lanes of the warp hold the same bound: 128 over the power of two above it
         float scale_o = 1.0f;
-        if (top * r.c > 128.0f) {
-            const int e = min(static_cast<int>(__float_as_uint(top) >> 23) - 126, 127);
+        if (steps * r.c > 128.0f) {
+            const int e = min(static_cast<int>(__float_as_uint(steps) >> 23) - 126, 127);
             const float c = exp2_int(7 - e);
             scale_o = c / r.c;
             r.c = c;
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            float f[2];
+            float2 best = both(kAttNone);
 #pragma unroll
-            for (int row = 0; row < 2; ++row) {
-                // (scores anew: beside the first reference their distance to it has no places left)
-                float best = kAttNone;
-                if (s[nt][row] != -INFINITY) best = fmaxf(best, s[nt][row] * r.a[nt][row]);
-                if (s[nt][2 + row] != -INFINITY) best = fmaxf(best, s[nt][2 + row] * r.a[nt][row]);
+            for (int h = 0; h < H; ++h)
 #pragma unroll
-                for (int d = 4; d < 32; d *= 2) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, d));
-                const float m = fmaxf(r.m[nt][row], best);
-                f[row] = ex2_approx(r.m[nt][row] - m);
-                r.m[nt][row] = m;
-                r.l[nt][row] *= f[row];
-                r.lo[nt][row] *= f[row];
-                s2[nt][row] = s[nt][row] == -INFINITY ? -INFINITY : __fmaf_rn(s[nt][row], r.a[nt][row], -m);
-                s2[nt][2 + row] = s[nt][2 + row] == -INFINITY ? -INFINITY : __fmaf_rn(s[nt][2 + row], r.a[nt][row], -m);
+                for (int i = 0; i < 2; ++i) {
+                    if (x[h][nt][2 * i] != -INFINITY) best.x = fmaxf(best.x, x[h][nt][2 * i] * r.a[nt].x);
+                    if (x[h][nt][2 * i + 1] != -INFINITY) best.y = fmaxf(best.y, x[h][nt][2 * i + 1] * r.a[nt].y);
+                }
+#pragma unroll
+            for (int d = 4; d < 32; d *= 2) {
+                best.x = fmaxf(best.x, __shfl_xor_sync(0xffffffffu, best.x, d));
+                best.y = fmaxf(best.y, __shfl_xor_sync(0xffffffffu, best.y, d));
             }
+            const float2 m = make_float2(fmaxf(r.m[nt].x, best.x), fmaxf(r.m[nt].y, best.y));
+            const float2 f = make_float2(ex2_approx(r.m[nt].x - m.x), ex2_approx(r.m[nt].y - m.y));
+            r.m[nt] = m;
+            r.l[nt] = __fmul2_rn(r.l[nt], f);
+            r.lo[nt] = __fmul2_rn(r.lo[nt], f);
 #pragma unroll
             for (int mt = 0; mt < D / 16; ++mt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) r.o[mt][nt][i] *= f[i & 1] * scale_o;
+                for (int i = 0; i < 4; ++i) r.o[mt][nt][i] *= (i & 1 ? f.y : f.x) * scale_o;
         }
     }
-    uint32_t pb[NT][2];
-    const float vs[2] = {vstep[0] * r.c, vstep[1] * r.c};
+    uint32_t pb[NT][2 * H];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        float w[4];
+    for (int h = 0; h < H; ++h)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float e = ex2_approx(s2[nt][i]);
-            const int tok = i >> 1, row = i & 1;
-            if (MASKED && s2[nt][i] == -INFINITY) {   // step and least of a key that the row does not see may be NaN
-                w[i] = 0.0f;
-            } else {
-                r.l[nt][row] += e;
-                r.lo[nt][row] = __fmaf_rn(e, vleast[tok], r.lo[nt][row]);
-                w[i] = e * vs[tok];
+        for (int i = 0; i < 2; ++i) {
+            const float2 vs = both(vstep[h][i] * r.c), least = both(__uint_as_float(pv[h][i] & 0xFFFF0000u));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const float2 v = make_float2(x[h][nt][2 * i], x[h][nt][2 * i + 1]);
+                const float2 d = __ffma2_rn(v, r.a[nt], make_float2(-r.m[nt].x, -r.m[nt].y));
+                float2 e = make_float2(ex2_approx(d.x), ex2_approx(d.y)), w;
+                if constexpr (MASKED) {   // step and least of a key that the row does not see may be NaN, and so may a
+                    const bool x_in = v.x != -INFINITY, y_in = v.y != -INFINITY;
+                    e = make_float2(x_in ? e.x : 0.0f, y_in ? e.y : 0.0f);
+                    r.lo[nt] = make_float2(x_in ? __fmaf_rn(e.x, least.x, r.lo[nt].x) : r.lo[nt].x, y_in ? __fmaf_rn(e.y, least.y, r.lo[nt].y) : r.lo[nt].y);
+                    w = make_float2(x_in ? e.x * vs.x : 0.0f, y_in ? e.y * vs.y : 0.0f);
+                } else {
+                    r.lo[nt] = __ffma2_rn(e, least, r.lo[nt]);
+                    w = __fmul2_rn(e, vs);
+                }
+                r.l[nt] = __fadd2_rn(r.l[nt], e);
+                pb[nt][2 * h + i] = movmatrix(pair_of<__half>(w.x, w.y));
             }
         }
-        pb[nt][0] = movmatrix(pair_of<__half>(w[0], w[1]));
-        pb[nt][1] = movmatrix(pair_of<__half>(w[2], w[3]));
-    }
     // values: the lane's D / 8 dimensions (8 to a word) of tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9 in the products' order
     const int p0 = (2 * t) ^ (t & 1), p1 = (2 * t + 1) ^ (t & 1);
-    uint32_t v0[D / 64], v1[D / 64], v2[D / 64], v3[D / 64];
-    const uint8_t* base = V + tk * (D / 2) + g * (D / 16);
-    load_words(v0, base + p0 * (D / 2));
-    load_words(v1, base + p1 * (D / 2));
-    load_words(v2, base + (p0 + 8) * (D / 2));
-    load_words(v3, base + (p1 + 8) * (D / 2));
 #pragma unroll
-    for (int w = 0; w < D / 64; ++w)
+    for (int h = 0; h < H; ++h) {
+        uint32_t v0[D / 64], v1[D / 64], v2[D / 64], v3[D / 64];
+        const uint8_t* base = V + (tk + 16 * h) * (D / 2) + g * (D / 16);
+        load_words(v0, base + p0 * (D / 2));
+        load_words(v1, base + p1 * (D / 2));
+        load_words(v2, base + (p0 + 8) * (D / 2));
+        load_words(v3, base + (p1 + 8) * (D / 2));
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const uint32_t x = __byte_perm(v0[w], v1[w], half ? 0x7632 : 0x5410), y = __byte_perm(v2[w], v3[w], half ? 0x7632 : 0x5410);
+        for (int w = 0; w < D / 64; ++w)
 #pragma unroll
-            for (int z = 0; z < 2; ++z) {
-                const uint32_t xs = z ? x >> 8 : x, ys = z ? y >> 8 : y;
+            for (int half = 0; half < 2; ++half) {
+                const uint32_t u = __byte_perm(v0[w], v1[w], half ? 0x7632 : 0x5410), v = __byte_perm(v2[w], v3[w], half ? 0x7632 : 0x5410);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-                    mma_16816(r.o[4 * w + 2 * half + z][nt], xs & kLow, xs & kHigh, ys & kLow, ys & kHigh, pb[nt][0], pb[nt][1]);
+                for (int z = 0; z < 2; ++z) {
+                    const uint32_t us = z ? u >> 8 : u, vs = z ? v >> 8 : v;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+                        mma_16816(r.o[4 * w + 2 * half + z][nt], us & kLow, us & kHigh, vs & kLow, vs & kHigh, pb[nt][2 * h], pb[nt][2 * h + 1]);
+                }
             }
-        }
+    }
 }
 
 // Where a unit lies.
 struct AttItem {
-    int b, head;
-    long long token0, len, base;   // base: its first unit
-    int n, rows, row0, tiles;      // tiles: those that some row sees, one at least
-    int seen;                      // positions that some row sees
+    int b, head, n, rows, row0;
+    int base, next;      // its first unit, and the one after its last
+    int tiles;           // those that some row sees, one at least
+    int seen;            // positions that some row sees
+    int index;           // among all row tiles, with one new token per sequence
+    long long token0, len;
 };
 
 template <int R>
-__device__ __forceinline__ AttItem att_item(const AttParams& p, const long long* first, long long unit) {
+__device__ __forceinline__ AttItem att_item(const AttParams& p, const int* first, int unit) {
     AttItem it;
     int lo = 0, hi = p.c.seqs;   // the last sequence whose units start at or before this one, and has some
     while (lo + 1 < hi) {
@@ -358,11 +395,13 @@ __device__ __forceinline__ AttItem att_item(const AttParams& p, const long long*
     const long long cap = static_cast<long long>(p.c.width) << p.c.shift;
     const int seen = static_cast<int>(min(max(it.len, 0LL), cap));
     const int row_tiles = (it.rows + R - 1) / R;
-    const long long tiles = p.by_item ? 1 : max(1, (seen + kAttTile - 1) / kAttTile);
-    const long long rest = unit - first[lo];
-    it.head = static_cast<int>(rest / (row_tiles * tiles));
-    int tile = static_cast<int>((rest - it.head * (row_tiles * tiles)) / tiles);
-    it.base = first[lo] + (it.head * static_cast<long long>(row_tiles) + tile) * tiles;
+    const int tiles = p.by_item ? 1 : kAttOver + max(1, (seen + kAttTile - 1) / kAttTile);
+    const int rest = static_cast<int>(static_cast<unsigned>(unit - first[lo]) / static_cast<unsigned>(tiles));   // head and row tile
+    it.head = row_tiles == 1 ? rest : rest / row_tiles;
+    int tile = rest - it.head * row_tiles;
+    it.base = first[lo] + rest * tiles;
+    it.next = it.base + tiles;
+    it.index = (lo * p.c.heads + it.head) * row_tiles + tile;
     if (p.by_item) tile = row_tiles - 1 - tile;   // the longest first
     it.row0 = tile * R;
     const int last = min(it.row0 + R, it.rows) - 1;
@@ -371,22 +410,37 @@ __device__ __forceinline__ AttItem att_item(const AttParams& p, const long long*
     return it;
 }
 
+// Tiles of an item among units beg .. end - 1.  An item's units are its overhead, then its tiles, then (of a tile of early rows)
+// those that none of its rows sees.
+__device__ __forceinline__ void att_tiles(const AttParams& p, const AttItem& it, int beg, int end, int& t0, int& t1) {
+    if (p.by_item) {
+        t0 = 0;
+        t1 = it.tiles;
+        return;
+    }
+    t0 = max(0, beg - it.base - kAttOver);
+    t1 = min(it.tiles, end - it.base - kAttOver);
+}
+
 template <int D, int NT, int RW>
 __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT, RW>::kPerSm) cache_attention_kernel(const AttParams p) {
     using Sh = AttShape<D, NT, RW>;
-    constexpr int R = Sh::R, TW = Sh::TW;
+    constexpr int R = Sh::R, TW = Sh::TW, H = Sh::H;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ __align__(8) uint64_t bars[2 * Sh::kStages];
+    __shared__ __align__(8) uint64_t bars[2 * Sh::kStages + 2];
     __shared__ uint32_t there[Sh::kStages];
     __shared__ int dead;   // a wait ran out: nothing more is loaded
     float* join = reinterpret_cast<float*>(smem + Sh::kStages * Sh::kStage);
-    float* stats = join + Sh::kJoin / 4;
-    long long* first = reinterpret_cast<long long*>(stats + Sh::kStats / 4);   // of each sequence, its first unit
+    uint8_t* queries = reinterpret_cast<uint8_t*>(join) + Sh::kJoin;
+    float* stats = reinterpret_cast<float*>(queries + Sh::kQueries);
+    int* first = reinterpret_cast<int*>(stats + Sh::kStats / 4);   // of each sequence, its first unit (the host keeps their number below 2^31)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t full = smem_u32(bars), empty = full + 8 * Sh::kStages, ring = smem_u32(smem);
+    const uint32_t full = smem_u32(bars), empty = full + 8 * Sh::kStages, q_full = empty + 8 * Sh::kStages, q_empty = q_full + 8, ring = smem_u32(smem);
     griddep_launch();
     if (threadIdx.x == 0) {
         for (int i = 0; i < Sh::kStages; ++i) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, kAttWarps);
+        mbar_init(q_full, 1);
+        mbar_init(q_empty, kAttWarps);
         fence_mbar_init();
         dead = 0;
     }
@@ -395,18 +449,18 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT, RW>::kPerSm) cach
     for (int b = threadIdx.x; b < p.c.seqs; b += kAttThreads) {
         long long beg, end;
         new_rows(p.c, b, beg, end);
-        const long long row_tiles = ((end - beg) * p.per + R - 1) / R;
-        const long long seen = min(max(static_cast<long long>(p.c.lengths[b]), 0LL), cap);
-        first[b + 1] = p.c.heads * row_tiles * (p.by_item ? 1 : max(1LL, (seen + kAttTile - 1) / kAttTile));
+        const int row_tiles = (static_cast<int>(end - beg) * p.per + R - 1) / R;
+        const int seen = static_cast<int>(min(max(static_cast<long long>(p.c.lengths[b]), 0LL), cap));
+        first[b + 1] = p.c.heads * row_tiles * (p.by_item ? 1 : kAttOver + max(1, (seen + kAttTile - 1) / kAttTile));
     }
     __syncthreads();
     if (warp == 0) {
-        long long sum = 0;
+        int sum = 0;
         for (int b0 = 0; b0 < p.c.seqs; b0 += 32) {
-            long long v = b0 + lane < p.c.seqs ? first[b0 + lane + 1] : 0;
+            int v = b0 + lane < p.c.seqs ? first[b0 + lane + 1] : 0;
 #pragma unroll
             for (int d = 1; d < 32; d *= 2) {
-                const long long o = __shfl_up_sync(0xffffffffu, v, d);
+                const int o = __shfl_up_sync(0xffffffffu, v, d);
                 if (lane >= d) v += o;
             }
             if (b0 + lane < p.c.seqs) first[b0 + lane + 1] = sum + v;
@@ -415,21 +469,40 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT, RW>::kPerSm) cach
         if (lane == 0) first[0] = 0;
     }
     __syncthreads();
-    const long long units = first[p.c.seqs], cta = blockIdx.x, ctas = min(static_cast<long long>(gridDim.x), units);   // a unit each at least
-    const long long beg = p.by_item ? min(cta, units) : cta < ctas ? cta * units / ctas : 0, end = p.by_item ? min(cta + 1, units) : cta < ctas ? (cta + 1) * units / ctas : 0;
-    const int shift = min(p.c.shift, 6);   // tokens of a piece: a page, or a tile
+    const int units = first[p.c.seqs], cta = blockIdx.x;
+    // equal shares, the first `more` CTAs one unit more; a unit each at least
+    const int ctas = min(static_cast<int>(gridDim.x), units), share = ctas ? units / ctas : 0, more = units - share * ctas;
+    const int beg = p.by_item ? min(cta, units) : cta < ctas ? cta * share + min(cta, more) : 0;
+    const int end = p.by_item ? min(cta + 1, units) : cta < ctas ? beg + share + (cta < more) : 0;
+    const int shift = min(p.c.shift, 7);   // tokens of a piece: a page, or a tile
     const int pieces = kAttTile >> shift;
 
-    int stage = 0, phase = 0;
+    int stage = 0, phase = 0, item = 0;   // item: how many this block has had
+    // Queries of all row tiles but the block's first, whose own loads begin as early.
+    const auto ahead = [&](int i) { return Sh::kAhead && p.vec_q && i > 0; };
     if (warp == kAttWarps) {   // ---- the producer
         const long long half = D / 2;
         const uint32_t codes = static_cast<uint32_t>(half) << shift, pairs = 4u << shift;
         long long issued = 0;   // tiles
-        for (long long u = beg; u < end;) {
+        for (int u = beg; u < end;) {
             const AttItem it = att_item<R>(p, first, u);
-            const int t0 = static_cast<int>(u - it.base);
-            const long long left = it.base + (p.by_item ? 1 : max(1LL, (min(max(it.len, 0LL), cap) + kAttTile - 1) / kAttTile));   // the item's last unit + 1
-            const int t1 = p.by_item ? it.tiles : static_cast<int>(min(static_cast<long long>(it.tiles), end - it.base));
+            int t0, t1;
+            att_tiles(p, it, beg, end, t0, t1);
+            u = it.next;
+            if (t0 >= t1) continue;
+            if (ahead(item)) {
+                if (!mbar_wait_warp(q_empty, item & 1, p.wait_limit) && lane == 0) *p.err = ERR_WAIT_EMPTY, *static_cast<volatile int*>(&dead) = 1;
+                if (__any_sync(0xffffffffu, *static_cast<volatile int*>(&dead))) goto drain;
+                const int rows = min(R, it.rows - it.row0);
+                if (lane == 0) mbar_expect_tx(q_full, rows * D * 2);
+                __syncwarp();
+                for (int row = lane; row < rows; row += 32) {
+                    const int i = (it.row0 + row) / p.per, j = it.row0 + row - i * p.per;
+                    bulk_load(smem_u32(queries) + row * D * 2,
+                              static_cast<const char*>(p.q) + 2 * ((it.token0 + i) * p.q_token + static_cast<long long>(it.head * p.per + j) * p.q_head), D * 2, q_full);
+                }
+            }
+            ++item;
             const int per = 32 / pieces;   // tiles whose pages the lanes look up at once
             for (int tb = t0; tb < t1; tb += per) {
                 const int mine = tb + lane / pieces;
@@ -452,7 +525,7 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT, RW>::kPerSm) cach
                             mbar_arrive(full + 8 * stage);
                     }
                     __syncwarp();
-                    if (lane / pieces == i && page >= 0 && !(p.stall && cta == 0 && u == beg && tb == t0 && i == 0)) {
+                    if (lane / pieces == i && page >= 0 && !(p.stall && cta == 0 && issued == 0)) {
                         const int at = lane % pieces << shift;                         // in the tile
                         const long long in = pos & (p.c.page - 1);                    // in the page
                         const uint32_t dst = ring + stage * Sh::kStage, bar = full + 8 * stage;
@@ -466,9 +539,9 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT, RW>::kPerSm) cach
                     ++issued;
                 }
             }
-            u = left;
         }
     drain:   // no copy is in flight when the block ends
+        if (ahead(item - 1) && !mbar_wait_warp(q_full, item & 1, p.wait_limit) && lane == 0) *p.err = ERR_DRAIN;
         for (long long i = max(0LL, issued - Sh::kStages); i < issued; ++i)
             if (!mbar_wait_warp(full + 8 * static_cast<int>(i % Sh::kStages), static_cast<int>(i / Sh::kStages) & 1, p.wait_limit) && lane == 0) *p.err = ERR_DRAIN;
         return;
@@ -479,16 +552,26 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT, RW>::kPerSm) cach
     const int g = lane >> 2, t = lane & 3;
     AttRows<D, NT> r;
     bool lost = false;
-    if (!p.by_item && threadIdx.x == 0) p.desc[cta].last = -1;
-    for (long long u = beg; u < end;) {
+    if (!p.by_item && !p.listed && threadIdx.x == 0) p.desc[cta].last = -1;
+    for (int u = beg; u < end;) {
         const AttItem it = att_item<R>(p, first, u);
-        const int t0 = static_cast<int>(u - it.base);
-        const long long left = it.base + (p.by_item ? 1 : max(1LL, (min(max(it.len, 0LL), cap) + kAttTile - 1) / kAttTile));
-        const int t1 = p.by_item ? it.tiles : static_cast<int>(min(static_cast<long long>(it.tiles), end - it.base));
-        u = left;
-        if (t0 >= t1) continue;   // units that no row of the tile sees
+        int t0, t1;
+        att_tiles(p, it, beg, end, t0, t1);
+        u = it.next;
+        if (t0 >= t1) continue;
         const int row0 = it.row0 + rw * 8 * NT;
-        att_queries<D, NT>(p, r, it.token0, it.n, it.head, row0, it.rows, it.len);
+        const bool here = ahead(item);
+        if (here && !lost && !mbar_wait_warp(q_full, (item & 1) ^ 1, p.wait_limit)) {
+            lost = true;
+            if (lane == 0) *p.err = ERR_WAIT_FULL, *static_cast<volatile int*>(&dead) = 1;
+        }
+        att_queries<D, NT>(p, r, reinterpret_cast<uint4*>(join + warp * (Sh::kWarp / 4)), it.token0, it.n, it.head, row0, it.rows, it.len,
+                            here ? queries + rw * 8 * NT * D * 2 : nullptr);
+        ++item;
+        if (here) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_empty);
+        }
         int all = it.seen;   // positions that all of the warp's rows see
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) all = min(all, min(r.lim[nt][0], r.lim[nt][1]));
@@ -507,12 +590,12 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT, RW>::kPerSm) cach
             const bool whole = have == (1u << pieces) - 1;
             if (row0 < it.rows && !lost) {
 #pragma unroll 1
-                for (int tk = tw * 16; tk < kAttTile; tk += TW * 16) {
+                for (int tk = tw * 16 * H; tk < kAttTile; tk += TW * 16 * H) {
                     const int pos = tile * kAttTile + tk;
-                    if (whole && pos + 16 <= all)
-                        att_step<D, NT, false>(r, K, V, KS, VS, tk, pos, it.seen, have, shift);
+                    if (whole && pos + 16 * H <= all)
+                        att_step<D, NT, H, false>(r, K, V, KS, VS, tk, pos, it.seen, have, shift);
                     else if (pos < it.seen)
-                        att_step<D, NT, true>(r, K, V, KS, VS, tk, pos, it.seen, have, shift);
+                        att_step<D, NT, H, true>(r, K, V, KS, VS, tk, pos, it.seen, have, shift);
                 }
             }
             __syncwarp();
@@ -520,32 +603,33 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT, RW>::kPerSm) cach
             if (++stage == Sh::kStages) stage = 0, phase ^= 1;
         }
         // ---- the segment's end: the warps' numerators, references and sums meet in shared memory
-        named_bar_sync(1, 32 * kAttWarps);   // the buffer is free
+        __syncwarp();   // all lanes are done with the queries
         const float inv = 1.0f / r.c;        // a power of two: exact
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
+            float m[2] = {r.m[nt].x, r.m[nt].y}, l[2] = {r.l[nt].x, r.l[nt].y}, lo[2] = {r.lo[nt].x, r.lo[nt].y};
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int d = 4; d < 32; d *= 2) {
-                    r.l[nt][i] += __shfl_xor_sync(0xffffffffu, r.l[nt][i], d);
-                    r.lo[nt][i] += __shfl_xor_sync(0xffffffffu, r.lo[nt][i], d);
+                    l[i] += __shfl_xor_sync(0xffffffffu, l[i], d);
+                    lo[i] += __shfl_xor_sync(0xffffffffu, lo[i], d);
                 }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int row = (warp * NT + nt) * 8 + 2 * t + i;
-                if (g == 0) stats[2 * row] = r.m[nt][i], stats[2 * row + 1] = r.l[nt][i];
+                if (g == 0) stats[2 * row] = m[i], stats[2 * row + 1] = l[i];
                 float* to = join + row * Sh::kPitch + g * (D / 8);
 #pragma unroll
                 for (int mt = 0; mt < D / 16; mt += 2)
                     *reinterpret_cast<float4*>(to + 2 * mt) =
-                        make_float4(__fmaf_rn(r.o[mt][nt][i] * 0x1p24f, inv, r.lo[nt][i]), __fmaf_rn(r.o[mt][nt][2 + i] * 0x1p20f, inv, r.lo[nt][i]),
-                                    __fmaf_rn(r.o[mt + 1][nt][i] * 0x1p24f, inv, r.lo[nt][i]), __fmaf_rn(r.o[mt + 1][nt][2 + i] * 0x1p20f, inv, r.lo[nt][i]));
+                        make_float4(__fmaf_rn(r.o[mt][nt][i] * 0x1p24f, inv, lo[i]), __fmaf_rn(r.o[mt][nt][2 + i] * 0x1p20f, inv, lo[i]),
+                                    __fmaf_rn(r.o[mt + 1][nt][i] * 0x1p24f, inv, lo[i]), __fmaf_rn(r.o[mt + 1][nt][2 + i] * 0x1p20f, inv, lo[i]));
             }
         }
         named_bar_sync(1, 32 * kAttWarps);
         const bool cut = t0 > 0 || t1 < it.tiles;
-        const long long slot = 2 * cta + (it.base < beg || t0 > 0 ? 0 : it.base > beg ? 1 : 0);
+        const long long slot = 2LL * cta + (t0 == 0);   // an item begins in one CTA, and only one that began before ends in it
         const int rows = min(R, it.rows - it.row0);
         for (int i = threadIdx.x; i < rows * (D / 8); i += 32 * kAttWarps) {
             const int row = i / (D / 8), d = i % (D / 8) * 8;
@@ -582,54 +666,97 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT, RW>::kPerSm) cach
                 }
             }
         }
-        if (cut && t0 == 0 && threadIdx.x == 0) {   // the tile begins here: this CTA says what there is to join
-            const long long last = it.base + it.tiles - 1;   // its owner: the c with c U / N <= last < (c + 1) U / N
-            p.desc[cta] = {static_cast<int>(slot), static_cast<int>(((last + 1) * ctas - 1) / units), it.rows, it.head, it.token0, it.row0, 0};
+        named_bar_sync(1, 32 * kAttWarps);   // the buffer is free
+        if (t0 == 0 && threadIdx.x == 0 && (p.listed || cut)) {   // the tile begins here: this CTA says what there is to join
+            int last = -1;
+            if (cut) {   // the owner of its last unit
+                const int u1 = it.base + kAttOver + it.tiles - 1, big = more * (share + 1);
+                last = u1 < big ? u1 / (share + 1) : more + (u1 - big) / share;
+            }
+            p.desc[p.listed ? it.index : cta] = {cta, last, it.rows, it.head, it.row0, static_cast<int>(it.token0), {0, 0}};
         }
     }
 }
 
-// Joins what a row tile's CTAs left.  A block a row, eight warps on different parts of it.
-template <int D>
+// Joins what a row tile's CTAs left: W warps a row, 32 parts of it at a time, each warp those that are its own modulo W.
+constexpr int kAttJoinWide = 8;
+
+template <int D, int W>
 __global__ void __launch_bounds__(256) cache_attention_join_kernel(const AttParams p, int R) {
-    constexpr int V = D / 32;   // dimensions a lane
-    __shared__ float part[8][D], sums[8][2];
-    griddep_launch();
+    constexpr int V = D / 32, ROWS = 8 / W;   // dimensions a lane, rows a block
+    __shared__ float part[W > 1 ? W : 1][W > 1 ? D : 1], sums[W][2];
+    // Only now: a next call's blocks that came while this kernel's still waited took SMs' room unevenly, and a few of its blocks
+    // then ran after all others (32 sequences of up to 8192 tokens: 35 us a call instead of 27).
     griddep_wait();
+    griddep_launch();
     const AttDesc a = p.desc[blockIdx.x];
-    const int row = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (a.last < 0 || a.row0 + row >= a.rows) return;
-    const int n = a.last - static_cast<int>(blockIdx.x) + 1;
-    // part i: this CTA's, then the first one of each that follows
-    const auto slot = [&](int i) { return static_cast<long long>(i == 0 ? a.slot : 2 * (static_cast<int>(blockIdx.x) + i)); };
-    float m = kAttNone, l = 0.0f, y[V] = {};
-    for (int i = warp; i < n; i += 8) {
-        const long long at = slot(i) * R + row;
-        const float mi = p.stat[2 * at], li = p.stat[2 * at + 1];
-        const float up = fmaxf(m, mi), f = ex2_approx(m - up), fi = ex2_approx(mi - up);
-        m = up;
-        l = l * f + li * fi;
+    if (a.last < 0) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = a.last - a.first + 1;
+    for (int row = blockIdx.y * ROWS + warp / W; row < R && a.row0 + row < a.rows; row += gridDim.y * ROWS) {
+        // part i: the first CTA's second, then the first one of each that follows
+        const auto at = [&](int i) { return (2LL * (a.first + i) + (i == 0)) * R + row; };
+        float m = kAttNone, l = 0.0f, y[V] = {};
+        for (int i0 = warp % W; i0 < n; i0 += 32 * W) {
+            const int mine = i0 + lane * W;
+            const float2 stat = mine < n ? *reinterpret_cast<const float2*>(p.stat + 2 * at(mine)) : make_float2(kAttNone, 0.0f);
+            float top = fmaxf(m, stat.x);
 #pragma unroll
-        for (int z = 0; z < V; ++z) y[z] = y[z] * f + fi * p.part[at * D + z * 32 + lane];
+            for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            const float f = ex2_approx(m - top), w = mine < n ? ex2_approx(stat.x - top) : 0.0f;
+            m = top;
+            l = l * f + w * stat.y;   // the lane's share of the sum
+#pragma unroll
+            for (int z = 0; z < V; ++z) y[z] *= f;
+            const int count = min(32, (n - i0 + W - 1) / W);
+            constexpr int AT_ONCE = 4;
+            for (int j0 = 0; j0 < count; j0 += AT_ONCE) {   // some parts' loads at once; those past the end are the last one's, with weight 0
+                float v[AT_ONCE][V];
+#pragma unroll
+                for (int j = 0; j < AT_ONCE; ++j) {
+                    const float* from = p.part + at(i0 + min(j0 + j, count - 1) * W) * D + lane;
+#pragma unroll
+                    for (int z = 0; z < V; ++z) v[j][z] = from[32 * z];
+                }
+#pragma unroll
+                for (int j = 0; j < AT_ONCE; ++j) {
+                    const float wj = j0 + j < count ? __shfl_sync(0xffffffffu, w, j0 + j) : 0.0f;
+#pragma unroll
+                    for (int z = 0; z < V; ++z) y[z] = __fmaf_rn(wj, v[j][z], y[z]);
+                }
+            }
+        }
+#pragma unroll
+        for (int d = 16; d; d /= 2) l += __shfl_xor_sync(0xffffffffu, l, d);
+        if constexpr (W > 1) {
+            if (lane == 0) sums[warp][0] = m, sums[warp][1] = l;
+#pragma unroll
+            for (int z = 0; z < V; ++z) part[warp][z * 32 + lane] = y[z];
+            __syncthreads();
+            if (warp == 0) {
+                float top = kAttNone;
+#pragma unroll
+                for (int w = 0; w < W; ++w) top = fmaxf(top, sums[w][0]);
+                l = 0.0f;
+#pragma unroll
+                for (int z = 0; z < V; ++z) y[z] = 0.0f;
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    const float f = ex2_approx(sums[w][0] - top);
+                    l = __fmaf_rn(f, sums[w][1], l);
+#pragma unroll
+                    for (int z = 0; z < V; ++z) y[z] = __fmaf_rn(f, part[w][z * 32 + lane], y[z]);
+                }
+            }
+        }
+        if (W == 1 || warp == 0) {
+            const float div = l == 0.0f ? 0.0f : 1.0f / l;
+            const int full_row = a.row0 + row, q = full_row / p.per;
+            const long long to = static_cast<long long>(a.token0 + q) * p.o_token + static_cast<long long>(a.head * p.per + full_row - q * p.per) * p.o_head + lane;
+#pragma unroll
+            for (int z = 0; z < V; ++z) store_y(p.out, to + 32 * z, y[z] * div, p.type);
+        }
+        if constexpr (W > 1) __syncthreads();
     }
-#pragma unroll
-    for (int z = 0; z < V; ++z) part[warp][z * 32 + lane] = y[z];
-    if (lane == 0) sums[warp][0] = m, sums[warp][1] = l;
-    __syncthreads();
-    if (threadIdx.x >= D) return;
-    float top = kAttNone;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) top = fmaxf(top, sums[w][0]);
-    float s = 0.0f, v = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) {
-        const float f = ex2_approx(sums[w][0] - top);
-        s = __fmaf_rn(f, sums[w][1], s);
-        v = __fmaf_rn(f, part[w][threadIdx.x], v);
-    }
-    v = s == 0.0f ? 0.0f : v / s;
-    const int full_row = a.row0 + row, q = full_row / p.per;
-    store_y(p.out, (a.token0 + q) * p.o_token + static_cast<long long>(a.head * p.per + full_row - q * p.per) * p.o_head + threadIdx.x, v, p.type);
 }
 
 }  // namespace ptq8

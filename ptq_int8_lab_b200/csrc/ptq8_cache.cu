@@ -151,6 +151,12 @@ const AttVariant kAttVariants[] = {
     att_variant<256, 1, 1>(), att_variant<256, 1, 2>(), att_variant<256, 1, 4>(),
 };
 
+using AttJoin = void (*)(AttParams, int);
+constexpr int kAttJoinSmem = 60 * 1024;   // none of it is used (see cache_attributes)
+const AttJoin kAttJoins[3][2] = {{cache_attention_join_kernel<64, 1>, cache_attention_join_kernel<64, kAttJoinWide>},
+                                 {cache_attention_join_kernel<128, 1>, cache_attention_join_kernel<128, kAttJoinWide>},
+                                 {cache_attention_join_kernel<256, 1>, cache_attention_join_kernel<256, kAttJoinWide>}};
+
 // The smallest tile that takes a sequence's query rows of a key head on average, or the largest.
 const AttVariant& att_choose(const ptq8_cache_attention_args& a) {
     const long long rows = (a.tokens * (a.heads / a.cache.kv_heads) + a.cache.sequences - 1) / a.cache.sequences;
@@ -160,10 +166,18 @@ const AttVariant& att_choose(const ptq8_cache_attention_args& a) {
     return *best;
 }
 
-// Many row tiles keep the SMs busy one CTA each; fewer are cut into equal shares.
-bool att_by_item(const ptq8_ops* o, const ptq8_cache_attention_args& a, const AttVariant& v) {
-    const long long rows = a.tokens * (a.heads / a.cache.kv_heads);
-    return a.cache.starts && rows / v.rows * a.cache.kv_heads >= 8LL * o->sms * v.per_sm;
+// Row tiles at most: each sequence's last may be partly filled.
+long long att_items(const ptq8_cache_attention_args& a, const AttVariant& v) {
+    const long long per = a.heads / a.cache.kv_heads, n = std::min<long long>(a.cache.sequences, a.tokens);
+    const long long tiles = a.cache.starts ? a.tokens * per / v.rows + n : n * ((per + v.rows - 1) / v.rows);
+    return tiles * a.cache.kv_heads;
+}
+
+// Many row tiles keep the SMs busy one CTA each; fewer are cut into equal shares.  (So are more units than an int counts.)
+bool att_by_item(const ptq8_ops* o, const ptq8_cache_attention_args& a, const AttVariant& v, int table_width) {
+    const long long most = static_cast<long long>(table_width) * a.cache.page / kAttTile + 1 + kAttOver, items = att_items(a, v);
+    if (items > 0x7FFFFFFFLL / most) return true;
+    return a.cache.starts && a.tokens * (a.heads / a.cache.kv_heads) / v.rows * a.cache.kv_heads >= 8LL * o->sms * v.per_sm;
 }
 
 int check_attention(ptq8_ops* o, const ptq8_cache_attention_args& a) {
@@ -182,7 +196,7 @@ int check_attention(ptq8_ops* o, const ptq8_cache_attention_args& a) {
 long long workspace_of(const ptq8_ops* o, const ptq8_cache_attention_args& a) {
     if (a.tokens == 0 || a.cache.sequences == 0) return 0;
     const AttVariant& v = att_choose(a);
-    if (att_by_item(o, a, v)) return 0;
+    if (att_by_item(o, a, v, 0)) return 0;   // (whatever the table's width)
     const long long n = static_cast<long long>(o->sms) * v.per_sm;
     return 2 * n * v.rows * (v.dim + 2) * 4 + n * static_cast<long long>(sizeof(AttDesc));
 }
@@ -196,26 +210,29 @@ int attention_call(ptq8_ops* o, const ptq8_cache_attention_args& a, cudaStream_t
     p.q_token = a.q_token, p.q_head = a.q_head, p.o_token = a.out_token, p.o_head = a.out_head;
     p.scale_log2 = a.scale * 1.4426950408889634f;
     p.per = a.heads / a.cache.kv_heads;
-    p.by_item = att_by_item(o, a, v);
+    p.by_item = att_by_item(o, a, v, a.cache.table_width);
     p.type = a.type;
     p.vec_q = vectors(a.q, a.q_token, a.q_head, a.type);
     p.vec_o = vectors(a.out, a.out_token, a.out_head, a.type);
     p.wait_limit = o->wait_limit;
     p.err = o->error_dev;
     p.stall = o->stall;
-    const long long rows = a.tokens * p.per;
+    const long long items = att_items(a, v);
     long long n = static_cast<long long>(o->sms) * v.per_sm;
-    if (p.by_item) {   // row tiles at most: each sequence's last may be partly filled
-        n = (rows / v.rows + std::min<long long>(a.cache.sequences, a.tokens)) * a.cache.kv_heads;
+    if (p.by_item) {
+        n = items;
     } else {
         p.part = static_cast<float*>(a.workspace);
         p.stat = p.part + 2 * n * v.rows * v.dim;
         p.desc = reinterpret_cast<AttDesc*>(p.stat + 2 * n * v.rows * 2);
+        p.listed = !a.cache.starts && items <= n;
     }
     cudaError_t e = launch(v.kernel, dim3(static_cast<unsigned>(n)), dim3(kAttThreads), v.smem_of(a.cache.sequences), 1, st, p);
     if (e == cudaSuccess && !p.by_item) {
-        const auto join = v.dim == 64 ? cache_attention_join_kernel<64> : v.dim == 128 ? cache_attention_join_kernel<128> : cache_attention_join_kernel<256>;
-        e = launch(join, dim3(static_cast<unsigned>(n), v.rows), dim3(256), 0, 1, st, p, v.rows);
+        // few row tiles have many parts each: eight warps a row; else a warp a row
+        const bool wide = p.listed && 4 * items <= n;
+        const int rows = p.listed ? std::min(v.rows, p.per) : v.rows;
+        e = launch(kAttJoins[v.dim == 64 ? 0 : v.dim == 128 ? 1 : 2][wide], dim3(static_cast<unsigned>(p.listed ? items : n), wide ? rows : (rows + 7) / 8), dim3(256), kAttJoinSmem, 1, st, p, v.rows);
     }
     return e == cudaSuccess ? PTQ8_OK : cuda_fail(o, "cache_attention", e);
 }
@@ -224,11 +241,28 @@ int attention_call(ptq8_ops* o, const ptq8_cache_attention_args& a, cudaStream_t
 
 namespace ptq8 {
 
+static cudaError_t most_shared(const void* kernel) {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+}
+
 cudaError_t cache_attributes() {
     for (const AttVariant& v : kAttVariants) {
         const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(v.kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, v.smem);
         if (e != cudaSuccess) return e;
     }
+    // An SM divides its memory anew between L1 and shared memory only when it is empty.  The kernels that run beside attention's
+    // under programmatic launch therefore ask for its division (one token over 2000 positions: 8.3 us a call instead of 8.8).
+    for (const auto& pair : kAttJoins)
+        for (const AttJoin join : pair)
+        {
+            if (const cudaError_t e = most_shared(reinterpret_cast<const void*>(join)); e != cudaSuccess) return e;
+            if (const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(join), cudaFuncAttributeMaxDynamicSharedMemorySize, kAttJoinSmem); e != cudaSuccess) return e;
+        }
+    for (const int dim : {64, 128, 256})
+        for (const bool write : {false, true})
+            for (const bool vec : {false, true})
+                for (const CacheKernel k : {rows_kernel_of<float>(dim, write, vec), rows_kernel_of<__half>(dim, write, vec), rows_kernel_of<__nv_bfloat16>(dim, write, vec)})
+                    if (const cudaError_t e = most_shared(reinterpret_cast<const void*>(k)); e != cudaSuccess) return e;
     return cudaSuccess;
 }
 

@@ -176,8 +176,8 @@ template <typename T, int D, bool VEC>
 __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(const CacheRowsParams p) {
     extern __shared__ int starts[];
     constexpr int LANES = D / 8;
-    griddep_launch();
     griddep_wait();
+    griddep_launch();
     if (p.c.starts) {
         for (int i = threadIdx.x; i <= p.c.seqs; i += kCacheThreads) starts[i] = p.c.starts[i];
         __syncthreads();
@@ -231,8 +231,8 @@ template <typename T, int D, bool VEC>
 __global__ void __launch_bounds__(kCacheThreads) cache_read_kernel(const CacheRowsParams p) {
     extern __shared__ int starts[];
     constexpr int LANES = D / 8;
-    griddep_launch();
     griddep_wait();
+    griddep_launch();
     if (p.c.starts) {
         for (int i = threadIdx.x; i <= p.c.seqs; i += kCacheThreads) starts[i] = p.c.starts[i];
         __syncthreads();

@@ -99,7 +99,7 @@ def _check_part(name: str, t: torch.Tensor, dtype, shape, device: int):
 def _check_rows(name: str, t: torch.Tensor, dtypes, shape, device: int):
     if t.dtype not in dtypes:
         raise Ptq8Error(f"{name}: dtype {t.dtype}")
-    if tuple(t.shape) != shape:
+    if t.dim() != 3 or tuple(t.shape) != shape:
         raise Ptq8Error(f"{name}: shape {tuple(t.shape)}, {shape} is wanted")
     if t.get_device() != device:
         raise Ptq8Error(f"{name}: on {t.device}, not on cuda:{device}")
@@ -167,6 +167,9 @@ class Int8Ops:
         self._w4_args = ctypes.create_string_buffer(_W4.size)
         self._cache_args = ctypes.create_string_buffer(_CACHE_ROWS.size)
         self._attention_args = ctypes.create_string_buffer(_ATTENTION.size)
+        self._linear_w4, self._cache_write, self._cache_read = self._lib.ptq8_linear_w4, self._lib.ptq8_cache_write, self._lib.ptq8_cache_read
+        self._cache_attention = self._lib.ptq8_cache_attention
+        self._workspaces = {}   # bytes, by the sizes of a call
 
     def _check(self, rc: int):
         if rc:
@@ -323,14 +326,24 @@ class Int8Ops:
             raise Ptq8Error(f"act {act}: EPI_NONE or EPI_SWIGLU")
         if not 0 < group <= 0x7FFFFFFF:
             raise Ptq8Error(f"group {group}")
-        for name, t, dtypes in (("x", x, _TYPES), ("w", w, _CODES[4]), ("w_scale", w_scale, _TYPES)):
-            if t.dim() != 2 or t.dtype not in dtypes or t.get_device() != d or t.stride(1) != 1:
-                _check_matrix(name, t, dtypes, 2, d)
+        x_type, s_type = _TYPES.get(x.dtype), _TYPES.get(w_scale.dtype)
+        if x_type is None or x.dim() != 2 or x.get_device() != d:
+            _check_matrix("x", x, _TYPES, 2, d)
+        if w.dtype not in _CODES[4] or w.dim() != 2 or w.get_device() != d:
+            _check_matrix("w", w, _CODES[4], 2, d)
+        if s_type is None or w_scale.dim() != 2 or w_scale.get_device() != d:
+            _check_matrix("w_scale", w_scale, _TYPES, 2, d)
         rows, k = x.shape
         channels, wide = w.shape
+        ldx, x_step = x.stride()
+        ldw, w_step = w.stride()
+        lds, s_step = w_scale.stride()
+        if x_step != 1 or w_step != 1 or s_step != 1:
+            for name, t, dtypes in (("x", x, _TYPES), ("w", w, _CODES[4]), ("w_scale", w_scale, _TYPES)):
+                _check_matrix(name, t, dtypes, 2, d)
         if wide != (k + 1) // 2:
             raise Ptq8Error(f"w: rows of {wide} bytes for {k} input features at 4 bits")
-        if w_scale.shape[0] != channels or w_scale.shape[1] != -(-k // group):
+        if w_scale.shape != (channels, -(-k // group)):
             raise Ptq8Error(f"w_scale: shape {tuple(w_scale.shape)}, {(channels, -(-k // group))} is wanted")
         b = 0
         if bias is not None:
@@ -348,40 +361,44 @@ class Int8Ops:
             if dtype not in _TYPES:
                 raise Ptq8Error(f"dtype {dtype}: f32, f16 or bf16")
             out = torch.empty((rows, n), dtype=dtype, device=x.device)
-        elif out.dim() != 2 or out.dtype not in _TYPES or out.get_device() != d or out.stride(1) != 1:
+        elif out.dim() != 2:
             _check_matrix("out", out, _TYPES, 2, d)
-        if out.shape[0] != rows or out.shape[1] != n:
+        y_type = _TYPES.get(out.dtype)
+        ldy, step = out.stride()
+        if y_type is None or step != 1 or out.get_device() != d:
+            _check_matrix("out", out, _TYPES, 2, d)
+        if out.shape != (rows, n):
             raise Ptq8Error(f"out: shape {tuple(out.shape)}, {(rows, n)} is wanted")
-        _W4.pack_into(self._w4_args, 0, x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), w_scale.data_ptr(), w_scale.stride(0), b,
-                      out.data_ptr(), out.stride(0), rows, k, n, group, act, _TYPES[x.dtype], _TYPES[w_scale.dtype], _TYPES[out.dtype], 0)
-        rc = self._lib.ptq8_linear_w4(self._h, self._w4_args, stream)
+        _W4.pack_into(self._w4_args, 0, x.data_ptr(), ldx, w.data_ptr(), ldw, w_scale.data_ptr(), lds, b, out.data_ptr(), ldy, rows, k, n,
+                      group, act, x_type, s_type, y_type, 0)
+        rc = self._linear_w4(self._h, self._w4_args, stream)
         if rc:
             self._check(rc)
         return out
 
     def _cache(self, cache, table, lengths, starts, tokens):
-        """The fields of ptq8_cache.  tokens: the new tokens, or None where starts is None (one per sequence)."""
+        """The fields of ptq8_cache.  tokens: the new tokens."""
         k, ks, v, vs = cache
         d = self.device
-        if k.dim() != 4:
-            raise Ptq8Error(f"cache.k: shape {tuple(k.shape)}, [pages, kv_heads, page, head_dim // 2] is wanted")
-        shape = tuple(k.shape)
-        pairs = (*shape[:3], 2)
-        # one look at what calls have in common; where it fails, _check_part says what is wrong
-        if (k.dtype is not _U8 or v.dtype is not _U8 or ks.dtype is not _BF16 or vs.dtype is not _BF16 or v.shape != k.shape
-                or tuple(ks.shape) != pairs or vs.shape != ks.shape):
-            for name, t, dtype, want in (("k", k, _U8, shape), ("v", v, _U8, shape), ("k_scale", ks, _BF16, pairs), ("v_scale", vs, _BF16, pairs)):
+        shape = k.shape
+        if len(shape) != 4:
+            raise Ptq8Error(f"cache.k: shape {tuple(shape)}, [pages, kv_heads, page, head_dim // 2] is wanted")
+        pages, heads, page, half = shape
+        pairs = (pages, heads, page, 2)
+        k_at, v_at, ks_at, vs_at = k.stride(), v.stride(), ks.stride(), vs.stride()
+        # one look at all that is wanted of the four; where it fails, _check_part says what is wrong
+        if not (k.dtype is _U8 and v.dtype is _U8 and ks.dtype is _BF16 and vs.dtype is _BF16 and v.shape == shape and ks.shape == pairs
+                and vs.shape == pairs and k_at[2:] == (half, 1) and v_at[2:] == (half, 1) and ks_at[2:] == (2, 1) and vs_at[2:] == (2, 1)
+                and k.get_device() == d and v.get_device() == d and ks.get_device() == d and vs.get_device() == d):
+            for name, t, dtype, want in (("k", k, _U8, tuple(shape)), ("v", v, _U8, tuple(shape)), ("k_scale", ks, _BF16, pairs), ("v_scale", vs, _BF16, pairs)):
                 _check_part(name, t, dtype, want, d)
-        (kp, kh, kr, k1), (vp, vh, vr, v1) = k.stride(), v.stride()
-        (ksp, ksh, ksr, ks1), (vsp, vsh, vsr, vs1) = ks.stride(), vs.stride()
-        half = shape[3]
-        if (k1 != 1 or v1 != 1 or ks1 != 1 or vs1 != 1 or kr != half or vr != half or ksr != 2 or vsr != 2 or k.get_device() != d
-                or v.get_device() != d or ks.get_device() != d or vs.get_device() != d):
-            for name, t, dtype, want in (("k", k, _U8, shape), ("v", v, _U8, shape), ("k_scale", ks, _BF16, pairs), ("v_scale", vs, _BF16, pairs)):
-                _check_part(name, t, dtype, want, d)
-        if table.dim() != 2 or table.dtype is not _I32 or table.get_device() != d or (table.stride(1) != 1 and table.shape[1] > 1):
+        shape = table.shape
+        if len(shape) != 2:
             _check_matrix("table", table, (_I32,), 2, d)
-        seqs, wide = table.shape
+        seqs, wide = shape
+        pitch, step = table.stride()
+        if table.dtype is not _I32 or step != 1 or table.get_device() != d:
+            _check_matrix("table", table, (_I32,), 2, d)
         if lengths.dtype is not _I32 or lengths.numel() != seqs or not lengths.is_contiguous() or lengths.get_device() != d:
             _check_vector("lengths", lengths, _I32, seqs, d)
         at = 0
@@ -391,22 +408,28 @@ class Int8Ops:
             at = starts.data_ptr()
         elif tokens != seqs:
             raise Ptq8Error(f"{tokens} tokens without starts, but {seqs} sequences")
-        return (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), kp, kh, vp, vh, 2 * ksp, 2 * ksh, 2 * vsp, 2 * vsh,
-                table.data_ptr(), table.stride(0), lengths.data_ptr(), at, shape[0], wide, shape[2], shape[1], 2 * half, seqs, 0)
+        return (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), k_at[0], k_at[1], v_at[0], v_at[1], 2 * ks_at[0], 2 * ks_at[1],
+                2 * vs_at[0], 2 * vs_at[1], table.data_ptr(), pitch, lengths.data_ptr(), at, pages, wide, page, heads, 2 * half, seqs, 0)
 
     def _cache_rows(self, call, cache, k, v, table, lengths, starts, stream):
-        if k.dim() != 3:
-            raise Ptq8Error(f"k: shape {tuple(k.shape)}, [tokens, kv_heads, head_dim] is wanted")
-        fields = self._cache(cache, table, lengths, starts, k.shape[0])
-        dtype = _TYPES.get(k.dtype)
-        want = (k.shape[0], fields[19], fields[20])
-        if dtype is None or tuple(k.shape) != want or k.get_device() != self.device or k.stride(2) != 1:
-            _check_rows("k", k, _TYPES, want, self.device)
-        if v.dtype is not k.dtype or tuple(v.shape) != want or v.get_device() != self.device or v.stride(2) != 1:
-            _check_rows("v", v, (k.dtype,), want, self.device)
-        _CACHE_ROWS.pack_into(self._cache_args, 0, *fields, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-                              want[0], dtype, 0)
-        rc = call(self._h, self._cache_args, self._stream(stream, True))
+        shape = k.shape
+        if len(shape) != 3:
+            raise Ptq8Error(f"k: shape {tuple(shape)}, [tokens, kv_heads, head_dim] is wanted")
+        tokens = shape[0]
+        fields = self._cache(cache, table, lengths, starts, tokens)
+        d, dtype = self.device, k.dtype
+        kind, want = _TYPES.get(dtype), (tokens, fields[19], fields[20])
+        if kind is None or shape != want or k.get_device() != d:
+            _check_rows("k", k, _TYPES, want, d)
+        if v.dtype is not dtype or v.shape != want or v.get_device() != d:
+            _check_rows("v", v, (dtype,), want, d)
+        k_token, k_head, k_step = k.stride()
+        v_token, v_head, v_step = v.stride()
+        if k_step != 1 or v_step != 1:
+            _check_rows("k", k, (dtype,), want, d)
+            _check_rows("v", v, (dtype,), want, d)
+        _CACHE_ROWS.pack_into(self._cache_args, 0, *fields, k.data_ptr(), v.data_ptr(), k_token, k_head, v_token, v_head, tokens, kind, 0)
+        rc = call(self._h, self._cache_args, stream)
         if rc:
             self._check(rc)
 
@@ -417,7 +440,7 @@ class Int8Ops:
         table int32 [sequences, n]: the pages of each sequence; lengths int32 [sequences]: its positions, the new tokens (its
         last ones) among them; starts int32 [sequences + 1]: sequence b's new tokens are starts[b] .. starts[b + 1] - 1, without
         it token b alone.  Positions without a page are skipped.  A page that is written belongs to one sequence."""
-        self._cache_rows(self._lib.ptq8_cache_write, cache, k, v, table, lengths, starts, stream)
+        self._cache_rows(self._cache_write, cache, k, v, table, lengths, starts, self._stream(stream, True))
 
     def cache_read(self, cache: Cache4, table: torch.Tensor, lengths: torch.Tensor, starts: Optional[torch.Tensor] = None,
                    tokens: Optional[int] = None, dtype: torch.dtype = torch.bfloat16, out=None, stream=None) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -435,7 +458,7 @@ class Int8Ops:
             shape = (tokens, cache[0].shape[1], 2 * cache[0].shape[3])
             out = tuple(torch.empty(shape, dtype=dtype, device=f"cuda:{self.device}") for _ in range(2))
         k, v = out
-        self._cache_rows(self._lib.ptq8_cache_read, cache, k, v, table, lengths, starts, stream)
+        self._cache_rows(self._cache_read, cache, k, v, table, lengths, starts, stream)
         return k, v
 
     def cache_attention(self, q: torch.Tensor, cache: Cache4, table: torch.Tensor, lengths: torch.Tensor,
@@ -447,47 +470,66 @@ class Int8Ops:
         nothing gets zeros; tokens of no sequence are not written.
 
         workspace: uint8, cache_attention_workspace() bytes; one is made where it is not given, which with stream it has to be."""
-        stream = self._stream(stream, out is not None and workspace is not None)
+        if stream is not None and (out is None or workspace is None):
+            raise Ptq8Error("with stream, out and workspace are wanted too: tensors made here would belong to the current stream")
+        stream = self._stream(stream, True)
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        args, need = self._attention(q, cache, table, lengths, starts, scale, out)
+        need = self._attention(q, cache, table, lengths, starts, scale, out)
         if workspace is None:
+            at, size = 0, 0
             if need:
                 workspace = torch.empty(need, dtype=_U8, device=q.device)
-        elif workspace.dtype is not _U8 or not workspace.is_contiguous() or workspace.get_device() != self.device:
-            raise Ptq8Error(f"workspace: {workspace.dtype} on {workspace.device}, consecutive uint8 on cuda:{self.device} is wanted")
-        at, size = (workspace.data_ptr(), workspace.numel()) if workspace is not None else (0, 0)
+                at, size = workspace.data_ptr(), need
+        else:
+            if workspace.dtype is not _U8 or not workspace.is_contiguous() or workspace.get_device() != self.device:
+                raise Ptq8Error(f"workspace: {workspace.dtype} on {workspace.device}, consecutive uint8 on cuda:{self.device} is wanted")
+            at, size = workspace.data_ptr(), workspace.numel()
+        args = self._attention_args
         _WORKSPACE.pack_into(args, _WORKSPACE_AT, at, size)
-        rc = self._lib.ptq8_cache_attention(self._h, args, stream)
+        rc = self._cache_attention(self._h, args, stream)
         if rc:
             self._check(rc)
         return out
 
-    def _attention(self, q, cache, table, lengths, starts, scale, out):
-        if q.dim() != 3:
-            raise Ptq8Error(f"q: shape {tuple(q.shape)}, [tokens, heads, head_dim] is wanted")
+    def _attention(self, q, cache, table, lengths, starts, scale, out) -> int:
+        """Fills the argument struct, all but its workspace; the bytes that that needs."""
+        shape = q.shape
+        if len(shape) != 3:
+            raise Ptq8Error(f"q: shape {tuple(shape)}, [tokens, heads, head_dim] is wanted")
         d = self.device
-        tokens, heads, dim = q.shape
+        tokens, heads, dim = shape
         fields = self._cache(cache, table, lengths, starts, tokens)
-        kind = _TYPES.get(q.dtype)
-        if not kind or dim != fields[20] or q.get_device() != d or q.stride(2) != 1:
+        dtype = q.dtype
+        kind = _TYPES.get(dtype)
+        if not kind or dim != fields[20] or q.get_device() != d:
             _check_rows("q", q, (torch.float16, _BF16), (tokens, heads, fields[20]), d)
-        if out.dtype is not q.dtype or out.shape != q.shape or out.get_device() != d or out.stride(2) != 1:
-            if out.dim() != 3:
-                raise Ptq8Error(f"out: shape {tuple(out.shape)}, {tuple(q.shape)} is wanted")
-            _check_rows("out", out, (q.dtype,), tuple(q.shape), d)
+        if out.dtype is not dtype or out.shape != shape or out.get_device() != d:
+            _check_rows("out", out, (dtype,), tuple(shape), d)
+        q_token, q_head, q_step = q.stride()
+        o_token, o_head, o_step = out.stride()
+        if q_step != 1 or o_step != 1:
+            _check_rows("q", q, (dtype,), tuple(shape), d)
+            _check_rows("out", out, (dtype,), tuple(shape), d)
         args = self._attention_args
-        _ATTENTION.pack_into(args, 0, *fields, q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1), tokens,
-                             0, 0, dim ** -0.5 if scale is None else scale, heads, kind, 0)
-        need = self._lib.ptq8_cache_attention_workspace(self._h, args)
-        if need < 0:
-            self._check(1)
-        return args, need
+        _ATTENTION.pack_into(args, 0, *fields, q.data_ptr(), out.data_ptr(), q_token, q_head, o_token, o_head, tokens, 0, 0,
+                             dim ** -0.5 if scale is None else scale, heads, kind, 0)
+        # a function of these numbers alone, asked for once
+        key = (tokens, heads, fields[19], dim, fields[21], starts is None)
+        need = self._workspaces.get(key)
+        if need is None:
+            need = self._lib.ptq8_cache_attention_workspace(self._h, args)
+            if need < 0:
+                self._check(1)
+            if len(self._workspaces) >= 4096:
+                self._workspaces.clear()
+            self._workspaces[key] = need
+        return need
 
     def cache_attention_workspace(self, q: torch.Tensor, cache: Cache4, table: torch.Tensor, lengths: torch.Tensor,
                                   starts: Optional[torch.Tensor] = None) -> int:
         """Bytes of workspace that cache_attention() needs for tensors of these shapes.  A workspace serves one call at a time."""
-        return self._attention(q, cache, table, lengths, starts, None, q)[1]
+        return self._attention(q, cache, table, lengths, starts, None, q)
 
     def check_device_error(self, stream=None):
         """Wait for the stream; raise Ptq8Error (status PTQ8_ERR_TIMEOUT) if a bounded device wait ran out."""
