@@ -38,17 +38,23 @@ int check_w4(ptq8_ops* o, const ptq8_linear_w4_args& a) {
     return PTQ8_OK;
 }
 
-using W4Kernel = void (*)(W4Params);
+struct W4Variant {
+    int type, vb, nt;   // of the activations; bytes that a lane takes at once; tiles of eight columns
+    void (*kernel)(W4Params, W4Plan, const CUtensorMap);
+    int sums, beside;
+    int (*frag)(int columns);
+};
 
-template <typename XT, int VB>
-W4Kernel w4_kernel(int rt, int nt) {
-    if (nt == 1) return rt == 1 ? linear_w4_kernel<XT, VB, 1, 1> : rt == 2 ? linear_w4_kernel<XT, VB, 2, 1> : linear_w4_kernel<XT, VB, 4, 1>;
-    return nt == 2 ? linear_w4_kernel<XT, VB, 2, 2> : linear_w4_kernel<XT, VB, 2, 4>;
+template <typename XT, int TYPE, int VB, int NT>
+W4Variant w4_variant() {
+    using Sh = W4Shape<XT, VB, NT>;
+    return {TYPE, VB, NT, linear_w4_kernel<XT, VB, NT>, Sh::kSums, Sh::kBeside, Sh::frag};
 }
-template <typename XT>
-W4Kernel w4_kernel(int vb, int rt, int nt) {
-    return vb == 16 ? w4_kernel<XT, 16>(rt, nt) : vb == 8 ? w4_kernel<XT, 8>(rt, nt) : w4_kernel<XT, 4>(rt, nt);
-}
+
+#define W4_TILES(XT, TYPE, VB) w4_variant<XT, TYPE, VB, 1>(), w4_variant<XT, TYPE, VB, 2>(), w4_variant<XT, TYPE, VB, 4>()
+#define W4_TYPE(XT, TYPE) W4_TILES(XT, TYPE, 4), W4_TILES(XT, TYPE, 8), W4_TILES(XT, TYPE, 16)
+
+const W4Variant kW4Variants[] = {W4_TYPE(float, PTQ8_F32), W4_TYPE(__half, PTQ8_F16), W4_TYPE(__nv_bfloat16, PTQ8_BF16)};
 
 int run_w4(ptq8_ops* o, const ptq8_linear_w4_args& a, cudaStream_t st) {
     W4Params p{};
@@ -64,20 +70,50 @@ int run_w4(ptq8_ops* o, const ptq8_linear_w4_args& a, cudaStream_t st) {
     p.x_type = a.x_type, p.s_type = a.scale_type, p.y_type = a.y_type;
     const long long lanes = 16 / static_cast<long long>(type_size(a.x_type));
     p.vec_x = aligned(a.x, 16) && (a.rows == 1 || a.ldx % lanes == 0);
+    p.wait_limit = o->wait_limit;
+    p.err = o->error_dev;
+    p.stall = o->stall;
+    p.shift = -1;
+    if ((a.group & (a.group - 1)) == 0)
+        while ((1LL << ++p.shift) < a.group) {
+        }
     // bytes that a lane takes at once: four lanes' stay within a group
     const int vb = a.group % 128 == 0 || a.group >= a.in_features ? 16 : a.group % 64 == 0 ? 8 : a.group % 32 == 0 ? 4 : 0;
     cudaError_t e;
-    if (vb && aligned(a.w, vb) && a.ldw % vb == 0) {
+    if (vb && a.lds < (1 << 28) && aligned(a.w, 16) && (a.ldw % 16 == 0 || (a.out_features == 1 && !p.gated)) && a.ldw < (1LL << 39)) {
         const int per_tile = a.x_type == PTQ8_F32 ? 4 : 8;   // tokens
-        const int nt = a.rows <= per_tile ? 1 : a.rows <= 2 * per_tile ? 2 : 4;
-        const long long tiles = (a.out_features + (p.gated ? 8 : 16) - 1LL) / (p.gated ? 8 : 16);
-        const int rt = nt > 1 ? 2 : tiles <= 3LL * o->sms ? 1 : tiles <= 8LL * o->sms ? 2 : 4;
-        const W4Kernel kernel = a.x_type == PTQ8_F32   ? w4_kernel<float>(vb, rt, nt)
-                                : a.x_type == PTQ8_F16 ? w4_kernel<__half>(vb, rt, nt)
-                                                       : w4_kernel<__nv_bfloat16>(vb, rt, nt);
-        const long long blocks = (a.rows + nt * per_tile - 1) / (nt * per_tile);
-        e = launch(kernel, dim3(static_cast<unsigned>((tiles + rt - 1) / rt), static_cast<unsigned>(std::min<long long>(blocks, 65535))), dim3(32 * kW4Warps),
-                   static_cast<size_t>(kW4Warps) * rt * nt * 128 * 4, 1, st, p);
+        const int chunks = (a.in_features + kW4Chunk - 1) / kW4Chunk;
+        const long long tiles = (a.out_features - 1LL) / (p.gated ? 16 : 32) + 1;   // pairs
+        // The fewest columns that take all tokens in a pass, fewer where all chunks' activations do not fit beside a stage of weights;
+        // then as long and as many stages as fit.  Not even with eight columns: a segment of 16 chunks at a time.
+        const W4Variant* v = nullptr;
+        W4Plan plan{};
+        long long passes = 0;
+        for (int nt = a.rows <= per_tile ? 1 : a.rows <= 2 * per_tile ? 2 : 4; !plan.stages; nt /= 2) {
+            const bool segments = nt == 0;
+            for (v = kW4Variants; v->type != a.x_type || v->vb != vb || v->nt != std::max(nt, 1);) ++v;
+            passes = (a.rows + v->nt * per_tile - 1) / (v->nt * per_tile);
+            plan = {8, segments ? 16 : chunks, 1, 4, 0};
+            if (v->nt == 1) plan.columns = static_cast<int>(std::min<long long>(8, a.rows * (a.x_type == PTQ8_F32 ? 2 : 1)));
+            // warps a tile: as many as leave the device's warps a tile each, if that many
+            while (plan.split < kW4Warps && plan.split < plan.held && tiles * passes * plan.split * 2 <= static_cast<long long>(kW4Warps) * o->sms) plan.split *= 2;
+            const long long left = kW4Smem - 1024 - v->sums - static_cast<long long>(plan.held) * (v->frag(plan.columns) + v->beside);
+            const auto room = [&](int run) { return static_cast<int>(std::max(0LL, std::min<long long>(kW4MostStages, left / (kW4Warps * run / 2 * kW4Box)))); };
+            plan.run = room(4) >= 2 ? 4 : 2;
+            plan.stages = room(plan.run);
+        }
+        const int slots = kW4Warps / plan.split, smem = v->sums + plan.held * (v->frag(plan.columns) + v->beside) + kW4Warps * plan.stages * plan.run / 2 * kW4Box + 1024;
+        const long long groups = (tiles + slots - 1) / slots;
+        const long long x = std::min<long long>(groups, std::max<long long>(1, o->sms / passes)), y = std::min<long long>(passes, std::max<long long>(1, o->sms / x));
+        const long long channels = static_cast<long long>(a.out_features) * (p.gated ? 2 : 1);
+        const int wide = (a.in_features + 1) / 2;
+        CUtensorMap map;
+        const cuuint64_t dims[2] = {static_cast<cuuint64_t>(wide), static_cast<cuuint64_t>(channels)}, pitch[1] = {static_cast<cuuint64_t>(channels > 1 ? a.ldw : (wide + 15) / 16 * 16)};
+        const cuuint32_t box[2] = {128, p.gated ? 16u : 32u}, one[2] = {1, 1};
+        const CUresult r = o->encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(a.w), dims, pitch, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (r != CUDA_SUCCESS) return fail(o, PTQ8_ERR_CUDA, "linear_w4: cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+        e = launch(v->kernel, dim3(static_cast<unsigned>(x), static_cast<unsigned>(y)), dim3(kW4Threads), smem, 1, st, p, plan, map);
     } else {
         const long long blocks = (a.rows + kW4AnyTokens - 1) / kW4AnyTokens;
         e = launch(linear_w4_any_kernel, dim3((a.out_features + 7) / 8, static_cast<unsigned>(std::min<long long>(blocks, 65535))), dim3(256), 0, 1, st, p);
@@ -89,7 +125,13 @@ int run_w4(ptq8_ops* o, const ptq8_linear_w4_args& a, cudaStream_t st) {
 
 namespace ptq8 {
 
-cudaError_t w4_attributes() { return cudaSuccess; }
+cudaError_t w4_attributes() {
+    for (const W4Variant& v : kW4Variants) {
+        const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(v.kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, kW4Smem);
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
+}
 
 }  // namespace ptq8
 

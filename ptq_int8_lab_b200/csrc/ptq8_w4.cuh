@@ -9,18 +9,21 @@
 // go in as two f16, the second with what the first leaves (22 places), in columns beside each other.  A group's sum is
 // f32 in the tensor cores, and meets its scale in f32.
 //
-// A warp owns 16 RT weight rows and a part of the input features, a lane 4, 8 or 16 bytes of two of them at a time; the
-// eight warps of a block have the same rows, and meet at the end in shared memory, in a fixed order.  Places of the
-// products' inner dimension are dealt to a row's bytes so that a group stays within an MMA (four lanes hold VB bytes
-// each: 32, 64 or 128 codes of a row).
+// A warp has pairs of tiles of 16 weight rows, or shares each with split - 1 others, which take other input features; their sums
+// meet in shared memory, in a fixed order.  Weights come by TMA through a ring of the warp's own in shared memory, two or
+// four chunks of 128 features of the 32 rows at a time.  (Bulk copies of single rows, a lane each, run one after another
+// in some 20 instructions each: 32 of them took 2 us.)  The activations are brought into the products' order in shared
+// memory: once, where they fit there as a whole, else a segment at a time.  Places of the products' inner dimension are
+// dealt to a row's bytes so that a group stays within an MMA (four lanes hold VB bytes each: 32, 64 or 128 codes of a row).
 #pragma once
 
 #include "ptq8_cache.cuh"
 #include "ptq8_linear.cuh"
+#include "ptq8_rows.cuh"
 
 namespace ptq8 {
 
-constexpr int kW4Warps = 8, kW4Chunk = 128;
+constexpr int kW4Warps = 16, kW4Chunk = 128;
 
 struct W4Params {
     const void* x;
@@ -31,7 +34,12 @@ struct W4Params {
     size_t ldx, ldw, lds, ldy;   // elements, bytes, elements, elements
     long long rows;
     int k, n, group;             // n: output features
-    int gated, x_type, s_type, y_type, vec_x;
+    int gated, x_type, s_type, y_type;
+    int vec_x;      // activations at multiples of 16 bytes
+    int shift;      // group = 1 << shift, or -1
+    long long wait_limit;
+    int* err;
+    int stall;
 };
 
 __device__ __forceinline__ float scale_at(const W4Params& p, size_t at) {
@@ -92,227 +100,350 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// The nibble's sign bit turned: code + 8 as an unsigned number, as f16 times 2^-24 (16 * 2^-24 for the high one).
-constexpr uint32_t kW4Low = 0x000F000Fu, kW4High = 0x00F000F0u, kW4FlipLow = 0x00080008u, kW4FlipHigh = 0x00800080u;
+// With every code's sign bit turned a nibble is code + 8: as f16 that times 2^-24 (times 2^-20 for the high one of a byte).
+constexpr uint32_t kW4Turn = 0x88888888u, kW4Low = 0x000F000Fu, kW4High = 0x00F000F0u;
 // -8 * 2^-24 and -128 * 2^-24
 constexpr uint32_t kW4ShiftLow = 0x80088008u, kW4ShiftHigh = 0x80808080u;
 
-// A lane's part of a chunk: for each of 128 / (8 VB) pieces VB bytes of 2 RT rows; their scales, piece min(t, last)'s.
-template <int VB, int RT>
-struct W4Load {
-    static constexpr int PIECES = 16 / VB;
-    uint32_t w[RT][2][4];
-    float s[RT][2];
+template <int VB>
+struct W4Pieces {
+    static constexpr int N = 16 / VB, RUN = 2 * VB;   // of a chunk, that a lane has; consecutive values of one
 };
 
-template <int VB, int RT>
-__device__ __forceinline__ void w4_load(W4Load<VB, RT>& l, const W4Params& p, const uint8_t* const (&row)[RT][2], const size_t (&srow)[RT][2], int chunk, int t) {
-    constexpr int PIECES = W4Load<VB, RT>::PIECES;
-    const int bytes = (p.k + 1) / 2, at = chunk * 64 + t * VB;
-    const int k = min(chunk * kW4Chunk + min(t, PIECES - 1) * 8 * VB, p.k - 1);
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            l.s[r][h] = scale_at(p, srow[r][h] + k / p.group);
-#pragma unroll
-            for (int i = 0; i < PIECES; ++i) {
-                const int from = at + i * 4 * VB;
-                uint32_t* w = &l.w[r][h][i * (VB / 4)];
-                if (from + VB <= bytes) {
-                    if constexpr (VB == 16) {
-                        const uint4 v = *reinterpret_cast<const uint4*>(row[r][h] + from);
-                        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-                    } else if constexpr (VB == 8) {
-                        const uint2 v = *reinterpret_cast<const uint2*>(row[r][h] + from);
-                        w[0] = v.x, w[1] = v.y;
-                    } else {
-                        w[0] = *reinterpret_cast<const uint32_t*>(row[r][h] + from);
-                    }
-                } else {   // the row's end: byte by byte (what is behind it meets zeros)
-#pragma unroll
-                    for (int j = 0; j < VB / 4; ++j) w[j] = join4(row[r][h] + from + 4 * j, min(4, bytes - from - 4 * j));
-                }
-            }
-        }
+__device__ __forceinline__ float w4_scale(uint32_t bits, int type) {
+    const float half = __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+    const float wide = __uint_as_float(type == Y_F32 ? bits : bits << 16);
+    return type == Y_F16 ? half : wide;
 }
 
-// 32 activations of a lane's token, of its places of a chunk, as f32 (zeros behind the row's end or without a token).
+// 32 activations of a lane's token and place of a chunk, as they lie in memory; zeros without a token and behind the row's end.
 template <typename XT, int VB>
-__device__ __forceinline__ void w4_tokens(const W4Params& p, float (&f)[32], long long token, int chunk, int t) {
-    constexpr int PIECES = 16 / VB, RUN = 2 * VB;   // consecutive values of a piece
+__device__ __forceinline__ void w4_tokens(uint4 (&x)[2 * sizeof(XT)], const W4Params& p, const char* token, int chunk, int t) {
+    constexpr int RUN = W4Pieces<VB>::RUN, PER = 16 / sizeof(XT);   // values of a vector
+    if (p.vec_x && (chunk + 1) * kW4Chunk <= p.k) {
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-        const int k0 = chunk * kW4Chunk + i * 8 * VB + t * RUN;
+        for (int i = 0; i < static_cast<int>(2 * sizeof(XT)); ++i) {
+            const int piece = i * PER / RUN, in = i * PER % RUN;
+            x[i] = token ? *reinterpret_cast<const uint4*>(token + (chunk * kW4Chunk + piece * 8 * VB + in) * sizeof(XT)) : make_uint4(0, 0, 0, 0);
+        }
+    } else {
+        uint32_t* w = reinterpret_cast<uint32_t*>(x);
 #pragma unroll
-        for (int j = 0; j < RUN / 8; ++j) {
-            const int k = k0 + 8 * j;
-            float e[8];
-            if (token >= 0 && p.vec_x && k + 8 <= p.k) {
-                load8<XT, true>(static_cast<const XT*>(p.x) + static_cast<size_t>(token) * p.ldx + k, e);
+        for (int i = 0; i < 32; ++i) {
+            const int k = chunk * kW4Chunk + i / RUN * 8 * VB + i % RUN;
+            const bool in = token && k + t * RUN < p.k;
+            if constexpr (sizeof(XT) == 4) {
+                w[i] = in ? reinterpret_cast<const uint32_t*>(token)[k] : 0u;
             } else {
-#pragma unroll
-                for (int z = 0; z < 8; ++z) e[z] = token >= 0 && k + z < p.k ? static_cast<float>(static_cast<const XT*>(p.x)[static_cast<size_t>(token) * p.ldx + k + z]) : 0.0f;
+                const uint32_t v = in ? reinterpret_cast<const unsigned short*>(token)[k] : 0u;
+                w[i / 2] = i & 1 ? w[i / 2] | v << 16 : v;
             }
-#pragma unroll
-            for (int z = 0; z < 8; ++z) f[i * RUN + 8 * j + z] = e[z];
         }
     }
 }
 
-// Their f16 as the products want them, four to a word of weights (codes 0, 4; 1, 5, which are 16 times too large; 2, 6; 3, 7),
-// and the power of two that their products with code * 2^-24 lack.  SPLIT: a lane of an odd column takes what the even
-// column's f16 leave, times 2^11.
-template <bool SPLIT>
-__device__ __forceinline__ float w4_fragments(uint32_t (&b)[4][4], const float (&f)[32], bool rest) {
-    float top = 0.0f;
+template <typename XT>
+__device__ __forceinline__ float w4_value(const uint32_t* raw, int i) {
+    if constexpr (sizeof(XT) == 4) return __uint_as_float(raw[i]);
+    if constexpr (__is_same(XT, __half)) return __half2float(__ushort_as_half(static_cast<unsigned short>(i & 1 ? raw[i / 2] >> 16 : raw[i / 2])));
+    return __uint_as_float(i & 1 ? raw[i / 2] & 0xFFFF0000u : raw[i / 2] << 16);
+}
+
+// They become f16, four to a word of weights (codes 0, 4; 1, 5, which come 16 times too large; 2, 6; 3, 7), times a power of two, at
+// to[stride w].  f32: the lanes of even columns take the first f16 of a number, those of odd ones what it leaves.  Beside
+// them, for each piece and column, -8 times its sum and the power of two that products with code * 2^-24 lack.
+template <typename XT, int VB>
+__device__ __forceinline__ void w4_fragments(uint4* to, int stride, bool kept, float2* beside, const uint4 (&x)[2 * sizeof(XT)], int g, int t) {
+    const uint32_t* raw = reinterpret_cast<const uint32_t*>(x);
+    float top;
+    if constexpr (sizeof(XT) == 4) {
+        top = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) top = max_nan(top, fabsf(f[i]));
+        for (int i = 0; i < 32; ++i) top = max_nan(top, fabsf(__uint_as_float(raw[i])));
+    } else {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) m = Vec<XT>::join(m, raw[i]);
+        top = __uint_as_float(Vec<XT>::top(m));
+    }
     top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const int e = min(max(14 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), -100), 100);
-    const float up = __int_as_float((e + 127) << 23);
-    float v[32];
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        v[i] = f[i] * up;
-        if (SPLIT) {
-            const float left = (v[i] - __half2float(__float2half_rn(v[i]))) * 2048.0f;
-            if (rest) v[i] = left;
-        }
-    }
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        const float* x = v + 8 * w;
-        b[w][0] = pair_of<__half>(x[0], x[4]);
-        b[w][1] = pair_of<__half>(x[1] * 0.0625f, x[5] * 0.0625f);
-        b[w][2] = pair_of<__half>(x[2], x[6]);
-        b[w][3] = pair_of<__half>(x[3] * 0.0625f, x[7] * 0.0625f);
-    }
+    const float up = __int_as_float((e + 127) << 23), up16 = up * 0.0625f;
     // a token that is not finite: NaN (as an infinity times a code of zero is)
-    return isfinite(top) ? __int_as_float((24 - e + 127) << 23) : __int_as_float(0x7FC00000);
+    const float l = isfinite(top) ? __int_as_float((24 - e + 127) << 23) : __int_as_float(0x7FC00000);
+    const float lack0 = __shfl_sync(0xffffffffu, l, 8 * t), lack1 = __shfl_sync(0xffffffffu, l, 8 * t + 4);
+#pragma unroll
+    for (int j = 0; j < 16 / VB; ++j) {
+        float shift[4] = {};
+#pragma unroll
+        for (int w = j * (VB / 4); w < (j + 1) * (VB / 4); ++w) {
+            uint32_t b[4];
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+                const float u = w4_value<XT>(raw, 8 * w + z) * (z & 1 ? up16 : up), v = w4_value<XT>(raw, 8 * w + z + 4) * (z & 1 ? up16 : up);
+                b[z] = pair_of<__half>(u, v);
+                if constexpr (sizeof(XT) == 4) {
+                    const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&b[z]));
+                    const uint32_t left = pair_of<__half>(u - h.x, v - h.y);
+                    if (g & 1) b[z] = left;
+                }
+            }
+            mma_f16(shift, kW4ShiftLow, kW4ShiftLow, kW4ShiftHigh, kW4ShiftHigh, b[0], b[1]);
+            mma_f16(shift, kW4ShiftLow, kW4ShiftLow, kW4ShiftHigh, kW4ShiftHigh, b[2], b[3]);
+            if (kept) to[stride * w] = make_uint4(b[0], b[1], b[2], b[3]);
+        }
+        if (g == 0) *reinterpret_cast<float4*>(beside + j * 8 + 2 * t) = make_float4(shift[0], lack0, shift[1], lack1);
+    }
 }
 
-template <typename XT, int VB, int RT, int NT>
-__global__ void __launch_bounds__(32 * kW4Warps) linear_w4_kernel(const W4Params p) {
-    constexpr bool SPLIT = sizeof(XT) == 4;
-    constexpr int TOKENS = NT * (SPLIT ? 4 : 8), PIECES = 16 / VB, WORDS = VB / 4;
-    extern __shared__ float sums[];   // [warp][RT][NT][4][32]
+constexpr int kW4Threads = 32 * kW4Warps, kW4MostStages = 4, kW4Smem = 224 * 1024, kW4Box = 32 * 128;   // two chunks of the 32 rows
+
+template <typename XT, int VB, int NT>
+struct W4Shape {
+    static constexpr bool kSplit = sizeof(XT) == 4;
+    static constexpr int kColumns = kSplit ? 4 : 8, kTokens = NT * kColumns;   // tokens of eight columns; of a pass
+    static constexpr int kPieces = W4Pieces<VB>::N;
+    static constexpr int kSums = kW4Warps * 2 * NT * 128 * 4;
+    // of a chunk; columns: those held (fewer than eight where there are no more)
+    static int frag(int columns) { return NT * 4 * columns * 64; }
+    static constexpr int kBeside = NT * kPieces * 64;
+};
+
+struct W4Plan {   // (see the host's choice)
+    int columns;   // of a tile, that hold a token
+    int held;      // chunks whose activations shared memory holds: all, or a segment's
+    int split;     // warps of a tile: a power of two
+    int run;       // chunks of a stage
+    int stages;    // of a warp
+};
+
+template <typename XT, int VB, int NT>
+__global__ void __launch_bounds__(kW4Threads, 1) linear_w4_kernel(const W4Params p, const W4Plan plan, const __grid_constant__ CUtensorMap map) {
+    using Sh = W4Shape<XT, VB, NT>;
+    constexpr int PIECES = Sh::kPieces, WORDS = VB / 4;
+    extern __shared__ uint8_t smem_any[];
+    uint8_t* smem = smem_any + (-smem_u32(smem_any) & 1023);   // TMA's pattern of 128 bytes goes by the address
+    __shared__ __align__(8) uint64_t bars[kW4Warps * kW4MostStages];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int part = warp & (plan.split - 1), slot = warp / plan.split, slots = kW4Warps / plan.split;
     // rows g and g + 8 of a tile: of a gated product a gate and its up row, else two output features
-    const int per = p.gated ? 8 : 16, c0 = blockIdx.x * per * RT;
-    const uint8_t* row[RT][2];
-    size_t srow[RT][2];
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {   // rows past the end repeat the last one; their sums are dropped
-            const int c = min(c0 + r * per + g + (p.gated ? 0 : 8 * h), p.n - 1);
-            const size_t at = static_cast<size_t>(c) + (p.gated ? static_cast<size_t>(h) * p.n : 0);
-            row[r][h] = p.w + at * p.ldw;
-            srow[r][h] = at * p.lds;
-        }
-    const int chunks = (p.k + kW4Chunk - 1) / kW4Chunk, beg = chunks * warp / kW4Warps, end = chunks * (warp + 1) / kW4Warps;
-    griddep_launch();
-    griddep_wait();
-    for (long long t0 = static_cast<long long>(blockIdx.y) * TOKENS; t0 < p.rows; t0 += static_cast<long long>(gridDim.y) * TOKENS) {
-        float acc[RT][NT][4] = {};
-        W4Load<VB, RT> cur, next;
-        if (beg < end) w4_load(next, p, row, srow, beg, t);
-        for (int chunk = beg; chunk < end; ++chunk) {
-            cur = next;
-            if (chunk + 1 < end) w4_load(next, p, row, srow, chunk + 1, t);
-            uint32_t b[NT][4][4];
-            float lack[NT][2];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                const long long token = t0 + nt * (TOKENS / NT) + (SPLIT ? g >> 1 : g);
-                float f[32];
-                w4_tokens<XT, VB>(p, f, token < p.rows ? token : -1, chunk, t);
-                const float l = w4_fragments<SPLIT>(b[nt], f, g & 1);
-                lack[nt][0] = __shfl_sync(0xffffffffu, l, 8 * t);
-                lack[nt][1] = __shfl_sync(0xffffffffu, l, 8 * t + 4);
-            }
-#pragma unroll
-            for (int i = 0; i < PIECES; ++i) {
-                float part[RT][NT][4];
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    float shift[4] = {};
-#pragma unroll
-                    for (int w = i * WORDS; w < (i + 1) * WORDS; ++w) {
-                        mma_f16(shift, kW4ShiftLow, kW4ShiftLow, kW4ShiftHigh, kW4ShiftHigh, b[nt][w][0], b[nt][w][1]);
-                        mma_f16(shift, kW4ShiftLow, kW4ShiftLow, kW4ShiftHigh, kW4ShiftHigh, b[nt][w][2], b[nt][w][3]);
-                    }
-#pragma unroll
-                    for (int r = 0; r < RT; ++r)
-#pragma unroll
-                        for (int z = 0; z < 4; ++z) part[r][nt][z] = shift[z];
+    const int per = p.gated ? 8 : 16, tiles = (p.n + 2 * per - 1) / (2 * per), rounds = (tiles + gridDim.x * slots - 1) / (gridDim.x * slots);
+    const int chunks = (p.k + kW4Chunk - 1) / kW4Chunk, segments = (chunks + plan.held - 1) / plan.held;
+    const int stage_bytes = plan.run / 2 * kW4Box;
+    uint8_t* ring = smem + warp * plan.stages * stage_bytes;
+    float* sums = reinterpret_cast<float*>(smem + kW4Warps * plan.stages * stage_bytes);   // [warp][2][NT][4][32]
+    uint4* frag = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(sums) + Sh::kSums);   // [held][NT][4][columns][4]
+    float2* beside = reinterpret_cast<float2*>(frag + plan.held * NT * 16 * plan.columns);   // [held][NT][PIECES][8]
+    const uint32_t full = smem_u32(bars + warp * kW4MostStages);
+    const int passes = static_cast<int>((p.rows + Sh::kTokens - 1) / Sh::kTokens);
+    if (lane < plan.stages) mbar_init(full + 8 * lane, 1);
+    fence_mbar_init();
+    __syncwarp();
+    // The pair of tiles that the warp has in a round (past the end: the last one's again; its sums are dropped), and its chunks of a segment.
+    // Of a gated product rows 8 r + g and 16 + 8 r + g are tile r's gate and up row g, else rows 16 r + g and 16 r + 8 + g two features.
+    const auto pair_of = [&](int round) { return min((round * static_cast<int>(gridDim.x) + static_cast<int>(blockIdx.x)) * slots + slot, tiles - 1); };
+    const auto chunk_of = [&](int segment, int i) { const int n = min(plan.held, chunks - segment * plan.held); return segment * plan.held + n * i / plan.split; };
+
+    // The warp's stages: for each pass, round and segment, its chunks, `run` at a time.  Loads go plan.stages ahead.
+    int l_pass = blockIdx.y, l_round = 0, l_segment = 0, l_chunk = chunk_of(0, part), l_end = chunk_of(0, part + 1), issued = 0, taken = 0;
+    bool lost = false;
+    const auto issue = [&]() {
+        while (l_chunk >= l_end) {   // (a part may be empty)
+            if (l_pass >= passes) return;
+            if (++l_segment == segments) {
+                l_segment = 0;
+                if (++l_round == rounds) {
+                    l_round = 0;
+                    l_pass += gridDim.y;
+                    if (l_pass >= passes) return;
                 }
+            }
+            l_chunk = chunk_of(l_segment, part), l_end = chunk_of(l_segment, part + 1);
+        }
+        const int stage = issued % plan.stages, boxes = (min(plan.run, l_end - l_chunk) + 1) / 2, row = pair_of(l_round) * 2 * per;
+        const uint32_t bar = full + 8 * stage, to = smem_u32(ring) + stage * stage_bytes;
+        if (elect_one()) {   // what lies outside of the weights comes as zeros, and counts
+            mbar_expect_tx(bar, boxes * kW4Box);
+            if (!(p.stall && blockIdx.x == 0 && blockIdx.y == 0 && warp == 0 && issued == 0))
+                for (int i = 0; i < boxes; ++i) {
+                    tma_load_2d(to + i * kW4Box, &map, bar, (l_chunk + 2 * i) * 64, row);
+                    if (p.gated) tma_load_2d(to + i * kW4Box + kW4Box / 2, &map, bar, (l_chunk + 2 * i) * 64, p.n + row);
+                }
+        }
+        __syncwarp();
+        ++issued;
+        l_chunk += plan.run;
+    };
+    // into L2 while the kernel before this one drains: what the first stages load
+    if (elect_one()) {
+        const int row = pair_of(0) * 2 * per;
+        for (int c = l_chunk; c < min(l_end, l_chunk + plan.run * plan.stages); c += 2)
+            for (int h = 0; h < (p.gated ? 2 : 1); ++h)
+                asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(&map)), "r"(c * 64), "r"(row + h * p.n) : "memory");
+    }
+    __syncwarp();
+    griddep_wait();
+    griddep_launch();
+    for (int i = 0; i < plan.stages; ++i) issue();
+    // Scales as bits, those of a stage's chunks while the one before is worked on: a conversion here would wait for the load.
+    const int scale_shift = p.s_type == Y_F32 ? 2 : 1, scale_pitch = static_cast<int>(p.lds) << scale_shift;   // (the host keeps it an int)
+    for (int pass = blockIdx.y; pass < passes; pass += gridDim.y) {
+        const long long t0 = static_cast<long long>(pass) * Sh::kTokens;
+        for (int round = 0; round < rounds; ++round) {
+            float2 acc[2][NT][2] = {};   // [tile][..][row g or g + 8]: columns 2 t, 2 t + 1
+            const char* scales[4];
 #pragma unroll
-                for (int w = i * WORDS; w < (i + 1) * WORDS; ++w)
+            for (int h = 0; h < 4; ++h) {   // row g + 8 (h % 2) of tile h / 2
+                const int c = min((2 * pair_of(round) + (h >> 1)) * per + g + (p.gated ? 0 : 8 * (h & 1)), p.n - 1) + (p.gated ? (h & 1) * p.n : 0);
+                scales[h] = static_cast<const char*>(p.s) + static_cast<long long>(c) * scale_pitch;
+            }
+            for (int segment = 0; segment < segments; ++segment) {
+                if (segments > 1 || round == 0) {   // the activations of its chunks
+                    __syncthreads();                // those before are read
+                    const int first = segment * plan.held, count = min(plan.held, chunks - first) * NT;
+                    for (int i = warp; i < count; i += kW4Warps) {
+                        const long long token = t0 + i % NT * Sh::kColumns + (Sh::kSplit ? g >> 1 : g);
+                        const char* from = token < p.rows ? static_cast<const char*>(p.x) + (static_cast<size_t>(token) * p.ldx + t * W4Pieces<VB>::RUN) * sizeof(XT) : nullptr;
+                        uint4 x[2 * sizeof(XT)];
+                        w4_tokens<XT, VB>(x, p, from, first + i / NT, t);
+                        w4_fragments<XT, VB>(frag + i * 16 * plan.columns + lane, 4 * plan.columns, g < plan.columns, beside + i * PIECES * 8, x, g, t);
+                    }
+                    __syncthreads();
+                }
+                const int end = chunk_of(segment, part + 1);
+                for (int c0 = chunk_of(segment, part); c0 < end; c0 += plan.run) {
+                    const int stage = taken % plan.stages, n = min(plan.run, end - c0);
+                    uint32_t scale[4][4];   // [chunk][row g + 8 h]
 #pragma unroll
-                    for (int r = 0; r < RT; ++r) {
-                        uint32_t u = cur.w[r][0][w], v = cur.w[r][1][w];
+                    for (int j = 0; j < 4; ++j) {
+                        if (j >= n) break;
+                        const int k = min((c0 + j) * kW4Chunk + min(t, PIECES - 1) * 8 * VB, p.k - 1), at = (p.shift >= 0 ? k >> p.shift : k / p.group) << scale_shift;
+                        if (scale_shift == 2) {
 #pragma unroll
-                        for (int z = 0; z < 4; z += 2) {
-                            const uint32_t a0 = (u & kW4Low) ^ kW4FlipLow, a1 = (v & kW4Low) ^ kW4FlipLow, a2 = (u & kW4High) ^ kW4FlipHigh, a3 = (v & kW4High) ^ kW4FlipHigh;
+                            for (int h = 0; h < 4; ++h) scale[j][h] = *reinterpret_cast<const uint32_t*>(scales[h] + at);
+                        } else {
 #pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) mma_f16(part[r][nt], a0, a1, a2, a3, b[nt][w][z], b[nt][w][z + 1]);
-                            u >>= 8, v >>= 8;
+                            for (int h = 0; h < 4; ++h) scale[j][h] = *reinterpret_cast<const unsigned short*>(scales[h] + at);
                         }
                     }
-#pragma unroll
-                for (int r = 0; r < RT; ++r) {
-                    float s[2];
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) s[h] = PIECES == 1 ? cur.s[r][h] : __shfl_sync(0xffffffffu, cur.s[r][h], (lane & 28) + i);
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int z = 0; z < 4; ++z) acc[r][nt][z] = __fmaf_rn(part[r][nt][z] * lack[nt][z & 1], s[z >> 1], acc[r][nt][z]);
-                }
-            }
-        }
-        // the warps' sums meet, in their order; lane's z: row g + 8 (z / 2), column 2 t + z % 2
-#pragma unroll
-        for (int r = 0; r < RT; ++r)
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int z = 0; z < 4; ++z) sums[((warp * RT + r) * NT + nt) * 128 + z * 32 + lane] = acc[r][nt][z];
-        __syncthreads();
-        constexpr int COLUMNS = SPLIT ? 4 : 8;   // tokens of a tile
-        for (int i = threadIdx.x; i < RT * NT * COLUMNS * per; i += 32 * kW4Warps) {
-            const int in = i % per, r = i / per % RT, col = i / (per * RT) % COLUMNS, nt = i / (per * RT * COLUMNS);
-            const int c = c0 + r * per + in;
-            const long long token = t0 + nt * COLUMNS + col;
-            if (c >= p.n || token >= p.rows) continue;
-            const auto sum = [&](int tile_row) {
-                float v = 0.0f;
-#pragma unroll
-                for (int w = 0; w < kW4Warps; ++w) {
-                    const float* at = sums + ((w * RT + r) * NT + nt) * 128;
-                    if (SPLIT) {   // columns 2 col and 2 col + 1
-                        const int l = (tile_row & 7) * 4 + col, z = tile_row >> 3 << 1;
-                        v += __fmaf_rn(at[(z + 1) * 32 + l], 1.0f / 2048.0f, at[z * 32 + l]);
-                    } else {
-                        v += at[((tile_row >> 3 << 1) + (col & 1)) * 32 + (tile_row & 7) * 4 + (col >> 1)];
+                    // (a warp that gives up goes on without loads, so that it meets the others at the barriers)
+                    if (!lost && !mbar_wait_warp(full + 8 * stage, (taken / plan.stages) & 1, p.wait_limit)) {
+                        lost = true;
+                        if (lane == 0) *p.err = ERR_WAIT_FULL;
                     }
+                    ++taken;
+                    const uint8_t* tile = ring + stage * stage_bytes + g * 128;
+                    // (a lane of a column that holds no token takes the last one's: what it adds to is not used)
+                    const uint4* b_at = frag + (c0 - segment * plan.held) * NT * 16 * plan.columns + 4 * min(g, plan.columns - 1) + t;
+                    const float2* beside_at = beside + (c0 - segment * plan.held) * NT * PIECES * 8 + 2 * t;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (j >= n) break;
+                        uint32_t weights[4][4];
+#pragma unroll
+                        for (int h = 0; h < 4; ++h)
+#pragma unroll
+                            for (int i = 0; i < PIECES; ++i) {
+                                // 16 bytes of a row lie at their place ^ the row's number % 8
+                                const int row = p.gated ? 16 * (h & 1) + 8 * (h >> 1) : 8 * h, at = (j & 1) * 64 + i * 4 * VB + t * VB;
+                                const uint8_t* from = tile + (j >> 1) * kW4Box + row * 128 + ((at ^ (g << 4)));
+                                uint32_t* w = &weights[h][i * WORDS];
+                                if constexpr (VB == 16) {
+                                    const uint4 v = *reinterpret_cast<const uint4*>(from);
+                                    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+                                } else if constexpr (VB == 8) {
+                                    const uint2 v = *reinterpret_cast<const uint2*>(from);
+                                    w[0] = v.x, w[1] = v.y;
+                                } else {
+                                    w[0] = *reinterpret_cast<const uint32_t*>(from);
+                                }
+                            }
+#pragma unroll
+                        for (int i = 0; i < PIECES; ++i) {
+                            float sum[2][NT][4];
+                            float2 lack[NT];
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                const float4 v = *reinterpret_cast<const float4*>(beside_at + ((j * NT + nt) * PIECES + i) * 8);
+#pragma unroll
+                                for (int r = 0; r < 2; ++r) sum[r][nt][0] = sum[r][nt][2] = v.x, sum[r][nt][1] = sum[r][nt][3] = v.z;
+                                lack[nt] = make_float2(v.y, v.w);
+                            }
+#pragma unroll
+                            for (int w = i * WORDS; w < (i + 1) * WORDS; ++w) {
+                                uint4 b[NT];
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt) b[nt] = b_at[((j * NT + nt) * 4 + w) * 4 * plan.columns];
+#pragma unroll
+                                for (int r = 0; r < 2; ++r) {
+                                    const uint32_t u = weights[2 * r][w] ^ kW4Turn, v = weights[2 * r + 1][w] ^ kW4Turn, u8 = u >> 8, v8 = v >> 8;
+#pragma unroll
+                                    for (int nt = 0; nt < NT; ++nt) {
+                                        mma_f16(sum[r][nt], u & kW4Low, v & kW4Low, u & kW4High, v & kW4High, b[nt].x, b[nt].y);
+                                        mma_f16(sum[r][nt], u8 & kW4Low, v8 & kW4Low, u8 & kW4High, v8 & kW4High, b[nt].z, b[nt].w);
+                                    }
+                                }
+                            }
+#pragma unroll
+                            for (int h = 0; h < 4; ++h) {
+                                const float2 s = both(w4_scale(PIECES == 1 ? scale[j][h] : __shfl_sync(0xffffffffu, scale[j][h], (lane & 28) + i), p.s_type));
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt) {
+                                    const float* x = sum[h >> 1][nt] + 2 * (h & 1);
+                                    acc[h >> 1][nt][h & 1] = __ffma2_rn(__fmul2_rn(make_float2(x[0], x[1]), lack[nt]), s, acc[h >> 1][nt][h & 1]);
+                                }
+                            }
+                        }
+                    }
+                    __syncwarp();   // the stage is read
+                    if (!lost) issue();
                 }
-                return v;
-            };
-            float v = sum(in);
-            if (p.bias) v += p.bias[c];
-            if (p.gated) {
-                float u = sum(in + 8);
-                if (p.bias) u += p.bias[p.n + c];
-                v = swiglu(v, u);
             }
-            store_y(p.y, static_cast<size_t>(token) * p.ldy + c, v, p.y_type);
+            // The parts' sums meet in the tile's first warp, in their order.
+            if (plan.split > 1) {
+                if (round || pass != static_cast<int>(blockIdx.y)) __syncthreads();   // those before are read
+                float2* mine = reinterpret_cast<float2*>(sums) + warp * 4 * NT * 32 + lane;
+                if (part)
+#pragma unroll
+                    for (int i = 0; i < 4 * NT; ++i) mine[32 * i] = acc[i / (2 * NT)][i / 2 % NT][i % 2];
+                __syncthreads();
+                if (part == 0)
+                    for (int w = 1; w < plan.split; ++w)
+#pragma unroll
+                        for (int i = 0; i < 4 * NT; ++i) {
+                            float2& x = acc[i / (2 * NT)][i / 2 % NT][i % 2];
+                            x = __fadd2_rn(x, mine[(w * 4 * NT + i) * 32]);
+                        }
+            }
+            const int pair = (round * gridDim.x + blockIdx.x) * slots + slot;
+            if (part || pair >= tiles) continue;
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int col = 0; col < (Sh::kSplit ? 1 : 2); ++col) {
+                        const long long token = t0 + nt * Sh::kColumns + (Sh::kSplit ? t : 2 * t + col);
+                        if (token >= p.rows) continue;
+                        float v[2];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) v[h] = Sh::kSplit ? acc[r][nt][h].x + acc[r][nt][h].y : col ? acc[r][nt][h].y : acc[r][nt][h].x;
+                        const size_t row = static_cast<size_t>(token) * p.ldy;
+                        if (p.gated) {
+                            const int c = (2 * pair + r) * 8 + g;
+                            if (c < p.n) store_y(p.y, row + c, swiglu(v[0] + (p.bias ? p.bias[c] : 0.0f), v[1] + (p.bias ? p.bias[p.n + c] : 0.0f)), p.y_type);
+                        } else {
+#pragma unroll
+                            for (int h = 0; h < 2; ++h)
+                                if (const int c = (2 * pair + r) * 16 + g + 8 * h; c < p.n) store_y(p.y, row + c, v[h] + (p.bias ? p.bias[c] : 0.0f), p.y_type);
+                        }
+                    }
         }
-        __syncthreads();
     }
+    if (lost)   // no copy is in flight when the block ends
+        for (int i = max(0, issued - plan.stages); i < issued; ++i)
+            if (!mbar_wait_warp(full + 8 * (i % plan.stages), (i / plan.stages) & 1, p.wait_limit) && lane == 0) *p.err = ERR_DRAIN;
 }
 
 }  // namespace ptq8
