@@ -56,6 +56,27 @@ W4Variant w4_variant() {
 
 const W4Variant kW4Variants[] = {W4_TYPE(float, PTQ8_F32), W4_TYPE(__half, PTQ8_F16), W4_TYPE(__nv_bfloat16, PTQ8_BF16)};
 
+using W4Few = void (*)(W4Params, int);
+template <typename XT>
+struct W4FewOf {
+    static constexpr W4Few kKernels[2] = {linear_w4_few_kernel<XT, 1>, linear_w4_few_kernel<XT, 2>};
+};
+const W4Few* const kW4Few[] = {W4FewOf<float>::kKernels, W4FewOf<__half>::kKernels, W4FewOf<__nv_bfloat16>::kKernels};   // by type
+
+// One or two tokens while the weights are small.  us here and on the tensor cores, tokens x in -> out:
+//                  1024 -> 1024   4096 -> 1024   4096 -> 4096   4096 -> 14336
+//   1 x bf16       2.1   4.5      2.6   6.6      4.9    6.5     15.4   13.4
+//   2 x bf16       4.1   4.5      5.1   6.6      9.2    6.6     26.8   13.4
+//   1 x f32        2.5   5.9      3.6   8.0      8.1    10.7    23.6   21.0
+//   2 x f32        4.4   5.9      6.2   8.0      13.7   10.7    43.3   21.0
+// (The activations are read again for every four weight rows, which is what large weights make it wait for.)  Rows of whole vectors.
+bool few_rows(const ptq8_linear_w4_args& a, bool vectors) {
+    const bool gated = a.epilogue == PTQ8_EPI_SWIGLU;
+    const long long bytes = static_cast<long long>(a.out_features) * (gated ? 2 : 1) * a.in_features / 2;
+    return a.rows <= 2 && bytes <= (a.rows == 1 ? 12LL << 20 : 4LL << 20) && vectors && a.in_features % 32 == 0 && aligned(a.w, 16) &&
+           (a.ldw % 16 == 0 || (a.out_features == 1 && !gated));
+}
+
 int run_w4(ptq8_ops* o, const ptq8_linear_w4_args& a, cudaStream_t st) {
     W4Params p{};
     p.x = a.x;
@@ -80,12 +101,18 @@ int run_w4(ptq8_ops* o, const ptq8_linear_w4_args& a, cudaStream_t st) {
     // bytes that a lane takes at once: four lanes' stay within a group
     const int vb = a.group % 128 == 0 || a.group >= a.in_features ? 16 : a.group % 64 == 0 ? 8 : a.group % 32 == 0 ? 4 : 0;
     cudaError_t e;
-    if (vb && a.lds < (1 << 28) && aligned(a.w, 16) && (a.ldw % 16 == 0 || (a.out_features == 1 && !p.gated)) && a.ldw < (1LL << 39)) {
+    if (few_rows(a, vb && p.vec_x)) {
+        const long long sets = (a.out_features - 1LL) / (p.gated ? 2 : 4) + 1;
+        int ks = 1;
+        while (ks < kW4FewWarps && sets * ks < 1LL * kW4FewWarps * o->sms) ks *= 2;
+        const int per = kW4FewWarps / ks;
+        e = launch(kW4Few[a.x_type][a.rows - 1], dim3(static_cast<unsigned>((sets + per - 1) / per)), dim3(32 * kW4FewWarps), 0, 1, st, p, ks);
+    } else if (vb && a.lds < (1 << 28) && aligned(a.w, 16) && (a.ldw % 16 == 0 || (a.out_features == 1 && !p.gated)) && a.ldw < (1LL << 39)) {
         const int per_tile = a.x_type == PTQ8_F32 ? 4 : 8;   // tokens
         const int chunks = (a.in_features + kW4Chunk - 1) / kW4Chunk;
-        const long long tiles = (a.out_features - 1LL) / (p.gated ? 16 : 32) + 1;   // pairs
+        const long long pairs = (a.out_features - 1LL) / (p.gated ? 16 : 32) + 1;   // of tiles
         // The fewest columns that take all tokens in a pass, fewer where all chunks' activations do not fit beside a stage of weights;
-        // then as long and as many stages as fit.  Not even with eight columns: a segment of 16 chunks at a time.
+        // then as many stages as fit.  Not even with eight columns: a segment of 16 chunks at a time.
         const W4Variant* v = nullptr;
         W4Plan plan{};
         long long passes = 0;
@@ -93,18 +120,17 @@ int run_w4(ptq8_ops* o, const ptq8_linear_w4_args& a, cudaStream_t st) {
             const bool segments = nt == 0;
             for (v = kW4Variants; v->type != a.x_type || v->vb != vb || v->nt != std::max(nt, 1);) ++v;
             passes = (a.rows + v->nt * per_tile - 1) / (v->nt * per_tile);
-            plan = {8, segments ? 16 : chunks, 1, 4, 0};
+            plan = {8, segments ? 16 : chunks, segments ? (chunks + 15) / 16 : 1, 0, static_cast<int>(pairs), 1, 0, static_cast<int>(passes)};
             if (v->nt == 1) plan.columns = static_cast<int>(std::min<long long>(8, a.rows * (a.x_type == PTQ8_F32 ? 2 : 1)));
-            // warps a tile: as many as leave the device's warps a tile each, if that many
-            while (plan.split < kW4Warps && plan.split < plan.held && tiles * passes * plan.split * 2 <= static_cast<long long>(kW4Warps) * o->sms) plan.split *= 2;
+            // warps a pair: as many as leave the device's warps one each, if that many
+            while (1 << plan.split_log < std::min(kW4Warps, plan.held) && (pairs * passes << plan.split_log) * 2 <= static_cast<long long>(kW4Warps) * o->sms) ++plan.split_log;
             const long long left = kW4Smem - 1024 - v->sums - static_cast<long long>(plan.held) * (v->frag(plan.columns) + v->beside);
-            const auto room = [&](int run) { return static_cast<int>(std::max(0LL, std::min<long long>(kW4MostStages, left / (kW4Warps * run / 2 * kW4Box)))); };
-            plan.run = room(4) >= 2 ? 4 : 2;
-            plan.stages = room(plan.run);
+            plan.stages = static_cast<int>(std::max(0LL, std::min<long long>(kW4MostStages, left / (kW4Warps * kW4Box))));
         }
-        const int slots = kW4Warps / plan.split, smem = v->sums + plan.held * (v->frag(plan.columns) + v->beside) + kW4Warps * plan.stages * plan.run / 2 * kW4Box + 1024;
-        const long long groups = (tiles + slots - 1) / slots;
+        const int slots = kW4Warps >> plan.split_log, smem = v->sums + plan.held * (v->frag(plan.columns) + v->beside) + kW4Warps * plan.stages * kW4Box + 1024;
+        const long long groups = (pairs + slots - 1) / slots;
         const long long x = std::min<long long>(groups, std::max<long long>(1, o->sms / passes)), y = std::min<long long>(passes, std::max<long long>(1, o->sms / x));
+        plan.rounds = static_cast<int>((groups + x - 1) / x);
         const long long channels = static_cast<long long>(a.out_features) * (p.gated ? 2 : 1);
         const int wide = (a.in_features + 1) / 2;
         CUtensorMap map;

@@ -10,8 +10,8 @@
 // f32 in the tensor cores, and meets its scale in f32.
 //
 // A warp has pairs of tiles of 16 weight rows, or shares each with split - 1 others, which take other input features; their sums
-// meet in shared memory, in a fixed order.  Weights come by TMA through a ring of the warp's own in shared memory, two or
-// four chunks of 128 features of the 32 rows at a time.  (Bulk copies of single rows, a lane each, run one after another
+// meet in shared memory, in a fixed order.  Weights come by TMA through a ring of the warp's own in shared memory, two
+// chunks of 128 features of the 32 rows at a time.  (Bulk copies of single rows, a lane each, run one after another
 // in some 20 instructions each: 32 of them took 2 us.)  The activations are brought into the products' order in shared
 // memory: once, where they fit there as a whole, else a segment at a time.  Places of the products' inner dimension are
 // dealt to a row's bytes so that a group stays within an MMA (four lanes hold VB bytes each: 32, 64 or 128 codes of a row).
@@ -94,6 +94,107 @@ __global__ void __launch_bounds__(256) linear_w4_any_kernel(const W4Params p) {
     }
 }
 
+__device__ __forceinline__ float w4_scale(uint32_t bits, int type) {
+    const float half = __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+    const float wide = __uint_as_float(type == Y_F32 ? bits : bits << 16);
+    return type == Y_F16 ? half : wide;
+}
+
+// One or two tokens: float multiply-adds on weights that go from memory straight to registers, as the few-token products of
+// int8 codes have it: a warp owns four weight rows (gated: two gate and two up rows), a lane 32 codes of each at a time, KS
+// warps of a block share a row's input features.  A code's byte becomes the float 2^23 + 8 + code by one byte permutation
+// and the code by half of a packed subtraction, exactly; with the packed multiply-adds of T tokens that makes 16 + 4 T
+// instructions for 8 codes, and bounds the kernel together with the launch.  Activations are exact floats here.
+constexpr int kW4FewWarps = 8, kW4FewRows = 4;
+
+template <typename XT, int MT>
+__global__ void __launch_bounds__(32 * kW4FewWarps, 1) linear_w4_few_kernel(const W4Params p, int ks) {
+    __shared__ float sums[kW4FewWarps][kW4FewRows * MT];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp & (ks - 1), set = warp / ks;
+    const int C = p.gated ? kW4FewRows / 2 : kW4FewRows;   // output features of a warp
+    const int c0 = (blockIdx.x * (kW4FewWarps / ks) + set) * C, bytes = p.k / 2;   // whole vectors of 16 (the host sees to it)
+    const int scale_shift = p.s_type == Y_F32 ? 2 : 1;
+    const uint8_t* row[kW4FewRows];
+    const char* scales[kW4FewRows];
+#pragma unroll
+    for (int r = 0; r < kW4FewRows; ++r) {   // rows past the end repeat the last one; their sums are dropped
+        const int c = min(c0 + (p.gated ? r & 1 : r), p.n - 1) + (p.gated && r > 1 ? p.n : 0);
+        row[r] = p.w + static_cast<size_t>(c) * p.ldw;
+        scales[r] = static_cast<const char*>(p.s) + (static_cast<size_t>(c) * p.lds << scale_shift);
+    }
+    const int strides = (bytes + 511) / 512, s0 = strides * part / ks, s1 = strides * (part + 1) / ks;
+    for (int s = s0; s < s1; ++s)   // into L2 while the kernel before this one drains
+        if (s * 512 + lane * 16 < bytes)
+#pragma unroll
+            for (int r = 0; r < kW4FewRows; ++r) asm volatile("prefetch.global.L2 [%0];" ::"l"(row[r] + s * 512 + lane * 16));
+    griddep_wait();
+    griddep_launch();
+    float acc[kW4FewRows][MT] = {};
+#pragma unroll 2
+    for (int s = s0; s < s1; ++s) {
+        const int byte = s * 512 + lane * 16;
+        if (byte >= bytes) break;   // (only in the row's last stride)
+        uint4 w[kW4FewRows];
+        uint32_t scale[kW4FewRows];
+        const int at = (p.shift >= 0 ? 2 * byte >> p.shift : 2 * byte / p.group) << scale_shift;
+#pragma unroll
+        for (int r = 0; r < kW4FewRows; ++r) {
+            w[r] = *reinterpret_cast<const uint4*>(row[r] + byte);
+            scale[r] = scale_shift == 2 ? *reinterpret_cast<const uint32_t*>(scales[r] + at) : *reinterpret_cast<const unsigned short*>(scales[r] + at);
+        }
+        float2 sum[kW4FewRows][MT] = {};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {   // eight codes
+            float2 x[MT][4];
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {   // missing tokens repeat the last one; their sums are dropped
+                float f[8];
+                load8<XT, true>(static_cast<const XT*>(p.x) + min(static_cast<long long>(t), p.rows - 1) * p.ldx + 2 * byte + 8 * i, f);
+#pragma unroll
+                for (int z = 0; z < 4; ++z) x[t][z] = make_float2(f[2 * z], f[2 * z + 1]);
+            }
+#pragma unroll
+            for (int r = 0; r < kW4FewRows; ++r) {
+                const uint32_t v = (&w[r].x)[i] ^ 0x88888888u, even = v & 0x0F0F0F0Fu, odd = v >> 4 & 0x0F0F0F0Fu;
+#pragma unroll
+                for (int z = 0; z < 4; ++z) {
+                    const float2 c = __fadd2_rn(make_float2(__uint_as_float(__byte_perm(even, 0x4B000000u, 0x7440 + z)), __uint_as_float(__byte_perm(odd, 0x4B000000u, 0x7440 + z))), both(-8388616.0f));
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) sum[r][t] = __ffma2_rn(c, x[t][z], sum[r][t]);
+                }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < kW4FewRows; ++r) {
+            const float f = w4_scale(scale[r], p.s_type);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) acc[r][t] = __fmaf_rn(sum[r][t].x + sum[r][t].y, f, acc[r][t]);
+        }
+    }
+    __syncwarp();
+    float mine = 0.0f;   // of row lane / MT, token lane % MT
+#pragma unroll
+    for (int r = 0; r < kW4FewRows; ++r)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            float v = acc[r][t];
+#pragma unroll
+            for (int d = 16; d; d /= 2) v += __shfl_xor_sync(0xffffffffu, v, d);
+            if (lane == r * MT + t) mine = v;
+        }
+    if (ks > 1) {
+        if (lane < kW4FewRows * MT) sums[warp][lane] = mine;
+        __syncthreads();
+        if (part == 0 && lane < kW4FewRows * MT)
+            for (int i = 1; i < ks; ++i) mine += sums[warp + i][lane];
+    }
+    const int r = lane / MT, t = lane % MT, c = c0 + (p.gated ? r & 1 : r);
+    const bool here = part == 0 && lane < kW4FewRows * MT && c < p.n && t < p.rows;
+    if (here && p.bias) mine += p.bias[c + (p.gated && r > 1 ? p.n : 0)];
+    const float up = __shfl_down_sync(0xffffffffu, mine, 2 * MT);
+    if (here && r < C) store_y(p.y, static_cast<size_t>(t) * p.ldy + c, p.gated ? swiglu(mine, up) : mine, p.y_type);
+}
+
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -109,12 +210,6 @@ template <int VB>
 struct W4Pieces {
     static constexpr int N = 16 / VB, RUN = 2 * VB;   // of a chunk, that a lane has; consecutive values of one
 };
-
-__device__ __forceinline__ float w4_scale(uint32_t bits, int type) {
-    const float half = __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
-    const float wide = __uint_as_float(type == Y_F32 ? bits : bits << 16);
-    return type == Y_F16 ? half : wide;
-}
 
 // 32 activations of a lane's token and place of a chunk, as they lie in memory; zeros without a token and behind the row's end.
 template <typename XT, int VB>
@@ -197,7 +292,7 @@ __device__ __forceinline__ void w4_fragments(uint4* to, int stride, bool kept, f
     }
 }
 
-constexpr int kW4Threads = 32 * kW4Warps, kW4MostStages = 4, kW4Smem = 224 * 1024, kW4Box = 32 * 128;   // two chunks of the 32 rows
+constexpr int kW4Threads = 32 * kW4Warps, kW4MostStages = 4, kW4Smem = 224 * 1024, kW4Run = 2, kW4Box = 32 * 64 * kW4Run;   // chunks of a stage; its bytes
 
 template <typename XT, int VB, int NT>
 struct W4Shape {
@@ -210,12 +305,14 @@ struct W4Shape {
     static constexpr int kBeside = NT * kPieces * 64;
 };
 
-struct W4Plan {   // (see the host's choice)
-    int columns;   // of a tile, that hold a token
-    int held;      // chunks whose activations shared memory holds: all, or a segment's
-    int split;     // warps of a tile: a power of two
-    int run;       // chunks of a stage
-    int stages;    // of a warp
+// What the host has worked out (quotients by numbers that are known at launch only cost a warp some hundred cycles each).
+struct W4Plan {
+    int columns;          // of a tile, that hold a token
+    int held, segments;   // chunks whose activations shared memory holds: all, or a segment's; how many segments
+    int split_log;        // 1 << split_log warps have a pair of tiles
+    int pairs, rounds;    // pairs of tiles; how many a warp has, at most
+    int stages;           // of a warp
+    int passes;           // over the tokens
 };
 
 template <typename XT, int VB, int NT>
@@ -226,98 +323,118 @@ __global__ void __launch_bounds__(kW4Threads, 1) linear_w4_kernel(const W4Params
     uint8_t* smem = smem_any + (-smem_u32(smem_any) & 1023);   // TMA's pattern of 128 bytes goes by the address
     __shared__ __align__(8) uint64_t bars[kW4Warps * kW4MostStages];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int part = warp & (plan.split - 1), slot = warp / plan.split, slots = kW4Warps / plan.split;
+    // the lane's row of eight: those of the lanes that read together lie in other banks of TMA's pattern
+    const int rg = VB == 16 ? (g >> 1) | (g & 1) << 2 : VB == 8 ? (g & 3) << 1 | g >> 2 : g;
+    const int part = warp & ((1 << plan.split_log) - 1), slot = warp >> plan.split_log, slots = kW4Warps >> plan.split_log;
     // rows g and g + 8 of a tile: of a gated product a gate and its up row, else two output features
-    const int per = p.gated ? 8 : 16, tiles = (p.n + 2 * per - 1) / (2 * per), rounds = (tiles + gridDim.x * slots - 1) / (gridDim.x * slots);
-    const int chunks = (p.k + kW4Chunk - 1) / kW4Chunk, segments = (chunks + plan.held - 1) / plan.held;
-    const int stage_bytes = plan.run / 2 * kW4Box;
-    uint8_t* ring = smem + warp * plan.stages * stage_bytes;
-    float* sums = reinterpret_cast<float*>(smem + kW4Warps * plan.stages * stage_bytes);   // [warp][2][NT][4][32]
+    const int per = p.gated ? 8 : 16, chunks = (p.k + kW4Chunk - 1) / kW4Chunk;
+    const int segments = plan.segments, rounds = plan.rounds, passes = plan.passes;
+    uint8_t* ring = smem + warp * plan.stages * kW4Box;
+    float* sums = reinterpret_cast<float*>(smem + kW4Warps * plan.stages * kW4Box);   // [warp][2][NT][4][32]
     uint4* frag = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(sums) + Sh::kSums);   // [held][NT][4][columns][4]
     float2* beside = reinterpret_cast<float2*>(frag + plan.held * NT * 16 * plan.columns);   // [held][NT][PIECES][8]
     const uint32_t full = smem_u32(bars + warp * kW4MostStages);
-    const int passes = static_cast<int>((p.rows + Sh::kTokens - 1) / Sh::kTokens);
     if (lane < plan.stages) mbar_init(full + 8 * lane, 1);
     fence_mbar_init();
     __syncwarp();
     // The pair of tiles that the warp has in a round (past the end: the last one's again; its sums are dropped), and its chunks of a segment.
     // Of a gated product rows 8 r + g and 16 + 8 r + g are tile r's gate and up row g, else rows 16 r + g and 16 r + 8 + g two features.
-    const auto pair_of = [&](int round) { return min((round * static_cast<int>(gridDim.x) + static_cast<int>(blockIdx.x)) * slots + slot, tiles - 1); };
-    const auto chunk_of = [&](int segment, int i) { const int n = min(plan.held, chunks - segment * plan.held); return segment * plan.held + n * i / plan.split; };
+    const auto pair_of = [&](int round) { return min((round * static_cast<int>(gridDim.x) + static_cast<int>(blockIdx.x)) * slots + slot, plan.pairs - 1); };
+    const auto chunk_of = [&](int segment, int i) { const int n = min(plan.held, chunks - segment * plan.held); return segment * plan.held + (n * i >> plan.split_log); };
 
-    // The warp's stages: for each pass, round and segment, its chunks, `run` at a time.  Loads go plan.stages ahead.
-    int l_pass = blockIdx.y, l_round = 0, l_segment = 0, l_chunk = chunk_of(0, part), l_end = chunk_of(0, part + 1), issued = 0, taken = 0;
-    bool lost = false;
-    const auto issue = [&]() {
-        while (l_chunk >= l_end) {   // (a part may be empty)
-            if (l_pass >= passes) return;
-            if (++l_segment == segments) {
-                l_segment = 0;
-                if (++l_round == rounds) {
-                    l_round = 0;
-                    l_pass += gridDim.y;
-                    if (l_pass >= passes) return;
+    // The warp's stages: for each pass, round and segment, its part of the chunks, two at a time.
+    struct Cursor {
+        int pass, round, segment, chunk, end;
+    };
+    const auto begin = [&]() { return Cursor{static_cast<int>(blockIdx.y), 0, 0, chunk_of(0, part), chunk_of(0, part + 1)}; };
+    const auto settle = [&](Cursor& c) {   // on to the next part that has chunks, where this one has no more; false: there is none
+        while (c.chunk >= c.end) {
+            if (c.pass >= passes) return false;
+            if (++c.segment == segments) {
+                c.segment = 0;
+                if (++c.round == rounds) {
+                    c.round = 0;
+                    c.pass += gridDim.y;
+                    if (c.pass >= passes) return false;
                 }
             }
-            l_chunk = chunk_of(l_segment, part), l_end = chunk_of(l_segment, part + 1);
+            c.chunk = chunk_of(c.segment, part), c.end = chunk_of(c.segment, part + 1);
         }
-        const int stage = issued % plan.stages, boxes = (min(plan.run, l_end - l_chunk) + 1) / 2, row = pair_of(l_round) * 2 * per;
-        const uint32_t bar = full + 8 * stage, to = smem_u32(ring) + stage * stage_bytes;
+        return true;
+    };
+    // Weights go plan.stages ahead of the products.
+    Cursor ahead = begin();
+    int issued = 0, issue_stage = 0, stage = 0, phase = 0;
+    bool lost = false;
+    const auto issue = [&]() {
+        if (!settle(ahead)) return;
+        const int row = pair_of(ahead.round) * 2 * per;
         if (elect_one()) {   // what lies outside of the weights comes as zeros, and counts
-            mbar_expect_tx(bar, boxes * kW4Box);
-            if (!(p.stall && blockIdx.x == 0 && blockIdx.y == 0 && warp == 0 && issued == 0))
-                for (int i = 0; i < boxes; ++i) {
-                    tma_load_2d(to + i * kW4Box, &map, bar, (l_chunk + 2 * i) * 64, row);
-                    if (p.gated) tma_load_2d(to + i * kW4Box + kW4Box / 2, &map, bar, (l_chunk + 2 * i) * 64, p.n + row);
-                }
+            const uint32_t bar = full + 8 * issue_stage, to = smem_u32(ring) + issue_stage * kW4Box;
+            mbar_expect_tx(bar, kW4Box);
+            if (!(p.stall && blockIdx.x == 0 && blockIdx.y == 0 && warp == 0 && issued == 0)) {
+                tma_load_2d(to, &map, bar, ahead.chunk * 64, row);
+                if (p.gated) tma_load_2d(to + kW4Box / 2, &map, bar, ahead.chunk * 64, p.n + row);
+            }
         }
         __syncwarp();
         ++issued;
-        l_chunk += plan.run;
+        if (++issue_stage == plan.stages) issue_stage = 0;
+        ahead.chunk += kW4Run;
     };
+    const int scale_shift = p.s_type == Y_F32 ? 2 : 1, scale_pitch = static_cast<int>(p.lds) << scale_shift;   // (the host keeps it an int)
     // into L2 while the kernel before this one drains: what the first stages load
     if (elect_one()) {
         const int row = pair_of(0) * 2 * per;
-        for (int c = l_chunk; c < min(l_end, l_chunk + plan.run * plan.stages); c += 2)
+        for (int c = ahead.chunk; c < min(ahead.end, ahead.chunk + kW4Run * plan.stages); c += kW4Run)
             for (int h = 0; h < (p.gated ? 2 : 1); ++h)
                 asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(&map)), "r"(c * 64), "r"(row + h * p.n) : "memory");
     }
     __syncwarp();
     griddep_wait();
     griddep_launch();
-    for (int i = 0; i < plan.stages; ++i) issue();
-    // Scales as bits, those of a stage's chunks while the one before is worked on: a conversion here would wait for the load.
-    const int scale_shift = p.s_type == Y_F32 ? 2 : 1, scale_pitch = static_cast<int>(p.lds) << scale_shift;   // (the host keeps it an int)
+    bool started = false;
     for (int pass = blockIdx.y; pass < passes; pass += gridDim.y) {
         const long long t0 = static_cast<long long>(pass) * Sh::kTokens;
         for (int round = 0; round < rounds; ++round) {
             float2 acc[2][NT][2] = {};   // [tile][..][row g or g + 8]: columns 2 t, 2 t + 1
             const char* scales[4];
 #pragma unroll
-            for (int h = 0; h < 4; ++h) {   // row g + 8 (h % 2) of tile h / 2
-                const int c = min((2 * pair_of(round) + (h >> 1)) * per + g + (p.gated ? 0 : 8 * (h & 1)), p.n - 1) + (p.gated ? (h & 1) * p.n : 0);
+            for (int h = 0; h < 4; ++h) {
+                const int c = min((2 * pair_of(round) + (h >> 1)) * per + rg + (p.gated ? 0 : 8 * (h & 1)), p.n - 1) + (p.gated ? (h & 1) * p.n : 0);
                 scales[h] = static_cast<const char*>(p.s) + static_cast<long long>(c) * scale_pitch;
             }
             for (int segment = 0; segment < segments; ++segment) {
                 if (segments > 1 || round == 0) {   // the activations of its chunks
-                    __syncthreads();                // those before are read
+                    if (round || segment || pass != static_cast<int>(blockIdx.y)) __syncthreads();   // those before are read
                     const int first = segment * plan.held, count = min(plan.held, chunks - first) * NT;
-                    for (int i = warp; i < count; i += kW4Warps) {
+                    const auto token_at = [&](int i) {
                         const long long token = t0 + i % NT * Sh::kColumns + (Sh::kSplit ? g >> 1 : g);
-                        const char* from = token < p.rows ? static_cast<const char*>(p.x) + (static_cast<size_t>(token) * p.ldx + t * W4Pieces<VB>::RUN) * sizeof(XT) : nullptr;
+                        return token < p.rows ? static_cast<const char*>(p.x) + (static_cast<size_t>(token) * p.ldx + t * W4Pieces<VB>::RUN) * sizeof(XT) : nullptr;
+                    };
+                    for (int i = warp; i < count; i += kW4Warps) {
                         uint4 x[2 * sizeof(XT)];
-                        w4_tokens<XT, VB>(x, p, from, first + i / NT, t);
+                        w4_tokens<XT, VB>(x, p, token_at(i), first + i / NT, t);
+                        if (!started) {   // (behind the first activations' loads)
+                            started = true;
+                            for (int i = 0; i < plan.stages; ++i) issue();
+                        }
                         w4_fragments<XT, VB>(frag + i * 16 * plan.columns + lane, 4 * plan.columns, g < plan.columns, beside + i * PIECES * 8, x, g, t);
+                    }
+                    if (!started) {   // a warp without a share of the activations
+                        started = true;
+                        for (int i = 0; i < plan.stages; ++i) issue();
                     }
                     __syncthreads();
                 }
                 const int end = chunk_of(segment, part + 1);
-                for (int c0 = chunk_of(segment, part); c0 < end; c0 += plan.run) {
-                    const int stage = taken % plan.stages, n = min(plan.run, end - c0);
-                    uint32_t scale[4][4];   // [chunk][row g + 8 h]
+                for (int c0 = chunk_of(segment, part); c0 < end; c0 += kW4Run) {
+                    const int n = min(kW4Run, end - c0);
+                    // Scales as bits: a conversion here would wait for the load.  [chunk][h]: row g + 8 (h % 2) of tile h / 2.  (Loaded a stage
+                    // ahead they took the registers that keep the products' operands out of local memory: 16.0 us instead of 15.8.)
+                    uint32_t scale[kW4Run][4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (j >= n) break;
+                    for (int j = 0; j < kW4Run; ++j) {
                         const int k = min((c0 + j) * kW4Chunk + min(t, PIECES - 1) * 8 * VB, p.k - 1), at = (p.shift >= 0 ? k >> p.shift : k / p.group) << scale_shift;
                         if (scale_shift == 2) {
 #pragma unroll
@@ -328,17 +445,16 @@ __global__ void __launch_bounds__(kW4Threads, 1) linear_w4_kernel(const W4Params
                         }
                     }
                     // (a warp that gives up goes on without loads, so that it meets the others at the barriers)
-                    if (!lost && !mbar_wait_warp(full + 8 * stage, (taken / plan.stages) & 1, p.wait_limit)) {
+                    if (!lost && !mbar_wait_warp(full + 8 * stage, phase, p.wait_limit)) {
                         lost = true;
                         if (lane == 0) *p.err = ERR_WAIT_FULL;
                     }
-                    ++taken;
-                    const uint8_t* tile = ring + stage * stage_bytes + g * 128;
+                    const uint8_t* tile = ring + stage * kW4Box + rg * 128;
                     // (a lane of a column that holds no token takes the last one's: what it adds to is not used)
                     const uint4* b_at = frag + (c0 - segment * plan.held) * NT * 16 * plan.columns + 4 * min(g, plan.columns - 1) + t;
                     const float2* beside_at = beside + (c0 - segment * plan.held) * NT * PIECES * 8 + 2 * t;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
+                    for (int j = 0; j < kW4Run; ++j) {
                         if (j >= n) break;
                         uint32_t weights[4][4];
 #pragma unroll
@@ -346,8 +462,8 @@ __global__ void __launch_bounds__(kW4Threads, 1) linear_w4_kernel(const W4Params
 #pragma unroll
                             for (int i = 0; i < PIECES; ++i) {
                                 // 16 bytes of a row lie at their place ^ the row's number % 8
-                                const int row = p.gated ? 16 * (h & 1) + 8 * (h >> 1) : 8 * h, at = (j & 1) * 64 + i * 4 * VB + t * VB;
-                                const uint8_t* from = tile + (j >> 1) * kW4Box + row * 128 + ((at ^ (g << 4)));
+                                const int row = p.gated ? 16 * (h & 1) + 8 * (h >> 1) : 8 * h, at = j * 64 + i * 4 * VB + t * VB;
+                                const uint8_t* from = tile + row * 128 + (at ^ (rg << 4));
                                 uint32_t* w = &weights[h][i * WORDS];
                                 if constexpr (VB == 16) {
                                     const uint4 v = *reinterpret_cast<const uint4*>(from);
@@ -397,11 +513,12 @@ __global__ void __launch_bounds__(kW4Threads, 1) linear_w4_kernel(const W4Params
                         }
                     }
                     __syncwarp();   // the stage is read
+                    if (++stage == plan.stages) stage = 0, phase ^= 1;
                     if (!lost) issue();
                 }
             }
             // The parts' sums meet in the tile's first warp, in their order.
-            if (plan.split > 1) {
+            if (plan.split_log) {
                 if (round || pass != static_cast<int>(blockIdx.y)) __syncthreads();   // those before are read
                 float2* mine = reinterpret_cast<float2*>(sums) + warp * 4 * NT * 32 + lane;
                 if (part)
@@ -409,7 +526,7 @@ __global__ void __launch_bounds__(kW4Threads, 1) linear_w4_kernel(const W4Params
                     for (int i = 0; i < 4 * NT; ++i) mine[32 * i] = acc[i / (2 * NT)][i / 2 % NT][i % 2];
                 __syncthreads();
                 if (part == 0)
-                    for (int w = 1; w < plan.split; ++w)
+                    for (int w = 1; w < 1 << plan.split_log; ++w)
 #pragma unroll
                         for (int i = 0; i < 4 * NT; ++i) {
                             float2& x = acc[i / (2 * NT)][i / 2 % NT][i % 2];
@@ -417,7 +534,7 @@ __global__ void __launch_bounds__(kW4Threads, 1) linear_w4_kernel(const W4Params
                         }
             }
             const int pair = (round * gridDim.x + blockIdx.x) * slots + slot;
-            if (part || pair >= tiles) continue;
+            if (part || pair >= plan.pairs) continue;
 #pragma unroll
             for (int r = 0; r < 2; ++r)
 #pragma unroll
@@ -431,12 +548,12 @@ __global__ void __launch_bounds__(kW4Threads, 1) linear_w4_kernel(const W4Params
                         for (int h = 0; h < 2; ++h) v[h] = Sh::kSplit ? acc[r][nt][h].x + acc[r][nt][h].y : col ? acc[r][nt][h].y : acc[r][nt][h].x;
                         const size_t row = static_cast<size_t>(token) * p.ldy;
                         if (p.gated) {
-                            const int c = (2 * pair + r) * 8 + g;
+                            const int c = (2 * pair + r) * 8 + rg;
                             if (c < p.n) store_y(p.y, row + c, swiglu(v[0] + (p.bias ? p.bias[c] : 0.0f), v[1] + (p.bias ? p.bias[p.n + c] : 0.0f)), p.y_type);
                         } else {
 #pragma unroll
                             for (int h = 0; h < 2; ++h)
-                                if (const int c = (2 * pair + r) * 16 + g + 8 * h; c < p.n) store_y(p.y, row + c, v[h] + (p.bias ? p.bias[c] : 0.0f), p.y_type);
+                                if (const int c = (2 * pair + r) * 16 + rg + 8 * h; c < p.n) store_y(p.y, row + c, v[h] + (p.bias ? p.bias[c] : 0.0f), p.y_type);
                         }
                     }
         }
