@@ -91,13 +91,14 @@ bool apart(long long tokens, long long token, int heads, long long head, int dim
 
 using CacheKernel = void (*)(CacheRowsParams);
 
-template <typename T, int D>
+template <typename T, int D, int U>
 CacheKernel rows_kernel_of(bool write, bool vec) {
-    return write ? (vec ? cache_write_kernel<T, D, true> : cache_write_kernel<T, D, false>) : (vec ? cache_read_kernel<T, D, true> : cache_read_kernel<T, D, false>);
+    return write ? (vec ? cache_write_kernel<T, D, true, U> : cache_write_kernel<T, D, false, U>) : (vec ? cache_read_kernel<T, D, true, U> : cache_read_kernel<T, D, false, U>);
 }
 template <typename T>
-CacheKernel rows_kernel_of(int dim, bool write, bool vec) {
-    return dim == 64 ? rows_kernel_of<T, 64>(write, vec) : dim == 128 ? rows_kernel_of<T, 128>(write, vec) : rows_kernel_of<T, 256>(write, vec);
+CacheKernel rows_kernel_of(int dim, bool write, bool vec, bool four) {
+    if (four) return dim == 64 ? rows_kernel_of<T, 64, 4>(write, vec) : dim == 128 ? rows_kernel_of<T, 128, 4>(write, vec) : rows_kernel_of<T, 256, 4>(write, vec);
+    return dim == 64 ? rows_kernel_of<T, 64, 1>(write, vec) : dim == 128 ? rows_kernel_of<T, 128, 1>(write, vec) : rows_kernel_of<T, 256, 1>(write, vec);
 }
 
 int rows_call(ptq8_ops* o, const ptq8_cache_rows_args* args, bool write, void* stream) {
@@ -118,12 +119,18 @@ int rows_call(ptq8_ops* o, const ptq8_cache_rows_args* args, bool write, void* s
         return fail(o, PTQ8_ERR_INVALID, "%s: k or v is not aligned to its element type", w);
     OnDevice on(o->device);
     if (on.rc != cudaSuccess) return cuda_fail(o, "cudaSetDevice", on.rc);
-    const CacheRowsParams p{view(c, a.tokens), a.k, a.v, a.k_token, a.k_head, a.v_token, a.v_head};
+    // A warp has 32 / (head_dim / 8) rows of a token at a time.  While there are few, that is all it has; then four times that,
+    // whose loads overlap (and, writing, whose lanes share the work on four rows' steps): 18 k tokens written and read back 80 us, row by row 92.
+    const long long steps = (2 * c.kv_heads * (c.head_dim / 8) + 31) / 32;
+    const bool four = steps >= 4 && a.tokens * steps > 64LL * o->sms;
+    const long long run = !four ? 1 : (steps + std::max<long long>(1, 64LL * o->sms / a.tokens) * 4 - 1) / (std::max<long long>(1, 64LL * o->sms / a.tokens) * 4) * 4;
+    const long long parts = (steps + run - 1) / run;
+    const CacheRowsParams p{view(c, a.tokens), a.k, a.v, a.k_token, a.k_head, a.v_token, a.v_head, static_cast<int>(parts), static_cast<int>(run)};
     const bool vec = vectors(a.k, a.k_token, a.k_head, a.type) && vectors(a.v, a.v_token, a.v_head, a.type);
-    const CacheKernel kernel = a.type == PTQ8_F32   ? rows_kernel_of<float>(c.head_dim, write, vec)
-                               : a.type == PTQ8_F16 ? rows_kernel_of<__half>(c.head_dim, write, vec)
-                                                    : rows_kernel_of<__nv_bfloat16>(c.head_dim, write, vec);
-    const long long per = kCacheThreads / (c.head_dim / 8), blocks = (a.tokens * 2 * c.kv_heads + per - 1) / per;
+    const CacheKernel kernel = a.type == PTQ8_F32   ? rows_kernel_of<float>(c.head_dim, write, vec, four)
+                               : a.type == PTQ8_F16 ? rows_kernel_of<__half>(c.head_dim, write, vec, four)
+                                                    : rows_kernel_of<__nv_bfloat16>(c.head_dim, write, vec, four);
+    const long long blocks = (a.tokens * parts + kCacheThreads / 32 - 1) / (kCacheThreads / 32);
     const size_t smem = c.starts ? (c.sequences + 1) * sizeof(int) : 0;
     const cudaError_t e = launch(kernel, dim3(static_cast<unsigned>(std::min<long long>(blocks, 8LL * o->sms))), dim3(kCacheThreads), smem, 1,
                                  static_cast<cudaStream_t>(stream), p);
@@ -260,8 +267,8 @@ cudaError_t cache_attributes() {
         }
     for (const int dim : {64, 128, 256})
         for (const bool write : {false, true})
-            for (const bool vec : {false, true})
-                for (const CacheKernel k : {rows_kernel_of<float>(dim, write, vec), rows_kernel_of<__half>(dim, write, vec), rows_kernel_of<__nv_bfloat16>(dim, write, vec)})
+            for (const int i : {0, 1, 2, 3})
+                for (const CacheKernel k : {rows_kernel_of<float>(dim, write, i & 1, i & 2), rows_kernel_of<__half>(dim, write, i & 1, i & 2), rows_kernel_of<__nv_bfloat16>(dim, write, i & 1, i & 2)})
                     if (const cudaError_t e = most_shared(reinterpret_cast<const void*>(k)); e != cudaSuccess) return e;
     return cudaSuccess;
 }
