@@ -4,11 +4,14 @@
     python -m ptq_int8_lab_b200.build
 
 The library is plain CUDA runtime + C++ (no torch linkage); the Python host
-side loads it with ctypes.  Output: ptq_int8_lab_b200/_lib/libptq8.so.
+side loads it with ctypes.  Output: ptq_int8_lab_b200/_lib/libptq8.so, and
+beside it ptq8_host.so, the Python extension that reads torch tensors for the
+token operators' calls (C++ against torch's headers, no CUDA).
 """
 import os
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
@@ -28,6 +31,18 @@ SOURCES = (
 )
 
 
+HOST = OUT / "ptq8_host.so"
+
+
+def host_command(out: Path) -> list:
+    import torch
+    root = Path(torch.__file__).resolve().parent
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-I", str(HERE.parent / "include"),
+            "-I", sysconfig.get_paths()["include"], "-I", str(root / "include"), "-I", str(root / "include/torch/csrc/api/include"),
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", str(SRC / "ptq8_host.cpp"), "-o", str(out),
+            "-L", str(root / "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"]
+
+
 def build(verbose_ptxas: bool = False) -> Path:
     OUT.mkdir(exist_ok=True)
     lib = OUT / "libptq8.so"
@@ -39,6 +54,9 @@ def build(verbose_ptxas: bool = False) -> Path:
         print(" ".join(cmd), flush=True)
         objs.append(OUT / obj)
         running.append((cmd, subprocess.Popen(cmd)))
+    cmd = host_command(OUT / "ptq8_host.so.tmp")
+    print(" ".join(cmd), flush=True)
+    running.append((cmd, subprocess.Popen(cmd)))
     failed = [cmd for cmd, p in running if p.wait() != 0]
     if failed:
         raise subprocess.CalledProcessError(1, failed[0])
@@ -47,6 +65,7 @@ def build(verbose_ptxas: bool = False) -> Path:
     print(" ".join(cmd), flush=True)
     subprocess.check_call(cmd)
     os.replace(tmp, lib)
+    os.replace(OUT / "ptq8_host.so.tmp", HOST)
     for o in objs:
         o.unlink()
     return lib

@@ -16,6 +16,7 @@ never require one, also where an input does.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import struct
 from typing import NamedTuple, Optional, Tuple
 
@@ -39,6 +40,26 @@ try:
 except AttributeError:   # a torch without CUDA
     def _raw_stream(device: int) -> int:
         return torch.cuda.current_stream(device).cuda_stream
+
+
+_host = None
+
+
+def _host_module():
+    """ptq8_host: the calls of the newer operators without the interpreter's share (built beside libptq8.so)."""
+    global _host
+    if _host is None:
+        from .build import HOST
+        if not HOST.exists():
+            raise Ptq8Error(f"{HOST} not found: build it with `python -m ptq_int8_lab_b200.build`")
+        spec = importlib.util.spec_from_file_location("ptq8_host", HOST)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        L = lib()
+        module.entries(*(ctypes.cast(f, ctypes.c_void_p).value for f in
+                         (L.ptq8_cache_write, L.ptq8_cache_read, L.ptq8_cache_attention, L.ptq8_cache_attention_workspace, L.ptq8_linear_w4)))
+        _host = module
+    return _host
 
 
 # Calls check their tensors with inline conditions; where one fails, these say what is wrong (or return:
@@ -169,6 +190,8 @@ class Int8Ops:
         self._attention_args = ctypes.create_string_buffer(_ATTENTION.size)
         self._linear_w4, self._cache_write, self._cache_read = self._lib.ptq8_linear_w4, self._lib.ptq8_cache_write, self._lib.ptq8_cache_read
         self._cache_attention = self._lib.ptq8_cache_attention
+        host = _host_module()
+        self._host_rows, self._host_attention, self._host_w4 = host.cache_rows, host.cache_attention, host.linear_w4
         self._workspaces = {}   # bytes, by the sizes of a call
 
     def _check(self, rc: int):
@@ -322,6 +345,13 @@ class Int8Ops:
         ceil(in / group)] (f32 / f16 / bf16).  act EPI_SWIGLU: channels = 2 * out, gate then up.  dtype: of y where out is not given
         (None: x's).  For generation: one to some tens of tokens."""
         d = self.device
+        if out is not None and stream is None:
+            rc = self._host_w4(self._h, d, x, w, w_scale, group, bias, act, out, _raw_stream(d))
+            if rc == 0:
+                return out
+            if rc > 0:
+                self._check(rc)
+        # (out of the ordinary: one look after another, and what is wrong is said)
         if act != EPI_NONE and act != EPI_SWIGLU:
             raise Ptq8Error(f"act {act}: EPI_NONE or EPI_SWIGLU")
         if not 0 < group <= 0x7FFFFFFF:
@@ -440,6 +470,12 @@ class Int8Ops:
         table int32 [sequences, n]: the pages of each sequence; lengths int32 [sequences]: its positions, the new tokens (its
         last ones) among them; starts int32 [sequences + 1]: sequence b's new tokens are starts[b] .. starts[b + 1] - 1, without
         it token b alone.  Positions without a page are skipped.  A page that is written belongs to one sequence."""
+        if stream is None:
+            rc = self._host_rows(True, self._h, self.device, cache, k, v, table, lengths, starts, _raw_stream(self.device))
+            if rc == 0:
+                return
+            if rc > 0:
+                self._check(rc)
         self._cache_rows(self._cache_write, cache, k, v, table, lengths, starts, self._stream(stream, True))
 
     def cache_read(self, cache: Cache4, table: torch.Tensor, lengths: torch.Tensor, starts: Optional[torch.Tensor] = None,
@@ -447,6 +483,13 @@ class Int8Ops:
         """(k, v) [T, kv_heads, head_dim] that the cache holds at the positions where cache_write with the same arguments
         writes; zeros where a position has no page.  With starts and without out, tokens is T.  Rows of no sequence are not
         written."""
+        if out is not None and stream is None:
+            k, v = out
+            rc = self._host_rows(False, self._h, self.device, cache, k, v, table, lengths, starts, _raw_stream(self.device))
+            if rc == 0:
+                return k, v
+            if rc > 0:
+                self._check(rc)
         stream = self._stream(stream, out is not None)
         if out is None:
             if dtype not in _TYPES:
@@ -472,9 +515,16 @@ class Int8Ops:
         workspace: uint8, cache_attention_workspace() bytes; one is made where it is not given, which with stream it has to be."""
         if stream is not None and (out is None or workspace is None):
             raise Ptq8Error("with stream, out and workspace are wanted too: tensors made here would belong to the current stream")
-        stream = self._stream(stream, True)
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        if stream is None and workspace is None:
+            rc = self._host_attention(self._h, self.device, q, cache, table, lengths, starts, q.shape[-1] ** -0.5 if scale is None else scale, out,
+                                      _raw_stream(self.device))
+            if rc == 0:
+                return out
+            if rc > 0:
+                self._check(rc)
+        stream = self._stream(stream, True)
         need = self._attention(q, cache, table, lengths, starts, scale, out)
         if workspace is None:
             at, size = 0, 0
