@@ -5,10 +5,14 @@
 // Five instructions widen eight codes; the powers of two, the steps and the least values go into the numbers around
 // the products:
 //   q . key    = step_k (q . codes) + least_k sum(q)                          queries as f16 times a power of two
-//   sum p v    = sum (p step_v) codes + sum p least_v                         p step_v as f16, over a bound of step_v
+//   sum p v    = sum (p step_v) (codes - 8) + sum p (least_v + 8 step_v)      p step_v as f16, over a bound of step_v
 // A query is scaled by the power of two that takes its largest value to 2^14 .. 2^15: f16 has three bits more than
 // bf16, and what is more than 2^28 below the largest loses places only then.  p step_v is rounded to f16's 11 bits (an
 // output has 11, or bf16's 8), with 2^-24 of the largest as its finest step; everything else is f32.
+// The values' codes enter as normal numbers, code - 8, and least + 8 step as their middle, for an instruction more for two of them: terms that do
+// not all have one sign lose less to p's rounding, and the tensor cores, which line the products of a sum up by their operands'
+// exponents and cut what is below, take a subnormal number's exponent for 2^-14.  (131072 f16 tokens, which average to 0.4 % of
+// a value: 7.5e-4 from 64 bits with codes as for the keys, 2.7e-4 like this; the output's own rounding is 2.1e-4.)
 //
 // A warp takes 16 tokens as the rows of its products, 8 NT query rows (query token x head of a key's group) as
 // the columns: keys codes [16 tokens x D] x queries [D x rows], then values codes [D x 16 tokens] x p [16 tokens x rows].
@@ -122,7 +126,7 @@ template <int D, int NT>
 struct AttRows {
     const uint4* q;               // fragments [NT][D / 32][32 lanes]: of a word of keys, those of its codes 0, 4; 1, 5; 2, 6; 3, 7
     float2 a[NT], b[NT];          // score in powers of two = a * (step (q . codes) + least b)
-    float2 m[NT], l[NT], lo[NT];  // reference, sum of p, sum of p least_v
+    float2 m[NT], l[NT], lo[NT];  // reference, sum of p, sum of p (least_v + 8 step_v)
     int lim[NT][2];               // positions that the row sees
     float o[D / 16][NT][4];
     float c;                             // what p step_v is multiplied by: a power of two
@@ -213,6 +217,18 @@ __device__ __forceinline__ void att_queries(const AttParams& p, AttRows<D, NT>& 
 }
 
 constexpr uint32_t kLow = 0x000F000Fu, kHigh = 0x00F000F0u;
+
+// Codes less eight (16 times that for the high one of a byte) as normal f16 numbers: 1024 + code, less 1032.
+__device__ __forceinline__ uint32_t centred_low(uint32_t word) {
+    const uint32_t a = mask_or(word, kLow, 0x64006400u), b = 0x64086408u;
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t centred_high(uint32_t word) {
+    const uint32_t a = mask_or(word, kHigh, 0x64006400u), b = 0x64806480u;
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
 
 // 16 H tokens, as H products: tk is the first one's place in the tile, pos its position.  MASKED: some row does not see
 // all of them, or not all are there: those before position `seen`, where bit i of `pieces` is set for piece i of the tile
@@ -320,7 +336,7 @@ __device__ __forceinline__ void att_step(AttRows<D, NT>& r, const uint8_t* K, co
     for (int h = 0; h < H; ++h)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const float2 vs = both(vstep[h][i] * r.c), least = both(__uint_as_float(pv[h][i] & 0xFFFF0000u));
+            const float2 vs = both(vstep[h][i] * r.c), middle = both(__fmaf_rn(8.0f, vstep[h][i], __uint_as_float(pv[h][i] & 0xFFFF0000u)));
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 const float2 v = make_float2(x[h][nt][2 * i], x[h][nt][2 * i + 1]);
@@ -329,10 +345,10 @@ __device__ __forceinline__ void att_step(AttRows<D, NT>& r, const uint8_t* K, co
                 if constexpr (MASKED) {   // step and least of a key that the row does not see may be NaN, and so may a
                     const bool x_in = v.x != -INFINITY, y_in = v.y != -INFINITY;
                     e = make_float2(x_in ? e.x : 0.0f, y_in ? e.y : 0.0f);
-                    r.lo[nt] = make_float2(x_in ? __fmaf_rn(e.x, least.x, r.lo[nt].x) : r.lo[nt].x, y_in ? __fmaf_rn(e.y, least.y, r.lo[nt].y) : r.lo[nt].y);
+                    r.lo[nt] = make_float2(x_in ? __fmaf_rn(e.x, middle.x, r.lo[nt].x) : r.lo[nt].x, y_in ? __fmaf_rn(e.y, middle.y, r.lo[nt].y) : r.lo[nt].y);
                     w = make_float2(x_in ? e.x * vs.x : 0.0f, y_in ? e.y * vs.y : 0.0f);
                 } else {
-                    r.lo[nt] = __ffma2_rn(e, least, r.lo[nt]);
+                    r.lo[nt] = __ffma2_rn(e, middle, r.lo[nt]);
                     w = __fmul2_rn(e, vs);
                 }
                 r.l[nt] = __fadd2_rn(r.l[nt], e);
@@ -357,9 +373,9 @@ __device__ __forceinline__ void att_step(AttRows<D, NT>& r, const uint8_t* K, co
 #pragma unroll
                 for (int z = 0; z < 2; ++z) {
                     const uint32_t us = z ? u >> 8 : u, vs = z ? v >> 8 : v;
+                    const uint32_t a0 = centred_low(us), a1 = centred_high(us), a2 = centred_low(vs), a3 = centred_high(vs);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-                        mma_16816(r.o[4 * w + 2 * half + z][nt], us & kLow, us & kHigh, vs & kLow, vs & kHigh, pb[nt][2 * h], pb[nt][2 * h + 1]);
+                    for (int nt = 0; nt < NT; ++nt) mma_16816(r.o[4 * w + 2 * half + z][nt], a0, a1, a2, a3, pb[nt][2 * h], pb[nt][2 * h + 1]);
                 }
             }
     }
@@ -623,8 +639,8 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT, RW>::kPerSm) cach
 #pragma unroll
                 for (int mt = 0; mt < D / 16; mt += 2)
                     *reinterpret_cast<float4*>(to + 2 * mt) =
-                        make_float4(__fmaf_rn(r.o[mt][nt][i] * 0x1p24f, inv, lo[i]), __fmaf_rn(r.o[mt][nt][2 + i] * 0x1p20f, inv, lo[i]),
-                                    __fmaf_rn(r.o[mt + 1][nt][i] * 0x1p24f, inv, lo[i]), __fmaf_rn(r.o[mt + 1][nt][2 + i] * 0x1p20f, inv, lo[i]));
+                        make_float4(__fmaf_rn(r.o[mt][nt][i], inv, lo[i]), __fmaf_rn(r.o[mt][nt][2 + i] * 0.0625f, inv, lo[i]),
+                                    __fmaf_rn(r.o[mt + 1][nt][i], inv, lo[i]), __fmaf_rn(r.o[mt + 1][nt][2 + i] * 0.0625f, inv, lo[i]));
             }
         }
         named_bar_sync(1, 32 * kAttWarps);

@@ -133,6 +133,13 @@ __device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
     }
 }
 
+// (word & mask) | ones, one instruction.
+__device__ __forceinline__ uint32_t mask_or(uint32_t word, uint32_t mask, uint32_t ones) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(word), "r"(mask), "r"(ones));
+    return r;
+}
+
 // NaN if either is (fminf and fmaxf would drop it).
 __device__ __forceinline__ float min_nan(float a, float b) {
     float r;

@@ -41,6 +41,7 @@ int check_w4(ptq8_ops* o, const ptq8_linear_w4_args& a) {
 struct W4Variant {
     int type, vb, nt;   // of the activations; bytes that a lane takes at once; tiles of eight columns
     void (*kernel)(W4Params, W4Plan, const CUtensorMap);
+    void (*exact)(W4Params, W4Plan, const CUtensorMap);   // for outputs of 32 bits
     int sums, beside;
     int (*frag)(int columns);
 };
@@ -48,7 +49,7 @@ struct W4Variant {
 template <typename XT, int TYPE, int VB, int NT>
 W4Variant w4_variant() {
     using Sh = W4Shape<XT, VB, NT>;
-    return {TYPE, VB, NT, linear_w4_kernel<XT, VB, NT>, Sh::kSums, Sh::kBeside, Sh::frag};
+    return {TYPE, VB, NT, linear_w4_kernel<XT, VB, NT, false>, linear_w4_kernel<XT, VB, NT, true>, Sh::kSums, Sh::kBeside, Sh::frag};
 }
 
 #define W4_TILES(XT, TYPE, VB) w4_variant<XT, TYPE, VB, 1>(), w4_variant<XT, TYPE, VB, 2>(), w4_variant<XT, TYPE, VB, 4>()
@@ -139,7 +140,7 @@ int run_w4(ptq8_ops* o, const ptq8_linear_w4_args& a, cudaStream_t st) {
         const CUresult r = o->encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(a.w), dims, pitch, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
         if (r != CUDA_SUCCESS) return fail(o, PTQ8_ERR_CUDA, "linear_w4: cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
-        e = launch(v->kernel, dim3(static_cast<unsigned>(x), static_cast<unsigned>(y)), dim3(kW4Threads), smem, 1, st, p, plan, map);
+        e = launch(a.y_type == PTQ8_F32 ? v->exact : v->kernel, dim3(static_cast<unsigned>(x), static_cast<unsigned>(y)), dim3(kW4Threads), smem, 1, st, p, plan, map);
     } else {
         const long long blocks = (a.rows + kW4AnyTokens - 1) / kW4AnyTokens;
         e = launch(linear_w4_any_kernel, dim3((a.out_features + 7) / 8, static_cast<unsigned>(std::min<long long>(blocks, 65535))), dim3(256), 0, 1, st, p);
@@ -152,10 +153,11 @@ int run_w4(ptq8_ops* o, const ptq8_linear_w4_args& a, cudaStream_t st) {
 namespace ptq8 {
 
 cudaError_t w4_attributes() {
-    for (const W4Variant& v : kW4Variants) {
-        const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(v.kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, kW4Smem);
-        if (e != cudaSuccess) return e;
-    }
+    for (const W4Variant& v : kW4Variants)
+        for (const auto kernel : {v.kernel, v.exact}) {
+            const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, kW4Smem);
+            if (e != cudaSuccess) return e;
+        }
     return cudaSuccess;
 }
 

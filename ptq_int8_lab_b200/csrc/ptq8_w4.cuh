@@ -203,6 +203,17 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
 
 // With every code's sign bit turned a nibble is code + 8: as f16 that times 2^-24 (times 2^-20 for the high one of a byte).
 constexpr uint32_t kW4Turn = 0x88888888u, kW4Low = 0x000F000Fu, kW4High = 0x00F000F0u;
+// The code itself (16 times it for the high one) as a normal number: 1024 + 8 + code, less 1032.
+__device__ __forceinline__ uint32_t w4_low(uint32_t word) {
+    const uint32_t a = mask_or(word, kW4Low, 0x64006400u), b = 0x64086408u;
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t w4_high(uint32_t word) {
+    const uint32_t a = mask_or(word, kW4High, 0x64006400u), b = 0x64806480u;
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
 // -8 * 2^-24 and -128 * 2^-24
 constexpr uint32_t kW4ShiftLow = 0x80088008u, kW4ShiftHigh = 0x80808080u;
 
@@ -247,7 +258,7 @@ __device__ __forceinline__ float w4_value(const uint32_t* raw, int i) {
 // They become f16, four to a word of weights (codes 0, 4; 1, 5, which come 16 times too large; 2, 6; 3, 7), times a power of two, at
 // to[stride w].  f32: the lanes of even columns take the first f16 of a number, those of odd ones what it leaves.  Beside
 // them, for each piece and column, -8 times its sum and the power of two that products with code * 2^-24 lack.
-template <typename XT, int VB>
+template <typename XT, int VB, bool EXACT>
 __device__ __forceinline__ void w4_fragments(uint4* to, int stride, bool kept, float2* beside, const uint4 (&x)[2 * sizeof(XT)], int g, int t) {
     const uint32_t* raw = reinterpret_cast<const uint32_t*>(x);
     float top;
@@ -266,7 +277,7 @@ __device__ __forceinline__ void w4_fragments(uint4* to, int stride, bool kept, f
     const int e = min(max(14 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), -100), 100);
     const float up = __int_as_float((e + 127) << 23), up16 = up * 0.0625f;
     // a token that is not finite: NaN (as an infinity times a code of zero is)
-    const float l = isfinite(top) ? __int_as_float((24 - e + 127) << 23) : __int_as_float(0x7FC00000);
+    const float l = isfinite(top) ? __int_as_float(((EXACT ? 0 : 24) - e + 127) << 23) : __int_as_float(0x7FC00000);
     const float lack0 = __shfl_sync(0xffffffffu, l, 8 * t), lack1 = __shfl_sync(0xffffffffu, l, 8 * t + 4);
 #pragma unroll
     for (int j = 0; j < 16 / VB; ++j) {
@@ -284,8 +295,10 @@ __device__ __forceinline__ void w4_fragments(uint4* to, int stride, bool kept, f
                     if (g & 1) b[z] = left;
                 }
             }
-            mma_f16(shift, kW4ShiftLow, kW4ShiftLow, kW4ShiftHigh, kW4ShiftHigh, b[0], b[1]);
-            mma_f16(shift, kW4ShiftLow, kW4ShiftLow, kW4ShiftHigh, kW4ShiftHigh, b[2], b[3]);
+            if constexpr (!EXACT) {
+                mma_f16(shift, kW4ShiftLow, kW4ShiftLow, kW4ShiftHigh, kW4ShiftHigh, b[0], b[1]);
+                mma_f16(shift, kW4ShiftLow, kW4ShiftLow, kW4ShiftHigh, kW4ShiftHigh, b[2], b[3]);
+            }
             if (kept) to[stride * w] = make_uint4(b[0], b[1], b[2], b[3]);
         }
         if (g == 0) *reinterpret_cast<float4*>(beside + j * 8 + 2 * t) = make_float4(shift[0], lack0, shift[1], lack1);
@@ -315,7 +328,11 @@ struct W4Plan {
     int passes;           // over the tokens
 };
 
-template <typename XT, int VB, int NT>
+// EXACT (outputs of 32 bits): the tensor cores line the products of a sum up by their operands' exponents and cut what is
+// below, and the exponent of a subnormal number is 2^-14 whatever it is.  So codes enter as normal numbers there, for an
+// instruction more for two of them, and each product of 16 features begins at zero and is added in f32 (45 f32 tokens
+// 2000 -> 1270: 2.2e-6 from 64 bits without, 8.6e-8 with).
+template <typename XT, int VB, int NT, bool EXACT>
 __global__ void __launch_bounds__(kW4Threads, 1) linear_w4_kernel(const W4Params p, const W4Plan plan, const __grid_constant__ CUtensorMap map) {
     using Sh = W4Shape<XT, VB, NT>;
     constexpr int PIECES = Sh::kPieces, WORDS = VB / 4;
@@ -419,7 +436,7 @@ __global__ void __launch_bounds__(kW4Threads, 1) linear_w4_kernel(const W4Params
                             started = true;
                             for (int i = 0; i < plan.stages; ++i) issue();
                         }
-                        w4_fragments<XT, VB>(frag + i * 16 * plan.columns + lane, 4 * plan.columns, g < plan.columns, beside + i * PIECES * 8, x, g, t);
+                        w4_fragments<XT, VB, EXACT>(frag + i * 16 * plan.columns + lane, 4 * plan.columns, g < plan.columns, beside + i * PIECES * 8, x, g, t);
                     }
                     if (!started) {   // a warp without a share of the activations
                         started = true;
@@ -496,8 +513,16 @@ __global__ void __launch_bounds__(kW4Threads, 1) linear_w4_kernel(const W4Params
                                     const uint32_t u = weights[2 * r][w] ^ kW4Turn, v = weights[2 * r + 1][w] ^ kW4Turn, u8 = u >> 8, v8 = v >> 8;
 #pragma unroll
                                     for (int nt = 0; nt < NT; ++nt) {
-                                        mma_f16(sum[r][nt], u & kW4Low, v & kW4Low, u & kW4High, v & kW4High, b[nt].x, b[nt].y);
-                                        mma_f16(sum[r][nt], u8 & kW4Low, v8 & kW4Low, u8 & kW4High, v8 & kW4High, b[nt].z, b[nt].w);
+                                        if constexpr (EXACT) {
+                                            float one[4] = {}, two[4] = {};
+                                            mma_f16(one, w4_low(u), w4_low(v), w4_high(u), w4_high(v), b[nt].x, b[nt].y);
+                                            mma_f16(two, w4_low(u8), w4_low(v8), w4_high(u8), w4_high(v8), b[nt].z, b[nt].w);
+#pragma unroll
+                                            for (int z = 0; z < 4; ++z) sum[r][nt][z] += one[z] + two[z];
+                                        } else {
+                                            mma_f16(sum[r][nt], u & kW4Low, v & kW4Low, u & kW4High, v & kW4High, b[nt].x, b[nt].y);
+                                            mma_f16(sum[r][nt], u8 & kW4Low, v8 & kW4Low, u8 & kW4High, v8 & kW4High, b[nt].z, b[nt].w);
+                                        }
                                     }
                                 }
                             }
