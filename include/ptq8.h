@@ -319,7 +319,7 @@ const char* ptq8_ops_last_error(const ptq8_ops* ops);
  * Until it is cleared here, every further call on the handle returns PTQ8_ERR_TIMEOUT too. */
 int ptq8_ops_check_device_error(ptq8_ops* ops, void* stream);
 /* Failure-detection test hook: wait limit in clock cycles (0: the default, about 2 s), and a switch that makes
- * the tensor-core product announce the first operand load of its first block without issuing it. */
+ * a kernel with such waits (tensor-core products, cache_attention) announce its first operand load without issuing it. */
 int ptq8_ops_set_wait_test(ptq8_ops* ops, long long wait_limit_cycles, int stall_first_load);
 
 /* int8 codes with one scale per row (token):

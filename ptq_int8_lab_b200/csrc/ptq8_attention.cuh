@@ -541,7 +541,7 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT, RW>::kPerSm) cach
                             mbar_arrive(full + 8 * stage);
                     }
                     __syncwarp();
-                    if (lane / pieces == i && page >= 0 && !(p.stall && cta == 0 && issued == 0)) {
+                    if (lane / pieces == i && page >= 0 && !(p.stall && it.base == 0 && mine == 0)) {   // (stall: the first tile of all)
                         const int at = lane % pieces << shift;                         // in the tile
                         const long long in = pos & (p.c.page - 1);                    // in the page
                         const uint32_t dst = ring + stage * Sh::kStage, bar = full + 8 * stage;

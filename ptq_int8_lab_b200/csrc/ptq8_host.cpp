@@ -8,6 +8,7 @@
 #include <ATen/ATen.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
 #include <cstdint>
 
 #include "ptq8.h"
@@ -92,6 +93,7 @@ PyObject* answer(int rc) { return PyLong_FromLong(rc); }
 // cache_rows(write, handle, device, cache, k, v, table, lengths, starts, stream)
 PyObject* cache_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (n != 10) return answer(-1);
+    if (a[1] == Py_None) return answer(-1);   // a closed handle
     const bool write = a[0] == Py_True;
     const int64_t device = PyLong_AsLongLong(a[2]);
     const at::Tensor *k = tensor(a[4]), *v = tensor(a[5]);
@@ -115,6 +117,7 @@ PyObject* cache_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // cache_attention(handle, device, q, cache, table, lengths, starts, scale, out, stream), its workspace made here
 PyObject* cache_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (n != 10) return answer(-1);
+    if (a[0] == Py_None) return answer(-1);   // a closed handle
     const int64_t device = PyLong_AsLongLong(a[1]);
     const at::Tensor *q = tensor(a[2]), *out = tensor(a[8]);
     if (!q || !out || q->dim() != 3 || out->sizes() != q->sizes() || out->scalar_type() != q->scalar_type() || !on(*q, device) || !on(*out, device)) return answer(-1);
@@ -128,7 +131,7 @@ PyObject* cache_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     args.q_token = q->stride(0), args.q_head = q->stride(1), args.out_token = out->stride(0), args.out_head = out->stride(1);
     args.tokens = q->size(0);
     args.heads = static_cast<int>(q->size(1));
-    args.scale = static_cast<float>(PyFloat_AsDouble(a[7]));
+    args.scale = static_cast<float>(a[7] == Py_None ? std::pow(static_cast<double>(args.cache.head_dim), -0.5) : PyFloat_AsDouble(a[7]));
     auto* ops = static_cast<ptq8_ops*>(PyLong_AsVoidPtr(a[0]));
     void* stream = PyLong_AsVoidPtr(a[9]);
     if (PyErr_Occurred()) return nullptr;
@@ -150,6 +153,7 @@ PyObject* cache_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // linear_w4(handle, device, x, w, w_scale, group, bias, act, out, stream)
 PyObject* linear_w4(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (n != 10) return answer(-1);
+    if (a[0] == Py_None) return answer(-1);   // a closed handle
     const int64_t device = PyLong_AsLongLong(a[1]), group = PyLong_AsLongLong(a[5]), act = PyLong_AsLongLong(a[7]);
     if (PyErr_Occurred()) {   // no whole numbers
         PyErr_Clear();

@@ -1,10 +1,11 @@
 # -*- coding: utf-8 -*-
 """Quantized SwiGLU MLPs on the token operators: one weight pair for every token, or experts.
 
-    python -m ptq_int8_lab_b200.mlp [--tokens 16] [--hidden 1024] [--width 2048] [--experts 8] [--top 2] [--bits 8]
+    python -m ptq_int8_lab_b200.mlp [--tokens 16] [--hidden 1024] [--width 2048] [--experts 8] [--top 2] [--bits 8] [--group 64]
 
 builds a dense MLP and one with experts from random weights, runs both on random hidden
-states and prints how far they are from the same MLPs in float.
+states and prints how far they are from the same MLPs in float; and, with --group, the dense one with 4-bit weights
+that have a scale per group of input features and float activations.
 
 Weights are quantized on the host with the engine's own quantizer (one scale per output
 channel, int8 or int4) and laid out once; activations are quantized per token on the way.
@@ -39,6 +40,42 @@ def lay_weights(w, bits: int = 8, device: int = 0) -> Tuple[torch.Tensor, torch.
     laid[:, :rows.shape[1]] = torch.from_numpy(np.ascontiguousarray(rows)).to(laid.device)
     laid = laid.view(*w.shape[:-1], pitch)[..., :rows.shape[1]]
     return laid, torch.from_numpy(scale).view(*w.shape[:-1]).to(laid.device)
+
+
+def lay_groups(w, group: int, device: int = 0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(codes, scale) on the device of float weights [channels, in]: int4 codes two per byte [channels, (in + 1) // 2], rows at
+    multiples of 16 bytes, and a scale per `group` consecutive input features, f32 [channels, ceil(in / group)]."""
+    w = np.asarray(w, dtype=np.float32)
+    if w.ndim != 2:
+        raise E.Ptq8Error(f"weights of shape {w.shape}: [channels, in] is wanted")
+    if group <= 0:
+        raise E.Ptq8Error(f"group {group}")
+    channels, inp = w.shape
+    groups = -(-inp // group)
+    padded = np.zeros((channels, groups * group), dtype=np.float32)
+    padded[:, :inp] = w
+    codes, scale = E.quantize_weight(padded.reshape(channels * groups, group), 4)   # (a row of the quantizer's is a group)
+    rows = pack_w4(np.ascontiguousarray(codes.reshape(channels, groups * group)[:, :inp]))
+    pitch = (rows.shape[1] + 15) // 16 * 16
+    laid = torch.zeros((channels, pitch), dtype=torch.uint8, device=f"cuda:{device}")
+    laid[:, :rows.shape[1]] = torch.from_numpy(np.ascontiguousarray(rows)).to(laid.device)
+    return laid[:, :rows.shape[1]], torch.from_numpy(scale.reshape(channels, groups)).to(laid.device)
+
+
+class Int4MLP:
+    """y = (silu(x Wg^T) * (x Wu^T)) Wd^T with float activations and 4-bit weights in groups: two launches.
+
+    gate_up [2 * width, hidden] (gate rows, then up rows), down [hidden, width], float."""
+
+    def __init__(self, gate_up, down, group: int = 128, device: int = 0, ops: Optional[Int8Ops] = None):
+        self.ops = ops or Int8Ops(device)
+        self.group = group
+        self.gate_up = lay_groups(gate_up, group, self.ops.device)
+        self.down = lay_groups(down, group, self.ops.device)
+
+    def __call__(self, x: torch.Tensor) -> torch.Tensor:
+        h = self.ops.linear_w4(x, *self.gate_up, self.group, act=EPI_SWIGLU)
+        return self.ops.linear_w4(h, *self.down, self.group)
 
 
 class Int8MLP:
@@ -102,10 +139,10 @@ def _float_mlp(x, gate_up, down):
     return (torch.nn.functional.silu(g) * u) @ down.t()
 
 
-def main(argv=None) -> Tuple[float, float]:
-    """Runs both; returns the relative differences from float (dense, experts)."""
+def main(argv=None) -> Tuple[float, ...]:
+    """Runs them; returns the relative differences from float (dense, experts, with --group that of grouped 4-bit weights)."""
     ap = argparse.ArgumentParser(description="Dense and expert MLPs with int8 activations, against float.")
-    for name, value in (("tokens", 16), ("hidden", 1024), ("width", 2048), ("experts", 8), ("top", 2), ("bits", 8), ("seed", 0)):
+    for name, value in (("tokens", 16), ("hidden", 1024), ("width", 2048), ("experts", 8), ("top", 2), ("bits", 8), ("group", 0), ("seed", 0)):
         ap.add_argument("--" + name, type=int, default=value)
     a = ap.parse_args(argv)
     rng = np.random.default_rng(a.seed)
@@ -129,7 +166,12 @@ def main(argv=None) -> Tuple[float, float]:
     ops.check_device_error()
     experts = float((got - want).norm() / want.norm())
     print(f"experts: top {a.top} of {a.experts}: relative difference from float {experts:.4f}")
-    return dense, experts
+    if not a.group:
+        return dense, experts
+    want = _float_mlp(x, f1[0], f2[0])
+    grouped = float((Int4MLP(w1[0], w2[0], a.group, ops=ops)(x) - want).norm() / want.norm())
+    print(f"dense, 4-bit weights with a scale per {a.group} input features, float activations: relative difference from float {grouped:.4f}")
+    return dense, experts, grouped
 
 
 if __name__ == "__main__":

@@ -8,6 +8,13 @@ token, int8 or packed int4 weights with one scale per output channel, exact int3
   ``linear``          product with one weight matrix, optional bias and SwiGLU
   ``linear_grouped``  the same with rows grouped by expert, each with its own weights
 
+And generation with 4 bits, activations kept as floats:
+
+  ``linear_w4``       product with 4-bit weights that have a scale per group of input features
+  ``cache_write``     keys and values of new tokens into a paged cache of 4-bit codes (``Cache4``, ``new_cache``)
+  ``cache_read``      the floats that stand there
+  ``cache_attention`` attention over it, causal, from one new token per sequence to pieces of prompts
+
 Calls enqueue on the current torch stream (or the one given) and return; nothing
 synchronises or allocates except outputs that the caller does not pass.  What is refused
 raises ``Ptq8Error``; tensors on the CPU are refused too.  There are no gradients: outputs
@@ -518,8 +525,7 @@ class Int8Ops:
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         if stream is None and workspace is None:
-            rc = self._host_attention(self._h, self.device, q, cache, table, lengths, starts, q.shape[-1] ** -0.5 if scale is None else scale, out,
-                                      _raw_stream(self.device))
+            rc = self._host_attention(self._h, self.device, q, cache, table, lengths, starts, scale, out, _raw_stream(self.device))
             if rc == 0:
                 return out
             if rc > 0:
