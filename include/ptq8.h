@@ -397,8 +397,8 @@ int ptq8_ops_set_choice_test(ptq8_ops* ops, int variant, int split);
 /* y[t][c] = sum_g w_scale[c][g] * (sum_{k in group g} code[c][k] * x[t][k]) + bias[c], then the epilogue, then one rounding to
  * y's type: float activations, 4-bit weights with a scale per `group` consecutive input features (the last group may be
  * shorter).  Codes lie as ptq8_linear's do with w_bits 4.  Sums are f32; f16 and bf16 activations are not rounded (what is less than
- * 2^-28 of the largest among 128 beside it may lose places), f32 ones keep 22 places.  A token that holds NaN or an infinity
- * gives NaN.
+ * 2^-28 of the largest among 128 beside it may lose places), f32 ones keep 22 places.  Outputs of a
+ * token that holds NaN or an infinity are NaN or infinite.
  * Groups of a multiple of 32 features (or of all) with weights and pitches at multiples of 16 bytes run on the tensor cores;
  * any other group and layout on a slower kernel. */
 typedef struct {

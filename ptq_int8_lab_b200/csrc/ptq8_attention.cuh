@@ -39,6 +39,8 @@ constexpr float kAttNone = -1e30f;   // reference of a row that has seen nothing
 constexpr float kAttSlack = 8.0f;
 // What a row tile costs beside its tokens (queries in, numerators joined and out), in units.
 constexpr int kAttOver = 2;
+// Units at most, which the host sees to; starts that decrease (their tokens count for several sequences) are held to it on the device.
+constexpr int kAttUnits = 0x3FFFFFFF;
 
 struct AttDesc {
     int first, last;       // the CTAs that have parts of a row tile that is cut (last -1: it is not)
@@ -449,7 +451,7 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT, RW>::kPerSm) cach
     float* join = reinterpret_cast<float*>(smem + Sh::kStages * Sh::kStage);
     uint8_t* queries = reinterpret_cast<uint8_t*>(join) + Sh::kJoin;
     float* stats = reinterpret_cast<float*>(queries + Sh::kQueries);
-    int* first = reinterpret_cast<int*>(stats + Sh::kStats / 4);   // of each sequence, its first unit (the host keeps their number below 2^31)
+    int* first = reinterpret_cast<int*>(stats + Sh::kStats / 4);   // of each sequence, its first unit
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t full = smem_u32(bars), empty = full + 8 * Sh::kStages, q_full = empty + 8 * Sh::kStages, q_empty = q_full + 8, ring = smem_u32(smem);
     griddep_launch();
@@ -467,7 +469,7 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT, RW>::kPerSm) cach
         new_rows(p.c, b, beg, end);
         const int row_tiles = (static_cast<int>(end - beg) * p.per + R - 1) / R;
         const int seen = static_cast<int>(min(max(static_cast<long long>(p.c.lengths[b]), 0LL), cap));
-        first[b + 1] = p.c.heads * row_tiles * (p.by_item ? 1 : kAttOver + max(1, (seen + kAttTile - 1) / kAttTile));
+        first[b + 1] = min(p.c.heads * row_tiles * (p.by_item ? 1 : kAttOver + max(1, (seen + kAttTile - 1) / kAttTile)), kAttUnits);
     }
     __syncthreads();
     if (warp == 0) {
@@ -477,10 +479,10 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT, RW>::kPerSm) cach
 #pragma unroll
             for (int d = 1; d < 32; d *= 2) {
                 const int o = __shfl_up_sync(0xffffffffu, v, d);
-                if (lane >= d) v += o;
+                if (lane >= d) v = min(v + o, kAttUnits);
             }
-            if (b0 + lane < p.c.seqs) first[b0 + lane + 1] = sum + v;
-            sum += __shfl_sync(0xffffffffu, v, 31);
+            if (b0 + lane < p.c.seqs) first[b0 + lane + 1] = min(sum + v, kAttUnits);
+            sum = min(sum + __shfl_sync(0xffffffffu, v, 31), kAttUnits);
         }
         if (lane == 0) first[0] = 0;
     }
@@ -687,7 +689,7 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT, RW>::kPerSm) cach
             int last = -1;
             if (cut) {   // the owner of its last unit
                 const int u1 = it.base + kAttOver + it.tiles - 1, big = more * (share + 1);
-                last = u1 < big ? u1 / (share + 1) : more + (u1 - big) / share;
+                last = min(u1 < big ? u1 / (share + 1) : more + (u1 - big) / share, ctas - 1);
             }
             p.desc[p.listed ? it.index : cta] = {cta, last, it.rows, it.head, it.row0, static_cast<int>(it.token0), {0, 0}};
         }

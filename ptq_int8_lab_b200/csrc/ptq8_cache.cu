@@ -183,7 +183,7 @@ long long att_items(const ptq8_cache_attention_args& a, const AttVariant& v) {
 // Many row tiles keep the SMs busy one CTA each; fewer are cut into equal shares.  (So are more units than an int counts.)
 bool att_by_item(const ptq8_ops* o, const ptq8_cache_attention_args& a, const AttVariant& v, int table_width) {
     const long long most = static_cast<long long>(table_width) * a.cache.page / kAttTile + 1 + kAttOver, items = att_items(a, v);
-    if (items > 0x7FFFFFFFLL / most) return true;
+    if (items > kAttUnits / most) return true;
     return a.cache.starts && a.tokens * (a.heads / a.cache.kv_heads) / v.rows * a.cache.kv_heads >= 8LL * o->sms * v.per_sm;
 }
 

@@ -38,6 +38,8 @@ int check_w4(ptq8_ops* o, const ptq8_linear_w4_args& a) {
     return PTQ8_OK;
 }
 
+constexpr int kW4Segment = 16;   // chunks
+
 struct W4Variant {
     int type, vb, nt;   // of the activations; bytes that a lane takes at once; tiles of eight columns
     void (*kernel)(W4Params, W4Plan, const CUtensorMap);
@@ -49,6 +51,7 @@ struct W4Variant {
 template <typename XT, int TYPE, int VB, int NT>
 W4Variant w4_variant() {
     using Sh = W4Shape<XT, VB, NT>;
+    static_assert(NT > 1 || kW4Smem - 1024 - Sh::kSums - kW4Segment * (Sh::frag(8) + Sh::kBeside) >= kW4Warps * kW4Box, "a segment fits beside a stage");
     return {TYPE, VB, NT, linear_w4_kernel<XT, VB, NT, false>, linear_w4_kernel<XT, VB, NT, true>, Sh::kSums, Sh::kBeside, Sh::frag};
 }
 
@@ -113,7 +116,7 @@ int run_w4(ptq8_ops* o, const ptq8_linear_w4_args& a, cudaStream_t st) {
         const int chunks = (a.in_features + kW4Chunk - 1) / kW4Chunk;
         const long long pairs = (a.out_features - 1LL) / (p.gated ? 16 : 32) + 1;   // of tiles
         // The fewest columns that take all tokens in a pass, fewer where all chunks' activations do not fit beside a stage of weights;
-        // then as many stages as fit.  Not even with eight columns: a segment of 16 chunks at a time.
+        // then as many stages as fit.  Not even with eight columns: a segment of kW4Segment chunks at a time.
         const W4Variant* v = nullptr;
         W4Plan plan{};
         long long passes = 0;
@@ -121,7 +124,7 @@ int run_w4(ptq8_ops* o, const ptq8_linear_w4_args& a, cudaStream_t st) {
             const bool segments = nt == 0;
             for (v = kW4Variants; v->type != a.x_type || v->vb != vb || v->nt != std::max(nt, 1);) ++v;
             passes = (a.rows + v->nt * per_tile - 1) / (v->nt * per_tile);
-            plan = {8, segments ? 16 : chunks, segments ? (chunks + 15) / 16 : 1, 0, static_cast<int>(pairs), 1, 0, static_cast<int>(passes)};
+            plan = {8, segments ? kW4Segment : chunks, segments ? (chunks + kW4Segment - 1) / kW4Segment : 1, 0, static_cast<int>(pairs), 1, 0, static_cast<int>(passes)};
             if (v->nt == 1) plan.columns = static_cast<int>(std::min<long long>(8, a.rows * (a.x_type == PTQ8_F32 ? 2 : 1)));
             // warps a pair: as many as leave the device's warps one each, if that many
             while (1 << plan.split_log < std::min(kW4Warps, plan.held) && (pairs * passes << plan.split_log) * 2 <= static_cast<long long>(kW4Warps) * o->sms) ++plan.split_log;

@@ -314,7 +314,7 @@ struct W4Shape {
     static constexpr int kPieces = W4Pieces<VB>::N;
     static constexpr int kSums = kW4Warps * 2 * NT * 128 * 4;
     // of a chunk; columns: those held (fewer than eight where there are no more)
-    static int frag(int columns) { return NT * 4 * columns * 64; }
+    static constexpr int frag(int columns) { return NT * 4 * columns * 64; }
     static constexpr int kBeside = NT * kPieces * 64;
 };
 
