@@ -103,6 +103,11 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[W], const uint8_t* p) {
 // 2^e for e within -126 .. 127.
 __device__ __forceinline__ float exp2_int(int e) { return __int_as_float((e + 127) << 23); }
 
+// a / b of powers of two within 2^+-121, 2^-126 at least.
+__device__ __forceinline__ float power_ratio(float a, float b) {
+    return exp2_int(max((__float_as_int(a) >> 23) - (__float_as_int(b) >> 23), -126));
+}
+
 template <int D, int NT, int RW>
 struct AttShape {
     static constexpr int R = 8 * NT * RW, TW = kAttWarps / RW;
@@ -114,7 +119,7 @@ struct AttShape {
     static constexpr int kJoin = kAttWarps * 8 * NT * kPitch * 4, kStats = kAttWarps * 8 * NT * 2 * 4;
     // a warp's query fragments lie in its own part of the joining buffer, which it writes when it is done with them
     static constexpr int kWarp = 8 * NT * kPitch * 4;
-    static_assert(NT * (D / 32) * 32 * 16 <= kWarp && kJoin == kAttWarps * kWarp, "query fragments fit");
+    static_assert(NT * (D / 32) * 32 * 16 + NT * 32 * 8 <= kWarp && kJoin == kAttWarps * kWarp, "query fragments and the rows' c fit");
     // query rows that the producer fetches ahead (the largest tile of 256 dimensions has no room for them)
     static constexpr bool kAhead = D < 256 || RW < 4;
     static constexpr int kQueries = kAhead ? R * D * 2 : 0;
@@ -131,7 +136,12 @@ struct AttRows {
     float2 m[NT], l[NT], lo[NT];  // reference, sum of p, sum of p (least_v + 8 step_v)
     int lim[NT][2];               // positions that the row sees
     float o[D / 16][NT][4];
-    float c;                             // what p step_v is multiplied by: a power of two
+    float c;                             // what p step_v is multiplied by: a power of two, by the steps of the values that a row sees
+    bool apart;                          // the rows' c differ and lie behind q ([NT][32 lanes], of rows 2 t and 2 t + 1): MASKED steps from here on
+    __device__ __forceinline__ float2* own_c() const {
+        return reinterpret_cast<float2*>(const_cast<uint4*>(q - (threadIdx.x & 31)) + NT * (D / 32) * 32) + (threadIdx.x & 31);
+    }
+    __device__ __forceinline__ float2 c_of(int nt) const { return apart ? own_c()[nt * 32] : make_float2(c, c); }
 };
 
 __device__ __forceinline__ float att_value(const void* p, long long at, int type) {
@@ -214,6 +224,7 @@ __device__ __forceinline__ void att_queries(const AttParams& p, AttRows<D, NT>& 
 #pragma unroll
             for (int i = 0; i < 4; ++i) r.o[mt][nt][i] = 0.0f;
     r.c = 0x1p120f;   // as for a bound of 2^-113 on step_v
+    r.apart = false;
     r.q = q + lane;
     __syncwarp();
 }
@@ -275,13 +286,16 @@ __device__ __forceinline__ void att_step(AttRows<D, NT>& r, const uint8_t* K, co
             }
     }
     // scores over a; `move`: one passes its row's reference by too much, or a value's step its bound
-    float vstep[H][2], steps = 0.0f, most = 0.0f;
+    float vstep[H][2], most = 0.0f;
+    float2 steps[NT];   // the largest step of a value that the row sees (MASKED), or that there is
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) steps[nt] = both(0.0f);
 #pragma unroll
     for (int h = 0; h < H; ++h)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             vstep[h][i] = __uint_as_float(pv[h][i] << 16);
-            steps = fmaxf(steps, vstep[h][i]);
+            if (!MASKED) steps[0].x = fmaxf(steps[0].x, vstep[h][i]);
             const float2 step = both(__uint_as_float(pk[h][i] << 16)), least = both(__uint_as_float(pk[h][i] & 0xFFFF0000u));
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -294,21 +308,34 @@ __device__ __forceinline__ void att_step(AttRows<D, NT>& r, const uint8_t* K, co
                 const float2 d = __ffma2_rn(v, r.a[nt], make_float2(-r.m[nt].x, -r.m[nt].y));
                 if (!MASKED || v.x != -INFINITY) most = fmaxf(most, d.x);
                 if (!MASKED || v.y != -INFINITY) most = fmaxf(most, d.y);
+                if (MASKED && v.x != -INFINITY) steps[nt].x = fmaxf(steps[nt].x, vstep[h][i]);
+                if (MASKED && v.y != -INFINITY) steps[nt].y = fmaxf(steps[nt].y, vstep[h][i]);
             }
         }
-    if (__any_sync(0xffffffffu, most > kAttSlack || steps * r.c > 128.0f)) {
+    bool wide = false;
 #pragma unroll
-        for (int d = 4; d < 32; d *= 2) steps = fmaxf(steps, __shfl_xor_sync(0xffffffffu, steps, d));
-        // all lanes of the warp hold the same bound: 128 over the power of two above it
-        float scale_o = 1.0f;
-        if (steps * r.c > 128.0f) {
-            const int e = min(static_cast<int>(__float_as_uint(steps) >> 23) - 126, 127);
-            const float c = exp2_int(7 - e);
-            scale_o = c / r.c;
-            r.c = c;
-        }
+    for (int nt = 0; nt < (MASKED ? NT : 1); ++nt) {
+        const float2 c = MASKED ? r.c_of(nt) : both(r.c);
+        wide |= steps[nt].x * c.x > 128.0f || (MASKED && steps[nt].y * c.y > 128.0f);
+    }
+    if (__any_sync(0xffffffffu, most > kAttSlack || wide)) {
+        float2 c[NT];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
+            if (MASKED || nt == 0) {
+#pragma unroll
+                for (int d = 4; d < 32; d *= 2) {   // (a row's eight lanes)
+                    steps[nt].x = fmaxf(steps[nt].x, __shfl_xor_sync(0xffffffffu, steps[nt].x, d));
+                    if (MASKED) steps[nt].y = fmaxf(steps[nt].y, __shfl_xor_sync(0xffffffffu, steps[nt].y, d));
+                }
+            }
+            if (!MASKED) steps[nt] = both(steps[0].x);
+            // 128 over the power of two above the largest step
+            const float2 old = MASKED ? r.c_of(nt) : both(r.c);
+            c[nt] = old;
+            if (steps[nt].x * old.x > 128.0f) c[nt].x = exp2_int(7 - min(static_cast<int>(__float_as_uint(steps[nt].x) >> 23) - 126, 127));
+            if (steps[nt].y * old.y > 128.0f) c[nt].y = exp2_int(7 - min(static_cast<int>(__float_as_uint(steps[nt].y) >> 23) - 126, 127));
+            const float2 scale_o = make_float2(power_ratio(c[nt].x, old.x), power_ratio(c[nt].y, old.y));
             float2 best = both(kAttNone);
 #pragma unroll
             for (int h = 0; h < H; ++h)
@@ -330,7 +357,20 @@ __device__ __forceinline__ void att_step(AttRows<D, NT>& r, const uint8_t* K, co
 #pragma unroll
             for (int mt = 0; mt < D / 16; ++mt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) r.o[mt][nt][i] *= (i & 1 ? f.y : f.x) * scale_o;
+                for (int i = 0; i < 4; ++i) r.o[mt][nt][i] *= i & 1 ? f.y * scale_o.y : f.x * scale_o.x;
+        }
+        if constexpr (MASKED) {
+            const float first = __shfl_sync(0xffffffffu, c[0].x, 0);
+            bool same = true;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                same &= c[nt].x == first && c[nt].y == first;
+                r.own_c()[nt * 32] = c[nt];   // (the lane's own)
+            }
+            r.apart = !__all_sync(0xffffffffu, same);
+            r.c = first;
+        } else {
+            r.c = c[0].x;
         }
     }
     uint32_t pb[NT][2 * H];
@@ -348,7 +388,7 @@ __device__ __forceinline__ void att_step(AttRows<D, NT>& r, const uint8_t* K, co
                     const bool x_in = v.x != -INFINITY, y_in = v.y != -INFINITY;
                     e = make_float2(x_in ? e.x : 0.0f, y_in ? e.y : 0.0f);
                     r.lo[nt] = make_float2(x_in ? __fmaf_rn(e.x, middle.x, r.lo[nt].x) : r.lo[nt].x, y_in ? __fmaf_rn(e.y, middle.y, r.lo[nt].y) : r.lo[nt].y);
-                    w = make_float2(x_in ? e.x * vs.x : 0.0f, y_in ? e.y * vs.y : 0.0f);
+                    w = make_float2(x_in ? e.x * (vstep[h][i] * r.c_of(nt).x) : 0.0f, y_in ? e.y * (vstep[h][i] * r.c_of(nt).y) : 0.0f);
                 } else {
                     r.lo[nt] = __ffma2_rn(e, middle, r.lo[nt]);
                     w = __fmul2_rn(e, vs);
@@ -610,7 +650,7 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT, RW>::kPerSm) cach
 #pragma unroll 1
                 for (int tk = tw * 16 * H; tk < kAttTile; tk += TW * 16 * H) {
                     const int pos = tile * kAttTile + tk;
-                    if (whole && pos + 16 * H <= all)
+                    if (whole && pos + 16 * H <= all && !r.apart)
                         att_step<D, NT, H, false>(r, K, V, KS, VS, tk, pos, it.seen, have, shift);
                     else if (pos < it.seen)
                         att_step<D, NT, H, true>(r, K, V, KS, VS, tk, pos, it.seen, have, shift);
@@ -621,10 +661,13 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT, RW>::kPerSm) cach
             if (++stage == Sh::kStages) stage = 0, phase ^= 1;
         }
         // ---- the segment's end: the warps' numerators, references and sums meet in shared memory
-        __syncwarp();   // all lanes are done with the queries
-        const float inv = 1.0f / r.c;        // a power of two: exact
+        float2 c[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) c[nt] = r.c_of(nt);
+        __syncwarp();   // all lanes are done with the queries, and what lies behind them
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
+            const float inv[2] = {power_ratio(1.0f, c[nt].x), power_ratio(1.0f, c[nt].y)};   // powers of two: exact
             float m[2] = {r.m[nt].x, r.m[nt].y}, l[2] = {r.l[nt].x, r.l[nt].y}, lo[2] = {r.lo[nt].x, r.lo[nt].y};
 #pragma unroll
             for (int i = 0; i < 2; ++i)
@@ -641,8 +684,8 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT, RW>::kPerSm) cach
 #pragma unroll
                 for (int mt = 0; mt < D / 16; mt += 2)
                     *reinterpret_cast<float4*>(to + 2 * mt) =
-                        make_float4(__fmaf_rn(r.o[mt][nt][i], inv, lo[i]), __fmaf_rn(r.o[mt][nt][2 + i] * 0.0625f, inv, lo[i]),
-                                    __fmaf_rn(r.o[mt + 1][nt][i], inv, lo[i]), __fmaf_rn(r.o[mt + 1][nt][2 + i] * 0.0625f, inv, lo[i]));
+                        make_float4(__fmaf_rn(r.o[mt][nt][i], inv[i], lo[i]), __fmaf_rn(r.o[mt][nt][2 + i] * 0.0625f, inv[i], lo[i]),
+                                    __fmaf_rn(r.o[mt + 1][nt][i], inv[i], lo[i]), __fmaf_rn(r.o[mt + 1][nt][2 + i] * 0.0625f, inv[i], lo[i]));
             }
         }
         named_bar_sync(1, 32 * kAttWarps);
