@@ -480,6 +480,57 @@ __device__ __forceinline__ void att_tiles(const AttParams& p, const AttItem& it,
     t1 = min(it.tiles, end - it.base - kAttOver);
 }
 
+// The first unit of each sequence, and of all after the last one's, in shared memory; by all threads.
+template <int R>
+__device__ __forceinline__ void att_units(const AttParams& p, int* first, int threads) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const long long cap = static_cast<long long>(p.c.width) << p.c.shift;
+    for (int b = threadIdx.x; b < p.c.seqs; b += threads) {
+        long long beg, end;
+        new_rows(p.c, b, beg, end);
+        const int row_tiles = (static_cast<int>(end - beg) * p.per + R - 1) / R;
+        const int seen = static_cast<int>(min(max(static_cast<long long>(p.c.lengths[b]), 0LL), cap));
+        first[b + 1] = min(p.c.heads * row_tiles * (p.by_item ? 1 : kAttOver + max(1, (seen + kAttTile - 1) / kAttTile)), kAttUnits);
+    }
+    __syncthreads();
+    if (warp == 0) {
+        int sum = 0;
+        for (int b0 = 0; b0 < p.c.seqs; b0 += 32) {
+            int v = b0 + lane < p.c.seqs ? first[b0 + lane + 1] : 0;
+#pragma unroll
+            for (int d = 1; d < 32; d *= 2) {
+                const int o = __shfl_up_sync(0xffffffffu, v, d);
+                if (lane >= d) v = min(v + o, kAttUnits);
+            }
+            if (b0 + lane < p.c.seqs) first[b0 + lane + 1] = min(sum + v, kAttUnits);
+            sum = min(sum + __shfl_sync(0xffffffffu, v, 31), kAttUnits);
+        }
+        if (lane == 0) first[0] = 0;
+    }
+    __syncthreads();
+}
+
+// This block's units: equal shares, the first `more` blocks one unit more; a unit each at least.
+struct AttShare {
+    int ctas, share, more, beg, end;
+    __device__ __forceinline__ AttShare(const AttParams& p, int units) {
+        const int cta = blockIdx.x;
+        ctas = min(static_cast<int>(gridDim.x), units), share = ctas ? units / ctas : 0, more = units - share * ctas;
+        beg = p.by_item ? min(cta, units) : cta < ctas ? cta * share + min(cta, more) : 0;
+        end = p.by_item ? min(cta + 1, units) : cta < ctas ? beg + share + (cta < more) : 0;
+    }
+};
+
+// What there is to join of a row tile that begins in this block: up to the owner of its last unit.
+__device__ __forceinline__ AttDesc att_described(const AttItem& it, const AttShare& s, int cta, bool cut) {
+    int last = -1;
+    if (cut) {
+        const int u1 = it.base + kAttOver + it.tiles - 1, big = s.more * (s.share + 1);
+        last = min(u1 < big ? u1 / (s.share + 1) : s.more + (u1 - big) / s.share, s.ctas - 1);
+    }
+    return {cta, last, it.rows, it.head, it.row0, static_cast<int>(it.token0), {0, 0}};
+}
+
 template <int D, int NT, int RW>
 __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT, RW>::kPerSm) cache_attention_kernel(const AttParams p) {
     using Sh = AttShape<D, NT, RW>;
@@ -503,35 +554,10 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT, RW>::kPerSm) cach
         dead = 0;
     }
     griddep_wait();
-    const long long cap = static_cast<long long>(p.c.width) << p.c.shift;
-    for (int b = threadIdx.x; b < p.c.seqs; b += kAttThreads) {
-        long long beg, end;
-        new_rows(p.c, b, beg, end);
-        const int row_tiles = (static_cast<int>(end - beg) * p.per + R - 1) / R;
-        const int seen = static_cast<int>(min(max(static_cast<long long>(p.c.lengths[b]), 0LL), cap));
-        first[b + 1] = min(p.c.heads * row_tiles * (p.by_item ? 1 : kAttOver + max(1, (seen + kAttTile - 1) / kAttTile)), kAttUnits);
-    }
-    __syncthreads();
-    if (warp == 0) {
-        int sum = 0;
-        for (int b0 = 0; b0 < p.c.seqs; b0 += 32) {
-            int v = b0 + lane < p.c.seqs ? first[b0 + lane + 1] : 0;
-#pragma unroll
-            for (int d = 1; d < 32; d *= 2) {
-                const int o = __shfl_up_sync(0xffffffffu, v, d);
-                if (lane >= d) v = min(v + o, kAttUnits);
-            }
-            if (b0 + lane < p.c.seqs) first[b0 + lane + 1] = min(sum + v, kAttUnits);
-            sum = min(sum + __shfl_sync(0xffffffffu, v, 31), kAttUnits);
-        }
-        if (lane == 0) first[0] = 0;
-    }
-    __syncthreads();
+    att_units<R>(p, first, kAttThreads);
     const int units = first[p.c.seqs], cta = blockIdx.x;
-    // equal shares, the first `more` CTAs one unit more; a unit each at least
-    const int ctas = min(static_cast<int>(gridDim.x), units), share = ctas ? units / ctas : 0, more = units - share * ctas;
-    const int beg = p.by_item ? min(cta, units) : cta < ctas ? cta * share + min(cta, more) : 0;
-    const int end = p.by_item ? min(cta + 1, units) : cta < ctas ? beg + share + (cta < more) : 0;
+    const AttShare own(p, units);
+    const int beg = own.beg, end = own.end;
     const int shift = min(p.c.shift, 7);   // tokens of a piece: a page, or a tile
     const int pieces = kAttTile >> shift;
 
@@ -729,12 +755,7 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT, RW>::kPerSm) cach
         }
         named_bar_sync(1, 32 * kAttWarps);   // the buffer is free
         if (t0 == 0 && threadIdx.x == 0 && (p.listed || cut)) {   // the tile begins here: this CTA says what there is to join
-            int last = -1;
-            if (cut) {   // the owner of its last unit
-                const int u1 = it.base + kAttOver + it.tiles - 1, big = more * (share + 1);
-                last = min(u1 < big ? u1 / (share + 1) : more + (u1 - big) / share, ctas - 1);
-            }
-            p.desc[p.listed ? it.index : cta] = {cta, last, it.rows, it.head, it.row0, static_cast<int>(it.token0), {0, 0}};
+            p.desc[p.listed ? it.index : cta] = att_described(it, own, cta, cut);
         }
     }
 }

@@ -4,7 +4,7 @@
 #include <algorithm>
 #include <cmath>
 
-#include "ptq8_attention.cuh"
+#include "ptq8_attention_tc.cuh"
 #include "ptq8_ops.cuh"
 
 using namespace ptq8;
@@ -144,17 +144,24 @@ struct AttVariant {
     AttKernel kernel;
     int per_sm, smem;   // of PTQ8_MAX_SEQUENCES
     int (*smem_of)(int seqs);
+    int threads;
 };
 
 template <int D, int NT, int RW>
 AttVariant att_variant() {
     using Sh = AttShape<D, NT, RW>;
-    return {D, Sh::R, cache_attention_kernel<D, NT, RW>, Sh::kPerSm, Sh::smem(PTQ8_MAX_SEQUENCES), Sh::smem};
+    return {D, Sh::R, cache_attention_kernel<D, NT, RW>, Sh::kPerSm, Sh::smem(PTQ8_MAX_SEQUENCES), Sh::smem, kAttThreads};
+}
+
+template <int D>
+AttVariant att_tiles_variant() {
+    using Sh = TcAttShape<D>;
+    return {D, kTcRows, cache_attention_tiles_kernel<D>, 1, Sh::smem(PTQ8_MAX_SEQUENCES), Sh::smem, kTcThreads};
 }
 
 const AttVariant kAttVariants[] = {
-    att_variant<64, 1, 1>(),  att_variant<64, 2, 1>(),  att_variant<64, 2, 2>(),  att_variant<64, 2, 4>(),
-    att_variant<128, 1, 1>(), att_variant<128, 2, 1>(), att_variant<128, 2, 2>(), att_variant<128, 2, 4>(),
+    att_variant<64, 1, 1>(),  att_variant<64, 2, 1>(),  att_variant<64, 2, 2>(),  att_variant<64, 2, 4>(), att_tiles_variant<64>(),
+    att_variant<128, 1, 1>(), att_variant<128, 2, 1>(), att_variant<128, 2, 2>(), att_variant<128, 2, 4>(), att_tiles_variant<128>(),
     att_variant<256, 1, 1>(), att_variant<256, 1, 2>(), att_variant<256, 1, 4>(),
 };
 
@@ -234,7 +241,7 @@ int attention_call(ptq8_ops* o, const ptq8_cache_attention_args& a, cudaStream_t
         p.desc = reinterpret_cast<AttDesc*>(p.stat + 2 * n * v.rows * 2);
         p.listed = !a.cache.starts && items <= n;
     }
-    cudaError_t e = launch(v.kernel, dim3(static_cast<unsigned>(n)), dim3(kAttThreads), v.smem_of(a.cache.sequences), 1, st, p);
+    cudaError_t e = launch(v.kernel, dim3(static_cast<unsigned>(n)), dim3(v.threads), v.smem_of(a.cache.sequences), 1, st, p);
     if (e == cudaSuccess && !p.by_item) {
         // few row tiles have many parts each: eight warps a row; else a warp a row
         const bool wide = p.listed && 4 * items <= n;
