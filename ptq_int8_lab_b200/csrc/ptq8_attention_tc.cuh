@@ -8,8 +8,9 @@
 // the same order, a token's row of 64 dimensions to 128 bytes: read as K-major for S, as N-major for O.  Where a word's
 // eight codes stand for dimensions in another order (0 4 1 5 2 6 3 7), queries and outputs follow it.
 //
-// A thread owns a row: no value of a softmax leaves it.  It goes over its 128 scores once, with the reference that it has; only
-// where one passes that by 2^8 (or a value's step its bound) does it go over them again with a new one, and over O.
+// A thread owns a row: no value of a softmax leaves it.  It goes over its 128 scores once, 16 at a time, with the reference that it
+// has; only where one passes that by 2^8 (or a value's step its bound) does it go over P so far and O with a new one, a
+// whole power of two away, so that P changes exactly.
 //
 // Warps: 0-3 and 4-7 softmax of 128 rows each, in turns with the tensor core: one's products run while the other's
 // exponentials do; 8-11 widen codes; 12 issues MMAs; 13 copies tiles in; 14, 15 idle.
@@ -27,21 +28,21 @@ struct TcAttShape {
     static constexpr int kCodes = kAttTile * D / 2, kPairs = kAttTile * 4, kStage = 2 * (kCodes + kPairs);
     static constexpr int kBlock = kAttTile * 128;              // 64 dimensions of 128 rows or tokens as f16
     static constexpr int kHalf = D / 64 * kBlock;              // an operand
-    static constexpr int kParam = kAttTile * 16 + 32;          // of a tile: for each two tokens step_k, middle_k, step_v, middle_v; then which there are, and the warps' largest steps
-    static constexpr int smem(int seqs) { return 1024 + 4 * kHalf + kStages * kStage + 2 * kParam + (seqs + 1) * 4; }
+    static constexpr int kParam = kAttTile * 16 + 32;          // of a tile: by 16 tokens, for each two step_k, middle_k, and for each two step_v, middle_v; then which there are, and the warps' largest steps
+    static constexpr int smem(int seqs) { return 1024 + 5 * kHalf + kStages * kStage + 2 * kParam + (seqs + 1) * 4; }
     static_assert(smem(1024) + 1024 <= 227 * 1024, "shared memory of an SM");
 };
 
-__device__ __forceinline__ void tmem_store32(uint32_t taddr, const uint32_t* v) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0],"
-        " {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16,"
-        " %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
-        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
-        "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
-        "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-        : "memory");
+__device__ __forceinline__ void tmem_store8(uint32_t taddr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
+                 "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_load8(uint32_t taddr, uint32_t (&v)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                 : "r"(taddr)
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -78,71 +79,111 @@ __device__ __forceinline__ uint64_t n_major_desc(uint32_t saddr, uint32_t block)
 struct TcRow {
     float a, b, m, l, lo, c;   // as in AttRows
     int lim;
+    bool fresh;                // it has seen nothing: m is 0, and says nothing
 };
 
-// One pass over the row's 128 scores of a tile with the reference m and the factor c: P (64 columns of two), the sums so far, and
-// what passes them by most.  MASKED: some row does not see all of the tile's tokens.
+// New references, whole powers of two from the old ones (`up` of them; P so far changes exactly), and new c: what there is of P (the
+// first `cols` columns at s) and O (`ocols` columns at o) follows.  By a whole warp.
+__device__ __noinline__ void tc_rescale(uint32_t s, int cols, uint32_t o, int ocols, float scale) {
+    tmem_stored();
+    const __half2 h = __float2half2_rn(scale);
+#pragma unroll 1
+    for (int i = 0; i < cols; i += 8) {
+        uint32_t x[8];
+        tmem_load8(s + i, x);
+        tmem_wait_ld();
+#pragma unroll
+        for (int z = 0; z < 8; ++z) {
+            __half2 v = *reinterpret_cast<__half2*>(&x[z]);
+            v = __hmul2(v, h);
+            x[z] = *reinterpret_cast<uint32_t*>(&v);
+        }
+        tmem_store8(s + i, x);
+    }
+#pragma unroll 1
+    for (int i = 0; i < ocols; i += 8) {
+        uint32_t x[8];
+        tmem_load8(o + i, x);
+        tmem_wait_ld();
+#pragma unroll
+        for (int z = 0; z < 8; ++z) x[z] = __float_as_uint(__uint_as_float(x[z]) * scale);
+        tmem_store8(o + i, x);
+    }
+    tmem_stored();
+}
+
+// The row's 128 scores of a tile at s become P there.  MASKED: some row does not see all of the tile's tokens.  largest: the tile's largest step.
 template <bool MASKED>
-__device__ __forceinline__ void tc_pass(const TcRow& r, uint32_t s, const float4* param, const uint32_t* there, int pos, uint32_t (&P)[64], float& l, float& lo, float& most, float& steps) {
-    const float2 a = both(r.a), b = both(r.b), m = both(-r.m), c = both(r.c);
+__device__ __forceinline__ void tc_tile(TcRow& r, uint32_t s, uint32_t o, int ocols, const float4* param, const uint32_t* there, int pos, float largest) {
     float2 sum = make_float2(r.l, 0.0f), low = make_float2(r.lo, 0.0f);
     uint32_t x[2][16];
     tmem_ld16(s, x[0]);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {   // 16 scores at a time, the next ones on their way
-        tmem_wait_ld(x[k & 1]);
-        if (k < 7) tmem_ld16(s + 16 * (k + 1), x[(k + 1) & 1]);
         uint32_t in = 0xFFFFu;
         if constexpr (MASKED) {
             const int n = min(max(r.lim - pos - 16 * k, 0), 16);
             in = (there[k >> 1] >> (16 * (k & 1))) & ((1u << n) - 1);
         }
+        float4 key[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) key[i] = param[16 * k + i];
+        tmem_wait_ld(x[k & 1]);
+        if (k < 7) tmem_ld16(s + 16 * (k + 1), x[(k + 1) & 1]);
+        float2 d[8];
+        float most = kAttNone, steps = k == 0 && !MASKED ? largest : 0.0f;
+        const float2 b = both(r.b), a = both(r.a);
+        float2 m = both(-r.m);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float4 key = param[2 * (8 * k + i)], value = param[2 * (8 * k + i) + 1];
-            float2 v = __ffma2_rn(make_float2(__uint_as_float(x[k & 1][2 * i]), __uint_as_float(x[k & 1][2 * i + 1])), make_float2(key.x, key.y), __fmul2_rn(make_float2(key.z, key.w), b));
-            float2 step = make_float2(value.x, value.y), middle = make_float2(value.z, value.w);
+            const float2 v = __ffma2_rn(make_float2(__uint_as_float(x[k & 1][2 * i]), __uint_as_float(x[k & 1][2 * i + 1])), make_float2(key[i].x, key[i].y), __fmul2_rn(make_float2(key[i].z, key[i].w), b));
+            d[i] = __ffma2_rn(v, a, m);
             if constexpr (MASKED) {   // (what a row does not see may be NaN)
-                if (!((in >> (2 * i)) & 1)) v.x = -INFINITY, step.x = middle.x = 0.0f;
-                if (!((in >> (2 * i + 1)) & 1)) v.y = -INFINITY, step.y = middle.y = 0.0f;
-                steps = fmaxf(steps, fmaxf(step.x, step.y));
+                if (!((in >> (2 * i)) & 1)) d[i].x = -INFINITY;
+                if (!((in >> (2 * i + 1)) & 1)) d[i].y = -INFINITY;
             }
-            float2 d = __ffma2_rn(v, a, m);
-            if constexpr (MASKED) {   // (and so may a be, or of either sign)
-                if (!((in >> (2 * i)) & 1)) d.x = -INFINITY;
-                if (!((in >> (2 * i + 1)) & 1)) d.y = -INFINITY;
-            }
-            most = fmaxf(most, fmaxf(d.x, d.y));
-            const float2 e = make_float2(ex2_approx(d.x), ex2_approx(d.y));
-            sum = __fadd2_rn(sum, e);
-            low = __ffma2_rn(e, middle, low);
-            const float2 w = __fmul2_rn(e, __fmul2_rn(step, c));
-            P[8 * k + i] = pair_of<__half>(w.x, w.y);
+            most = fmaxf(most, fmaxf(d[i].x, d[i].y));
         }
-    }
-    l = sum.x + sum.y;
-    lo = low.x + low.y;
-}
-
-// The largest score of the row's in a tile, in powers of two.
-__device__ __noinline__ float tc_most(float ra, float rb, int lim, uint32_t s, const float4* param, const uint32_t* there, int pos) {
-    float best = kAttNone;
-#pragma unroll 1
-    for (int k = 0; k < 8; ++k) {
-        uint32_t x[16];
-        tmem_ld16(s + 16 * k, x);
-        tmem_wait_ld(x);
-        const int n = min(max(lim - pos - 16 * k, 0), 16);
-        const uint32_t in = (there[k >> 1] >> (16 * (k & 1))) & ((1u << n) - 1);
+        float4 value[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) value[i] = param[16 * k + 8 + i];
+        if constexpr (MASKED) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (!((in >> (2 * i)) & 1)) value[i].x = value[i].z = 0.0f;
+                if (!((in >> (2 * i + 1)) & 1)) value[i].y = value[i].w = 0.0f;
+                steps = fmaxf(steps, fmaxf(value[i].x, value[i].y));
+            }
+        }
+        if (__any_sync(0xffffffffu, most > kAttSlack || (r.fresh && most > kAttNone) || steps * r.c > 128.0f)) {
+            float up = 0.0f, f = 1.0f;
+            if (most > kAttSlack || (r.fresh && most > kAttNone)) {
+                up = ceilf(most);
+                if (!r.fresh) f = exp2_int(static_cast<int>(fmaxf(-up, -126.0f)));
+                r.fresh = false;
+            }
+            float c = r.c;
+            if (steps * r.c > 128.0f) c = exp2_int(7 - min(static_cast<int>(__float_as_uint(steps) >> 23) - 126, 127));
+            tc_rescale(s, 8 * k, o, ocols, f * power_ratio(c, r.c));
+            r.m += up, r.c = c;
+            sum = __fmul2_rn(sum, both(f)), low = __fmul2_rn(low, both(f));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) d[i] = make_float2(d[i].x - up, d[i].y - up);
+        }
+        const float2 c = both(r.c);
+        uint32_t P[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float4 key = param[2 * (8 * k + i)];
-            const float v = __fmaf_rn(__uint_as_float(x[2 * i]), key.x, key.z * rb) * ra, w = __fmaf_rn(__uint_as_float(x[2 * i + 1]), key.y, key.w * rb) * ra;
-            if ((in >> (2 * i)) & 1) best = fmaxf(best, v);
-            if ((in >> (2 * i + 1)) & 1) best = fmaxf(best, w);
+            const float2 e = make_float2(ex2_approx(d[i].x), ex2_approx(d[i].y));
+            sum = __fadd2_rn(sum, e);
+            low = __ffma2_rn(e, make_float2(value[i].z, value[i].w), low);
+            const float2 w = __fmul2_rn(e, __fmul2_rn(make_float2(value[i].x, value[i].y), c));
+            P[i] = pair_of<__half>(w.x, w.y);
         }
+        tmem_store8(s + 8 * k, P);
     }
-    return best;
+    r.l = sum.x + sum.y;
+    r.lo = low.x + low.y;
 }
 
 template <int D>
@@ -150,23 +191,23 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tiles_kernel(co
     using Sh = TcAttShape<D>;
     constexpr int R = kTcRows;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bars[2 * Sh::kStages + 14];
+    __shared__ __align__(8) uint64_t bars[2 * Sh::kStages + 16];
     __shared__ uint32_t there[Sh::kStages], slot;
     __shared__ int dead;
     uint8_t* const smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
     uint8_t* const q_smem = smem;                       // two halves of 128 rows
     uint8_t* const k_smem = q_smem + 2 * Sh::kHalf;
     uint8_t* const v_smem = k_smem + Sh::kHalf;
-    uint8_t* const ring = v_smem + Sh::kHalf;
+    uint8_t* const ring = v_smem + 2 * Sh::kHalf;
     uint8_t* const params = ring + Sh::kStages * Sh::kStage;
     int* const first = reinterpret_cast<int*>(params + 2 * Sh::kParam);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t full = smem_u32(bars), empty = full + 8 * Sh::kStages, k_full = empty + 8 * Sh::kStages, k_empty = k_full + 8, v_full = k_empty + 8, v_empty = v_full + 8,
-                   s_full = v_empty + 8, p_full = s_full + 16, o_full = p_full + 16, par_full = o_full + 16, q_full = par_full + 16, done = q_full + 8;
+    const uint32_t full = smem_u32(bars), empty = full + 8 * Sh::kStages, k_full = empty + 8 * Sh::kStages, k_empty = k_full + 8, v_full = k_empty + 8, v_empty = v_full + 16,
+                   s_full = v_empty + 16, p_full = s_full + 16, o_full = p_full + 16, par_full = o_full + 16, q_full = par_full + 16, done = q_full + 8;
     if (threadIdx.x == 0) {
         for (int i = 0; i < Sh::kStages; ++i) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, 4);
-        mbar_init(k_full, 4), mbar_init(k_empty, 1), mbar_init(v_full, 4), mbar_init(v_empty, 1);
-        for (int i = 0; i < 2; ++i) mbar_init(s_full + 8 * i, 1), mbar_init(p_full + 8 * i, 4), mbar_init(o_full + 8 * i, 1), mbar_init(par_full + 8 * i, 4);
+        mbar_init(k_full, 4), mbar_init(k_empty, 1);
+        for (int i = 0; i < 2; ++i) mbar_init(s_full + 8 * i, 1), mbar_init(p_full + 8 * i, 4), mbar_init(o_full + 8 * i, 1), mbar_init(par_full + 8 * i, 4), mbar_init(v_full + 8 * i, 4), mbar_init(v_empty + 8 * i, 1);
         mbar_init(q_full, 8), mbar_init(done, 1);
         fence_mbar_init();
         dead = 0;
@@ -270,20 +311,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tiles_kernel(co
             wait(k_full, tile & 1, ERR_WAIT_FULL);
             for (int g = 0; g < groups; ++g) scores(g, g == groups - 1);
             for (int t = t0; t < t1; ++t, ++tile) {
-                wait(v_full, tile & 1, ERR_WAIT_FULL);
-                if (t + 1 < t1) wait(k_full, (tile + 1) & 1, ERR_WAIT_FULL);
+                wait(v_full + 8 * (tile & 1), (tile >> 1) & 1, ERR_WAIT_FULL);
                 for (int g = 0; g < groups; ++g) {
                     wait(p_full + 8 * g, turns[g]++ & 1, ERR_WAIT_ACC);
                     if (lost) continue;
                     tc_fence_after();
 #pragma unroll
                     for (int k = 0; k < 8; ++k)
-                        mma_f16_tmem(tmem + 256 + 128 * g, tmem + 128 * g + 8 * k, vd + (k * 2048 >> 4), idesc_f16(D, true), t > t0 || k > 0);
-                    if (g == groups - 1) mma_commit_elect(v_empty);
-                    if (t + 1 < t1)
+                        mma_f16_tmem(tmem + 256 + 128 * g, tmem + 128 * g + 8 * k, vd + (((tile & 1) * Sh::kHalf + k * 2048) >> 4), idesc_f16(D, true), t > t0 || k > 0);
+                    if (g == groups - 1) mma_commit_elect(v_empty + 8 * (tile & 1));
+                    if (t + 1 < t1) {
+                        if (g == 0) wait(k_full, (tile + 1) & 1, ERR_WAIT_FULL);
                         scores(g, g == groups - 1);
-                    else
+                    } else {
                         mma_commit_elect(o_full + 8 * g);
+                    }
                 }
             }
         }
@@ -298,8 +340,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tiles_kernel(co
         constexpr int LANES = D / 32, ROWS = 32 / LANES;   // lanes of a token's row, 32 codes each; tokens of a warp at a time
         const int part = lane % LANES, row = lane / LANES;
         const auto widen = [&](const uint8_t* from, uint32_t to) {
-#pragma unroll 2
-            for (int tok = (warp - 8) * 32 + row; tok < (warp - 7) * 32; tok += ROWS) {
+#pragma unroll
+            for (int i0 = 0; i0 < 32; i0 += ROWS) {
+                const int tok = (warp - 8) * 32 + row + i0;
                 const uint4 w = *reinterpret_cast<const uint4*>(from + tok * (D / 2) + part * 16);
                 const uint32_t words[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -328,9 +371,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tiles_kernel(co
                     const bool ok = t * kAttTile + mine < it.seen && ((there[stage] >> (mine >> shift)) & 1);
                     if (!ok) pk = pv = 0;   // what lies there is not looked at
                     const float ks = __uint_as_float(pk << 16), vs = __uint_as_float(pv << 16);
-                    float* to = reinterpret_cast<float*>(params + (tile & 1) * Sh::kParam) + mine / 2 * 8 + mine % 2;
+                    float* to = reinterpret_cast<float*>(params + (tile & 1) * Sh::kParam) + mine / 16 * 64 + mine % 16 / 2 * 4 + mine % 2;
                     to[0] = ks, to[2] = __fmaf_rn(8.0f, ks, __uint_as_float(pk & 0xFFFF0000u));
-                    to[4] = vs, to[6] = __fmaf_rn(8.0f, vs, __uint_as_float(pv & 0xFFFF0000u));
+                    to[32] = vs, to[34] = __fmaf_rn(8.0f, vs, __uint_as_float(pv & 0xFFFF0000u));
                     const uint32_t have = __ballot_sync(0xffffffffu, ok);
                     float most = fmaxf(vs, 0.0f);   // (NaN counts for nothing)
 #pragma unroll
@@ -343,11 +386,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tiles_kernel(co
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(k_full), mbar_arrive(par_full + 8 * (tile & 1));
-                wait(v_empty, (tile & 1) ^ 1, ERR_WAIT_EMPTY);
-                if (!lost) widen(V, kv[1]);
+                wait(v_empty + 8 * (tile & 1), ((tile >> 1) & 1) ^ 1, ERR_WAIT_EMPTY);
+                if (!lost) widen(V, kv[1] + (tile & 1) * Sh::kHalf);
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(v_full), mbar_arrive(empty + 8 * stage);
+                if (lane == 0) mbar_arrive(v_full + 8 * (tile & 1)), mbar_arrive(empty + 8 * stage);
                 if (++stage == Sh::kStages) stage = 0, phase ^= 1;
             }
         }
@@ -408,7 +451,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tiles_kernel(co
                 // NaN and infinities in a row make all of its scores NaN
                 r.a = isfinite(top) ? exp2_int(-e) * p.scale_log2 : __int_as_float(0x7FC00000);
                 r.b = sum;
-                r.m = kAttNone, r.l = r.lo = 0.0f, r.c = 0x1p120f;
+                r.m = r.l = r.lo = 0.0f, r.c = 0x1p120f, r.fresh = true;
                 r.lim = mine ? static_cast<int>(min(max(it.len - it.n + row / p.per + 1, 0LL), cap)) : 0x7FFFFFFF;
             }
             fence_proxy_async_smem();
@@ -431,40 +474,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tiles_kernel(co
                 if (!lost) {
                     tc_fence_after();
                     const bool masked = (t + 1) * kAttTile > all || (have[0] & have[1] & have[2] & have[3]) != 0xFFFFFFFFu;
-                    uint32_t P[64];
-                    for (int again = 0; again < 2; ++again) {
-                        float l, lo, most = kAttNone, steps = 0.0f;
-                        if (masked) {
-                            tc_pass<true>(r, s, param, have, t * kAttTile, P, l, lo, most, steps);
-                        } else {
-                            tc_pass<false>(r, s, param, have, t * kAttTile, P, l, lo, most, steps);
-                            steps = fmaxf(fmaxf(largest[0], largest[1]), fmaxf(largest[2], largest[3]));
-                        }
-                        if (again || !__any_sync(0xffffffffu, most > kAttSlack || steps * r.c > 128.0f)) {
-                            r.l = l, r.lo = lo;
-                            break;
-                        }
-                        // the reference becomes the row's largest score so far, c 128 over the power of two above the largest step
-                        const float m = fmaxf(r.m, tc_most(r.a, r.b, r.lim, s, param, have, t * kAttTile));
-                        const float f = ex2_approx(r.m - m);
-                        float c = r.c;
-                        if (steps * r.c > 128.0f) c = exp2_int(7 - min(static_cast<int>(__float_as_uint(steps) >> 23) - 126, 127));
-                        const float scale = f * power_ratio(c, r.c);
-                        r.m = m, r.c = c, r.l *= f, r.lo *= f;
-                        if (t > t0) {
-#pragma unroll 1
-                            for (int d = 0; d < D; d += 32) {
-                                uint32_t x[32];
-                                tmem_ld32(o + d, x);
-                                tmem_wait_ld();
-#pragma unroll
-                                for (int z = 0; z < 32; ++z) x[z] = __float_as_uint(__uint_as_float(x[z]) * scale);
-                                tmem_store32(o + d, x);
-                            }
-                        }
-                    }
-                    tmem_store32(s, P);
-                    tmem_store32(s + 32, P + 32);
+                    const float step = fmaxf(fmaxf(largest[0], largest[1]), fmaxf(largest[2], largest[3]));
+                    const int ocols = t > t0 ? D : 0;
+                    if (masked)
+                        tc_tile<true>(r, s, o, ocols, param, have, t * kAttTile, step);
+                    else
+                        tc_tile<false>(r, s, o, ocols, param, have, t * kAttTile, step);
                     tmem_stored();
                     tc_fence_before();
                 }
@@ -509,7 +524,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tiles_kernel(co
                 }
             }
             __syncwarp();
-            if (cut && mine) p.stat[2 * slot_row] = r.m, p.stat[2 * slot_row + 1] = r.l;
+            if (cut && mine) p.stat[2 * slot_row] = r.fresh ? kAttNone : r.m, p.stat[2 * slot_row + 1] = r.l;
             if (t0 == 0 && threadIdx.x == 0 && (p.listed || cut)) p.desc[p.listed ? it.index : cta] = att_described(it, sh, cta, cut);
             tc_fence_before();
         }
