@@ -112,52 +112,43 @@ __device__ __noinline__ void tc_rescale(uint32_t s, int cols, uint32_t o, int oc
     tmem_stored();
 }
 
+// Of 16 tokens of a tile, the k-th ones: their scores above the reference, the most of them and the largest step; `in` says which the row sees (MASKED).
+template <bool MASKED>
+__device__ __forceinline__ void tc_scores(const TcRow& r, const uint32_t (&x)[16], const float4* param, int k, uint32_t in, float2 (&d)[8], float& most, float& steps) {
+    const float2 a = both(r.a), b = both(r.b), m = both(-r.m);
+    most = kAttNone;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float4 key = param[16 * k + i];
+        const float2 v = __ffma2_rn(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), make_float2(key.x, key.y), __fmul2_rn(make_float2(key.z, key.w), b));
+        d[i] = __ffma2_rn(v, a, m);
+        if constexpr (MASKED) {   // (what a row does not see may be NaN)
+            if (!((in >> (2 * i)) & 1)) d[i].x = -INFINITY;
+            if (!((in >> (2 * i + 1)) & 1)) d[i].y = -INFINITY;
+            const float4 value = param[16 * k + 8 + i];
+            if ((in >> (2 * i)) & 1) steps = fmaxf(steps, value.x);
+            if ((in >> (2 * i + 1)) & 1) steps = fmaxf(steps, value.y);
+        }
+        most = fmaxf(most, fmaxf(d[i].x, d[i].y));
+    }
+}
+
 // The row's 128 scores of a tile at s become P there.  MASKED: some row does not see all of the tile's tokens.  largest: the tile's largest step.
 template <bool MASKED>
 __device__ __forceinline__ void tc_tile(TcRow& r, uint32_t s, uint32_t o, int ocols, const float4* param, const uint32_t* there, int pos, float largest) {
     float2 sum = make_float2(r.l, 0.0f), low = make_float2(r.lo, 0.0f);
-    uint32_t x[2][16];
-    tmem_ld16(s, x[0]);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {   // 16 scores at a time, the next ones on their way
-        uint32_t in = 0xFFFFu;
-        if constexpr (MASKED) {
-            const int n = min(max(r.lim - pos - 16 * k, 0), 16);
-            in = (there[k >> 1] >> (16 * (k & 1))) & ((1u << n) - 1);
-        }
-        float4 key[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) key[i] = param[16 * k + i];
-        tmem_wait_ld(x[k & 1]);
-        if (k < 7) tmem_ld16(s + 16 * (k + 1), x[(k + 1) & 1]);
-        float2 d[8];
-        float most = kAttNone, steps = k == 0 && !MASKED ? largest : 0.0f;
-        const float2 b = both(r.b), a = both(r.a);
-        float2 m = both(-r.m);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float2 v = __ffma2_rn(make_float2(__uint_as_float(x[k & 1][2 * i]), __uint_as_float(x[k & 1][2 * i + 1])), make_float2(key[i].x, key[i].y), __fmul2_rn(make_float2(key[i].z, key[i].w), b));
-            d[i] = __ffma2_rn(v, a, m);
-            if constexpr (MASKED) {   // (what a row does not see may be NaN)
-                if (!((in >> (2 * i)) & 1)) d[i].x = -INFINITY;
-                if (!((in >> (2 * i + 1)) & 1)) d[i].y = -INFINITY;
-            }
-            most = fmaxf(most, fmaxf(d[i].x, d[i].y));
-        }
-        float4 value[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) value[i] = param[16 * k + 8 + i];
-        if constexpr (MASKED) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (!((in >> (2 * i)) & 1)) value[i].x = value[i].z = 0.0f;
-                if (!((in >> (2 * i + 1)) & 1)) value[i].y = value[i].w = 0.0f;
-                steps = fmaxf(steps, fmaxf(value[i].x, value[i].y));
-            }
-        }
-        if (__any_sync(0xffffffffu, most > kAttSlack || (r.fresh && most > kAttNone) || steps * r.c > 128.0f)) {
+    const auto seen = [&](int k) {
+        if (!MASKED) return 0xFFFFu;
+        const int n = min(max(r.lim - pos - 16 * k, 0), 16);
+        return (there[k >> 1] >> (16 * (k & 1))) & ((1u << n) - 1);
+    };
+    // a new reference where one is wanted, before the k-th 16 scores become P
+    const auto check = [&](int k, float2 (&d)[8], float most, float steps, uint32_t (&coming)[16]) {
+        const bool move = most > kAttSlack || (r.fresh && most > kAttNone);
+        if (__any_sync(0xffffffffu, move || steps * r.c > 128.0f)) {
+            tmem_wait_ld(coming);   // registers that a load has yet to write do not go through a call
             float up = 0.0f, f = 1.0f;
-            if (most > kAttSlack || (r.fresh && most > kAttNone)) {
+            if (move) {
                 up = ceilf(most);
                 if (!r.fresh) f = exp2_int(static_cast<int>(fmaxf(-up, -126.0f)));
                 r.fresh = false;
@@ -170,17 +161,42 @@ __device__ __forceinline__ void tc_tile(TcRow& r, uint32_t s, uint32_t o, int oc
 #pragma unroll
             for (int i = 0; i < 8; ++i) d[i] = make_float2(d[i].x - up, d[i].y - up);
         }
+    };
+    // 16 scores at a time: while some become P, the next ones are looked at and the ones after those are on their way
+    uint32_t x[2][16];
+    float2 d[2][8];
+    float most, steps = MASKED ? 0.0f : largest;
+    tmem_ld16(s, x[0]);
+    tmem_wait_ld(x[0]);
+    tmem_ld16(s + 16, x[1]);
+    tc_scores<MASKED>(r, x[0], param, 0, seen(0), d[0], most, steps);
+    check(0, d[0], most, steps, x[1]);
+#pragma unroll 2   // (all eight in a row, 32 KB of instructions that a warp goes through once a tile, wait for them)
+    for (int k = 0; k < 8; ++k) {
+        steps = 0.0f;
+        if (k < 7) {
+            tmem_wait_ld(x[(k + 1) & 1]);
+            if (k < 6) tmem_ld16(s + 16 * (k + 2), x[k & 1]);
+            tc_scores<MASKED>(r, x[(k + 1) & 1], param, k + 1, seen(k + 1), d[(k + 1) & 1], most, steps);
+        }
+        const uint32_t in = seen(k);
         const float2 c = both(r.c);
         uint32_t P[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float2 e = make_float2(ex2_approx(d[i].x), ex2_approx(d[i].y));
+            float4 value = param[16 * k + 8 + i];
+            if constexpr (MASKED) {
+                if (!((in >> (2 * i)) & 1)) value.x = value.z = 0.0f;
+                if (!((in >> (2 * i + 1)) & 1)) value.y = value.w = 0.0f;
+            }
+            const float2 e = make_float2(ex2_approx(d[k & 1][i].x), ex2_approx(d[k & 1][i].y));
             sum = __fadd2_rn(sum, e);
-            low = __ffma2_rn(e, make_float2(value[i].z, value[i].w), low);
-            const float2 w = __fmul2_rn(e, __fmul2_rn(make_float2(value[i].x, value[i].y), c));
+            low = __ffma2_rn(e, make_float2(value.z, value.w), low);
+            const float2 w = __fmul2_rn(e, __fmul2_rn(make_float2(value.x, value.y), c));
             P[i] = pair_of<__half>(w.x, w.y);
         }
         tmem_store8(s + 8 * k, P);
+        if (k < 7) check(k + 1, d[(k + 1) & 1], most, steps, x[k & 1]);
     }
     r.l = sum.x + sum.y;
     r.lo = low.x + low.y;
@@ -197,17 +213,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tiles_kernel(co
     uint8_t* const smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
     uint8_t* const q_smem = smem;                       // two halves of 128 rows
     uint8_t* const k_smem = q_smem + 2 * Sh::kHalf;
-    uint8_t* const v_smem = k_smem + Sh::kHalf;
-    uint8_t* const ring = v_smem + 2 * Sh::kHalf;
+    uint8_t* const v_smem = k_smem + 2 * Sh::kHalf;   // (keys are widened a tile ahead)
+    uint8_t* const ring = v_smem + Sh::kHalf;
     uint8_t* const params = ring + Sh::kStages * Sh::kStage;
     int* const first = reinterpret_cast<int*>(params + 2 * Sh::kParam);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t full = smem_u32(bars), empty = full + 8 * Sh::kStages, k_full = empty + 8 * Sh::kStages, k_empty = k_full + 8, v_full = k_empty + 8, v_empty = v_full + 16,
-                   s_full = v_empty + 16, p_full = s_full + 16, o_full = p_full + 16, par_full = o_full + 16, q_full = par_full + 16, done = q_full + 8;
+    const uint32_t full = smem_u32(bars), empty = full + 8 * Sh::kStages, k_full = empty + 8 * Sh::kStages, k_empty = k_full + 16, v_full = k_empty + 16, v_empty = v_full + 8,
+                   s_full = v_empty + 8, p_full = s_full + 16, o_full = p_full + 16, par_full = o_full + 16, q_full = par_full + 16, done = q_full + 8;
     if (threadIdx.x == 0) {
         for (int i = 0; i < Sh::kStages; ++i) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, 4);
-        mbar_init(k_full, 4), mbar_init(k_empty, 1);
-        for (int i = 0; i < 2; ++i) mbar_init(s_full + 8 * i, 1), mbar_init(p_full + 8 * i, 4), mbar_init(o_full + 8 * i, 1), mbar_init(par_full + 8 * i, 4), mbar_init(v_full + 8 * i, 4), mbar_init(v_empty + 8 * i, 1);
+        mbar_init(v_full, 4), mbar_init(v_empty, 1);
+        for (int i = 0; i < 2; ++i) mbar_init(s_full + 8 * i, 1), mbar_init(p_full + 8 * i, 4), mbar_init(o_full + 8 * i, 1), mbar_init(par_full + 8 * i, 4), mbar_init(k_full + 8 * i, 4), mbar_init(k_empty + 8 * i, 1);
         mbar_init(q_full, 8), mbar_init(done, 1);
         fence_mbar_init();
         dead = 0;
@@ -289,16 +305,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tiles_kernel(co
         const uint64_t qd = make_sdesc(smem_u32(q_smem), 128), kd = make_sdesc(smem_u32(k_smem), 128), vd = n_major_desc(smem_u32(v_smem), Sh::kBlock);
         int tile = 0, item = 0;   // how many so far
         int turns[2] = {0, 0};    // of P
-        const auto scores = [&](int g, bool last) {
+        const auto scores = [&](int g, int which, bool last) {   // which: of the keys' buffers
             if (lost) return;
             tc_fence_after();
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
                 const uint64_t at = static_cast<uint64_t>((k / 4 * Sh::kBlock + k % 4 * 32) >> 4);
-                mma_f16(tmem + 128 * g, qd + (g * Sh::kHalf >> 4) + at, kd + at, idesc_f16(128, false), k > 0);
+                mma_f16(tmem + 128 * g, qd + (g * Sh::kHalf >> 4) + at, kd + (which * Sh::kHalf >> 4) + at, idesc_f16(128, false), k > 0);
             }
             mma_commit_elect(s_full + 8 * g);
-            if (last) mma_commit_elect(k_empty);
+            if (last) mma_commit_elect(k_empty + 8 * which);
         };
         for (int u = sh.beg; u < sh.end;) {
             const AttItem it = att_item<R>(p, first, u);
@@ -308,21 +324,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tiles_kernel(co
             if (t0 >= t1) continue;
             const int groups = it.rows - it.row0 > 128 ? 2 : 1;
             wait(q_full, item++ & 1, ERR_WAIT_FULL);
-            wait(k_full, tile & 1, ERR_WAIT_FULL);
-            for (int g = 0; g < groups; ++g) scores(g, g == groups - 1);
+            wait(k_full + 8 * (tile & 1), (tile >> 1) & 1, ERR_WAIT_FULL);
+            for (int g = 0; g < groups; ++g) scores(g, tile & 1, g == groups - 1);
             for (int t = t0; t < t1; ++t, ++tile) {
-                wait(v_full + 8 * (tile & 1), (tile >> 1) & 1, ERR_WAIT_FULL);
+                wait(v_full, tile & 1, ERR_WAIT_FULL);
                 for (int g = 0; g < groups; ++g) {
                     wait(p_full + 8 * g, turns[g]++ & 1, ERR_WAIT_ACC);
                     if (lost) continue;
                     tc_fence_after();
 #pragma unroll
                     for (int k = 0; k < 8; ++k)
-                        mma_f16_tmem(tmem + 256 + 128 * g, tmem + 128 * g + 8 * k, vd + (((tile & 1) * Sh::kHalf + k * 2048) >> 4), idesc_f16(D, true), t > t0 || k > 0);
-                    if (g == groups - 1) mma_commit_elect(v_empty + 8 * (tile & 1));
+                        mma_f16_tmem(tmem + 256 + 128 * g, tmem + 128 * g + 8 * k, vd + (k * 2048 >> 4), idesc_f16(D, true), t > t0 || k > 0);
+                    if (g == groups - 1) mma_commit_elect(v_empty);
                     if (t + 1 < t1) {
-                        if (g == 0) wait(k_full, (tile + 1) & 1, ERR_WAIT_FULL);
-                        scores(g, g == groups - 1);
+                        if (g == 0) wait(k_full + 8 * ((tile + 1) & 1), ((tile + 1) >> 1) & 1, ERR_WAIT_FULL);
+                        scores(g, (tile + 1) & 1, g == groups - 1);
                     } else {
                         mma_commit_elect(o_full + 8 * g);
                     }
@@ -364,9 +380,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tiles_kernel(co
                 const uint8_t* K = ring + stage * Sh::kStage;
                 const uint8_t* V = K + Sh::kCodes;
                 wait(full + 8 * stage, phase, ERR_WAIT_FULL);
-                wait(k_empty, (tile & 1) ^ 1, ERR_WAIT_EMPTY);
+                wait(k_empty + 8 * (tile & 1), ((tile >> 1) & 1) ^ 1, ERR_WAIT_EMPTY);
                 if (!lost) {
-                    widen(K, kv[0]);
+                    widen(K, kv[0] + (tile & 1) * Sh::kHalf);
                     uint32_t pk = reinterpret_cast<const uint32_t*>(V + Sh::kCodes)[mine], pv = reinterpret_cast<const uint32_t*>(V + Sh::kCodes + Sh::kPairs)[mine];
                     const bool ok = t * kAttTile + mine < it.seen && ((there[stage] >> (mine >> shift)) & 1);
                     if (!ok) pk = pv = 0;   // what lies there is not looked at
@@ -385,12 +401,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tiles_kernel(co
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(k_full), mbar_arrive(par_full + 8 * (tile & 1));
-                wait(v_empty + 8 * (tile & 1), ((tile >> 1) & 1) ^ 1, ERR_WAIT_EMPTY);
-                if (!lost) widen(V, kv[1] + (tile & 1) * Sh::kHalf);
+                if (lane == 0) mbar_arrive(k_full + 8 * (tile & 1)), mbar_arrive(par_full + 8 * (tile & 1));
+                wait(v_empty, (tile & 1) ^ 1, ERR_WAIT_EMPTY);
+                if (!lost) widen(V, kv[1]);
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(v_full + 8 * (tile & 1)), mbar_arrive(empty + 8 * stage);
+                if (lane == 0) mbar_arrive(v_full), mbar_arrive(empty + 8 * stage);
                 if (++stage == Sh::kStages) stage = 0, phase ^= 1;
             }
         }
