@@ -479,7 +479,7 @@ int ptq8_cache_read(ptq8_ops* ops, const ptq8_cache_rows_args* args, void* strea
 /* out[token][h] = sum_j p_j v_j, p = softmax_j(scale * q[token][h] . k_j), over the positions j up to the token's own, keys and
  * values of head h / (heads / kv_heads).  A token that sees no position gets zeros; tokens of no sequence are left as they
  * were.  Queries are f16 or bf16, the output has their type; sums and the softmax are f32, p (times the value's step) is rounded
- * to f16's 11 bits for its product with the codes.  Rows of keys or values that a token does not see have no part in its
+ * to f16's 11 bits for its product with the codes less eight, 2^-30 of the largest step that the token sees being the finest.  Rows of keys or values that a token does not see have no part in its
  * output, whatever they hold.
  * workspace: device memory of ptq8_cache_attention_workspace() bytes, aligned to 16 bytes, which this call alone uses until its
  * kernels have run: calls on one stream may share it, calls on two streams or of two graphs that may run at once may not. */

@@ -86,7 +86,6 @@ struct TcRow {
 // first `cols` columns at s) and O (`ocols` columns at o) follows.  By a whole warp.
 __device__ __noinline__ void tc_rescale(uint32_t s, int cols, uint32_t o, int ocols, float scale) {
     tmem_stored();
-    const __half2 h = __float2half2_rn(scale);
 #pragma unroll 1
     for (int i = 0; i < cols; i += 8) {
         uint32_t x[8];
@@ -94,9 +93,8 @@ __device__ __noinline__ void tc_rescale(uint32_t s, int cols, uint32_t o, int oc
         tmem_wait_ld();
 #pragma unroll
         for (int z = 0; z < 8; ++z) {
-            __half2 v = *reinterpret_cast<__half2*>(&x[z]);
-            v = __hmul2(v, h);
-            x[z] = *reinterpret_cast<uint32_t*>(&v);
+            const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&x[z]));   // (a scale below 2^-24 is no f16 number, its product may be)
+            x[z] = pair_of<__half>(v.x * scale, v.y * scale);
         }
         tmem_store8(s + i, x);
     }

@@ -145,18 +145,19 @@ struct AttVariant {
     int per_sm, smem;   // of PTQ8_MAX_SEQUENCES
     int (*smem_of)(int seqs);
     int threads;
+    long long work;   // query rows x tokens that a table has room for, from which on it is taken
 };
 
 template <int D, int NT, int RW>
 AttVariant att_variant() {
     using Sh = AttShape<D, NT, RW>;
-    return {D, Sh::R, cache_attention_kernel<D, NT, RW>, Sh::kPerSm, Sh::smem(PTQ8_MAX_SEQUENCES), Sh::smem, kAttThreads};
+    return {D, Sh::R, cache_attention_kernel<D, NT, RW>, Sh::kPerSm, Sh::smem(PTQ8_MAX_SEQUENCES), Sh::smem, kAttThreads, 0};
 }
 
 template <int D>
 AttVariant att_tiles_variant() {
     using Sh = TcAttShape<D>;
-    return {D, kTcRows, cache_attention_tiles_kernel<D>, 1, Sh::smem(PTQ8_MAX_SEQUENCES), Sh::smem, kTcThreads};
+    return {D, kTcRows, cache_attention_tiles_kernel<D>, 1, Sh::smem(PTQ8_MAX_SEQUENCES), Sh::smem, kTcThreads, D == 128 ? 1 << 24 : 1 << 25};
 }
 
 const AttVariant kAttVariants[] = {
@@ -171,12 +172,18 @@ const AttJoin kAttJoins[3][2] = {{cache_attention_join_kernel<64, 1>, cache_atte
                                  {cache_attention_join_kernel<128, 1>, cache_attention_join_kernel<128, kAttJoinWide>},
                                  {cache_attention_join_kernel<256, 1>, cache_attention_join_kernel<256, kAttJoinWide>}};
 
-// The smallest tile that takes a sequence's query rows of a key head on average, or the largest.
-const AttVariant& att_choose(const ptq8_cache_attention_args& a) {
+// The smallest tile that takes a sequence's query rows of a key head on average, or the largest.  Tiles of 256 rows while there is enough
+// to do: their blocks take some us more to begin and to join.  us with them and without, 8 key heads, bf16, sequences x
+// query rows of a key head x positions:
+//              1 x 512 x 500   1 x 384 x 4000   1 x 512 x 4000   1 x 1024 x 4000   8 x 68 x 4000   8 x 136 x 4000   8 x 512 x 4000
+//   D = 64     25   19         37   33          39   38          55   60           64   58         76   81          148   189
+//   D = 128    34   25         47   46          49   56          74   92           79   90         96   128         179   310
+// The host knows only what the table has room for: a table much wider than its sequences are long takes them early.
+const AttVariant& att_choose(const ptq8_cache_attention_args& a, long long room) {
     const long long rows = (a.tokens * (a.heads / a.cache.kv_heads) + a.cache.sequences - 1) / a.cache.sequences;
     const AttVariant* best = nullptr;
     for (const AttVariant& v : kAttVariants)
-        if (v.dim == a.cache.head_dim && (!best || best->rows < rows)) best = &v;
+        if (v.dim == a.cache.head_dim && (!best || best->rows < rows) && a.tokens * a.heads * room >= v.work) best = &v;
     return *best;
 }
 
@@ -209,14 +216,17 @@ int check_attention(ptq8_ops* o, const ptq8_cache_attention_args& a) {
 
 long long workspace_of(const ptq8_ops* o, const ptq8_cache_attention_args& a) {
     if (a.tokens == 0 || a.cache.sequences == 0) return 0;
-    const AttVariant& v = att_choose(a);
-    if (att_by_item(o, a, v, 0)) return 0;   // (whatever the table's width)
-    const long long n = static_cast<long long>(o->sms) * v.per_sm;
-    return 2 * n * v.rows * (v.dim + 2) * 4 + n * static_cast<long long>(sizeof(AttDesc));
+    long long need = 0;
+    for (const long long room : {0LL, 1LL << 31}) {   // whatever the table's width
+        const AttVariant& v = att_choose(a, room);
+        const long long n = static_cast<long long>(o->sms) * v.per_sm;
+        if (!att_by_item(o, a, v, 0)) need = std::max(need, 2 * n * v.rows * (v.dim + 2) * 4 + n * static_cast<long long>(sizeof(AttDesc)));
+    }
+    return need;
 }
 
 int attention_call(ptq8_ops* o, const ptq8_cache_attention_args& a, cudaStream_t st) {
-    const AttVariant& v = att_choose(a);
+    const AttVariant& v = att_choose(a, static_cast<long long>(a.cache.table_width) * a.cache.page);
     AttParams p{};
     p.c = view(a.cache, a.tokens);
     p.q = a.q;
