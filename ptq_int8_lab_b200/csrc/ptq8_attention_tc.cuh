@@ -14,6 +14,13 @@
 //
 // Warps: 0-3 and 4-7 softmax of 128 rows each, in turns with the tensor core: one's products run while the other's
 // exponentials do; 8-11 widen codes; 12 issues MMAs; 13 copies tiles in; 14, 15 idle.
+//
+// What bounds it: the softmax's instructions.  2 x 512 new tokens of 32 heads (8 key heads, D = 128, bf16) over 4500 to 8192
+// positions take 243 us, 420 TFLOP/s, against 463 us with warp-level products; a tile of 128 tokens takes some 7600 cycles, of
+// which the tensor cores need 2000 and the exponentials 2000 (4 a cycle and scheduler); the rest are the other twelve instructions for
+// two scores and what they wait for, with two warps of the softmax a scheduler.  All eight steps of a tile's loop written out, 32 KB of
+// instructions, waited for those (285 us instead of 243).  The tokens' pairs as they lie in the cache, half the bytes from shared memory for four more instructions
+// for two scores: 270.  More registers for the softmax warps by setmaxnreg: 559, the others spilled.
 #pragma once
 
 #include "ptq8_attention.cuh"
@@ -85,6 +92,7 @@ struct TcRow {
 // New references, whole powers of two from the old ones (`up` of them; P so far changes exactly), and new c: what there is of P (the
 // first `cols` columns at s) and O (`ocols` columns at o) follows.  By a whole warp.
 __device__ __noinline__ void tc_rescale(uint32_t s, int cols, uint32_t o, int ocols, float scale) {
+    __syncwarp();
     tmem_stored();
 #pragma unroll 1
     for (int i = 0; i < cols; i += 8) {
@@ -508,6 +516,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tiles_kernel(co
             const long long at = mine ? (it.token0 + row / p.per) * p.o_token + static_cast<long long>(it.head * p.per + row % p.per) * p.o_head : 0;
             for (int d = 0; d < D && !lost; d += 16) {   // (a block that gives up leaves what it would; its row tiles are described all the same)
                 uint32_t x[16];
+                __syncwarp();   // (the loads are the whole warp's; what follows is not)
                 tmem_ld16(o + d, x);
                 tmem_wait_ld(x);
                 if (!mine) continue;

@@ -5,6 +5,9 @@
 // another, so that a tile of keys is one piece of memory.  Step and least are bf16 for its range (half the bytes of
 // f32); what their rounding costs stays inside a step, since the codes are computed with the rounded numbers: least is
 // rounded down and step up, which keeps 15 steps from least no shorter than the row's spread.
+//
+// What bounds them: few rows, a launch after another (32 tokens of 8 heads written and one read 4.1 us); many, instructions: issue 68 %
+// for writing 18 k tokens of 8 heads x 128 (38 us, floor 14) and reading 33 k of 8 x 128 (40 us, floor 26).
 #pragma once
 
 #include <cuda_bf16.h>

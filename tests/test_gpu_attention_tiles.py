@@ -64,6 +64,20 @@ def test_prompts_by_row_tile(ops, dim):  # noqa: F811
 
 
 @pytest.mark.parametrize("dim", [64, 128])
+def test_one_token_of_many_heads(ops, dim):  # noqa: F811
+    """No starts: a token's heads alone fill the tiles."""
+    g = generator(8)
+    lengths = [3000, 77, 0, 129]
+    pages, table = layout(g, lengths, 64, width=ROOM // 64)
+    cache = random_cache(g, pages, 1, 64, dim)
+    q = torch.randn((4, 300, dim), generator=g, device="cuda").to(torch.bfloat16)
+    got = ops.cache_attention(q, cache, table, ints(lengths), out=torch.full_like(q, 3.0))
+    ops.check_device_error()
+    want, bound = reference(q, cache, table, ints(lengths), None, dim ** -0.5, torch.full_like(q, 3.0))
+    assert bool(((got.double() - want).abs() <= bound).all()) and not got[2].any()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
 def test_rows_that_see_nothing(ops, dim):  # noqa: F811
     g = generator(1)
     got = check(ops, g, "bf16", dim, 2, 4, 16, [60, 200], [100, 150], width=ROOM // 16)
