@@ -220,3 +220,31 @@ def test_a_wait_runs_out(dim, per, lengths, news):
         ops.set_wait_test()
         assert torch.equal(ops.cache_attention(*args), good)
         ops.check_device_error()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_two_streams_at_once(dim):
+    """Tiles on one stream and tiles and products on another, each taking the tensor memory that the other leaves."""
+    from ptq_int8_lab_b200.ops import Int8Ops
+    with Int8Ops(0) as one, Int8Ops(0) as two:
+        g = generator(9)
+        pages, table = layout(g, [900], 64, width=ROOM // 64)
+        cache = random_cache(g, pages, 2, 64, dim)
+        q = torch.randn((400, 8, dim), generator=g, device="cuda").to(torch.bfloat16)
+        x, xs = torch.randint(-127, 128, (300, 512), generator=g, device="cuda").to(torch.int8), torch.ones(300, device="cuda")
+        w, ws = torch.randint(-127, 128, (1024, 512), generator=g, device="cuda").to(torch.int8), torch.ones(1024, device="cuda")
+        args = (cache, table, ints([900]), begins([400]))
+        want, product = one.cache_attention(q, *args), one.linear(x, xs, w, ws)
+        need = one.cache_attention_workspace(q, *args)
+        outs = [torch.zeros_like(q) for _ in range(2)]
+        rooms = [torch.empty(need, dtype=torch.uint8, device="cuda") for _ in range(2)]
+        y = torch.zeros_like(product)
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        torch.cuda.synchronize()
+        for _ in range(40):
+            one.cache_attention(q, *args, out=outs[0], workspace=rooms[0], stream=streams[0])
+            two.linear(x, xs, w, ws, out=y, stream=streams[1])
+            two.cache_attention(q, *args, out=outs[1], workspace=rooms[1], stream=streams[1])
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want) and torch.equal(outs[1], want) and torch.equal(y, product)
+        one.check_device_error(), two.check_device_error()
