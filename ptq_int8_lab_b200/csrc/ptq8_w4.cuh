@@ -109,9 +109,10 @@ __device__ __forceinline__ float w4_scale(uint32_t bits, int type) {
 
 // One or two tokens: float multiply-adds on weights that go from memory straight to registers, as the few-token products of
 // int8 codes have it: a warp owns four weight rows (gated: two gate and two up rows), a lane 32 codes of each at a time, KS
-// warps of a block share a row's input features.  A code's byte becomes the float 2^23 + 8 + code by one byte permutation
+// warps of a block share a row's input features.  A code's byte becomes the float 2^11 + 2^-12 (8 + code) by one byte permutation
 // and the code by half of a packed subtraction, exactly; with the packed multiply-adds of T tokens that makes 16 + 4 T
-// instructions for 8 codes, and bounds the kernel together with the launch.  Activations are exact floats here.
+// instructions for 8 codes, and bounds the kernel together with the launch.  Activations are exact floats here.  (All of it times
+// 2^-12, by the exponent of those floats: the largest activations times codes stay within f32.)
 constexpr int kW4FewWarps = 8, kW4FewRows = 4;
 
 template <typename XT, int MT>
@@ -165,7 +166,7 @@ __global__ void __launch_bounds__(32 * kW4FewWarps, 1) linear_w4_few_kernel(cons
                 const uint32_t v = (&w[r].x)[i] ^ 0x88888888u, even = v & 0x0F0F0F0Fu, odd = v >> 4 & 0x0F0F0F0Fu;
 #pragma unroll
                 for (int z = 0; z < 4; ++z) {
-                    const float2 c = __fadd2_rn(make_float2(__uint_as_float(__byte_perm(even, 0x4B000000u, 0x7440 + z)), __uint_as_float(__byte_perm(odd, 0x4B000000u, 0x7440 + z))), both(-8388616.0f));
+                    const float2 c = __fadd2_rn(make_float2(__uint_as_float(__byte_perm(even, 0x45000000u, 0x7440 + z)), __uint_as_float(__byte_perm(odd, 0x45000000u, 0x7440 + z))), both(-0x1.00001p11f));
 #pragma unroll
                     for (int t = 0; t < MT; ++t) sum[r][t] = __ffma2_rn(c, x[t][z], sum[r][t]);
                 }
@@ -197,6 +198,7 @@ __global__ void __launch_bounds__(32 * kW4FewWarps, 1) linear_w4_few_kernel(cons
     }
     const int r = lane / MT, t = lane % MT, c = c0 + (p.gated ? r & 1 : r);
     const bool here = part == 0 && lane < kW4FewRows * MT && c < p.n && t < p.rows;
+    mine *= 0x1p12f;
     if (here && p.bias) mine += p.bias[c + (p.gated && r > 1 ? p.n : 0)];
     const float up = __shfl_down_sync(0xffffffffu, mine, 2 * MT);
     if (here && r < C) store_y(p.y, static_cast<size_t>(t) * p.ldy + c, p.gated ? swiglu(mine, up) : mine, p.y_type);
@@ -262,6 +264,10 @@ __device__ __forceinline__ float w4_value(const uint32_t* raw, int i) {
     return __uint_as_float(i & 1 ? raw[i / 2] & 0xFFFF0000u : raw[i / 2] << 16);
 }
 
+// Outputs are summed in units of 2^11, so that no group's sum of the largest floats, and no power of two that takes one back to
+// its size, leaves f32's range.
+constexpr int kW4Units = 11;
+
 // They become f16, four to a word of weights (codes 0, 4; 1, 5, which come 16 times too large; 2, 6; 3, 7), times a power of two, at
 // to[stride w].  f32: the lanes of even columns take the first f16 of a number, those of odd ones what it leaves.  Beside
 // them, for each piece and column, -8 times its sum and the power of two that products with code * 2^-24 lack.
@@ -281,10 +287,11 @@ __device__ __forceinline__ void w4_fragments(uint4* to, int stride, bool kept, f
     }
     top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const int e = min(max(14 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), -100), 100);
+    // from -113 for the largest floats on; what is below 2^-100 stays below 2^14, and loses places by that much
+    const int e = min(14 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), 114);
     const float up = __int_as_float((e + 127) << 23), up16 = up * 0.0625f;
     // a token that is not finite: NaN (as an infinity times a code of zero is)
-    const float l = isfinite(top) ? __int_as_float(((EXACT ? 0 : 24) - e + 127) << 23) : __int_as_float(0x7FC00000);
+    const float l = isfinite(top) ? __int_as_float(((EXACT ? 0 : 24) - kW4Units - e + 127) << 23) : __int_as_float(0x7FC00000);
     const float lack0 = __shfl_sync(0xffffffffu, l, 8 * t), lack1 = __shfl_sync(0xffffffffu, l, 8 * t + 4);
 #pragma unroll
     for (int j = 0; j < 16 / VB; ++j) {
@@ -577,7 +584,7 @@ __global__ void __launch_bounds__(kW4Threads, 1) linear_w4_kernel(const W4Params
                         if (token >= p.rows) continue;
                         float v[2];
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) v[h] = Sh::kSplit ? acc[r][nt][h].x + acc[r][nt][h].y : col ? acc[r][nt][h].y : acc[r][nt][h].x;
+                        for (int h = 0; h < 2; ++h) v[h] = (Sh::kSplit ? acc[r][nt][h].x + acc[r][nt][h].y : col ? acc[r][nt][h].y : acc[r][nt][h].x) * (1 << kW4Units);
                         const size_t row = static_cast<size_t>(token) * p.ldy;
                         if (p.gated) {
                             const int c = (2 * pair + r) * 8 + rg;
