@@ -2,9 +2,11 @@
 //   y[t][c] = sum_g s[c][g] (sum_{k in group g} code[c][k] x[t][k]) + b[c], then the epilogue
 // for a few tokens, whose activations stay as they are (f32, f16 or bf16).
 //
-// A code enters the tensor cores as it lies in memory: code + 8, masked out of a word, is as f16 the subnormal number
-// (code + 8) * 2^-24 (or 16 times it, for the second code of a byte), exact and without a conversion; the 8 leaves with
-// a product of a constant row, which starts the sum at -8 sum(x).  Activations become f16 times a power of two, which
+// A code enters the tensor cores as a normal f16 number around zero (16 times it, for the second code of a byte): masked out of
+// a word together with the exponent of 1024, less 1032.  (code + 8 alone, as the subnormal number that it is in a word, is an
+// instruction less for two codes, but the tensor cores line the products of a sum up by their operands' exponents, take a
+// subnormal number's for 2^-14, and cut what is below: an activation 2^12 times the others cost an output 2^-10 of itself, even
+// where its code is zero.  8 tokens, 4096 -> 2 x 8192: 14.9 us, 14.8 so.)  Activations become f16 times a power of two, which
 // takes the largest of 128 to 2^14 .. 2^15: what is less than 2^28 below it keeps all places of bf16 and f16.  f32 ones
 // go in as two f16, the second with what the first leaves (22 places), in columns beside each other.  A group's sum is
 // f32 in the tensor cores, and meets its scale in f32.
@@ -15,12 +17,11 @@
 // in some 20 instructions each: 32 of them took 2 us.)  The activations are brought into the products' order in shared
 // memory: once, where they fit there as a whole, else a segment at a time.  Places of the products' inner dimension are
 // dealt to a row's bytes so that a group stays within an MMA (four lanes hold VB bytes each: 32, 64 or 128 codes of a row).
-// EXACT (outputs of 32 bits): codes less eight as normal f16 numbers, for an instruction more for two of them: the tensor cores take
-// a subnormal number's exponent for 2^-14 and cut what is below the largest of a sum (45 tokens x 2000, f32: 8.6e-8 from 64 bits).
+// EXACT (outputs of 32 bits): each product of 16 features begins at zero and is added in f32 (45 tokens x 2000, f32: 8.6e-8 from 64 bits).
 //
 // What bounds it (B200, in a graph of calls): one token, 4096 -> 4096, 4.9 us: latency and launch (3.4 TB/s of weights from L2);
 // 8 tokens, 4096 -> 2 x 8192, 15 us, floor 5.5: the weights' and fragments' way through shared memory and the instructions that mask them
-// (issue 49 %), after 3 us in which every block brings the activations into order; 45 tokens f32, 2000 -> 1270, 10.7 us:
+// (issue 49 %), after 3 us in which every block brings the activations into order; 45 tokens f32, 2000 -> 1270, 10.1 us:
 // that same start, for three passes of 16 tokens.
 #pragma once
 
@@ -210,9 +211,9 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// With every code's sign bit turned a nibble is code + 8: as f16 that times 2^-24 (times 2^-20 for the high one of a byte).
+// With every code's sign bit turned a nibble is code + 8.
 constexpr uint32_t kW4Turn = 0x88888888u, kW4Low = 0x000F000Fu, kW4High = 0x00F000F0u;
-// The code itself (16 times it for the high one) as a normal number: 1024 + 8 + code, less 1032.
+// The code itself (16 times it for the high one) as a normal f16 number: 1024 + 8 + code, less 1032.
 __device__ __forceinline__ uint32_t w4_low(uint32_t word) {
     const uint32_t a = mask_or(word, kW4Low, 0x64006400u), b = 0x64086408u;
     const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
@@ -223,8 +224,6 @@ __device__ __forceinline__ uint32_t w4_high(uint32_t word) {
     const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&r);
 }
-// -8 * 2^-24 and -128 * 2^-24
-constexpr uint32_t kW4ShiftLow = 0x80088008u, kW4ShiftHigh = 0x80808080u;
 
 template <int VB>
 struct W4Pieces {
@@ -270,9 +269,9 @@ constexpr int kW4Units = 11;
 
 // They become f16, four to a word of weights (codes 0, 4; 1, 5, which come 16 times too large; 2, 6; 3, 7), times a power of two, at
 // to[stride w].  f32: the lanes of even columns take the first f16 of a number, those of odd ones what it leaves.  Beside
-// them, for each piece and column, -8 times its sum and the power of two that products with code * 2^-24 lack.
-template <typename XT, int VB, bool EXACT>
-__device__ __forceinline__ void w4_fragments(uint4* to, int stride, bool kept, float2* beside, const uint4 (&x)[2 * sizeof(XT)], int g, int t) {
+// them, for each column, the power of two that its products lack.
+template <typename XT, int VB>
+__device__ __forceinline__ void w4_fragments(uint4* to, int stride, bool kept, float* beside, const uint4 (&x)[2 * sizeof(XT)], int g, int t) {
     const uint32_t* raw = reinterpret_cast<const uint32_t*>(x);
     float top;
     if constexpr (sizeof(XT) == 4) {
@@ -291,31 +290,21 @@ __device__ __forceinline__ void w4_fragments(uint4* to, int stride, bool kept, f
     const int e = min(14 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), 114);
     const float up = __int_as_float((e + 127) << 23), up16 = up * 0.0625f;
     // a token that is not finite: NaN (as an infinity times a code of zero is)
-    const float l = isfinite(top) ? __int_as_float(((EXACT ? 0 : 24) - kW4Units - e + 127) << 23) : __int_as_float(0x7FC00000);
-    const float lack0 = __shfl_sync(0xffffffffu, l, 8 * t), lack1 = __shfl_sync(0xffffffffu, l, 8 * t + 4);
+    if (t == 0) beside[g] = isfinite(top) ? __int_as_float((-kW4Units - e + 127) << 23) : __int_as_float(0x7FC00000);
 #pragma unroll
-    for (int j = 0; j < 16 / VB; ++j) {
-        float shift[4] = {};
+    for (int w = 0; w < 4; ++w) {
+        uint32_t b[4];
 #pragma unroll
-        for (int w = j * (VB / 4); w < (j + 1) * (VB / 4); ++w) {
-            uint32_t b[4];
-#pragma unroll
-            for (int z = 0; z < 4; ++z) {
-                const float u = w4_value<XT>(raw, 8 * w + z) * (z & 1 ? up16 : up), v = w4_value<XT>(raw, 8 * w + z + 4) * (z & 1 ? up16 : up);
-                b[z] = pair_of<__half>(u, v);
-                if constexpr (sizeof(XT) == 4) {
-                    const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&b[z]));
-                    const uint32_t left = pair_of<__half>(u - h.x, v - h.y);
-                    if (g & 1) b[z] = left;
-                }
+        for (int z = 0; z < 4; ++z) {
+            const float u = w4_value<XT>(raw, 8 * w + z) * (z & 1 ? up16 : up), v = w4_value<XT>(raw, 8 * w + z + 4) * (z & 1 ? up16 : up);
+            b[z] = pair_of<__half>(u, v);
+            if constexpr (sizeof(XT) == 4) {
+                const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&b[z]));
+                const uint32_t left = pair_of<__half>(u - h.x, v - h.y);
+                if (g & 1) b[z] = left;
             }
-            if constexpr (!EXACT) {
-                mma_f16(shift, kW4ShiftLow, kW4ShiftLow, kW4ShiftHigh, kW4ShiftHigh, b[0], b[1]);
-                mma_f16(shift, kW4ShiftLow, kW4ShiftLow, kW4ShiftHigh, kW4ShiftHigh, b[2], b[3]);
-            }
-            if (kept) to[stride * w] = make_uint4(b[0], b[1], b[2], b[3]);
         }
-        if (g == 0) *reinterpret_cast<float4*>(beside + j * 8 + 2 * t) = make_float4(shift[0], lack0, shift[1], lack1);
+        if (kept) to[stride * w] = make_uint4(b[0], b[1], b[2], b[3]);
     }
 }
 
@@ -329,7 +318,7 @@ struct W4Shape {
     static constexpr int kSums = kW4Warps * 2 * NT * 128 * 4;
     // of a chunk; columns: those held (fewer than eight where there are no more)
     static constexpr int frag(int columns) { return NT * 4 * columns * 64; }
-    static constexpr int kBeside = NT * kPieces * 64;
+    static constexpr int kBeside = NT * 32;
 };
 
 // What the host has worked out (quotients by numbers that are known at launch only cost a warp some hundred cycles each).
@@ -342,10 +331,8 @@ struct W4Plan {
     int passes;           // over the tokens
 };
 
-// EXACT (outputs of 32 bits): the tensor cores line the products of a sum up by their operands' exponents and cut what is
-// below, and the exponent of a subnormal number is 2^-14 whatever it is.  So codes enter as normal numbers there, for an
-// instruction more for two of them, and each product of 16 features begins at zero and is added in f32 (45 f32 tokens
-// 2000 -> 1270: 2.2e-6 from 64 bits without, 8.6e-8 with).
+// EXACT (outputs of 32 bits): what the tensor cores cut of a sum goes by its largest term, so each product of 16 features begins at
+// zero there and is added in f32.
 template <typename XT, int VB, int NT, bool EXACT>
 __global__ void __launch_bounds__(kW4Threads, 1) linear_w4_kernel(const W4Params p, const W4Plan plan, const __grid_constant__ CUtensorMap map) {
     using Sh = W4Shape<XT, VB, NT>;
@@ -363,7 +350,7 @@ __global__ void __launch_bounds__(kW4Threads, 1) linear_w4_kernel(const W4Params
     uint8_t* ring = smem + warp * plan.stages * kW4Box;
     float* sums = reinterpret_cast<float*>(smem + kW4Warps * plan.stages * kW4Box);   // [warp][2][NT][4][32]
     uint4* frag = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(sums) + Sh::kSums);   // [held][NT][4][columns][4]
-    float2* beside = reinterpret_cast<float2*>(frag + plan.held * NT * 16 * plan.columns);   // [held][NT][PIECES][8]
+    float* beside = reinterpret_cast<float*>(frag + plan.held * NT * 16 * plan.columns);   // [held][NT][8]
     const uint32_t full = smem_u32(bars + warp * kW4MostStages);
     if (lane < plan.stages) mbar_init(full + 8 * lane, 1);
     fence_mbar_init();
@@ -450,7 +437,7 @@ __global__ void __launch_bounds__(kW4Threads, 1) linear_w4_kernel(const W4Params
                             started = true;
                             for (int i = 0; i < plan.stages; ++i) issue();
                         }
-                        w4_fragments<XT, VB, EXACT>(frag + i * 16 * plan.columns + lane, 4 * plan.columns, g < plan.columns, beside + i * PIECES * 8, x, g, t);
+                        w4_fragments<XT, VB>(frag + i * 16 * plan.columns + lane, 4 * plan.columns, g < plan.columns, beside + i * 8, x, g, t);
                     }
                     if (!started) {   // a warp without a share of the activations
                         started = true;
@@ -483,7 +470,7 @@ __global__ void __launch_bounds__(kW4Threads, 1) linear_w4_kernel(const W4Params
                     const uint8_t* tile = ring + stage * kW4Box + rg * 128;
                     // (a lane of a column that holds no token takes the last one's: what it adds to is not used)
                     const uint4* b_at = frag + (c0 - segment * plan.held) * NT * 16 * plan.columns + 4 * min(g, plan.columns - 1) + t;
-                    const float2* beside_at = beside + (c0 - segment * plan.held) * NT * PIECES * 8 + 2 * t;
+                    const float* beside_at = beside + (c0 - segment * plan.held) * NT * 8 + 2 * t;
 #pragma unroll
                     for (int j = 0; j < kW4Run; ++j) {
                         if (j >= n) break;
@@ -506,17 +493,12 @@ __global__ void __launch_bounds__(kW4Threads, 1) linear_w4_kernel(const W4Params
                                     w[0] = *reinterpret_cast<const uint32_t*>(from);
                                 }
                             }
+                        float2 lack[NT];
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) lack[nt] = *reinterpret_cast<const float2*>(beside_at + (j * NT + nt) * 8);
 #pragma unroll
                         for (int i = 0; i < PIECES; ++i) {
-                            float sum[2][NT][4];
-                            float2 lack[NT];
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) {
-                                const float4 v = *reinterpret_cast<const float4*>(beside_at + ((j * NT + nt) * PIECES + i) * 8);
-#pragma unroll
-                                for (int r = 0; r < 2; ++r) sum[r][nt][0] = sum[r][nt][2] = v.x, sum[r][nt][1] = sum[r][nt][3] = v.z;
-                                lack[nt] = make_float2(v.y, v.w);
-                            }
+                            float sum[2][NT][4] = {};
 #pragma unroll
                             for (int w = i * WORDS; w < (i + 1) * WORDS; ++w) {
                                 uint4 b[NT];
@@ -534,8 +516,8 @@ __global__ void __launch_bounds__(kW4Threads, 1) linear_w4_kernel(const W4Params
 #pragma unroll
                                             for (int z = 0; z < 4; ++z) sum[r][nt][z] += one[z] + two[z];
                                         } else {
-                                            mma_f16(sum[r][nt], u & kW4Low, v & kW4Low, u & kW4High, v & kW4High, b[nt].x, b[nt].y);
-                                            mma_f16(sum[r][nt], u8 & kW4Low, v8 & kW4Low, u8 & kW4High, v8 & kW4High, b[nt].z, b[nt].w);
+                                            mma_f16(sum[r][nt], w4_low(u), w4_low(v), w4_high(u), w4_high(v), b[nt].x, b[nt].y);
+                                            mma_f16(sum[r][nt], w4_low(u8), w4_low(v8), w4_high(u8), w4_high(v8), b[nt].z, b[nt].w);
                                         }
                                     }
                                 }
