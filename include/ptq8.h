@@ -396,9 +396,11 @@ int ptq8_ops_set_choice_test(ptq8_ops* ops, int variant, int split);
 
 /* y[t][c] = sum_g w_scale[c][g] * (sum_{k in group g} code[c][k] * x[t][k]) + bias[c], then the epilogue, then one rounding to
  * y's type: float activations, 4-bit weights with a scale per `group` consecutive input features (the last group may be
- * shorter).  Codes lie as ptq8_linear's do with w_bits 4.  Sums are f32; f16 and bf16 activations are not rounded (what is less than
- * 2^-28 of the largest among 128 beside it may lose places), f32 ones keep 22 places.  Outputs of a
- * token that holds NaN or an infinity are NaN or infinite.
+ * shorter).  Codes lie as ptq8_linear's do with w_bits 4.  Sums are f32.
+ * On the tensor cores an activation is an f16 number times a power of two that goes by the largest, top, of the 128 that it lies
+ * among (from a multiple of 128 on): off by at most 2^-39 top, or 2^-35 top where its feature's number is odd.  f16 and bf16 ones
+ * within 2^-24 of top are exact; f32 ones take two f16 numbers and are off by at most 2^-22 of themselves more.  (A top below 2^-100
+ * counts as 2^-100.)  Outputs of a token that holds NaN or an infinity are NaN or infinite.
  * Groups of a multiple of 32 features (or of all) with weights and pitches at multiples of 16 bytes run on the tensor cores;
  * any other group and layout on a slower kernel. */
 typedef struct {

@@ -6,8 +6,8 @@
 // the products:
 //   q . key    = step_k (q . codes) + least_k sum(q)                          queries as f16 times a power of two
 //   sum p v    = sum (p step_v) (codes - 8) + sum p (least_v + 8 step_v)      p step_v as f16, over a bound of step_v
-// A query is scaled by the power of two that takes its largest value to 2^14 .. 2^15: f16 has three bits more than
-// bf16, and what is more than 2^28 below the largest loses places only then.  p step_v is rounded to f16's 11 bits (an
+// A query is scaled by the power of two that takes its largest value to 2^14 .. 2^15, dimensions that meet a byte's second code to
+// a sixteenth of that: what is within 2^28 (2^24) of the largest keeps f16's and bf16's places.  p step_v is rounded to f16's 11 bits (an
 // output has 11, or bf16's 8), with 2^-24 of the largest as its finest step; everything else is f32.
 // The values' codes enter as normal numbers, code - 8, and least + 8 step as their middle, for an instruction more for two of them: terms that do
 // not all have one sign lose less to p's rounding, and the tensor cores, which line the products of a sum up by their operands'

@@ -7,9 +7,10 @@
 // instruction less for two codes, but the tensor cores line the products of a sum up by their operands' exponents, take a
 // subnormal number's for 2^-14, and cut what is below: an activation 2^12 times the others cost an output 2^-10 of itself, even
 // where its code is zero.  8 tokens, 4096 -> 2 x 8192: 14.9 us, 14.8 so.)  Activations become f16 times a power of two, which
-// takes the largest of 128 to 2^14 .. 2^15: what is less than 2^28 below it keeps all places of bf16 and f16.  f32 ones
-// go in as two f16, the second with what the first leaves (22 places), in columns beside each other.  A group's sum is
-// f32 in the tensor cores, and meets its scale in f32.
+// takes the largest of 128 to 2^14 .. 2^15, those that meet a byte's second code a sixteenth of it: what is within 2^28 (2^24) of
+// the largest keeps f16's and bf16's places, and f16's finest step is 2^-38 (2^-34) of it.  f32 ones go in as two f16, the second
+// with what the first leaves (22 places, down to that step), in columns beside each other.  A group's sum is f32 in the tensor cores, and
+// meets its scale in f32.
 //
 // A warp has pairs of tiles of 16 weight rows, or shares each with split - 1 others, which take other input features; their sums
 // meet in shared memory, in a fixed order.  Weights come by TMA through a ring of the warp's own in shared memory, two

@@ -46,3 +46,21 @@ def test_outliers_beside_codes_of_zero(ops, tokens, group, x_type, out_type):  #
             want, bound = expected(x, w, s, group, TYPES[out_type])
             worst = float(((y - want).abs() / bound).max())
             assert worst <= 1.0, (exponent, at, worst)
+
+
+@pytest.mark.parametrize("x_type", ["f16", "bf16"])
+@pytest.mark.parametrize("at", [0, 1])
+def test_activations_within_a_range_are_exact(ops, at, x_type):  # noqa: F811
+    """16-bit activations within 2^-24 of the largest among 128 lose nothing: one of them alone meets a code of one."""
+    g = generator(at)
+    inp = 256
+    for below in (0, 10, 20, 23):
+        x = torch.zeros((8, inp), device="cuda")
+        x[:, 6] = 2.0 ** 8
+        x[:, 130] = 1.0
+        x[:, 32 + at] = (torch.rand(8, generator=g, device="cuda") + 1.0) * 2.0 ** (8 - below - 1)
+        x = x.to(TYPES[x_type])
+        w = torch.zeros((16, inp // 2), dtype=torch.uint8, device="cuda")
+        w[:, 16] = 16 if at else 1
+        y = ops.linear_w4(x, w, torch.ones((16, 2), device="cuda"), 128, dtype=torch.float32)
+        assert torch.equal(y, x[:, 32 + at:33 + at].float().expand(8, 16))
