@@ -39,7 +39,7 @@
 namespace ptq8 {
 
 constexpr int kAttTile = 128, kAttWarps = 4, kAttThreads = 32 * (kAttWarps + 1);
-constexpr float kAttNone = -1e30f;   // reference of a row that has seen nothing
+constexpr float kAttNone = -0x1.fffffep127f;   // reference of a row that has seen nothing: no score is less
 constexpr float kAttSlack = 8.0f;
 // What a row tile costs beside its tokens (queries in, numerators joined and out), in units.
 constexpr int kAttOver = 2;

@@ -1,0 +1,76 @@
+"""cache_attention where scores are far larger than usual, or far apart: few query rows and tiles of many, against 64 bits."""
+import math
+
+import pytest
+import torch
+
+from tests import cache_reference as R
+from tests.test_gpu_cache import TYPES, begins, generator, ints, layout, ops, random_cache  # noqa: F401  (ops: the fixture)
+
+pytestmark = pytest.mark.gpu
+
+ROOM = 1 << 18   # tokens that a table has room for: tiles of 256 rows where a sequence has more than 64
+CASES = [(64, 2, 0), (128, 2, 0), (256, 2, 0), (128, 40, 0), (64, 100, ROOM), (128, 100, ROOM), (256, 100, 0)]   # dim, new tokens, room
+
+
+def expected(q, cache, table, length, news, scale):
+    """(y, bound) like q in 64 bits for one sequence of whole pages.  Scores are off by delta: sums of dim products and a few more
+    roundings of 2^-23 of their terms' magnitudes, counted where a token's p is more than 2^-60 (elsewhere p stays nothing), and
+    not where all such tokens' keys are the same, whose scores are off alike.  A term enters as p step (code - 8), p step rounded to f16 (2^-11, and 2^-31 of the largest step that is seen as its finest), beside
+    p (least + 8 step) in f32."""
+    page, kv, dim = cache[0].shape[2], cache[0].shape[1], q.shape[2]
+    per = q.shape[1] // kv
+    (kc, ks, kl), (vc, vs, vl), _ = R.gathered(cache, table[0], length, page)
+    y, bound = torch.zeros(q.shape, dtype=torch.float64, device="cuda"), torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+    seen = torch.arange(length, device="cuda")[None] <= torch.arange(length - news, length, device="cuda")[:, None]
+    for h in range(kv):
+        x = q[:, h * per:(h + 1) * per].double()
+        z = torch.einsum("npd,jd->npj", x, kc[:, h] * ks[:, h] + kl[:, h]) * scale
+        size = torch.einsum("npd,jd->npj", x.abs(), kc[:, h] * ks[:, h].abs() + kl[:, h].abs()) * abs(scale)
+        z = z.masked_fill(~seen[:, None], -math.inf)
+        z = z - z.amax(-1, keepdim=True)
+        p = torch.exp(z)
+        delta = ((dim + 16) * 2.0 ** -23 * size).masked_fill(p < 2.0 ** -60, 0).amax(-1, keepdim=True)
+        delta = torch.where(((p >= 2.0 ** -60) & (z < 0)).any(-1, keepdim=True), delta, 0.0)
+        p = p / p.sum(-1, keepdim=True)
+        v = vc[:, h] * vs[:, h] + vl[:, h]
+        y[:, h * per:(h + 1) * per] = p @ v
+        steps = (p @ vs[:, h]) * 8
+        adds = length / 16 + 64
+        bound[:, h * per:(h + 1) * per] = (torch.finfo(q.dtype).eps / 2 * 1.01 * (p @ v).abs() + 2.0 ** -11 * steps + 2 * length * 8 * 2.0 ** -31 * vs.max()
+                                           + (adds * 2.0 ** -22 + 2.5 * delta) * (p @ (v.abs() + 8 * vs[:, h])))
+    return y, bound + 2.0 ** -24
+
+
+def constant_keys(cache, table, values):
+    """The keys of position i become values[i] in every dimension (values: f32 that bf16 holds); codes of zero."""
+    page = cache[0].shape[2]
+    at = torch.arange(values.numel(), device="cuda")
+    name = table[0].long()[at // page]
+    cache[0][name, :, at % page] = 0
+    cache[1][name, :, at % page, 0] = 0.0
+    cache[1][name, :, at % page, 1] = values.to(torch.bfloat16)[:, None]
+
+
+def run(ops, g, dim, news, room, length, keys, q_value, kind="bf16", scale=None):  # noqa: F811
+    page = 64
+    pages, table = layout(g, [length], page, width=max(room // page, -(-length // page)))
+    cache = random_cache(g, pages, 2, page, dim)
+    constant_keys(cache, table, keys)
+    q = torch.full((news, 8, dim), q_value, device="cuda").to(TYPES[kind])
+    got = ops.cache_attention(q, cache, table, ints([length]), begins([news]), scale=scale)
+    ops.check_device_error()
+    want, bound = expected(q, cache, table, length, news, dim ** -0.5 if scale is None else scale)
+    far = (got.double() - want).abs()
+    assert bool((far <= bound).all()), (float((far / bound).max()), float(far.max()))
+
+
+@pytest.mark.parametrize("dim,news,room", CASES)
+@pytest.mark.parametrize("top", [1.0, 2.0 ** 100, 2.0 ** 103])
+def test_all_scores_far_below_zero(ops, dim, news, room, top):  # noqa: F811
+    """However low they are, the largest ones have the weight (ties: the same)."""
+    g = generator(dim + news)
+    length = 500
+    keys = -top * (torch.randint(2, 9, (length,), generator=g, device="cuda").float())
+    keys[5], keys[200], keys[390] = -top, -top, -top
+    run(ops, g, dim, news, room, length, keys, 1.0)
