@@ -58,7 +58,9 @@ struct AttParams {
     const void* q;
     void* out;
     long long q_token, q_head, o_token, o_head;   // elements
-    float scale_log2;   // scale * log2(e)
+    // scale * log2(e) = key_scale * score_scale, a power of two: products of scores with that are exact, so that a row's largest score
+    // becomes its reference exactly, however large it is
+    float key_scale, score_scale;
     int per;            // query heads of a key head
     int by_item;        // 1: a CTA per row tile, none cut; 0: equal shares
     int listed;         // descriptions by row tile (one new token per sequence, no more row tiles than CTAs), not by CTA
@@ -136,7 +138,7 @@ struct AttShape {
 template <int D, int NT>
 struct AttRows {
     const uint4* q;               // fragments [NT][D / 32][32 lanes]: of a word of keys, those of its codes 0, 4; 1, 5; 2, 6; 3, 7
-    float2 a[NT], b[NT];          // score in powers of two = a * (step (q . codes) + least b)
+    float2 a[NT], b[NT];          // score in powers of two = a * (step (q . codes) + least b), step and least times key_scale; a: a power of two
     float2 m[NT], l[NT], lo[NT];  // reference, sum of p, sum of p (least_v + 8 step_v)
     int lim[NT][2];               // positions that the row sees
     float o[D / 16][NT][4];
@@ -208,7 +210,7 @@ __device__ __forceinline__ void att_queries(const AttParams& p, AttRows<D, NT>& 
                                                             pair_of<__half>(x[2], x[6]), pair_of<__half>(x[3] * 0.0625f, x[7] * 0.0625f));
         }
         // the products are 2^(e - 24) of the true ones; NaN and infinities in a row make all of its scores NaN
-        const float a = isfinite(top) ? exp2_int(24 - e) * p.scale_log2 : __int_as_float(0x7FC00000);
+        const float a = isfinite(top) ? exp2_int(24 - e) * p.score_scale : __int_as_float(0x7FC00000);
         const float b = sum * 0x1p-24f;
         r.a[nt] = make_float2(__shfl_sync(0xffffffffu, a, 8 * t), __shfl_sync(0xffffffffu, a, 8 * t + 4));
         r.b[nt] = make_float2(__shfl_sync(0xffffffffu, b, 8 * t), __shfl_sync(0xffffffffu, b, 8 * t + 4));
@@ -251,8 +253,8 @@ __device__ __forceinline__ uint32_t centred_high(uint32_t word) {
 // all of them, or not all are there: those before position `seen`, where bit i of `pieces` is set for piece i of the tile
 // (1 << piece_shift tokens).
 template <int D, int NT, int H, bool MASKED>
-__device__ __forceinline__ void att_step(AttRows<D, NT>& r, const uint8_t* K, const uint8_t* V, const uint32_t* KS, const uint32_t* VS, int tk,
-                                         int pos, int seen, uint32_t pieces, int piece_shift) {
+__device__ __forceinline__ void att_step(AttRows<D, NT>& r, const uint8_t* K, const uint8_t* V, const uint32_t* KS, const uint32_t* VS, float key_scale,
+                                         int tk, int pos, int seen, uint32_t pieces, int piece_shift) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     // row m of a product is token m ^ (m / 2 % 2): the lanes that read values together then meet fewer banks twice
     const int pg = g ^ ((g >> 1) & 1);
@@ -300,7 +302,7 @@ __device__ __forceinline__ void att_step(AttRows<D, NT>& r, const uint8_t* K, co
         for (int i = 0; i < 2; ++i) {
             vstep[h][i] = __uint_as_float(pv[h][i] << 16);
             if (!MASKED) steps[0].x = fmaxf(steps[0].x, vstep[h][i]);
-            const float2 step = both(__uint_as_float(pk[h][i] << 16)), least = both(__uint_as_float(pk[h][i] & 0xFFFF0000u));
+            const float2 step = both(__uint_as_float(pk[h][i] << 16) * key_scale), least = both(__uint_as_float(pk[h][i] & 0xFFFF0000u) * key_scale);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 float2 v = __ffma2_rn(make_float2(x[h][nt][2 * i], x[h][nt][2 * i + 1]), step, __fmul2_rn(least, r.b[nt]));
@@ -681,9 +683,9 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT, RW>::kPerSm) cach
                 for (int tk = tw * 16 * H; tk < kAttTile; tk += TW * 16 * H) {
                     const int pos = tile * kAttTile + tk;
                     if (whole && pos + 16 * H <= all && !r.apart)
-                        att_step<D, NT, H, false>(r, K, V, KS, VS, tk, pos, it.seen, have, shift);
+                        att_step<D, NT, H, false>(r, K, V, KS, VS, p.key_scale, tk, pos, it.seen, have, shift);
                     else if (pos < it.seen)
-                        att_step<D, NT, H, true>(r, K, V, KS, VS, tk, pos, it.seen, have, shift);
+                        att_step<D, NT, H, true>(r, K, V, KS, VS, p.key_scale, tk, pos, it.seen, have, shift);
                 }
             }
             __syncwarp();

@@ -118,24 +118,23 @@ __device__ __noinline__ void tc_rescale(uint32_t s, int cols, uint32_t o, int oc
     tmem_stored();
 }
 
-// Of 16 tokens of a tile, the k-th ones: their scores above the reference, the most of them and the largest step; `in` says which the row sees (MASKED).
+// Of 16 tokens of a tile, the k-th ones: their scores over a, the most of them and the largest step; `in` says which the row sees (MASKED).
 template <bool MASKED>
-__device__ __forceinline__ void tc_scores(const TcRow& r, const uint32_t (&x)[16], const float4* param, int k, uint32_t in, float2 (&d)[8], float& most, float& steps) {
-    const float2 a = both(r.a), b = both(r.b), m = both(-r.m);
-    most = kAttNone;
+__device__ __forceinline__ void tc_scores(const TcRow& r, const uint32_t (&x)[16], const float4* param, int k, uint32_t in, float2 (&v)[8], float& most, float& steps) {
+    const float2 b = both(r.b);
+    most = -INFINITY;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const float4 key = param[16 * k + i];
-        const float2 v = __ffma2_rn(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), make_float2(key.x, key.y), __fmul2_rn(make_float2(key.z, key.w), b));
-        d[i] = __ffma2_rn(v, a, m);
+        v[i] = __ffma2_rn(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), make_float2(key.x, key.y), __fmul2_rn(make_float2(key.z, key.w), b));
         if constexpr (MASKED) {   // (what a row does not see may be NaN)
-            if (!((in >> (2 * i)) & 1)) d[i].x = -INFINITY;
-            if (!((in >> (2 * i + 1)) & 1)) d[i].y = -INFINITY;
+            if (!((in >> (2 * i)) & 1)) v[i].x = -INFINITY;
+            if (!((in >> (2 * i + 1)) & 1)) v[i].y = -INFINITY;
             const float4 value = param[16 * k + 8 + i];
             if ((in >> (2 * i)) & 1) steps = fmaxf(steps, value.x);
             if ((in >> (2 * i + 1)) & 1) steps = fmaxf(steps, value.y);
         }
-        most = fmaxf(most, fmaxf(d[i].x, d[i].y));
+        most = fmaxf(most, fmaxf(v[i].x, v[i].y));
     }
 }
 
@@ -148,42 +147,52 @@ __device__ __forceinline__ void tc_tile(TcRow& r, uint32_t s, uint32_t o, int oc
         const int n = min(max(r.lim - pos - 16 * k, 0), 16);
         return (there[k >> 1] >> (16 * (k & 1))) & ((1u << n) - 1);
     };
-    // a new reference where one is wanted, before the k-th 16 scores become P
-    const auto check = [&](int k, float2 (&d)[8], float most, float steps, uint32_t (&coming)[16]) {
-        const bool move = most > kAttSlack || (r.fresh && most > kAttNone);
+    // A new reference where one is wanted, before the k-th 16 scores become P.  (Scores are kept as they are until then: a difference from a
+    // reference far below them would say only roughly how far they are from the new one.)
+    const auto check = [&](int k, float2 (&v)[8], float most, float steps, uint32_t (&coming)[16]) {
+        const float top = most * r.a;   // (a: a power of two)
+        const bool move = top - r.m > kAttSlack || (r.fresh && top > kAttNone);
         if (__any_sync(0xffffffffu, move || steps * r.c > 128.0f)) {
             tmem_wait_ld(coming);   // registers that a load has yet to write do not go through a call
-            float up = 0.0f, f = 1.0f;
+            float f = 1.0f;
             if (move) {
-                up = ceilf(most);
-                if (!r.fresh) f = exp2_int(static_cast<int>(fmaxf(-up, -126.0f)));
-                r.fresh = false;
+                const float m = ceilf(top);
+                if (!r.fresh) f = exp2_int(static_cast<int>(fmaxf(r.m - m, -126.0f)));
+                r.m = m, r.fresh = false;
             }
             float c = r.c;
             if (steps * r.c > 128.0f) c = exp2_int(7 - min(static_cast<int>(__float_as_uint(steps) >> 23) - 126, 127));
             tc_rescale(s, 8 * k, o, ocols, f * power_ratio(c, r.c));
-            r.m += up, r.c = c;
+            r.c = c;
             sum = __fmul2_rn(sum, both(f)), low = __fmul2_rn(low, both(f));
+        }
+        const uint32_t in = seen(k);
+        const float2 a = both(r.a), m = both(-r.m);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) d[i] = make_float2(d[i].x - up, d[i].y - up);
+        for (int i = 0; i < 8; ++i) {
+            v[i] = __ffma2_rn(v[i], a, m);
+            if constexpr (MASKED) {   // (a may be zero or NaN)
+                if (!((in >> (2 * i)) & 1)) v[i].x = -INFINITY;
+                if (!((in >> (2 * i + 1)) & 1)) v[i].y = -INFINITY;
+            }
         }
     };
     // 16 scores at a time: while some become P, the next ones are looked at and the ones after those are on their way
     uint32_t x[2][16];
-    float2 d[2][8];
+    float2 v[2][8];
     float most, steps = MASKED ? 0.0f : largest;
     tmem_ld16(s, x[0]);
     tmem_wait_ld(x[0]);
     tmem_ld16(s + 16, x[1]);
-    tc_scores<MASKED>(r, x[0], param, 0, seen(0), d[0], most, steps);
-    check(0, d[0], most, steps, x[1]);
+    tc_scores<MASKED>(r, x[0], param, 0, seen(0), v[0], most, steps);
+    check(0, v[0], most, steps, x[1]);
 #pragma unroll 2   // (all eight in a row, 32 KB of instructions that a warp goes through once a tile, wait for them)
     for (int k = 0; k < 8; ++k) {
         steps = 0.0f;
         if (k < 7) {
             tmem_wait_ld(x[(k + 1) & 1]);
             if (k < 6) tmem_ld16(s + 16 * (k + 2), x[k & 1]);
-            tc_scores<MASKED>(r, x[(k + 1) & 1], param, k + 1, seen(k + 1), d[(k + 1) & 1], most, steps);
+            tc_scores<MASKED>(r, x[(k + 1) & 1], param, k + 1, seen(k + 1), v[(k + 1) & 1], most, steps);
         }
         const uint32_t in = seen(k);
         const float2 c = both(r.c);
@@ -195,14 +204,14 @@ __device__ __forceinline__ void tc_tile(TcRow& r, uint32_t s, uint32_t o, int oc
                 if (!((in >> (2 * i)) & 1)) value.x = value.z = 0.0f;
                 if (!((in >> (2 * i + 1)) & 1)) value.y = value.w = 0.0f;
             }
-            const float2 e = make_float2(ex2_approx(d[k & 1][i].x), ex2_approx(d[k & 1][i].y));
+            const float2 e = make_float2(ex2_approx(v[k & 1][i].x), ex2_approx(v[k & 1][i].y));
             sum = __fadd2_rn(sum, e);
             low = __ffma2_rn(e, make_float2(value.z, value.w), low);
             const float2 w = __fmul2_rn(e, __fmul2_rn(make_float2(value.x, value.y), c));
             P[i] = pair_of<__half>(w.x, w.y);
         }
         tmem_store8(s + 8 * k, P);
-        if (k < 7) check(k + 1, d[(k + 1) & 1], most, steps, x[k & 1]);
+        if (k < 7) check(k + 1, v[(k + 1) & 1], most, steps, x[k & 1]);
     }
     r.l = sum.x + sum.y;
     r.lo = low.x + low.y;
@@ -392,9 +401,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tiles_kernel(co
                     uint32_t pk = reinterpret_cast<const uint32_t*>(V + Sh::kCodes)[mine], pv = reinterpret_cast<const uint32_t*>(V + Sh::kCodes + Sh::kPairs)[mine];
                     const bool ok = t * kAttTile + mine < it.seen && ((there[stage] >> (mine >> shift)) & 1);
                     if (!ok) pk = pv = 0;   // what lies there is not looked at
-                    const float ks = __uint_as_float(pk << 16), vs = __uint_as_float(pv << 16);
+                    const float ks = __uint_as_float(pk << 16) * p.key_scale, vs = __uint_as_float(pv << 16);
                     float* to = reinterpret_cast<float*>(params + (tile & 1) * Sh::kParam) + mine / 16 * 64 + mine % 16 / 2 * 4 + mine % 2;
-                    to[0] = ks, to[2] = __fmaf_rn(8.0f, ks, __uint_as_float(pk & 0xFFFF0000u));
+                    to[0] = ks, to[2] = __fmaf_rn(8.0f, ks, __uint_as_float(pk & 0xFFFF0000u) * p.key_scale);
                     to[32] = vs, to[34] = __fmaf_rn(8.0f, vs, __uint_as_float(pv & 0xFFFF0000u));
                     const uint32_t have = __ballot_sync(0xffffffffu, ok);
                     float most = fmaxf(vs, 0.0f);   // (NaN counts for nothing)
@@ -471,7 +480,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tiles_kernel(co
                                  : "memory");
                 }
                 // NaN and infinities in a row make all of its scores NaN
-                r.a = isfinite(top) ? exp2_int(-e) * p.scale_log2 : __int_as_float(0x7FC00000);
+                r.a = isfinite(top) ? exp2_int(-e) * p.score_scale : __int_as_float(0x7FC00000);
                 r.b = sum;
                 r.m = r.l = r.lo = 0.0f, r.c = 0x1p120f, r.fresh = true;
                 r.lim = mine ? static_cast<int>(min(max(it.len - it.n + row / p.per + 1, 0LL), cap)) : 0x7FFFFFFF;

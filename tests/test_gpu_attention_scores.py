@@ -74,3 +74,29 @@ def test_all_scores_far_below_zero(ops, dim, news, room, top):  # noqa: F811
     keys = -top * (torch.randint(2, 9, (length,), generator=g, device="cuda").float())
     keys[5], keys[200], keys[390] = -top, -top, -top
     run(ops, g, dim, news, room, length, keys, 1.0)
+
+
+@pytest.mark.parametrize("dim,news,room", CASES)
+@pytest.mark.parametrize("scale", [None, 0.3, -0.7])
+@pytest.mark.parametrize("top", [2.0 ** 16, 2.0 ** 24, 2.0 ** 30, 2.0 ** 60, 2.0 ** 100])
+def test_large_scores(ops, dim, news, room, top, scale):  # noqa: F811
+    """Scores of any size: the largest ones share the weight, wherever they lie."""
+    g = generator(dim + news)
+    length = 500
+    keys = top * torch.randint(-8, 9, (length,), generator=g, device="cuda").float()
+    run(ops, g, dim, news, room, length, keys, 1.0, scale=scale)
+    keys = top * (1 + torch.arange(length, device="cuda") // 90 / 128)   # growing, each of them a hundred times
+    run(ops, g, dim, news, room, length, keys, 1.0, scale=scale)
+
+
+@pytest.mark.parametrize("dim,news,room", CASES)
+@pytest.mark.parametrize("low", [2.0 ** 10, 2.0 ** 17, 2.0 ** 20, 2.0 ** 30, 2.0 ** 80])
+@pytest.mark.parametrize("first", [16, 40, 128, 300])
+def test_ordinary_scores_after_far_lower_ones(ops, dim, news, room, low, first):  # noqa: F811
+    g = generator(first)
+    length = 450
+    keys = torch.randn(length, generator=g, device="cuda").to(torch.bfloat16).float() * 0.25
+    keys[:first] = -low * (1 + torch.arange(first, device="cuda") % 3)
+    run(ops, g, dim, news, room, length, keys, 1.0)
+    keys = keys.flip(0)
+    run(ops, g, dim, news, room, length, keys, 1.0)
