@@ -482,7 +482,9 @@ int ptq8_cache_read(ptq8_ops* ops, const ptq8_cache_rows_args* args, void* strea
  * values of head h / (heads / kv_heads).  A token that sees no position gets zeros; tokens of no sequence are left as they
  * were.  Queries are f16 or bf16, the output has their type; sums and the softmax are f32, p (times the value's step) is rounded
  * to f16's 11 bits for its product with the codes less eight, 2^-30 of the largest step that the token sees being the finest.  Rows of keys or values that a token does not see have no part in its
- * output, whatever they hold.
+ * output, whatever they hold.  Queries are f16 numbers times a power of two that goes by a row's largest: off by at most 2^-39 of it,
+ * or 2^-35 in dimensions of odd number.  Any finite query is taken; keys up to 2^115, and scores (times log2(e)) as well as sums of p v
+ * (p up to 2^8 a position, before they are divided by the sum of p), that f32 numbers hold.
  * workspace: device memory of ptq8_cache_attention_workspace() bytes, aligned to 16 bytes, which this call alone uses until its
  * kernels have run: calls on one stream may share it, calls on two streams or of two graphs that may run at once may not. */
 typedef struct {

@@ -58,7 +58,7 @@ struct AttParams {
     const void* q;
     void* out;
     long long q_token, q_head, o_token, o_head;   // elements
-    // scale * log2(e) = key_scale * score_scale, a power of two: products of scores with that are exact, so that a row's largest score
+    // scale * log2(e) = 2^kAttKeys key_scale * score_scale, a power of two: products of scores with that are exact, so that a row's largest score
     // becomes its reference exactly, however large it is
     float key_scale, score_scale;
     int per;            // query heads of a key head
@@ -108,6 +108,13 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[W], const uint8_t* p) {
 
 // 2^e for e within -126 .. 127.
 __device__ __forceinline__ float exp2_int(int e) { return __int_as_float((e + 127) << 23); }
+
+// 2^e takes a query's largest value to 2^14 .. 2^15 (below 2^-112 it stays below, as subnormal numbers do).
+__device__ __forceinline__ int att_power(float top) { return min(14 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), 126); }
+
+// Keys are multiplied by 2^-kAttKeys (in key_scale), so that neither what takes a product back to its size, 2^(kAttKeys - e), leaves f32's
+// range for any query, nor products with queries of 2^14 do for keys up to 2^115.
+constexpr int kAttKeys = 13;
 
 // a / b of powers of two within 2^+-121, 2^-126 at least.
 __device__ __forceinline__ float power_ratio(float a, float b) {
@@ -192,8 +199,7 @@ __device__ __forceinline__ void att_queries(const AttParams& p, AttRows<D, NT>& 
         for (int k = 0; k < DL; ++k) top = max_nan(top, fabsf(f[k]));
         top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // 2^e takes the largest to 2^14 .. 2^15 (rows below 2^-86 stay below; their scores are zero for any key)
-        const int e = min(max(14 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), -100), 100);
+        const int e = att_power(top);
         const float up = exp2_int(e);
 #pragma unroll
         for (int k = 0; k < DL; ++k) {
@@ -209,8 +215,8 @@ __device__ __forceinline__ void att_queries(const AttParams& p, AttRows<D, NT>& 
             q[(nt * (D / 32) + w) * 32 + lane] = make_uint4(pair_of<__half>(x[0], x[4]), pair_of<__half>(x[1] * 0.0625f, x[5] * 0.0625f),
                                                             pair_of<__half>(x[2], x[6]), pair_of<__half>(x[3] * 0.0625f, x[7] * 0.0625f));
         }
-        // the products are 2^(e - 24) of the true ones; NaN and infinities in a row make all of its scores NaN
-        const float a = isfinite(top) ? exp2_int(24 - e) * p.score_scale : __int_as_float(0x7FC00000);
+        // the products are 2^(e - 24) of the true ones, keys 2^(24 - 13); NaN and infinities in a row make all of its scores NaN
+        const float a = isfinite(top) ? exp2_int(kAttKeys - e) * p.score_scale : __int_as_float(0x7FC00000);
         const float b = sum * 0x1p-24f;
         r.a[nt] = make_float2(__shfl_sync(0xffffffffu, a, 8 * t), __shfl_sync(0xffffffffu, a, 8 * t + 4));
         r.b[nt] = make_float2(__shfl_sync(0xffffffffu, b, 8 * t), __shfl_sync(0xffffffffu, b, 8 * t + 4));
@@ -639,6 +645,7 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT, RW>::kPerSm) cach
 
     // ---- the computing warps
     const int rw = warp % RW, tw = warp / RW;   // which rows, which tokens of a tile
+    const float key_scale = p.key_scale * 0x1p24f;   // (codes are 2^-24 of themselves)
     const int g = lane >> 2, t = lane & 3;
     AttRows<D, NT> r;
     bool lost = false;
@@ -683,9 +690,9 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT, RW>::kPerSm) cach
                 for (int tk = tw * 16 * H; tk < kAttTile; tk += TW * 16 * H) {
                     const int pos = tile * kAttTile + tk;
                     if (whole && pos + 16 * H <= all && !r.apart)
-                        att_step<D, NT, H, false>(r, K, V, KS, VS, p.key_scale, tk, pos, it.seen, have, shift);
+                        att_step<D, NT, H, false>(r, K, V, KS, VS, key_scale, tk, pos, it.seen, have, shift);
                     else if (pos < it.seen)
-                        att_step<D, NT, H, true>(r, K, V, KS, VS, p.key_scale, tk, pos, it.seen, have, shift);
+                        att_step<D, NT, H, true>(r, K, V, KS, VS, key_scale, tk, pos, it.seen, have, shift);
                 }
             }
             __syncwarp();

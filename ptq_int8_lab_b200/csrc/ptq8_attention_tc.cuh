@@ -443,7 +443,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tiles_kernel(co
             const long long from = mine ? (it.token0 + row / p.per) * p.q_token + static_cast<long long>(it.head * p.per + row % p.per) * p.q_head : 0;
             TcRow r;
             {   // the row's queries: scaled so that the largest is 2^14 .. 2^15
-                uint32_t top_bits = 0;
                 float top = 0.0f, sum = 0.0f;
                 const auto value = [&](int k) { return mine ? att_value(p.q, from + k, p.type) : 0.0f; };
                 const auto eight = [&](int k, float (&f)[8]) {
@@ -464,8 +463,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tiles_kernel(co
 #pragma unroll
                     for (int z = 0; z < 8; ++z) top = max_nan(top, fabsf(f[z]));
                 }
-                top_bits = __float_as_uint(top);
-                const int e = min(max(14 - (static_cast<int>(top_bits >> 23) - 127), -100), 100);
+                const int e = att_power(top);
                 const float up = exp2_int(e);
                 const uint32_t to = smem_u32(q_smem) + g * Sh::kHalf + my * 128;
 #pragma unroll 4
@@ -480,7 +478,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tiles_kernel(co
                                  : "memory");
                 }
                 // NaN and infinities in a row make all of its scores NaN
-                r.a = isfinite(top) ? exp2_int(-e) * p.score_scale : __int_as_float(0x7FC00000);
+                r.a = isfinite(top) ? exp2_int(kAttKeys - e) * p.score_scale : __int_as_float(0x7FC00000);
                 r.b = sum;
                 r.m = r.l = r.lo = 0.0f, r.c = 0x1p120f, r.fresh = true;
                 r.lim = mine ? static_cast<int>(min(max(it.len - it.n + row / p.per + 1, 0LL), cap)) : 0x7FFFFFFF;

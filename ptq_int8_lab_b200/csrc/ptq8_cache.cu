@@ -234,8 +234,8 @@ int attention_call(ptq8_ops* o, const ptq8_cache_attention_args& a, cudaStream_t
     p.q_token = a.q_token, p.q_head = a.q_head, p.o_token = a.out_token, p.o_head = a.out_head;
     int power = 0;
     const double fraction = std::frexp(a.scale * 1.4426950408889634, &power);
-    const int held = std::min(std::max(power, -126), 127);   // (a power of two that is a float)
-    p.key_scale = fraction == 0.0 ? 1.0f : static_cast<float>(std::ldexp(fraction, power - held));
+    const int held = std::min(std::max(power, -126), 1);   // (with what takes the largest queries' products back, a power of two that is a float)
+    p.key_scale = fraction == 0.0 ? std::ldexp(1.0f, -kAttKeys) : static_cast<float>(std::ldexp(fraction, power - held - kAttKeys));
     p.score_scale = fraction == 0.0 ? 0.0f : std::ldexp(1.0f, held);
     p.per = a.heads / a.cache.kv_heads;
     p.by_item = att_by_item(o, a, v, a.cache.table_width);

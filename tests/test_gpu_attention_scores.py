@@ -100,3 +100,31 @@ def test_ordinary_scores_after_far_lower_ones(ops, dim, news, room, low, first):
     run(ops, g, dim, news, room, length, keys, 1.0)
     keys = keys.flip(0)
     run(ops, g, dim, news, room, length, keys, 1.0)
+
+
+@pytest.mark.parametrize("dim,news,room", CASES)
+@pytest.mark.parametrize("exponent", [-120, -110, -60, 60, 115, 117, 120, 126])
+def test_queries_of_any_size(ops, dim, news, room, exponent):  # noqa: F811
+    """Queries over bf16's range, keys so that the scores are ordinary ones: as accurate as any."""
+    g = generator(dim + news)
+    length, page = 500, 64
+    pages, table = layout(g, [length], page, width=max(room // page, -(-length // page)))
+    cache = random_cache(g, pages, 2, page, dim)
+    cache[1].copy_((cache[1].float() * 2.0 ** -max(-110, min(exponent, 118))).to(torch.bfloat16))
+    q = (torch.randn((news, 8, dim), generator=g, device="cuda").clamp(-1.9, 1.9) * 2.0 ** exponent).to(torch.bfloat16)
+    q[0, 0] = 0
+    args = (table, ints([length]), begins([news]))
+    got = ops.cache_attention(q, cache, *args).double()
+    want, bound = expected(q, cache, table, length, news, dim ** -0.5)
+    assert bool(((got - want).abs() <= bound).all()), float(((got - want).abs() / bound).max())
+    ops.check_device_error()
+
+
+@pytest.mark.parametrize("dim,news,room", CASES)
+def test_keys_and_scores_near_the_largest_float(ops, dim, news, room):  # noqa: F811
+    g = generator(dim + news)
+    length = 300
+    for top, q_value in ((2.0 ** 112, 1.0), (2.0 ** 112, 2.0 ** -100), (2.0 ** -8, 1.5 * 2.0 ** 120)):
+        keys = top * torch.randint(-8, 9, (length,), generator=g, device="cuda").float()
+        run(ops, g, dim, news, room, length, keys, q_value, scale=2.0 ** -5)
+        run(ops, g, dim, news, room, length, keys, -q_value)
