@@ -1,18 +1,18 @@
 // Attention over the cache of 4-bit keys and values.
 //
-// A code enters the tensor cores as it lies in the cache: four bits masked out of a word are, read as two f16, the
-// subnormal numbers code * 2^-24 (or 16 code * 2^-24, the second code of a byte), exact, with no conversion at all.
-// Five instructions widen eight codes; the powers of two, the steps and the least values go into the numbers around
-// the products:
-//   q . key    = step_k (q . codes) + least_k sum(q)                          queries as f16 times a power of two
+// A code enters the tensor cores as a normal f16 number around zero (16 times it, for the second code of a byte): masked out of a word
+// together with the exponent of 1024, less 1032.  Nine instructions widen eight codes; the steps and the middles go into the numbers
+// around the products:
+//   q . key    = step_k (q . (codes - 8)) + (least_k + 8 step_k) sum(q)       queries as f16 times a power of two
 //   sum p v    = sum (p step_v) (codes - 8) + sum p (least_v + 8 step_v)      p step_v as f16, over a bound of step_v
 // A query is scaled by the power of two that takes its largest value to 2^14 .. 2^15, dimensions that meet a byte's second code to
 // a sixteenth of that: what is within 2^28 (2^24) of the largest keeps f16's and bf16's places.  p step_v is rounded to f16's 11 bits (an
 // output has 11, or bf16's 8), with 2^-24 of the largest as its finest step; everything else is f32.
-// The values' codes enter as normal numbers, code - 8, and least + 8 step as their middle, for an instruction more for two of them: terms that do
-// not all have one sign lose less to p's rounding, and the tensor cores, which line the products of a sum up by their operands'
-// exponents and cut what is below, take a subnormal number's exponent for 2^-14.  (131072 f16 tokens, which average to 0.4 % of
-// a value: 7.5e-4 from 64 bits with codes as for the keys, 2.7e-4 like this; the output's own rounding is 2.1e-4.)
+// (The four bits alone are, read as f16, the subnormal number code * 2^-24: five instructions for eight codes.  But terms that do not all
+// have one sign lose less to p's rounding, and the tensor cores, which line the products of a sum up by their operands' exponents and
+// cut what is below, take a subnormal number's exponent for 2^-14.  131072 f16 tokens, which average to 0.4 % of a value: 7.5e-4 from 64
+// bits with such codes of values, 2.7e-4 like this; the output's own rounding is 2.1e-4.  One dimension of queries 2^12 times the
+// others, where keys are zero: 4e-3 with such codes of keys.)
 //
 // A warp takes 16 tokens as the rows of its products, 8 NT query rows (query token x head of a key's group) as
 // the columns: keys codes [16 tokens x D] x queries [D x rows], then values codes [D x 16 tokens] x p [16 tokens x rows].
@@ -145,7 +145,7 @@ struct AttShape {
 template <int D, int NT>
 struct AttRows {
     const uint4* q;               // fragments [NT][D / 32][32 lanes]: of a word of keys, those of its codes 0, 4; 1, 5; 2, 6; 3, 7
-    float2 a[NT], b[NT];          // score in powers of two = a * (step (q . codes) + least b), step and least times key_scale; a: a power of two
+    float2 a[NT], b[NT];          // score in powers of two = a * (step (q . (codes - 8)) + middle b), step and middle times key_scale; a: a power of two
     float2 m[NT], l[NT], lo[NT];  // reference, sum of p, sum of p (least_v + 8 step_v)
     int lim[NT][2];               // positions that the row sees
     float o[D / 16][NT][4];
@@ -215,9 +215,9 @@ __device__ __forceinline__ void att_queries(const AttParams& p, AttRows<D, NT>& 
             q[(nt * (D / 32) + w) * 32 + lane] = make_uint4(pair_of<__half>(x[0], x[4]), pair_of<__half>(x[1] * 0.0625f, x[5] * 0.0625f),
                                                             pair_of<__half>(x[2], x[6]), pair_of<__half>(x[3] * 0.0625f, x[7] * 0.0625f));
         }
-        // the products are 2^(e - 24) of the true ones, keys 2^(24 - 13); NaN and infinities in a row make all of its scores NaN
+        // the products are 2^e of the true ones, keys 2^-kAttKeys; NaN and infinities in a row make all of its scores NaN
         const float a = isfinite(top) ? exp2_int(kAttKeys - e) * p.score_scale : __int_as_float(0x7FC00000);
-        const float b = sum * 0x1p-24f;
+        const float b = sum;
         r.a[nt] = make_float2(__shfl_sync(0xffffffffu, a, 8 * t), __shfl_sync(0xffffffffu, a, 8 * t + 4));
         r.b[nt] = make_float2(__shfl_sync(0xffffffffu, b, 8 * t), __shfl_sync(0xffffffffu, b, 8 * t + 4));
         r.m[nt] = both(kAttNone);
@@ -293,8 +293,9 @@ __device__ __forceinline__ void att_step(AttRows<D, NT>& r, const uint8_t* K, co
 #pragma unroll
             for (int h = 0; h < H; ++h) {
                 const uint32_t u = z ? keys[h][0][w] >> 8 : keys[h][0][w], v = z ? keys[h][1][w] >> 8 : keys[h][1][w];
+                const uint32_t a0 = centred_low(u), a1 = centred_low(v), a2 = centred_high(u), a3 = centred_high(v);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mma_16816(x[h][nt], u & kLow, v & kLow, u & kHigh, v & kHigh, z ? q[nt].z : q[nt].x, z ? q[nt].w : q[nt].y);
+                for (int nt = 0; nt < NT; ++nt) mma_16816(x[h][nt], a0, a1, a2, a3, z ? q[nt].z : q[nt].x, z ? q[nt].w : q[nt].y);
             }
     }
     // scores over a; `move`: one passes its row's reference by too much, or a value's step its bound
@@ -308,10 +309,11 @@ __device__ __forceinline__ void att_step(AttRows<D, NT>& r, const uint8_t* K, co
         for (int i = 0; i < 2; ++i) {
             vstep[h][i] = __uint_as_float(pv[h][i] << 16);
             if (!MASKED) steps[0].x = fmaxf(steps[0].x, vstep[h][i]);
-            const float2 step = both(__uint_as_float(pk[h][i] << 16) * key_scale), least = both(__uint_as_float(pk[h][i] & 0xFFFF0000u) * key_scale);
+            const float s = __uint_as_float(pk[h][i] << 16);
+            const float2 step = both(s * key_scale), middle = both(__fmaf_rn(8.0f, s, __uint_as_float(pk[h][i] & 0xFFFF0000u)) * key_scale);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                float2 v = __ffma2_rn(make_float2(x[h][nt][2 * i], x[h][nt][2 * i + 1]), step, __fmul2_rn(least, r.b[nt]));
+                float2 v = __ffma2_rn(make_float2(x[h][nt][2 * i], x[h][nt][2 * i + 1]), step, __fmul2_rn(middle, r.b[nt]));
                 if (MASKED) {
                     if (at[h][i] == 0x7FFFFFFF || at[h][i] >= r.lim[nt][0]) v.x = -INFINITY;
                     if (at[h][i] == 0x7FFFFFFF || at[h][i] >= r.lim[nt][1]) v.y = -INFINITY;
@@ -645,7 +647,6 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT, RW>::kPerSm) cach
 
     // ---- the computing warps
     const int rw = warp % RW, tw = warp / RW;   // which rows, which tokens of a tile
-    const float key_scale = p.key_scale * 0x1p24f;   // (codes are 2^-24 of themselves)
     const int g = lane >> 2, t = lane & 3;
     AttRows<D, NT> r;
     bool lost = false;
@@ -690,9 +691,9 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT, RW>::kPerSm) cach
                 for (int tk = tw * 16 * H; tk < kAttTile; tk += TW * 16 * H) {
                     const int pos = tile * kAttTile + tk;
                     if (whole && pos + 16 * H <= all && !r.apart)
-                        att_step<D, NT, H, false>(r, K, V, KS, VS, key_scale, tk, pos, it.seen, have, shift);
+                        att_step<D, NT, H, false>(r, K, V, KS, VS, p.key_scale, tk, pos, it.seen, have, shift);
                     else if (pos < it.seen)
-                        att_step<D, NT, H, true>(r, K, V, KS, VS, key_scale, tk, pos, it.seen, have, shift);
+                        att_step<D, NT, H, true>(r, K, V, KS, VS, p.key_scale, tk, pos, it.seen, have, shift);
                 }
             }
             __syncwarp();

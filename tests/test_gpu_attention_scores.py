@@ -128,3 +128,30 @@ def test_keys_and_scores_near_the_largest_float(ops, dim, news, room):  # noqa: 
         keys = top * torch.randint(-8, 9, (length,), generator=g, device="cuda").float()
         run(ops, g, dim, news, room, length, keys, q_value, scale=2.0 ** -5)
         run(ops, g, dim, news, room, length, keys, -q_value)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("dim,news,room", CASES)
+@pytest.mark.parametrize("exponent", [4, 8, 12, 14])
+@pytest.mark.parametrize("at", [2, 3, 60])
+def test_a_large_dimension_of_queries_where_keys_are_zero(ops, dim, news, room, exponent, at, kind):  # noqa: F811
+    """It has no part in the scores, and takes no place from those that have: they are sums in f32."""
+    g = generator(dim + exponent)
+    length, page = 512, 64
+    pages, table = layout(g, [length], page, width=max(room // page, -(-length // page)))
+    cache = random_cache(g, pages, 2, page, dim)
+    keys, step = cache[0], cache[1][..., :1].float()
+    cache[1][..., 1:] = (-8 * step).to(torch.bfloat16)   # code 8 is zero
+    keys[..., at // 2] = (keys[..., at // 2] & 0xF0) | 0x08 if at % 2 == 0 else (keys[..., at // 2] & 0x0F) | 0x80
+    q = torch.randn((news, 8, dim), generator=g, device="cuda")
+    q[..., at] = 2.0 ** exponent
+    q = q.to(TYPES[kind])
+    args = (table, ints([length]), begins([news]))
+    got = ops.cache_attention(q, cache, *args).double()
+    # Without that dimension the same tokens are as far from 64 bits as the kernel's roundings take them.  With it the other dimensions are
+    # f16 numbers down to 2^-35 of it, 2^-21 at most: no more than a hundredth of an output's rounding.
+    blank = q.clone()
+    blank[..., at] = 0
+    want = expected(blank, cache, table, length, news, dim ** -0.5)[0]
+    usual = (ops.cache_attention(blank, cache, *args).double() - want).norm()
+    assert float((got - want).norm() / usual) <= 1.25, float((got - want).norm() / usual)
