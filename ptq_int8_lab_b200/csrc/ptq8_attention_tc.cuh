@@ -51,6 +51,10 @@ __device__ __forceinline__ void tmem_load8(uint32_t taddr, uint32_t (&v)[8]) {
                  : "r"(taddr)
                  : "memory");
 }
+// (naming the registers: their uses stay behind it)
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&v)[8]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7])::"memory");
+}
 __device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // D[tmem] (+)= A B^T, f16 -> f32; A in shared memory or in TMEM.  By one lane of a converged warp.
@@ -98,7 +102,7 @@ __device__ __noinline__ void tc_rescale(uint32_t s, int cols, uint32_t o, int oc
     for (int i = 0; i < cols; i += 8) {
         uint32_t x[8];
         tmem_load8(s + i, x);
-        tmem_wait_ld();
+        tmem_wait_ld(x);
 #pragma unroll
         for (int z = 0; z < 8; ++z) {
             const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&x[z]));   // (a scale below 2^-24 is no f16 number, its product may be)
@@ -110,7 +114,7 @@ __device__ __noinline__ void tc_rescale(uint32_t s, int cols, uint32_t o, int oc
     for (int i = 0; i < ocols; i += 8) {
         uint32_t x[8];
         tmem_load8(o + i, x);
-        tmem_wait_ld();
+        tmem_wait_ld(x);
 #pragma unroll
         for (int z = 0; z < 8; ++z) x[z] = __float_as_uint(__uint_as_float(x[z]) * scale);
         tmem_store8(o + i, x);
