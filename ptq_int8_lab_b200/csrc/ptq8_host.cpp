@@ -3,6 +3,10 @@
 // it return -1 before any call, and ops.py goes through the arguments one by one and says what is wrong with them.
 //
 // A call of cache_write took 8 us of host time with the same steps in Python, of which this takes one.
+//
+// The interpreter's lock is given back around the calls of libptq8 and the allocator, as ctypes does: a launch may wait for room in its
+// stream's queue, and that stream for a host function that wants the lock.  Meanwhile the tensors are held, whatever other
+// threads do with the caller's containers.
 #include <Python.h>
 
 #include <ATen/ATen.h>
@@ -10,6 +14,7 @@
 
 #include <cmath>
 #include <cstdint>
+#include <initializer_list>
 
 #include "ptq8.h"
 
@@ -43,7 +48,26 @@ bool part(const at::Tensor& t, at::ScalarType type, const int64_t* shape, int64_
            t.stride(2) == wide && on(t, device);
 }
 
-bool fill(ptq8_cache& c, PyObject* cache, PyObject* table_o, PyObject* lengths_o, PyObject* starts_o, int64_t tokens, int64_t device) {
+// Tensors that a call reads and writes, kept until it is over.
+struct Held {
+    at::Tensor tensors[10];
+    int n = 0;
+    void add(std::initializer_list<const at::Tensor*> more) {
+        for (const at::Tensor* t : more)
+            if (t) tensors[n++] = *t;
+    }
+};
+
+// What a call gives, without the interpreter's lock meanwhile.
+template <typename F>
+auto unlocked(const F& call) {
+    PyThreadState* state = PyEval_SaveThread();
+    const auto result = call();   // (throws nothing)
+    PyEval_RestoreThread(state);
+    return result;
+}
+
+bool fill(ptq8_cache& c, Held& held, PyObject* cache, PyObject* table_o, PyObject* lengths_o, PyObject* starts_o, int64_t tokens, int64_t device) {
     PyObject* const* items;
     if (PyTuple_Check(cache) && PyTuple_GET_SIZE(cache) == 4)
         items = &PyTuple_GET_ITEM(cache, 0);
@@ -66,6 +90,7 @@ bool fill(ptq8_cache& c, PyObject* cache, PyObject* table_o, PyObject* lengths_o
     } else {
         const at::Tensor* starts = tensor(starts_o);
         if (!starts || !ints(*starts, seqs + 1, device)) return false;
+        held.add({starts});
         c.starts = static_cast<const int*>(starts->data_ptr());
     }
     constexpr int64_t most = 0x7FFFFFFF;
@@ -85,6 +110,7 @@ bool fill(ptq8_cache& c, PyObject* cache, PyObject* table_o, PyObject* lengths_o
     c.kv_heads = static_cast<int>(shape[1]);
     c.head_dim = static_cast<int>(2 * half);
     c.sequences = static_cast<int>(seqs);
+    held.add({k, ks, v, vs, table, lengths});
     return true;
 }
 
@@ -100,7 +126,9 @@ PyObject* cache_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!k || !v || k->dim() != 3 || v->dim() != 3 || k->scalar_type() != v->scalar_type()) return answer(-1);
     ptq8_cache_rows_args args{};
     const int64_t tokens = k->size(0);
-    if (!fill(args.cache, a[3], a[6], a[7], a[8], tokens, device)) return answer(-1);
+    Held held;
+    held.add({k, v});
+    if (!fill(args.cache, held, a[3], a[6], a[7], a[8], tokens, device)) return answer(-1);
     args.type = type_of(*k);
     for (const at::Tensor* t : {k, v})
         if (t->size(0) != tokens || t->size(1) != args.cache.kv_heads || t->size(2) != args.cache.head_dim || t->stride(2) != 1 || !on(*t, device)) return answer(-1);
@@ -111,7 +139,7 @@ PyObject* cache_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
     auto* ops = static_cast<ptq8_ops*>(PyLong_AsVoidPtr(a[1]));
     void* stream = PyLong_AsVoidPtr(a[9]);
     if (PyErr_Occurred()) return nullptr;
-    return answer((write ? cache_write_entry : cache_read_entry)(ops, &args, stream));
+    return answer(unlocked([&]() noexcept { return (write ? cache_write_entry : cache_read_entry)(ops, &args, stream); }));
 }
 
 // cache_attention(handle, device, q, cache, table, lengths, starts, scale, out, stream), its workspace made here
@@ -123,7 +151,9 @@ PyObject* cache_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!q || !out || q->dim() != 3 || out->sizes() != q->sizes() || out->scalar_type() != q->scalar_type() || !on(*q, device) || !on(*out, device)) return answer(-1);
     if (q->stride(2) != 1 || out->stride(2) != 1) return answer(-1);
     ptq8_cache_attention_args args{};
-    if (!fill(args.cache, a[3], a[4], a[5], a[6], q->size(0), device)) return answer(-1);
+    Held held;
+    held.add({q, out});
+    if (!fill(args.cache, held, a[3], a[4], a[5], a[6], q->size(0), device)) return answer(-1);
     args.type = type_of(*q);
     if (args.type != PTQ8_F16 && args.type != PTQ8_BF16) return answer(-1);
     if (q->size(2) != args.cache.head_dim || q->size(1) > 0x7FFFFFFF) return answer(-1);
@@ -135,19 +165,22 @@ PyObject* cache_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     auto* ops = static_cast<ptq8_ops*>(PyLong_AsVoidPtr(a[0]));
     void* stream = PyLong_AsVoidPtr(a[9]);
     if (PyErr_Occurred()) return nullptr;
-    const long long need = workspace_entry(ops, &args);
-    if (need < 0) return answer(-1);
     at::Tensor workspace;
-    if (need) {
-        try {
-            workspace = at::empty({need}, q->options().dtype(at::kByte));
-        } catch (const std::exception&) {   // out of memory: the way through Python raises torch's own error
-            return answer(-1);
+    const auto options = q->options().dtype(at::kByte);
+    return answer(unlocked([&]() noexcept {
+        const long long need = workspace_entry(ops, &args);
+        if (need < 0) return -1;
+        if (need) {
+            try {
+                workspace = at::empty({need}, options);
+            } catch (...) {   // out of memory: the way through Python raises torch's own error
+                return -1;
+            }
+            args.workspace = workspace.data_ptr();
+            args.workspace_bytes = need;
         }
-        args.workspace = workspace.data_ptr();
-        args.workspace_bytes = need;
-    }
-    return answer(attention_entry(ops, &args, stream));
+        return attention_entry(ops, &args, stream);
+    }));
 }
 
 // linear_w4(handle, device, x, w, w_scale, group, bias, act, out, stream)
@@ -184,7 +217,10 @@ PyObject* linear_w4(PyObject*, PyObject* const* a, Py_ssize_t n) {
     auto* ops = static_cast<ptq8_ops*>(PyLong_AsVoidPtr(a[0]));
     void* stream = PyLong_AsVoidPtr(a[9]);
     if (PyErr_Occurred()) return nullptr;
-    return answer(w4_entry(ops, &args, stream));
+    Held held;
+    held.add({x, w, s, y});
+    if (a[6] != Py_None) held.add({tensor(a[6])});
+    return answer(unlocked([&]() noexcept { return w4_entry(ops, &args, stream); }));
 }
 
 // entries(cache_write, cache_read, cache_attention, cache_attention_workspace, linear_w4): addresses
