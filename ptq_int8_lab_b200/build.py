@@ -5,8 +5,9 @@
 
 The library is plain CUDA runtime + C++ (no torch linkage); the Python host
 side loads it with ctypes.  Output: ptq_int8_lab_b200/_lib/libptq8.so, and
-beside it ptq8_host.so, the Python extension that reads torch tensors for the
-token operators' calls (C++ against torch's headers, no CUDA).
+where torch is installed ptq8_host.so beside it, the Python extension that reads
+torch tensors for the newer token operators' calls (C++ against torch's headers,
+no CUDA).  The library does not depend on it, in its build or in its use.
 """
 import os
 import subprocess
@@ -35,7 +36,11 @@ HOST = OUT / "ptq8_host.so"
 
 
 def host_command(out: Path) -> list:
-    import torch
+    """The compiler's command for ptq8_host.so; empty where there is no torch to read tensors of."""
+    try:
+        import torch
+    except ImportError:
+        return []
     root = Path(torch.__file__).resolve().parent
     return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-I", str(HERE.parent / "include"),
             "-I", sysconfig.get_paths()["include"], "-I", str(root / "include"), "-I", str(root / "include/torch/csrc/api/include"),
@@ -54,10 +59,15 @@ def build(verbose_ptxas: bool = False) -> Path:
         print(" ".join(cmd), flush=True)
         objs.append(OUT / obj)
         running.append((cmd, subprocess.Popen(cmd)))
-    cmd = host_command(OUT / "ptq8_host.so.tmp")
-    print(" ".join(cmd), flush=True)
-    running.append((cmd, subprocess.Popen(cmd)))
+    host_tmp = OUT / "ptq8_host.so.tmp"
+    host_cmd, host = host_command(host_tmp), None
+    if host_cmd:
+        print(" ".join(host_cmd), flush=True)
+        host = subprocess.Popen(host_cmd)
+    else:
+        print("no torch: libptq8.so alone, without ptq8_host.so", flush=True)
     failed = [cmd for cmd, p in running if p.wait() != 0]
+    host_failed = host is not None and host.wait() != 0
     if failed:
         raise subprocess.CalledProcessError(1, failed[0])
     tmp = OUT / "libptq8.so.tmp"
@@ -65,9 +75,12 @@ def build(verbose_ptxas: bool = False) -> Path:
     print(" ".join(cmd), flush=True)
     subprocess.check_call(cmd)
     os.replace(tmp, lib)
-    os.replace(OUT / "ptq8_host.so.tmp", HOST)
     for o in objs:
         o.unlink()
+    if host_failed:   # (libptq8.so is there, and all that does not need the extension works)
+        raise subprocess.CalledProcessError(1, host_cmd)
+    if host is not None:
+        os.replace(host_tmp, HOST)
     return lib
 
 

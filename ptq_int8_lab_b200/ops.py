@@ -25,6 +25,7 @@ from __future__ import annotations
 import ctypes
 import importlib.util
 import struct
+from functools import cached_property
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -53,15 +54,19 @@ _host = None
 
 
 def _host_module():
-    """ptq8_host: the calls of the newer operators without the interpreter's share (built beside libptq8.so)."""
+    """ptq8_host: the calls of linear_w4 and the cache operators without the interpreter's share (built beside libptq8.so against the
+    installed torch).  Loaded at their first call; the operators that do without it never look for it."""
     global _host
     if _host is None:
         from .build import HOST
         if not HOST.exists():
             raise Ptq8Error(f"{HOST} not found: build it with `python -m ptq_int8_lab_b200.build`")
         spec = importlib.util.spec_from_file_location("ptq8_host", HOST)
-        module = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(module)
+        try:
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+        except ImportError as e:
+            raise Ptq8Error(f"{HOST} does not fit this Python or torch ({e}): build it with `python -m ptq_int8_lab_b200.build`") from e
         L = lib()
         module.entries(*(ctypes.cast(f, ctypes.c_void_p).value for f in
                          (L.ptq8_cache_write, L.ptq8_cache_read, L.ptq8_cache_attention, L.ptq8_cache_attention_workspace, L.ptq8_linear_w4)))
@@ -197,9 +202,19 @@ class Int8Ops:
         self._attention_args = ctypes.create_string_buffer(_ATTENTION.size)
         self._linear_w4, self._cache_write, self._cache_read = self._lib.ptq8_linear_w4, self._lib.ptq8_cache_write, self._lib.ptq8_cache_read
         self._cache_attention = self._lib.ptq8_cache_attention
-        host = _host_module()
-        self._host_rows, self._host_attention, self._host_w4 = host.cache_rows, host.cache_attention, host.linear_w4
         self._workspaces = {}   # bytes, by the sizes of a call
+
+    @cached_property
+    def _host_rows(self):
+        return _host_module().cache_rows
+
+    @cached_property
+    def _host_attention(self):
+        return _host_module().cache_attention
+
+    @cached_property
+    def _host_w4(self):
+        return _host_module().linear_w4
 
     def _check(self, rc: int):
         if rc:
