@@ -300,7 +300,7 @@ __device__ __forceinline__ void att_step(AttRows<D, NT>& r, const uint8_t* K, co
     }
     // scores over a; `move`: one passes its row's reference by too much, or a value's step its bound
     float vstep[H][2], most = 0.0f;
-    float2 steps[NT];   // the largest step of a value that the row sees (MASKED), or that there is
+    float2 steps[NT];   // the largest step, in magnitude, of a value that the row sees (MASKED), or that there is
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) steps[nt] = both(0.0f);
 #pragma unroll
@@ -308,7 +308,7 @@ __device__ __forceinline__ void att_step(AttRows<D, NT>& r, const uint8_t* K, co
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             vstep[h][i] = __uint_as_float(pv[h][i] << 16);
-            if (!MASKED) steps[0].x = fmaxf(steps[0].x, vstep[h][i]);
+            if (!MASKED) steps[0].x = fmaxf(steps[0].x, fabsf(vstep[h][i]));
             const float s = __uint_as_float(pk[h][i] << 16);
             const float2 step = both(s * key_scale), middle = both(__fmaf_rn(8.0f, s, __uint_as_float(pk[h][i] & 0xFFFF0000u)) * key_scale);
 #pragma unroll
@@ -322,8 +322,8 @@ __device__ __forceinline__ void att_step(AttRows<D, NT>& r, const uint8_t* K, co
                 const float2 d = __ffma2_rn(v, r.a[nt], make_float2(-r.m[nt].x, -r.m[nt].y));
                 if (!MASKED || v.x != -INFINITY) most = fmaxf(most, d.x);
                 if (!MASKED || v.y != -INFINITY) most = fmaxf(most, d.y);
-                if (MASKED && v.x != -INFINITY) steps[nt].x = fmaxf(steps[nt].x, vstep[h][i]);
-                if (MASKED && v.y != -INFINITY) steps[nt].y = fmaxf(steps[nt].y, vstep[h][i]);
+                if (MASKED && v.x != -INFINITY) steps[nt].x = fmaxf(steps[nt].x, fabsf(vstep[h][i]));
+                if (MASKED && v.y != -INFINITY) steps[nt].y = fmaxf(steps[nt].y, fabsf(vstep[h][i]));
             }
         }
     bool wide = false;

@@ -135,8 +135,8 @@ __device__ __forceinline__ void tc_scores(const TcRow& r, const uint32_t (&x)[16
             if (!((in >> (2 * i)) & 1)) v[i].x = -INFINITY;
             if (!((in >> (2 * i + 1)) & 1)) v[i].y = -INFINITY;
             const float4 value = param[16 * k + 8 + i];
-            if ((in >> (2 * i)) & 1) steps = fmaxf(steps, value.x);
-            if ((in >> (2 * i + 1)) & 1) steps = fmaxf(steps, value.y);
+            if ((in >> (2 * i)) & 1) steps = fmaxf(steps, fabsf(value.x));
+            if ((in >> (2 * i + 1)) & 1) steps = fmaxf(steps, fabsf(value.y));
         }
         most = fmaxf(most, fmaxf(v[i].x, v[i].y));
     }
@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tiles_kernel(co
                     to[0] = ks, to[2] = __fmaf_rn(8.0f, ks, __uint_as_float(pk & 0xFFFF0000u) * p.key_scale);
                     to[32] = vs, to[34] = __fmaf_rn(8.0f, vs, __uint_as_float(pv & 0xFFFF0000u));
                     const uint32_t have = __ballot_sync(0xffffffffu, ok);
-                    float most = fmaxf(vs, 0.0f);   // (NaN counts for nothing)
+                    float most = fmaxf(fabsf(vs), 0.0f);   // (NaN counts for nothing)
 #pragma unroll
                     for (int d = 1; d < 32; d *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
                     if (lane == 0) {

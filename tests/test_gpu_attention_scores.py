@@ -155,3 +155,32 @@ def test_a_large_dimension_of_queries_where_keys_are_zero(ops, dim, news, room, 
     want = expected(blank, cache, table, length, news, dim ** -0.5)[0]
     usual = (ops.cache_attention(blank, cache, *args).double() - want).norm()
     assert float((got - want).norm() / usual) <= 1.25, float((got - want).norm() / usual)
+
+
+@pytest.mark.parametrize("dim,news,room", CASES)
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_steps_below_zero(ops, dim, news, room, which):  # noqa: F811
+    """A cache that another program has filled: a code stands for least + step * code whatever the step's sign."""
+    g = generator(dim + news)
+    length, page = 400, 64
+    pages, table = layout(g, [length], page, width=max(room // page, -(-length // page)))
+    cache = random_cache(g, pages, 2, page, dim)
+    plain = [t.clone() for t in cache]
+    flip = torch.rand(cache[1].shape[:3], generator=g, device="cuda") < (0.0, 0.5, 1.0)[which]
+    for i in (0, 2):   # the same values: codes from the other end, least + 15 step and -step
+        cache[i][flip] = 255 - cache[i][flip]
+        step, least = cache[i + 1][..., 0].float(), cache[i + 1][..., 1].float()
+        step = (step * 8).ceil() / 8   # (numbers whose multiples by 15 bf16 holds)
+        least = (least * 2).round() / 2
+        for to, sign in ((plain, 1.0), (cache, -1.0)):
+            to[i + 1][..., 0] = torch.where(flip, sign * step, step).to(torch.bfloat16)
+            to[i + 1][..., 1] = torch.where(flip, least + (15 * step if sign < 0 else 0), least).to(torch.bfloat16)
+    for i in (0, 2):
+        (ca, sa, la), (cb, sb, lb) = (R.rows_of(c[i], c[i + 1]) for c in (plain, cache))
+        assert torch.equal(ca * sa + la, cb * sb + lb)
+    q = torch.randn((news, 8, dim), generator=g, device="cuda").to(torch.float16)
+    args = (table, ints([length]), begins([news]))
+    got = ops.cache_attention(q, cache, *args).double()
+    want, bound = expected(q, plain, table, length, news, dim ** -0.5)
+    assert bool(((got - want).abs() <= bound).all()), float(((got - want).abs() / bound).max())
+    ops.check_device_error()
