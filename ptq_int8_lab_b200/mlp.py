@@ -51,6 +51,7 @@ def lay_groups(w, group: int, device: int = 0) -> Tuple[torch.Tensor, torch.Tens
     if group <= 0:
         raise E.Ptq8Error(f"group {group}")
     channels, inp = w.shape
+    group = min(group, max(inp, 1))   # (one group of all features, however large it is said to be)
     groups = -(-inp // group)
     padded = np.zeros((channels, groups * group), dtype=np.float32)
     padded[:, :inp] = w
