@@ -26,9 +26,10 @@
 // those from c U / N to (c + 1) U / N: equal shares whatever the lengths are, known on the device only.  A row tile cut
 // by a share's end leaves (numerators, reference, sum) in the workspace, and a second kernel joins them.
 //
-// What bounds it: for few rows the way from one launch to the next (one token over 2000 positions 8.9 us, of which the join's launch and
-// set-up are half), then DRAM at the loop's 6.1 TB/s and the ends (32 sequences of up to 8192 tokens 28 us, floor 12: 3 us to the first
-// bytes, shares that end apart, the join 6); warp-level products reach 42 % of their rate with 8 computing warps an SM.
+// What it spends its time on: for few rows the way from one launch to the next (one token over 2000 positions 9.2 us, of which the join's
+// launch and set-up are half), then the loop and the ends (32 sequences of up to 8192 tokens 30 us, floor 12, issue 56 %: 3 us to the first
+// bytes, shares that end apart, the join 6); warp-level products reach 42 % of their rate with 8 computing warps an SM.  All variants
+// spill a little (48 to 166 bytes of stores), 64 dimensions with 8 rows aside.
 // A producer warp keeps bulk copies of whole tiles in flight; four warps compute, RW of them on different rows, 4 / RW on
 // different tokens of a tile.
 #pragma once

@@ -16,10 +16,10 @@
 // exponentials do; 8-11 widen codes; 12 issues MMAs; 13 copies tiles in; 14, 15 idle.
 //
 // What bounds it: the softmax's instructions.  2 x 512 new tokens of 32 heads (8 key heads, D = 128, bf16) over 4500 to 8192
-// positions take 243 us, 420 TFLOP/s, against 463 us with warp-level products; a tile of 128 tokens takes some 7600 cycles, of
+// positions take 247 us, 413 TFLOP/s, against 463 us with warp-level products; a tile of 128 tokens takes some 7700 cycles, of
 // which the tensor cores need 2000 and the exponentials 2000 (4 a cycle and scheduler); the rest are the other twelve instructions for
 // two scores and what they wait for, with two warps of the softmax a scheduler.  All eight steps of a tile's loop written out, 32 KB of
-// instructions, waited for those (285 us instead of 243).  The tokens' pairs as they lie in the cache, half the bytes from shared memory for four more instructions
+// instructions, waited for those (285 us where this took 243).  The kernel spills 68 bytes (132 of loads).  The tokens' pairs as they lie in the cache, half the bytes from shared memory for four more instructions
 // for two scores: 270.  More registers for the softmax warps by setmaxnreg: 559, the others spilled.
 #pragma once
 

@@ -176,9 +176,11 @@ const AttJoin kAttJoins[3][2] = {{cache_attention_join_kernel<64, 1>, cache_atte
 // to do: their blocks take some us more to begin and to join.  us with them and without, 8 key heads, bf16, sequences x
 // query rows of a key head x positions:
 //              1 x 512 x 500   1 x 384 x 4000   1 x 512 x 4000   1 x 1024 x 4000   8 x 68 x 4000   8 x 136 x 4000   8 x 512 x 4000
-//   D = 64     25   19         37   33          39   38          55   60           64   58         76   81          148   189
-//   D = 128    34   25         47   46          49   56          74   92           79   90         96   128         179   310
-// The host knows only what the table has room for: a table much wider than its sequences are long takes them early.
+//   D = 64     26   19         37   34          41   40          57   63           65   62         79   86          152   201
+//   D = 128    34   26         47   48          51   59          75   98           81   97         99   137         183   332
+// (The last but four are 16.5 M rows x tokens, just below the limit of 128 dimensions: a limit that took them would take 1 x 384 x 4000 and
+// wider tables of shorter sequences with them.)  The host knows only what the table has room for: a table much wider than its
+// sequences are long takes tiles early.  It goes by the mean of the sequences: pieces beside many single tokens may stay on narrow tiles.
 const AttVariant& att_choose(const ptq8_cache_attention_args& a, long long room) {
     const long long rows = (a.tokens * (a.heads / a.cache.kv_heads) + a.cache.sequences - 1) / a.cache.sequences;
     const AttVariant* best = nullptr;

@@ -6,8 +6,9 @@
 // f32); what their rounding costs stays inside a step, since the codes are computed with the rounded numbers: least is
 // rounded down and step up, which keeps 15 steps from least no shorter than the row's spread.
 //
-// What bounds them: few rows, a launch after another (32 tokens of 8 heads written and one read 4.1 us); many, instructions: issue 68 %
-// for writing 18 k tokens of 8 heads x 128 (38 us, floor 14) and reading 33 k of 8 x 128 (40 us, floor 26).
+// What they spend their time on (in a graph of calls): few rows, a launch after another (32 tokens of 8 heads written and read back 4.1 us);
+// many, instructions and what they wait for, at issue 68 %: writing 18 k tokens of 8 heads x 128 (34 us, floor 14) and reading 33 k of 8 x 128
+// (40 us, floor 26).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -248,7 +249,7 @@ constexpr int kCacheThreads = 256;
 // 1.5 * 2^23 rounds a quotient to its code, which is then the sum's low bits; the sums' bits, shifted to their places, add
 // up to the codes and a constant.  Each operation rounds by itself (no contraction: packed f32 products and sums would be).
 // A row that holds NaN or an infinity, or whose spread is no finite number, gets codes 0 and NaN for step and least.
-// Instructions bound it: 291 k rows of 128 bf16 (75 MB in, 20 MB out) in 39 us.
+// 291 k rows of 128 bf16 (75 MB in, 20 MB out) in 34 us, issue 68 %.
 // U: rows that a lane has at a time.
 template <typename T, int D, bool VEC, int U>
 __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(const CacheRowsParams p) {

@@ -69,10 +69,10 @@ const W4Few* const kW4Few[] = {W4FewOf<float>::kKernels, W4FewOf<__half>::kKerne
 
 // One or two tokens while the weights are small.  us here and on the tensor cores, tokens x in -> out:
 //                  1024 -> 1024   4096 -> 1024   4096 -> 4096   4096 -> 14336
-//   1 x bf16       2.1   4.5      2.6   6.6      4.9    6.5     15.4   13.4
-//   2 x bf16       4.1   4.5      5.1   6.6      9.2    6.6     26.8   13.4
-//   1 x f32        2.5   5.9      3.6   8.0      8.1    10.7    23.6   21.0
-//   2 x f32        4.4   5.9      6.2   8.0      13.7   10.7    43.3   21.0
+//   1 x bf16       2.0   4.3      2.6   6.1      4.9    6.3     14.5   12.8
+//   2 x bf16       4.1   4.6      5.2   6.3      8.4    6.5     25.3   12.8
+//   1 x f32        2.4   4.3      3.3   6.7      7.5    7.1     23.4   13.9
+//   2 x f32        4.4   4.3      6.1   7.1      13.3   7.3     42.5   14.1
 // (The activations are read again for every four weight rows, which is what large weights make it wait for.)  Rows of whole vectors.
 bool few_rows(const ptq8_linear_w4_args& a, bool vectors) {
     const bool gated = a.epilogue == PTQ8_EPI_SWIGLU;

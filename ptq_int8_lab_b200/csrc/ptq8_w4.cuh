@@ -20,10 +20,12 @@
 // dealt to a row's bytes so that a group stays within an MMA (four lanes hold VB bytes each: 32, 64 or 128 codes of a row).
 // EXACT (outputs of 32 bits): each product of 16 features begins at zero and is added in f32 (45 tokens x 2000, f32: 8.6e-8 from 64 bits).
 //
-// What bounds it (B200, in a graph of calls): one token, 4096 -> 4096, 4.9 us: latency and launch (3.4 TB/s of weights from L2);
-// 8 tokens, 4096 -> 2 x 8192, 15 us, floor 5.5: the weights' and fragments' way through shared memory and the instructions that mask them
-// (issue 49 %), after 3 us in which every block brings the activations into order; 45 tokens f32, 2000 -> 1270, 10.1 us:
-// that same start, for three passes of 16 tokens.
+// What it spends its time on (B200, in a graph of calls): one token, 4096 -> 4096, 4.9 us, floor 1.3: latency and launch (8.7 MB at
+// 1.8 TB/s, from L2; 5.2 us with weights from DRAM); 8 tokens, 4096 -> 2 x 8192, 15 us, floor 5.5: waits for the weights' and fragments'
+// way through shared memory and for the instructions that widen them (issue 53 %), after 3 us in which every block brings the activations
+// into order; 45 tokens f32, 2000 -> 1270, 10.1 us: that same start, for three passes of 16 tokens.  Beyond some tens of tokens every
+// pass of at most 32 reads and widens all weights again: 512 bf16 tokens, 4096 -> 4096, 127 us where the operations' floor is 11.
+// Kernels of four tiles of eight columns spill (up to 282 bytes of stores and 372 of loads), those of one do not.
 #pragma once
 
 #include "ptq8_cache.cuh"
